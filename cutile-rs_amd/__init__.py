@@ -164,6 +164,14 @@ def lib() -> C.CDLL:
                                                 P(TensorArg), f32, P(LaunchOpts)],
             "cutile_launch_linear_tile_nvfp4": [vp, P(PartitionArg), P(TensorArg), P(TensorArg), P(TensorArg),
                                                 P(TensorArg), f32, P(LaunchOpts)],
+            "cutile_launch_linear_tile_mxfp4": [vp, P(PartitionArg), P(TensorArg), P(TensorArg), P(TensorArg),
+                                                P(TensorArg), f32, P(LaunchOpts)],
+            "cutile_launch_block_quantize": [vp, P(TensorArg), P(PartitionArg), P(PartitionArg), f32, P(LaunchOpts)],
+            "cutile_launch_block_dequantize": [vp, P(TensorArg), P(TensorArg), f32, P(PartitionArg), P(LaunchOpts)],
+            "cutile_launch_rms_norm_quantize": [vp, P(TensorArg), P(TensorArg), P(PartitionArg), P(PartitionArg), f32, f32, P(LaunchOpts)],
+            "cutile_launch_add_rms_norm_quantize": [vp, P(TensorArg), P(TensorArg), P(TensorArg), P(PartitionArg), P(PartitionArg), P(PartitionArg),
+                                                    f32, f32, P(LaunchOpts)],
+            "cutile_launch_silu_mul_quantize": [vp, P(TensorArg), P(TensorArg), P(PartitionArg), P(PartitionArg), f32, P(LaunchOpts)],
             "cutile_partition_grid": [P(PartitionArg), P(C.c_uint32 * 3)],
             "cutile_mapped_partition_grid": [P(MappedPartitionArg), P(C.c_uint32 * 3)],
             "cutile_mapped_partition_index": [P(MappedPartitionArg), C.c_uint32, P(C.c_uint32 * 3), P(C.c_uint32)],
@@ -760,6 +768,70 @@ def linear_tile_nvfp4(z: Partition, x, y, x_scales, y_scales, alpha: float = 1.0
     nibble first); scales [M, K/16], [N, K/16]: uint8 (or float8_e4m3fn) tensors of e4m3fn bytes; z f32 or bf16."""
     _c.linear_tile_nvfp4(stream, z, (x, F4E2M1FNX2), (y, F4E2M1FNX2), (x_scales, F8E4M3FN), (y_scales, F8E4M3FN), float(alpha),
             (grid, generics, variant))
+
+
+def linear_tile_mxfp4(z: Partition, x, y, x_scales, y_scales, alpha: float = 1.0, *, stream=None, grid=None,
+                      generics=None, variant=None) -> None:
+    """linear_tile on MXFP4 operands: x [M, K/2], y [N, K/2]: uint8 tensors of packed e2m1 pairs (low nibble first); scales
+    [M, K/32], [N, K/32]: uint8 (or float8_e8m0fnu) tensors of e8m0 bytes; z f32 or bf16."""
+    _c.linear_tile_mxfp4(stream, z, (x, F4E2M1FNX2), (y, F4E2M1FNX2), (x_scales, F8E8M0FNU), (y_scales, F8E8M0FNU), float(alpha),
+            (grid, generics, variant))
+
+
+# ---- block-scaled rows: format -> element types of the data and of the scales ------------------------------------------------
+BLOCK_FORMATS = {"mxfp8": (F8E4M3FN, F8E8M0FNU), "mxfp4": (F4E2M1FNX2, F8E8M0FNU), "nvfp4": (F4E2M1FNX2, F8E4M3FN)}
+
+
+def _block_types(fmt: str, *tensors):
+    """the element types of a format; `tensors` hold its bytes (data, scales)"""
+    if fmt not in BLOCK_FORMATS:
+        raise CutileError(-2, f"unknown block-scaled format {fmt!r}: one of {', '.join(BLOCK_FORMATS)}")
+    for t in tensors:
+        if t.element_size() != 1:
+            raise CutileError(-2, f"{fmt}: data and scales are tensors of bytes (uint8 or an 8-bit float), not {t.dtype}")
+    return BLOCK_FORMATS[fmt]
+
+
+def _block_outputs(fmt: str, out: Partition, scales: Partition):
+    d, s = _block_types(fmt, out.tensor, scales.tensor)
+    return Partition(out.tensor, out.shape, out.prefix, d), Partition(scales.tensor, scales.shape, scales.prefix, s)
+
+
+def block_quantize(x, out: Partition, scales: Partition, fmt: str, tensor_scale: float = 1.0, *, stream=None, grid=None, generics=None,
+                   variant=None) -> None:
+    """x [M, N] (f16, bf16, f32; any strides) as block-scaled rows.  ``fmt`` "mxfp8": out [M, K] e4m3 bytes, scales [M, K/32] e8m0;
+    "mxfp4": out [M, K/2] packed e2m1 pairs, scales [M, K/32] e8m0; "nvfp4": out [M, K/2], scales [M, K/16] e4m3 and ``tensor_scale``.
+    K >= N whole blocks, the columns behind N zeros; partitions [BM, whole row]."""
+    o, s = _block_outputs(fmt, out, scales)
+    _c.block_quantize(stream, x, o, s, float(tensor_scale), (grid, generics, variant))
+
+
+def block_dequantize(x, scales, out: Partition, fmt: str, tensor_scale: float = 1.0, *, stream=None, grid=None, generics=None,
+                     variant=None) -> None:
+    """out [M, N] (f16, bf16, f32; any strides, N <= K) <- the values that block-scaled rows stand for"""
+    d, s = _block_types(fmt, x, scales)
+    _c.block_dequantize(stream, (x, d), (scales, s), float(tensor_scale), out, (grid, generics, variant))
+
+
+def rms_norm_quantize(x, w, out: Partition, scales: Partition, eps: float, fmt: str, tensor_scale: float = 1.0, *, stream=None, grid=None,
+                      generics=None, variant=None) -> None:
+    """x / sqrt(mean(x^2) + eps) * w as block-scaled rows (formats: block_quantize); x and w f16 or bf16"""
+    o, s = _block_outputs(fmt, out, scales)
+    _c.rms_norm_quantize(stream, x, w, o, s, float(eps), float(tensor_scale), (grid, generics, variant))
+
+
+def add_rms_norm_quantize(residual, x, w, out: Partition, scales: Partition, residual_out: Partition, eps: float, fmt: str,
+                          tensor_scale: float = 1.0, *, stream=None, grid=None, generics=None, variant=None) -> None:
+    """rms_norm_quantize of residual + x; the sum goes to residual_out too (which may be residual or x itself)"""
+    o, s = _block_outputs(fmt, out, scales)
+    _c.add_rms_norm_quantize(stream, residual, x, w, o, s, residual_out, float(eps), float(tensor_scale), (grid, generics, variant))
+
+
+def silu_mul_quantize(gate, up, out: Partition, scales: Partition, fmt: str, tensor_scale: float = 1.0, *, stream=None, grid=None,
+                      generics=None, variant=None) -> None:
+    """silu(gate) * up as block-scaled rows (formats: block_quantize); gate and up f16 or bf16"""
+    o, s = _block_outputs(fmt, out, scales)
+    _c.silu_mul_quantize(stream, gate, up, o, s, float(tensor_scale), (grid, generics, variant))
 
 
 # ---- table / device helpers -------------------------------------------------------------------

@@ -41,6 +41,8 @@ IMAGES = {
     "mxtiles": "mxfp8_tiles.hip",
     "gemmgroup": "gemm_group.hip",
     "fmhakeys": "fmha_keys.hip",
+    "mxfp4flat": "mxfp4_flat.hip",
+    "blockscale": "block_scale.hip",
 }
 HOST_SOURCES = ["hip_api.cpp", "driver.cpp", "kernel_table.cpp", "launch.cpp", "runtime.cpp", "tuning.cpp", "workspace.cpp"]
 # The recording stand-in for the HIP runtime (include/cutile_hip_testing.h) is not part of the product library: the CPU
@@ -191,6 +193,7 @@ CPP_TESTS = {
     # binary -> (source, library it links: True = the product library, "testing" = the one with the recording runtime, extra flags)
     "test_host_surface": ("test_host_surface.cpp", "testing", []),
     "test_gpu_surface": ("test_gpu_surface.cpp", True, []),
+    "test_block_scale": ("test_block_scale.cpp", True, []),
     "write_record": ("write_record.cpp", True, []),
     "test_slot_table": ("test_slot_table.cpp", False, []),
     "test_slot_table_tsan": ("test_slot_table.cpp", False, ["-fsanitize=thread"]),

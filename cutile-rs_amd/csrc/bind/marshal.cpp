@@ -318,7 +318,8 @@ PyObject* call(cutile_status_t (*fn)(cutile_stream_t, A...), const Binding& b, P
   X(add_rms_norm_decode_raw_f16) X(qk_norm_rope_kv_prefill_raw_f16) X(qk_norm_rope_kv_decode_raw_f16) X(group_gemm_f16_nt_desc) \
   X(argmax_blocks_f16) X(lm_head_argmax_blocks_f16) X(argmax_reduce_blocks_to_u32) X(embedding_batch_f16) X(gather_row_f16)   \
   X(fmha_prefill_gqa_lpt_raw_f16) X(fmha_seq_f16) X(linear_tile_mxfp8) X(linear_tile_nvfp4) \
-  X(attention_decode_kernel_grouped_f16)
+  X(attention_decode_kernel_grouped_f16) X(linear_tile_mxfp4) X(block_quantize) X(block_dequantize) X(rms_norm_quantize) \
+  X(add_rms_norm_quantize) X(silu_mul_quantize)
 
 struct Launcher {
   PyObject_HEAD

@@ -29,6 +29,8 @@ extern const unsigned char cutile_img_gemmgroup_start[], cutile_img_gemmgroup_en
 extern const unsigned char cutile_img_fmhakeys_start[], cutile_img_fmhakeys_end[];
 extern const unsigned char cutile_img_gemmtiles_start[], cutile_img_gemmtiles_end[];
 extern const unsigned char cutile_img_scaledflat_start[], cutile_img_scaledflat_end[];
+extern const unsigned char cutile_img_mxfp4flat_start[], cutile_img_mxfp4flat_end[];
+extern const unsigned char cutile_img_blockscale_start[], cutile_img_blockscale_end[];
 }
 
 namespace cutile {
@@ -71,6 +73,8 @@ ImageRef image_ref(Image img) {
     case IMG_GEMM_TILES: return {cutile_img_gemmtiles_start, cutile_img_gemmtiles_end};
     case IMG_GEMM_SMALL: return {cutile_img_gemmsmall_start, cutile_img_gemmsmall_end};
     case IMG_SCALED_FLAT: return {cutile_img_scaledflat_start, cutile_img_scaledflat_end};
+    case IMG_MXFP4_FLAT: return {cutile_img_mxfp4flat_start, cutile_img_mxfp4flat_end};
+    case IMG_BLOCK_SCALE: return {cutile_img_blockscale_start, cutile_img_blockscale_end};
     default: return {nullptr, nullptr};
   }
 }
@@ -467,6 +471,23 @@ std::vector<KernelEntry> build_table() {
         const int stages = 8 * ((64 + t[3]) * (128 + (mx8 ? 4 : 16)) + 32), sums = t[2] * t[0] * (t[1] + 4) * 4;
         add(mx8 ? "linear_tile" : "linear_tile_nvfp4", keep(v), keep((mx8 ? "linear_tile_entry__" : "linear_tile_nvfp4_entry__") + v), IMG_SCALED_FLAT, 512,
             (uint32_t)(std::max(stages, sums) + 4), 0, t[1], 0, t[0], dt, 0, 2);
+      }
+  // the same strips on MXFP4 operands (mxfp4_flat.hip)
+  for (const char* dt : {"bf16", "f32"})
+    for (auto t : {std::array<int, 4>{16, 64, 8, 16}, std::array<int, 4>{32, 64, 8, 32}, std::array<int, 4>{64, 64, 8, 64}, std::array<int, 4>{64, 128, 4, 64},
+                   std::array<int, 4>{128, 128, 2, 64}}) {
+      const std::string v = std::string(dt) + "_flat" + std::to_string(t[0]) + "x" + std::to_string(t[1]);
+      const int stages = 8 * ((64 + t[3]) * (128 + 8) + 32), sums = t[2] * t[0] * (t[1] + 4) * 4;
+      add("linear_tile_mxfp4", keep(v), keep("linear_tile_mxfp4_entry__" + v), IMG_MXFP4_FLAT, 512, (uint32_t)(std::max(stages, sums) + 4), 0, t[1], 0, t[0], dt, 0, 2);
+    }
+
+  // ---- block-scaled rows (block_scale.hip) ----
+  for (const char* fmt : {"mxfp8", "mxfp4", "nvfp4"})
+    for (const char* dt : {"f16", "bf16", "f32"})
+      for (const char* fn : {"block_quantize", "block_dequantize", "silu_mul_quantize", "rms_norm_quantize", "add_rms_norm_quantize"}) {
+        if (dt[1] == '3' && strncmp(fn, "block_", 6) != 0) continue;   // (the fused forms read 16-bit rows)
+        const std::string v = std::string(fmt) + "_" + dt + "_any";
+        add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_BLOCK_SCALE, 256, strstr(fn, "norm") ? 16 : 0, 0, 0, 0, 0, dt, 0, 2);
       }
   return t;
 }

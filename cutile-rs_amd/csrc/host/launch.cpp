@@ -384,7 +384,7 @@ bool is_gemm_small(const KernelEntry* e) { return ((e->image == IMG_GEMM_SMALL |
 bool is_gemm_tile(const KernelEntry* e) { return (e->image == IMG_GEMM_TILES || e->image == IMG_GEMM_SMALL) && e->tile[0] != 0; }
 bool is_thin(const KernelEntry* e) { return is_gemm_small(e) && e->tile[2] == 0; }
 // The block-scaled kernels on wave-private stages (scaled_flat.hip): tile[3] x tile[1] outputs a workgroup, any partition shape.
-bool is_scaled_flat(const KernelEntry* e) { return e->image == IMG_SCALED_FLAT; }
+bool is_scaled_flat(const KernelEntry* e) { return e->image == IMG_SCALED_FLAT || e->image == IMG_MXFP4_FLAT; }
 
 // Room for the partial tiles of a block-scaled product, and the workspace once somebody has asked for it.
 struct ScaledRoom {
@@ -469,7 +469,7 @@ cutile_status_t launch_scaled(Resolved& res, cutile_stream_t stream, const cutil
     const uint32_t tiles_m = div_up(zt.shape[0], res.entry->tile[3]), tiles_n = div_up(zt.shape[1], res.entry->tile[1]);
     const uint64_t blocks = (uint64_t)tiles_m * tiles_n;
     SplitWorkspace ws;
-    uint32_t splits = std::min(scaled_launch_splits(blocks, pieces, cus, x->dtype == CUTILE_DTYPE_F4E2M1FNX2, res.entry->tile[3], res.entry->tile[1]),
+    uint32_t splits = std::min(scaled_launch_splits(blocks, pieces, cus, xs->dtype == CUTILE_DTYPE_F8E4M3FN, res.entry->tile[3], res.entry->tile[1]),
                                split_limit(blocks, (uint64_t)res.entry->tile[1] * res.entry->tile[3]));
     if (splits > 1 && g_launch_mode == 0) {
       ws = split_workspace(res.device, (hipStream_t)stream);
@@ -3277,6 +3277,261 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
   ScaledRoom room;
   if (cutile_status_t s = resolve_scaled("linear_tile_nvfp4", "", dt, bm, bn, full_cover, flat, {M, N, (KP + 63) / 64, true}, opts, missing, stream, &cus, &room, &res)) return s;
   return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, (KP + 63) / 64, cus, room);
+}
+
+}  // extern "C"
+
+// ---- block-scaled rows (block_scale.hip) and the MXFP4 product ---------------------------------------------------------
+namespace {
+
+struct BlockFormat {
+  const char* name = nullptr;
+  int32_t block = 0, per_byte = 0;   // values of a block and of a byte of data
+};
+
+// The format that data and scales stand for, their shapes and layout; `k` = values of a row.
+cutile_status_t check_blocks(const char* fn, const cutile_tensor_arg_t& data, const cutile_tensor_arg_t& scales, BlockFormat* f, int64_t* k) {
+  const bool e4m3 = data.dtype == CUTILE_DTYPE_F8E4M3FN, e2m1 = data.dtype == CUTILE_DTYPE_F4E2M1FNX2;
+  if (scales.dtype == CUTILE_DTYPE_F8E8M0FNU && e4m3) *f = {"mxfp8", 32, 1};
+  if (scales.dtype == CUTILE_DTYPE_F8E8M0FNU && e2m1) *f = {"mxfp4", 32, 2};
+  if (scales.dtype == CUTILE_DTYPE_F8E4M3FN && e2m1) *f = {"nvfp4", 16, 2};
+  CUTILE_REQUIRE(f->name, CUTILE_ERR_KERNEL_NOT_FOUND, "%s: no block-scaled format has %s data with %s scales (mxfp8: f8e4m3fn, f8e8m0fnu; mxfp4: f4e2m1fnx2, f8e8m0fnu; "
+                 "nvfp4: f4e2m1fnx2, f8e4m3fn)", fn, cutile_dtype_name(data.dtype), cutile_dtype_name(scales.dtype));
+  *k = (int64_t)data.shape[1] * f->per_byte;
+  CUTILE_REQUIRE(*k % f->block == 0 && scales.shape[0] == data.shape[0] && scales.shape[1] == *k / f->block, CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: %s data of %d rows of %lld values needs whole blocks of %d and scales [%d, %lld], not [%d, %d]", fn, f->name, data.shape[0], (long long)*k, f->block,
+                 data.shape[0], (long long)(*k / f->block), scales.shape[0], scales.shape[1]);
+  const bool one = data.shape[0] == 1;
+  CUTILE_REQUIRE(data.strides[1] == 1 && ((uintptr_t)data.ptr & 7) == 0 && (one || (data.strides[0] % 8 == 0 && data.strides[0] >= data.shape[1])) &&
+                     (scales.shape[1] == 1 || scales.strides[1] == 1) && (one || scales.strides[0] >= scales.shape[1]),
+                 CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants need contiguous rows of data and scales that do not overlap, and data rows on 8-byte boundaries", fn);
+  return CUTILE_SUCCESS;
+}
+
+// g and 1 / (6 g), as the kernels take them.
+struct TensorScale {
+  float g, inv6g;
+};
+cutile_status_t tensor_scale_of(const char* fn, const BlockFormat& f, float g, TensorScale* t) {
+  if (f.block == 16)
+    CUTILE_REQUIRE(g >= 0x1p-100f && g <= 0x1p100f, CUTILE_ERR_KERNEL_LAUNCH, "%s: tensor_scale must lie between 2^-100 and 2^100, got %g", fn, (double)g);
+  else
+    CUTILE_REQUIRE(g == 1.0f, CUTILE_ERR_KERNEL_LAUNCH, "%s: %s has no tensor_scale (nvfp4 has): it must be 1, got %g", fn, f.name, (double)g);
+  *t = {g, (float)(1.0 / (6.0 * (double)g))};
+  return CUTILE_SUCCESS;
+}
+
+// Whole-row partitions of a launch and the rows that its grid covers.
+cutile_status_t rows_of(const char* fn, const cutile_partition_arg_t* const* parts, int n, const cutile_launch_opts_t* opts, int64_t* rows) {
+  for (int i = 0; i < n; ++i)
+    CUTILE_REQUIRE(parts[i]->partition_shape[1] == parts[i]->tensor.shape[1] && parts[i]->partition_shape[0] == parts[0]->partition_shape[0] &&
+                       parts[i]->tensor.shape[0] == parts[0]->tensor.shape[0],
+                   CUTILE_ERR_KERNEL_LAUNCH, "%s: outputs must have the same rows and be partitioned [BM, whole row] alike", fn);
+  uint32_t explicit_grid[3] = {0, 0, 0}, tg[3];
+  if (opts) memcpy(explicit_grid, opts->grid, sizeof(explicit_grid));
+  if (cutile_status_t s = cutile_infer_launch_grid(explicit_grid, parts, n, tg)) return s;
+  CUTILE_REQUIRE(tg[0] > 0 && tg[1] > 0 && tg[2] > 0, CUTILE_ERR_KERNEL_LAUNCH, "launch grid (%u, %u, %u) has a zero axis", tg[0], tg[1], tg[2]);
+  *rows = std::min<int64_t>((int64_t)tg[0] * parts[0]->partition_shape[0], parts[0]->tensor.shape[0]);
+  return CUTILE_SUCCESS;
+}
+
+bool is_16bit_float(cutile_dtype_t dt) { return dt == CUTILE_DTYPE_F16 || dt == CUTILE_DTYPE_BF16; }
+
+// Workgroups of 256 threads, a unit of 8 values to a thread; the kernels stride over what is beyond.
+void unit_grid(int64_t units, uint32_t grid[3]) {
+  grid[0] = (uint32_t)std::min<int64_t>((units + 255) / 256, 1 << 24);
+  grid[1] = grid[2] = 1;
+}
+
+// block_quantize (up == nullptr) and silu_mul_quantize
+cutile_status_t launch_quantize(const char* fn, cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* up, const cutile_partition_arg_t* out,
+                                const cutile_partition_arg_t* scales, float tensor_scale, const cutile_launch_opts_t* opts) {
+  if (cutile_status_t s = check_tensor(x, up ? "gate" : "x", 2, 2)) return s;
+  if (up)
+    if (cutile_status_t s = check_tensor(up, "up", 2, 2)) return s;
+  if (cutile_status_t s = check_partition(out, "out", 2, 2)) return s;
+  if (cutile_status_t s = check_partition(scales, "scales", 2, 2)) return s;
+  CUTILE_REQUIRE(up ? is_16bit_float(x->dtype) && up->dtype == x->dtype : is_16bit_float(x->dtype) || x->dtype == CUTILE_DTYPE_F32, CUTILE_ERR_KERNEL_NOT_FOUND,
+                 up ? "%s: gate and up must both be f16 or both bf16" : "%s: x must be f16, bf16 or f32", fn);
+  BlockFormat f;
+  int64_t k, rows;
+  if (cutile_status_t s = check_blocks(fn, out->tensor, scales->tensor, &f, &k)) return s;
+  CUTILE_REQUIRE(x->shape[1] <= k && x->shape[0] >= out->tensor.shape[0] && (!up || same_shape(*x, *up)), CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: out holds %d rows of %lld values, %s is [%d, %d]%s", fn, out->tensor.shape[0], (long long)k, up ? "gate" : "x", x->shape[0], x->shape[1],
+                 up && !same_shape(*x, *up) ? " and up has another shape" : "");
+  if (cutile_status_t s = check_generic(opts, 0, num(x->shape[1]), "N")) return s;
+  TensorScale t;
+  if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
+  const cutile_partition_arg_t* parts[2] = {out, scales};
+  if (cutile_status_t s = rows_of(fn, parts, 2, opts, &rows)) return s;
+  const Name any = Name(f.name) + "_" + cutile_dtype_name(x->dtype) + "_any";
+  Resolved res;
+  if (cutile_status_t s = resolve_entry(fn, opts, any, {any}, &res)) return s;
+  ArgPacker args;
+  args.push_tensor(*x);
+  if (up) args.push_tensor(*up);
+  args.push_partition(*out);
+  args.push_partition(*scales);
+  args.push_val<TensorScale>(t);
+  args.push_val<int64_t>(rows);
+  args.push_val<int32_t>((int32_t)(k / 8));
+  uint32_t grid[3];
+  unit_grid(rows * (k / 8), grid);
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+}
+
+// rms_norm_quantize (residual == nullptr) and add_rms_norm_quantize
+cutile_status_t launch_norm_quantize(const char* fn, cutile_stream_t stream, const cutile_tensor_arg_t* residual, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* w,
+                                     const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales, const cutile_partition_arg_t* residual_out, float eps,
+                                     float tensor_scale, const cutile_launch_opts_t* opts) {
+  if (residual)
+    if (cutile_status_t s = check_tensor(residual, "residual", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(x, "x", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(w, "w", 1, 1)) return s;
+  if (cutile_status_t s = check_partition(out, "out", 2, 2)) return s;
+  if (cutile_status_t s = check_partition(scales, "scales", 2, 2)) return s;
+  if (residual)
+    if (cutile_status_t s = check_partition(residual_out, "residual_out", 2, 2)) return s;
+  const int32_t n = x->shape[1];
+  CUTILE_REQUIRE(is_16bit_float(x->dtype) && w->dtype == x->dtype && (!residual || (residual->dtype == x->dtype && residual_out->tensor.dtype == x->dtype)),
+                 CUTILE_ERR_KERNEL_NOT_FOUND, "%s: the rows and w must all be f16 or all bf16", fn);
+  CUTILE_REQUIRE(w->shape[0] == n && (!residual || (residual->shape[1] == n && residual_out->tensor.shape[1] == n)), CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: row length N = %d must be shared by all tensors", fn, n);
+  BlockFormat f;
+  int64_t k, rows;
+  if (cutile_status_t s = check_blocks(fn, out->tensor, scales->tensor, &f, &k)) return s;
+  CUTILE_REQUIRE(n <= k && x->shape[0] >= out->tensor.shape[0] && (!residual || residual->shape[0] >= out->tensor.shape[0]), CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: out holds %d rows of %lld values, x is [%d, %d]%s", fn, out->tensor.shape[0], (long long)k, x->shape[0], n, residual ? " and residual must have its rows" : "");
+  if (cutile_status_t s = check_generic(opts, 0, num(n), "N")) return s;
+  TensorScale t;
+  if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
+  const cutile_partition_arg_t* parts[3] = {out, scales, residual_out};
+  if (cutile_status_t s = rows_of(fn, parts, residual ? 3 : 2, opts, &rows)) return s;
+  const Name any = Name(f.name) + "_" + cutile_dtype_name(x->dtype) + "_any";
+  Resolved res;
+  if (cutile_status_t s = resolve_entry(fn, opts, any, {any}, &res)) return s;
+  ArgPacker args;
+  if (residual) args.push_tensor(*residual);
+  args.push_tensor(*x);
+  args.push_tensor(*w);
+  args.push_partition(*out);
+  args.push_partition(*scales);
+  if (residual) args.push_partition(*residual_out);
+  args.push_val<float>(eps);
+  args.push_val<TensorScale>(t);
+  args.push_val<int64_t>(rows);
+  args.push_val<int32_t>((int32_t)(k / 8));
+  const uint32_t grid[3] = {(uint32_t)std::min<int64_t>(rows, 1 << 24), 1, 1};
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+}
+
+}  // namespace
+
+extern "C" {
+
+cutile_status_t cutile_launch_block_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_partition_arg_t* out,
+                                             const cutile_partition_arg_t* scales, float tensor_scale, const cutile_launch_opts_t* opts) {
+  return launch_quantize("block_quantize", stream, x, nullptr, out, scales, tensor_scale, opts);
+}
+cutile_status_t cutile_launch_silu_mul_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* gate, const cutile_tensor_arg_t* up,
+                                                const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales, float tensor_scale,
+                                                const cutile_launch_opts_t* opts) {
+  CUTILE_REQUIRE(up, CUTILE_ERR_INVALID_ARGUMENT, "up is null");
+  return launch_quantize("silu_mul_quantize", stream, gate, up, out, scales, tensor_scale, opts);
+}
+cutile_status_t cutile_launch_rms_norm_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* w, const cutile_partition_arg_t* out,
+                                                const cutile_partition_arg_t* scales, float eps, float tensor_scale, const cutile_launch_opts_t* opts) {
+  return launch_norm_quantize("rms_norm_quantize", stream, nullptr, x, w, out, scales, nullptr, eps, tensor_scale, opts);
+}
+cutile_status_t cutile_launch_add_rms_norm_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* residual, const cutile_tensor_arg_t* x,
+                                                    const cutile_tensor_arg_t* w, const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales,
+                                                    const cutile_partition_arg_t* residual_out, float eps, float tensor_scale, const cutile_launch_opts_t* opts) {
+  CUTILE_REQUIRE(residual, CUTILE_ERR_INVALID_ARGUMENT, "residual is null");
+  return launch_norm_quantize("add_rms_norm_quantize", stream, residual, x, w, out, scales, residual_out, eps, tensor_scale, opts);
+}
+
+cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* scales, float tensor_scale,
+                                               const cutile_partition_arg_t* out, const cutile_launch_opts_t* opts) {
+  const char* const fn = "block_dequantize";
+  if (cutile_status_t s = check_tensor(x, "x", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(scales, "scales", 2, 2)) return s;
+  if (cutile_status_t s = check_partition(out, "out", 2, 2)) return s;
+  const cutile_tensor_arg_t& ot = out->tensor;
+  CUTILE_REQUIRE(is_16bit_float(ot.dtype) || ot.dtype == CUTILE_DTYPE_F32, CUTILE_ERR_KERNEL_NOT_FOUND, "%s: out must be f16, bf16 or f32", fn);
+  BlockFormat f;
+  int64_t k, rows;
+  if (cutile_status_t s = check_blocks(fn, *x, *scales, &f, &k)) return s;
+  CUTILE_REQUIRE(ot.shape[1] <= k && x->shape[0] >= ot.shape[0], CUTILE_ERR_KERNEL_LAUNCH, "%s: out is [%d, %d], x holds %d rows of %lld values", fn, ot.shape[0], ot.shape[1],
+                 x->shape[0], (long long)k);
+  if (cutile_status_t s = check_generic(opts, 0, num(ot.shape[1]), "N")) return s;
+  TensorScale t;
+  if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
+  const cutile_partition_arg_t* parts[1] = {out};
+  if (cutile_status_t s = rows_of(fn, parts, 1, opts, &rows)) return s;
+  const Name any = Name(f.name) + "_" + cutile_dtype_name(ot.dtype) + "_any";
+  Resolved res;
+  if (cutile_status_t s = resolve_entry(fn, opts, any, {any}, &res)) return s;
+  const int32_t units = (int32_t)div_up(ot.shape[1], 8);
+  ArgPacker args;
+  args.push_tensor(*x);
+  args.push_tensor(*scales);
+  args.push_partition(*out);
+  args.push_val<float>(t.g);
+  args.push_val<int64_t>(rows);
+  args.push_val<int32_t>(units);
+  uint32_t grid[3];
+  unit_grid(rows * units, grid);
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+}
+
+cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cutile_partition_arg_t* z, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* y,
+                                                const cutile_tensor_arg_t* xs, const cutile_tensor_arg_t* ys, float alpha, const cutile_launch_opts_t* opts) {
+  if (cutile_status_t s = check_partition(z, "z", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(x, "x", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(y, "y", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(xs, "x_scales", 2, 2)) return s;
+  if (cutile_status_t s = check_tensor(ys, "y_scales", 2, 2)) return s;
+  const cutile_tensor_arg_t& zt = z->tensor;
+  CUTILE_REQUIRE(x->dtype == CUTILE_DTYPE_F4E2M1FNX2 && y->dtype == CUTILE_DTYPE_F4E2M1FNX2 && xs->dtype == CUTILE_DTYPE_F8E8M0FNU && ys->dtype == CUTILE_DTYPE_F8E8M0FNU,
+                 CUTILE_ERR_KERNEL_NOT_FOUND, "linear_tile (mxfp4): precompiled variants take f4e2m1fnx2 data with f8e8m0fnu scales");
+  CUTILE_REQUIRE(zt.dtype == CUTILE_DTYPE_F32 || zt.dtype == CUTILE_DTYPE_BF16, CUTILE_ERR_KERNEL_NOT_FOUND, "linear_tile (mxfp4): z must be f32 or bf16");
+  const int32_t M = x->shape[0], KP = x->shape[1], N = y->shape[0];
+  const int64_t K = 2 * (int64_t)KP;
+  CUTILE_REQUIRE(y->shape[1] == KP, CUTILE_ERR_KERNEL_LAUNCH, "linear_tile (mxfp4): x is [%d, %d] but y is [%d, %d] (packed bytes)", M, KP, N, y->shape[1]);
+  CUTILE_REQUIRE(K % 32 == 0 && xs->shape[0] == M && xs->shape[1] == K / 32 && ys->shape[0] == N && ys->shape[1] == K / 32, CUTILE_ERR_KERNEL_LAUNCH,
+                 "linear_tile (mxfp4): scales must be [M, K/32] and [N, K/32] with K = %lld a multiple of 32", (long long)K);
+  CUTILE_REQUIRE(zt.shape[0] == M && zt.shape[1] == N, CUTILE_ERR_KERNEL_LAUNCH, "linear_tile (mxfp4): z is [%d, %d], expected [%d, %d]", zt.shape[0], zt.shape[1], M, N);
+  const int32_t bm = z->partition_shape[0], bn = z->partition_shape[1];
+  if (cutile_status_t s = check_generic(opts, 0, num(bm), "BM")) return s;
+  if (cutile_status_t s = check_generic(opts, 1, num(bn), "BN")) return s;
+  const int bk_user = generic_int(opts, 2, 128);
+  CUTILE_REQUIRE(bk_user > 0 && bk_user % 32 == 0 && generic_int(opts, 3, bk_user / 2) == bk_user / 2 && generic_int(opts, 4, bk_user / 32) == bk_user / 32,
+                 CUTILE_ERR_KERNEL_LAUNCH, "linear_tile (mxfp4): BK must be a multiple of 32, BK_PACKED = BK/2 and BK_SCALES = BK/32");
+  CUTILE_REQUIRE(K % bk_user == 0, CUTILE_ERR_KERNEL_LAUNCH, "linear_tile (mxfp4): K = %lld is not a multiple of BK = %d", (long long)K, bk_user);
+  uint32_t tg[3], full[3];
+  if (cutile_status_t s = resolve_grid(z, opts, tg)) return s;
+  cutile_partition_grid(z, full);
+  const bool full_cover = tg[0] == full[0] && tg[1] == full[1];
+  CUTILE_REQUIRE(K % 128 == 0 && x->strides[1] == 1 && y->strides[1] == 1 && xs->strides[1] == 1 && ys->strides[1] == 1 && zt.strides[1] == 1 && x->strides[0] % 16 == 0 &&
+                     y->strides[0] % 16 == 0 && xs->strides[0] % 4 == 0 && ys->strides[0] % 4 == 0 && zt.strides[0] % 4 == 0 && zt.shape[1] % 4 == 0 && aligned16(x->ptr) &&
+                     aligned16(y->ptr) && aligned16(zt.ptr) && ((uintptr_t)xs->ptr & 3) == 0 && ((uintptr_t)ys->ptr & 3) == 0,
+                 CUTILE_ERR_KERNEL_NOT_FOUND, "linear_tile (mxfp4): precompiled variants need K a multiple of 128, unit inner strides and aligned rows");
+  CUTILE_REQUIRE(extent_bytes_2d(*x) < kDescriptorLimit && extent_bytes_2d(*y) < kDescriptorLimit && extent_bytes_2d(*xs) < kDescriptorLimit &&
+                     extent_bytes_2d(*ys) < kDescriptorLimit && extent_bytes_2d(zt) < kDescriptorLimit,
+                 CUTILE_ERR_KERNEL_NOT_FOUND,
+                 "linear_tile (mxfp4): precompiled variants address an operand with 32-bit byte offsets: x, y, the scales and z must each end below 2 GiB from their first "
+                 "element (x spans %lld bytes, y %lld, z %lld)",
+                 (long long)extent_bytes_2d(*x), (long long)extent_bytes_2d(*y), (long long)extent_bytes_2d(zt));
+  CUTILE_REQUIRE(full_cover, CUTILE_ERR_KERNEL_NOT_FOUND, "linear_tile (mxfp4): no precompiled variant covers a part of z");
+  const Name dt = zt.dtype == CUTILE_DTYPE_F32 ? "f32" : "bf16";
+  Names acceptable;
+  for (const KernelEntry* e : kernels_of("linear_tile_mxfp4"))
+    if (dt == e->dtype) acceptable.push_back(e->variant);
+  Resolved res;
+  int cus = 256;
+  if (cutile_status_t s = current_device_units(&cus)) return s;
+  if (cutile_status_t s = resolve_entry("linear_tile_mxfp4", opts, dt + (M <= 16 ? "_flat16x64" : M <= 32 ? "_flat32x64" : "_flat64x128"), acceptable, &res)) return s;
+  return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, KP / 64, cus, ScaledRoom{});
 }
 
 }  // extern "C"

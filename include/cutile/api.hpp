@@ -665,9 +665,57 @@ struct LinearTileMxfp8Fn {
   static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, Z& z, X& x, Yv& y, XS& xs, YS& ys, float alpha) {
     auto zp = z.arg();
     auto xa = input_arg(x), ya = input_arg(y), xsa = input_arg(xs), ysa = input_arg(ys);
-    // the reference has one `linear_tile` per module (mxfp8.rs, nvfp4.rs); here the operand type picks the kernel
+    // the reference has one `linear_tile` per module (mxfp8.rs, nvfp4.rs); here the operand types pick the kernel
+    if (xa.dtype == CUTILE_DTYPE_F4E2M1FNX2 && xsa.dtype == CUTILE_DTYPE_F8E8M0FNU) return cutile_launch_linear_tile_mxfp4(s, &zp, &xa, &ya, &xsa, &ysa, alpha, o);
     if (xa.dtype == CUTILE_DTYPE_F4E2M1FNX2) return cutile_launch_linear_tile_nvfp4(s, &zp, &xa, &ya, &xsa, &ysa, alpha, o);
     return cutile_launch_linear_tile_mxfp8(s, &zp, &xa, &ya, &xsa, &ysa, alpha, o);
+  }
+};
+// ---- block-scaled rows: the element types of out (or x) and scales name the format ----
+struct BlockQuantizeFn {
+  static constexpr const char* name = "block_quantize";
+  template <class X, class O, class S>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, X& x, O& out, S& scales, float tensor_scale) {
+    auto xa = input_arg(x);
+    auto op = out.arg(), sp = scales.arg();
+    return cutile_launch_block_quantize(s, &xa, &op, &sp, tensor_scale, o);
+  }
+};
+struct BlockDequantizeFn {
+  static constexpr const char* name = "block_dequantize";
+  template <class X, class S, class O>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, X& x, S& scales, float tensor_scale, O& out) {
+    auto xa = input_arg(x), sa = input_arg(scales);
+    auto op = out.arg();
+    return cutile_launch_block_dequantize(s, &xa, &sa, tensor_scale, &op, o);
+  }
+};
+struct RmsNormQuantizeFn {
+  static constexpr const char* name = "rms_norm_quantize";
+  template <class X, class W, class O, class S>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, X& x, W& w, O& out, S& scales, float eps, float tensor_scale) {
+    auto xa = input_arg(x), wa = input_arg(w);
+    auto op = out.arg(), sp = scales.arg();
+    return cutile_launch_rms_norm_quantize(s, &xa, &wa, &op, &sp, eps, tensor_scale, o);
+  }
+};
+struct AddRmsNormQuantizeFn {
+  static constexpr const char* name = "add_rms_norm_quantize";
+  template <class R, class X, class W, class O, class S, class RO>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, R& residual, X& x, W& w, O& out, S& scales, RO& residual_out, float eps,
+                                float tensor_scale) {
+    auto ra = input_arg(residual), xa = input_arg(x), wa = input_arg(w);
+    auto op = out.arg(), sp = scales.arg(), rop = residual_out.arg();
+    return cutile_launch_add_rms_norm_quantize(s, &ra, &xa, &wa, &op, &sp, &rop, eps, tensor_scale, o);
+  }
+};
+struct SiluMulQuantizeFn {
+  static constexpr const char* name = "silu_mul_quantize";
+  template <class G, class U, class O, class S>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, G& gate, U& up, O& out, S& scales, float tensor_scale) {
+    auto ga = input_arg(gate), ua = input_arg(up);
+    auto op = out.arg(), sp = scales.arg();
+    return cutile_launch_silu_mul_quantize(s, &ga, &ua, &op, &sp, tensor_scale, o);
   }
 };
 // ---- transformer-block kernels (cutile-kernels/src/{norms,pointwise,positional}.rs) ----
@@ -893,6 +941,13 @@ template <class O, class Q, class K, class V> auto fmha(O&& out, Q&& q, K&& k, V
 template <class O, class Q, class K, class V> auto fmha_causal(O&& out, Q&& q, K&& k, V&& v, float scale, int32_t input_pos, int32_t group) { return make_launcher<kernels::FmhaFn<true>>(std::forward<O>(out), std::forward<Q>(q), std::forward<K>(k), std::forward<V>(v), scale, input_pos, group); }
 // linear_tile(z: partition [BM,BN], x, y, x_scales, y_scales, alpha)   cutile-examples/examples/mxfp8.rs:35-42 (f8e4m3fn x, y) and nvfp4.rs:39-51 (f4e2m1fnx2 x, y)
 template <class Z, class X, class Y, class XS, class YS> auto linear_tile(Z&& z, X&& x, Y&& y, XS&& xs, YS&& ys, float alpha) { return make_launcher<kernels::LinearTileMxfp8Fn>(std::forward<Z>(z), std::forward<X>(x), std::forward<Y>(y), std::forward<XS>(xs), std::forward<YS>(ys), alpha); }
+//   (f4e2m1fnx2 x, y with f8e8m0fnu scales: the MXFP4 product, which has no counterpart there)
+// block_quantize(x, out: [BM, row], scales: [BM, row], tensor_scale) and the kernels that end in it: no counterpart in the reference; formats and rounding in cutile_hip.h
+template <class X, class O, class S> auto block_quantize(X&& x, O&& out, S&& scales, float tensor_scale = 1.0f) { return make_launcher<kernels::BlockQuantizeFn>(std::forward<X>(x), std::forward<O>(out), std::forward<S>(scales), tensor_scale); }
+template <class X, class S, class O> auto block_dequantize(X&& x, S&& scales, float tensor_scale, O&& out) { return make_launcher<kernels::BlockDequantizeFn>(std::forward<X>(x), std::forward<S>(scales), tensor_scale, std::forward<O>(out)); }
+template <class X, class W, class O, class S> auto rms_norm_quantize(X&& x, W&& w, O&& out, S&& scales, float eps, float tensor_scale = 1.0f) { return make_launcher<kernels::RmsNormQuantizeFn>(std::forward<X>(x), std::forward<W>(w), std::forward<O>(out), std::forward<S>(scales), eps, tensor_scale); }
+template <class R, class X, class W, class O, class S, class RO> auto add_rms_norm_quantize(R&& residual, X&& x, W&& w, O&& out, S&& scales, RO&& residual_out, float eps, float tensor_scale = 1.0f) { return make_launcher<kernels::AddRmsNormQuantizeFn>(std::forward<R>(residual), std::forward<X>(x), std::forward<W>(w), std::forward<O>(out), std::forward<S>(scales), std::forward<RO>(residual_out), eps, tensor_scale); }
+template <class G, class U, class O, class S> auto silu_mul_quantize(G&& gate, U&& up, O&& out, S&& scales, float tensor_scale = 1.0f) { return make_launcher<kernels::SiluMulQuantizeFn>(std::forward<G>(gate), std::forward<U>(up), std::forward<O>(out), std::forward<S>(scales), tensor_scale); }
 // add_rms_norm_f16(residual, x, w, out: [1,N], residual_out: [1,N], eps)      cutile-kernels/src/norms.rs:76-83
 template <class R, class X, class W, class O, class RO> auto add_rms_norm_f16(R&& residual, X&& x, W&& w, O&& out, RO&& residual_out, float eps) { return make_launcher<kernels::AddRmsNormF16Fn>(std::forward<R>(residual), std::forward<X>(x), std::forward<W>(w), std::forward<O>(out), std::forward<RO>(residual_out), eps); }
 // qk_norm_f16(q, k, q_weight, k_weight, out: [1,N], eps, num_q_rows)          cutile-kernels/src/norms.rs:152-160

@@ -748,6 +748,50 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
                                                 const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* y,
                                                 const cutile_tensor_arg_t* x_scales, const cutile_tensor_arg_t* y_scales,
                                                 float alpha, const cutile_launch_opts_t* opts);
+/* ---- block-scaled operands: made, read back, multiplied.  No counterpart in the reference, whose block-scaled products
+ * (mxfp8.rs, nvfp4.rs) take operands that a program already has. -------------------------------------------------------
+ * A format is named by the types of its data and its scales:
+ *   mxfp8  f8e4m3fn [M, K],           f8e8m0fnu [M, K/32]   value = element * 2^(byte - 127)
+ *   mxfp4  f4e2m1fnx2 [M, K/2 bytes], f8e8m0fnu [M, K/32]
+ *   nvfp4  f4e2m1fnx2 [M, K/2 bytes], f8e4m3fn  [M, K/16]   value = element * scale * tensor_scale
+ * block_quantize: for the largest magnitude a of a block (32 values, nvfp4 16)
+ *   mxfp8, mxfp4   byte = clamp(floor(log2 a) - emax + 127, 0, 254), emax 8 (e4m3) or 2 (e2m1); a = 0: byte 0; elements
+ *                  round(x * 2^(127 - byte)) to nearest even, saturated at 448 or 6   (OCP MX 1.0, section 6.3)
+ *   nvfp4          scale = e4m3(min(a / (6 tensor_scale), 448)), elements e2m1(x / (scale * tensor_scale)), 0 where the scale is
+ *   A block that holds a NaN or an infinity gets a NaN scale (0xff, 0x7f) and elements 0: it stands for NaN throughout.
+ * x: [M, N] f16, bf16 or f32 with any strides; N of any length up to K.  out: K whole blocks a row, columns N .. K - 1 zeros
+ * (so rows can be made as long as the product that reads them wants).  out and scales are partitioned [BM, whole row] alike
+ * and may have fewer rows than x; their rows are contiguous and apart, those of out on 8-byte boundaries.  tensor_scale is 1 for
+ * the mx formats and between 2^-100 and 2^100 for nvfp4.  Generic 0, when given, is N. */
+cutile_status_t cutile_launch_block_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_partition_arg_t* out,
+                                             const cutile_partition_arg_t* scales, float tensor_scale, const cutile_launch_opts_t* opts);
+/* block_dequantize: out [M, N] <- the values that x and scales stand for, N up to K, rounded once to f16, bf16 or f32; out has
+ * any strides and is partitioned [BM, N]; the block of a NaN scale is NaN. */
+cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* scales,
+                                               float tensor_scale, const cutile_partition_arg_t* out, const cutile_launch_opts_t* opts);
+/* The kernels in front of a block-scaled product with its operand as their output (x, w, gate, up f16 or bf16 alike, any
+ * strides; f32 from the loads to the one rounding of block_quantize, nothing rounded to 16 bits in between):
+ *   rms_norm_quantize       x / sqrt(mean(x^2) + eps) * w
+ *   add_rms_norm_quantize   the same of c = residual + x; residual_out <- c, rounded once; it may be residual or x itself
+ *   silu_mul_quantize       gate / (1 + exp(-gate)) * up */
+cutile_status_t cutile_launch_rms_norm_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* w,
+                                                const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales, float eps,
+                                                float tensor_scale, const cutile_launch_opts_t* opts);
+cutile_status_t cutile_launch_add_rms_norm_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* residual,
+                                                    const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* w,
+                                                    const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales,
+                                                    const cutile_partition_arg_t* residual_out, float eps, float tensor_scale,
+                                                    const cutile_launch_opts_t* opts);
+cutile_status_t cutile_launch_silu_mul_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* gate, const cutile_tensor_arg_t* up,
+                                                const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales,
+                                                float tensor_scale, const cutile_launch_opts_t* opts);
+/* linear_tile on MXFP4 operands: z [M, N] (f32 or bf16) = alpha * sum_k x[i,k] sx[i,k/32] * y[j,k] sy[j,k/32], x [M, K/2 bytes],
+ * y [N, K/2 bytes], scales [M, K/32], [N, K/32] e8m0; f32 accumulation.  The rules of linear_tile_mxfp8: K a multiple of 128, N of
+ * 4, 16-byte aligned data rows, 4-byte aligned scale rows, every operand within 2 GiB.  Generics, when given: BM, BN, BK,
+ * BK_PACKED = BK/2, BK_SCALES = BK/32. */
+cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cutile_partition_arg_t* z, const cutile_tensor_arg_t* x,
+                                                const cutile_tensor_arg_t* y, const cutile_tensor_arg_t* x_scales,
+                                                const cutile_tensor_arg_t* y_scales, float alpha, const cutile_launch_opts_t* opts);
 
 /* ======================================================================== */
 /* Part E — asynchronous runtime                                             */

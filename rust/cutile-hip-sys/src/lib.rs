@@ -322,6 +322,12 @@ extern "C" {
     pub fn cutile_launch_fmha(stream: cutile_stream_t, out: *const cutile_partition_arg_t, q: *const cutile_tensor_arg_t, k: *const cutile_tensor_arg_t, v: *const cutile_tensor_arg_t, qk_scale: f32, input_pos: i32, query_group_size: i32, causal: i32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
     pub fn cutile_launch_linear_tile_mxfp8(stream: cutile_stream_t, z: *const cutile_partition_arg_t, x: *const cutile_tensor_arg_t, y: *const cutile_tensor_arg_t, x_scales: *const cutile_tensor_arg_t, y_scales: *const cutile_tensor_arg_t, alpha: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
     pub fn cutile_launch_linear_tile_nvfp4(stream: cutile_stream_t, z: *const cutile_partition_arg_t, x: *const cutile_tensor_arg_t, y: *const cutile_tensor_arg_t, x_scales: *const cutile_tensor_arg_t, y_scales: *const cutile_tensor_arg_t, alpha: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_block_quantize(stream: cutile_stream_t, x: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, scales: *const cutile_partition_arg_t, tensor_scale: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_block_dequantize(stream: cutile_stream_t, x: *const cutile_tensor_arg_t, scales: *const cutile_tensor_arg_t, tensor_scale: f32, out: *const cutile_partition_arg_t, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_rms_norm_quantize(stream: cutile_stream_t, x: *const cutile_tensor_arg_t, w: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, scales: *const cutile_partition_arg_t, eps: f32, tensor_scale: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_add_rms_norm_quantize(stream: cutile_stream_t, residual: *const cutile_tensor_arg_t, x: *const cutile_tensor_arg_t, w: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, scales: *const cutile_partition_arg_t, residual_out: *const cutile_partition_arg_t, eps: f32, tensor_scale: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_silu_mul_quantize(stream: cutile_stream_t, gate: *const cutile_tensor_arg_t, up: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, scales: *const cutile_partition_arg_t, tensor_scale: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_linear_tile_mxfp4(stream: cutile_stream_t, z: *const cutile_partition_arg_t, x: *const cutile_tensor_arg_t, y: *const cutile_tensor_arg_t, x_scales: *const cutile_tensor_arg_t, y_scales: *const cutile_tensor_arg_t, alpha: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
     pub fn cutile_execution_lock_acquire() -> cutile_status_t;
     pub fn cutile_execution_lock_release();
     pub fn cutile_execution_lock_held() -> i32;

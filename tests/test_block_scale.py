@@ -1,0 +1,405 @@
+"""Block-scaled rows: quantisation, reading back, and the norm and gated activation that end in it (block_scale.hip)."""
+import math
+
+import pytest
+import torch
+
+import block_ref as ref
+
+FORMATS = ["mxfp8", "mxfp4", "nvfp4"]
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+# one value, one short of a block, a block, one more, lengths that are no multiple of a unit, several workgroups, a long row
+LENGTHS = [1, 15, 16, 31, 32, 33, 100, 256, 1000, 5001, 8192, 20000]
+
+
+def whole(ct, t):
+    return ct.partition(t, [1, t.shape[1]])
+
+
+def normal(shape, seed, device, dtype=torch.float32, std=1.0):
+    g = torch.Generator(device="cpu")
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to(device).to(dtype)
+
+
+def g_of(x, fmt):
+    return float(x[torch.isfinite(x)].abs().max().float()) / (6 * 448.0) if fmt == "nvfp4" else 1.0
+
+
+# ---- refusals, without a GPU ---------------------------------------------------------------------------------------------
+def test_refusals(fake_hip):
+    ct = fake_hip
+    n0 = ct.lib().cutile_testing_launch_count()
+    x = torch.zeros(4, 64, dtype=torch.half)
+    data, scales = torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    q = lambda x=x, d=data, s=scales, fmt="mxfp8", *a, **kw: ct.block_quantize(x, whole(ct, d), whole(ct, s), fmt, *a, **kw)
+    w = torch.zeros(64, dtype=torch.half)
+    norm = lambda r=x, x=x, w=w, d=data, s=scales, ro=x, **kw: ct.add_rms_norm_quantize(r, x, w, whole(ct, d), whole(ct, s), whole(ct, ro), 1e-6, "mxfp8", **kw)
+    silu = lambda g=x, u=x, **kw: ct.silu_mul_quantize(g, u, whole(ct, data), whole(ct, scales), "mxfp8", **kw)
+    deq = lambda d=data, s=scales, o=x, fmt="mxfp8", *a: ct.block_dequantize(d, s, whole(ct, o), fmt, *a)
+    wide = torch.zeros(4, 80, dtype=torch.uint8)
+    cases = [
+        (lambda: q(fmt="mxfp6"), "unknown block-scaled format"),
+        (lambda: q(d=data.float()), "tensors of bytes"),
+        (lambda: q(x=x.double()), "x must be f16, bf16 or f32"),
+        (lambda: q(x=x.to(torch.uint8)), "x must be f16, bf16 or f32"),
+        (lambda: q(x=torch.zeros(64, dtype=torch.half)), "expected rank 2"),
+        (lambda: q(s=torch.zeros(4, 4, dtype=torch.uint8)), "whole blocks of 32 and scales"),
+        (lambda: q(d=torch.zeros(4, 48, dtype=torch.uint8)), "whole blocks of 32"),
+        (lambda: q(s=torch.zeros(3, 2, dtype=torch.uint8)), "whole blocks of 32 and scales"),
+        (lambda: q(x=torch.zeros(4, 65, dtype=torch.half)), "out holds 4 rows of 64 values"),
+        (lambda: q(x=torch.zeros(3, 64, dtype=torch.half)), "out holds 4 rows of 64 values"),
+        (lambda: q(d=torch.zeros(64, 4, dtype=torch.uint8).t()), "contiguous rows"),
+        (lambda: q(d=torch.zeros(4, 65, dtype=torch.uint8)[:, :64]), "8-byte boundaries"),
+        (lambda: q(d=torch.zeros(4, 72, dtype=torch.uint8)[:, 1:65]), "8-byte boundaries"),
+        (lambda: q(d=torch.zeros(1, 64, dtype=torch.uint8).expand(4, 64)), "do not overlap"),
+        (lambda: q(s=torch.zeros(1, 2, dtype=torch.uint8).expand(4, 2)), "do not overlap"),
+        (lambda: q(s=torch.zeros(2, 4, dtype=torch.uint8).t()), "contiguous rows"),
+        (lambda: q(x, data, scales, "mxfp8", 2.0), "no tensor_scale"),
+        (lambda: q(x, data[:, :32], torch.zeros(4, 4, dtype=torch.uint8), "nvfp4", 0.0), "tensor_scale must lie"),
+        (lambda: q(x, data[:, :32], torch.zeros(4, 4, dtype=torch.uint8), "nvfp4", -1.0), "tensor_scale must lie"),
+        (lambda: q(x, data[:, :32], torch.zeros(4, 4, dtype=torch.uint8), "nvfp4", math.nan), "tensor_scale must lie"),
+        (lambda: q(x, data[:, :32], torch.zeros(4, 4, dtype=torch.uint8), "nvfp4", math.inf), "tensor_scale must lie"),
+        (lambda: q(generics=[32]), "generic N"),
+        (lambda: q(grid=(3, 1, 1)), "does not match the inferred partition grid"),
+        (lambda: q(variant="mxfp4_f16_any"), "does not fit these arguments"),
+        (lambda: ct.block_quantize(x, ct.partition(data, [1, 32]), whole(ct, scales), "mxfp8"), "whole row"),
+        (lambda: ct.block_quantize(x, ct.partition(data, [2, 64]), whole(ct, scales), "mxfp8"), "whole row"),
+        (lambda: ct.block_quantize(x, ct.partition(data, [1, 64], prefix=True), ct.partition(scales, [1, 2], prefix=True), "mxfp8"), "Launch grid required"),
+        (lambda: norm(w=w[:32]), "must be shared by all tensors"),
+        (lambda: norm(w=w.float()), "all be f16 or all bf16"),
+        (lambda: norm(x=x.bfloat16()), "all be f16 or all bf16"),
+        (lambda: norm(r=x[:2]), "residual must have its rows"),
+        (lambda: norm(r=x[:, :32]), "must be shared by all tensors"),
+        (lambda: norm(ro=x[:2]), "same rows"),
+        (lambda: norm(ro=x.float()), "all be f16 or all bf16"),
+        (lambda: norm(variant="none"), "does not fit these arguments"),
+        (lambda: ct.rms_norm_quantize(x.float(), w.float(), whole(ct, data), whole(ct, scales), 1e-6, "mxfp8"), "all be f16 or all bf16"),
+        (lambda: silu(u=x[:, :32]), "up has another shape"),
+        (lambda: silu(u=x.bfloat16()), "both be f16 or both bf16"),
+        (lambda: silu(g=x.float(), u=x.float()), "both be f16 or both bf16"),
+        (lambda: deq(o=torch.zeros(4, 65, dtype=torch.half)), "x holds 4 rows of 64 values"),
+        (lambda: deq(o=torch.zeros(5, 64, dtype=torch.half)), "x holds 4 rows of 64 values"),
+        (lambda: deq(o=torch.zeros(4, 64, dtype=torch.double)), "out must be f16, bf16 or f32"),
+        (lambda: deq(s=wide), "whole blocks of 32 and scales"),
+        (lambda: deq(data, scales, x, "mxfp4", 3.0), "whole blocks of 32 and scales"),
+    ]
+    for i, (fn, msg) in enumerate(cases):
+        with pytest.raises(ct.CutileError, match=msg):
+            fn()
+            print("case", i, msg)
+    assert ct.lib().cutile_testing_launch_count() == n0
+
+
+def test_null_arguments_of_the_c_entries(fake_hip):
+    """every pointer of the C entries may be null by mistake: an error, not a fault"""
+    import ctypes as C
+
+    ct = fake_hip
+    x, data, scales, w = (torch.zeros(4, 64, dtype=torch.half), torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8), torch.zeros(64, dtype=torch.half))
+    t = lambda v, d=None: C.pointer(ct.tensor_arg(v, d))
+    p = lambda v, d=None: C.pointer(ct.Partition(v, [1, v.shape[1]], False, d).arg())
+    f32 = C.c_float
+    calls = {
+        "block_quantize": [t(x), p(data, ct.F8E4M3FN), p(scales, ct.F8E8M0FNU), f32(1.0)],
+        "block_dequantize": [t(data, ct.F8E4M3FN), t(scales, ct.F8E8M0FNU), f32(1.0), p(x)],
+        "rms_norm_quantize": [t(x), t(w), p(data, ct.F8E4M3FN), p(scales, ct.F8E8M0FNU), f32(1e-6), f32(1.0)],
+        "add_rms_norm_quantize": [t(x), t(x), t(w), p(data, ct.F8E4M3FN), p(scales, ct.F8E8M0FNU), p(x), f32(1e-6), f32(1.0)],
+        "silu_mul_quantize": [t(x), t(x), p(data, ct.F8E4M3FN), p(scales, ct.F8E8M0FNU), f32(1.0)],
+    }
+    for name, args in calls.items():
+        fn = getattr(ct.lib(), "cutile_launch_" + name)
+        assert fn(None, *args, None) == 0, name
+        for i, a in enumerate(args):
+            if isinstance(a, C.c_float):
+                continue
+            assert fn(None, *[None if j == i else b for j, b in enumerate(args)], None) == -2, (name, i)
+
+
+def test_launch_modes_and_coverage(fake_hip):
+    """a prefix partition covers the rows that its grid says; compile-only launches enqueue nothing"""
+    import struct
+
+    ct = fake_hip
+    x = torch.zeros(10, 64, dtype=torch.half)
+    data, scales = torch.zeros(10, 64, dtype=torch.uint8), torch.zeros(10, 2, dtype=torch.uint8)
+    ct.block_quantize(x, ct.partition(data, [4, 64], prefix=True), ct.partition(scales, [4, 2], prefix=True), "mxfp8", grid=(2, 1, 1), generics=[64])
+    from test_host_abi import _last
+    rec, args = _last(ct)
+    assert rec.symbol.startswith(b"block_quantize_entry__mxfp8_f16")
+    n0 = ct.lib().cutile_testing_launch_count()
+    ct.check(ct.lib().cutile_set_launch_mode(1))
+    try:
+        ct.block_quantize(x, whole(ct, data), whole(ct, scales), "mxfp8")
+        assert ct.last_resolved()["function"] == "block_quantize"
+    finally:
+        ct.check(ct.lib().cutile_set_launch_mode(0))
+    assert ct.lib().cutile_testing_launch_count() == n0
+
+
+# ---- quantisation ----------------------------------------------------------------------------------------------------------
+def quantised(ct, x, fmt, k=None, g=1.0, rows=None, **kw):
+    rows = x.shape[0] if rows is None else rows
+    data, scales = ref.buffers(rows, ref.padded(x.shape[1], fmt) if k is None else k, fmt, x.device, extra_rows=1)
+    ct.block_quantize(x, whole(ct, data[:rows]), whole(ct, scales[:rows]), fmt, g, **kw)
+    torch.cuda.synchronize()
+    assert int((data[rows:] != 0xA5).sum() + (scales[rows:] != 0xA5).sum()) == 0, "rows behind the last"
+    return data[:rows], scales[:rows]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", LENGTHS)
+def test_gpu_quantize(ct, dev, fmt, dtype, n):
+    """rows of any length, from tight to wide apart; the input is exact, so every code is the rounding (nvfp4: its scale is found with
+    two f32 roundings)"""
+    for rows, pad in ((1, 0), (5, 0), (37, 3)):
+        x = normal((rows, n + pad), 100 + n + rows, dev, TYPES[dtype]) * torch.exp2(torch.arange(rows, device=dev) % 13 - 6.0).to(TYPES[dtype])[:, None]
+        x = x[:, pad:]
+        g = g_of(x, fmt)
+        k = ref.padded(n, fmt) + (ref.BLOCK[fmt] * 3 if rows == 5 else 0)      # blocks of nothing but padding
+        data, scales = quantised(ct, x, fmt, k, g)
+        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gpu_quantize_strides(ct, dev, fmt, dtype):
+    """transposed, every second column, one row repeated, a part of wider rows whose start is on no boundary"""
+    base = normal((300, 517), 7, dev, TYPES[dtype])
+    wide = normal((70, 1030), 8, dev, TYPES[dtype])
+    for x in (base.t(), base[:, ::2], base[:1].expand(9, 517), wide[:, 3:1027], wide[1:, 1:130], wide[:, 6:70], base.t()[5:, 3:200], base[::3].t()):
+        g = g_of(x, fmt)
+        data, scales = quantised(ct, x, fmt, None, g)
+        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gpu_quantize_special_values(ct, dev, fmt):
+    """zeros of both signs, NaN, infinities, subnormals, the type's extremes, values halfway between two codes: each in a block of its own"""
+    b = ref.BLOCK[fmt]
+    for name, dt in TYPES.items():
+        info = torch.finfo(dt)
+        grid = ref.grid_of(fmt)
+        mids = ((grid[1:] + grid[:-1]) / 2)[-b + 1:]
+        rows = [torch.zeros(b), -torch.zeros(b), torch.full((b,), info.max), torch.full((b,), -info.max), torch.full((b,), info.tiny), torch.full((b,), info.smallest_normal / 4),
+                torch.cat((torch.tensor([float(grid[-1])]), torch.nn.functional.pad(mids.float(), (0, b - 1 - mids.numel())))),
+                torch.cat((torch.tensor([-float(grid[-1])]), torch.nn.functional.pad(-mids.float(), (0, b - 1 - mids.numel()))))]
+        for at in (0, b // 2, b - 1):
+            for bad in (math.nan, math.inf, -math.inf):
+                rows.append(torch.ones(b))
+                rows[-1][at] = bad
+        rows.append(torch.ones(b))                                        # a block beside those
+        x = torch.stack(rows).to(dt).reshape(1, -1).to(dev)
+        g = 2.0 ** -9 if fmt == "nvfp4" else 1.0
+        data, scales = quantised(ct, x, fmt, None, g)
+        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+        back = torch.zeros(x.shape, device=dev)
+        ct.block_dequantize(data, scales, whole(ct, back), fmt, g)
+        lost = ~torch.isfinite(x.view(-1, b)).all(-1)
+        assert bool(torch.isnan(back.view(-1, b)[lost]).all()) and bool(torch.isfinite(back.view(-1, b)[~lost]).all()), name
+
+
+@pytest.mark.gpu
+def test_gpu_quantize_tensor_scale_range(ct, dev):
+    """nvfp4: the ends of tensor_scale, values too small for any scale and too large for the largest"""
+    x = torch.cat([normal((1, 64), 3, dev) * s for s in (1e-30, 1e-6, 1.0, 1e6, 1e30)], 1)
+    for g in (2.0 ** -100, 1.0, 1e3, 2.0 ** 100):
+        data, scales = quantised(ct, x, "nvfp4", None, g)
+        ref.assert_quantised(data, scales, x.double(), "nvfp4", g, slack=2 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+def test_gpu_quantize_covers_the_rows_of_its_grid(ct, dev):
+    x = normal((10, 96), 5, dev, torch.half)
+    data, scales = ref.buffers(10, 96, "mxfp8", dev)
+    ct.block_quantize(x, ct.partition(data, [4, 96], prefix=True), ct.partition(scales, [4, 3], prefix=True), "mxfp8", grid=(2, 1, 1))
+    torch.cuda.synchronize()
+    ref.assert_quantised(data[:8], scales[:8], x[:8].double(), "mxfp8")
+    assert int((data[8:] != 0xA5).sum() + (scales[8:] != 0xA5).sum()) == 0
+    data, scales = ref.buffers(7, 96, "mxfp8", dev)                         # fewer rows than x
+    ct.block_quantize(x, ct.partition(data, [3, 96]), ct.partition(scales, [3, 3]), "mxfp8")
+    ref.assert_quantised(data, scales, x[:7].double(), "mxfp8")
+
+
+@pytest.mark.gpu
+def test_gpu_quantize_and_back_beyond_32_bit_offsets(ct, dev):
+    """more than 2^32 bytes of input: the last rows are where their offsets say"""
+    rows, n = 300000, 8192
+    x = torch.zeros((rows, n), dtype=torch.bfloat16, device=dev)
+    tail = normal((64, n), 11, dev, torch.bfloat16)
+    x[-64:] = tail
+    x[:64] = tail
+    for fmt in ("mxfp8", "mxfp4"):
+        data, scales = ref.buffers(rows, n, fmt, dev)
+        ct.block_quantize(x, whole(ct, data), whole(ct, scales), fmt)
+        for part in (slice(0, 64), slice(rows - 64, rows)):
+            ref.assert_quantised(data[part], scales[part], tail.double(), fmt)
+        assert int(scales[64:-64].view(torch.uint8).max()) == 0
+        x.fill_(1.0)
+        ct.block_dequantize(data, scales, whole(ct, x), fmt)
+        assert torch.equal(x[-64:].double(), ref.values(data[-64:], scales[-64:], fmt)) and int(torch.count_nonzero(x[64:-64])) == 0
+        x[-64:] = tail
+        x[:64] = tail
+        del data, scales
+
+
+# ---- reading back ----------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gpu_dequantize_every_code_and_scale(ct, dev, fmt, dtype):
+    """each scale byte against each data byte, one rounding to out's type (f32: exact but for 2^-149, and nvfp4's factor)"""
+    b = ref.BLOCK[fmt]
+    per_row = 256 if fmt == "mxfp8" else 512
+    data = torch.arange(256, dtype=torch.uint8, device=dev).repeat(256, 1)
+    scales = torch.arange(256, dtype=torch.uint8, device=dev)[:, None].repeat(1, per_row // b)
+    g = 0.37 if fmt == "nvfp4" else 1.0
+    out = torch.full((257, per_row), 7.0, dtype=TYPES[dtype], device=dev)
+    ct.block_dequantize(data, scales, whole(ct, out[:256]), fmt, g)
+    want = ref.values(data, scales, fmt, torch.tensor(g, dtype=torch.float32).double().item())
+    got = out[:256].double()
+    assert bool((out[256] == 7.0).all())
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    info = torch.finfo(TYPES[dtype])
+    over = want.abs() >= info.max * (1 + info.eps / 4)
+    assert torch.equal(got[over], torch.copysign(torch.full_like(want, math.inf), want)[over])
+    fine = torch.isfinite(want) & ~over
+    # a step is eps of the value, or of the smallest normal number below it; f32 holds the product before the rounding to out
+    step = info.eps / 2 * want.abs().clamp(min=info.smallest_normal) + 2.0 ** -24 * want.abs() * (fmt == "nvfp4") + 2.0 ** -150
+    assert bool(((got - want).abs() <= step)[fine].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gpu_dequantize_lengths_and_strides(ct, dev, fmt):
+    for rows, n in ((1, 1), (3, 33), (2, 100), (40, 1000), (7, 5001)):
+        x = normal((rows, n), rows + n, dev)
+        g = g_of(x, fmt)
+        data, scales = quantised(ct, x, fmt, None, g)
+        want = ref.values(data, scales, fmt, torch.tensor(g, dtype=torch.float32).double().item())[:, :n]
+        for out in (torch.full((rows + 1, n), 7.0, device=dev)[:rows], torch.zeros((n, rows), device=dev).t(), torch.full((rows, n + 5), 7.0, device=dev)[:, 3:n + 3],
+                    torch.full((rows, 2 * n), 7.0, device=dev)[:, ::2], torch.zeros((rows, max(1, n - 9)), dtype=torch.half, device=dev)):
+            ct.block_dequantize(data, scales, whole(ct, out), fmt, g)
+            assert bool(((out.double() - want[:, : out.shape[1]]).abs() <= torch.finfo(out.dtype).eps * want[:, : out.shape[1]].abs()).all())
+            if out.dtype == torch.float32 and out._base is not None and out._base.shape != out.shape and out.stride(1) == 1:
+                assert int((out._base == 7.0).sum()) >= out._base.numel() - out.numel(), "around out"
+
+
+# ---- norm ------------------------------------------------------------------------------------------------------------------
+def norm_slack(n):
+    """relative to 2^-24: the sum's own rounding; half of what the sum of squares collects - 2 per square and one per addition, of which a
+    value passes at most n / 256 in its thread and 16 across lanes and threads; mean, eps, root and reciprocal; two products"""
+    return (1 + 0.5 * (2 + n / 256 + 8 + 16) + 4 + 2) * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", LENGTHS + [40000])
+@pytest.mark.parametrize("add", [False, True])
+def test_gpu_norm(ct, dev, fmt, dtype, n, add):
+    dt = TYPES[dtype]
+    for rows, pad in ((1, 0), (6, 0), (11, 5)):
+        x, r = (normal((rows, n + pad), 31 * n + rows + i, dev, dt, 1.0 + i)[:, pad:] for i in range(2))
+        w = (1 + 0.3 * normal((n,), n, dev)).to(dt)
+        c = x.double() + r.double() if add else x.double()
+        want = c / torch.sqrt(c.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+        g = g_of(want, fmt)
+        data, scales = ref.buffers(rows, ref.padded(n, fmt) + (ref.BLOCK[fmt] * 2 if rows == 6 else 0), fmt, dev, extra_rows=1)
+        outs = whole(ct, data[:rows]), whole(ct, scales[:rows])
+        if add:
+            ro = torch.full((rows + 1, n), 7.0, dtype=dt, device=dev)
+            ct.add_rms_norm_quantize(r, x, w, *outs, whole(ct, ro[:rows]), 1e-6, fmt, g)
+            assert bool((ro[rows] == 7.0).all())
+            assert torch.equal(ro[:rows], (x.float() + r.float()).to(dt))       # f32 sum, one rounding
+        else:
+            ct.rms_norm_quantize(x, w, *outs, 1e-6, fmt, g)
+        torch.cuda.synchronize()
+        assert int((data[rows:] != 0xA5).sum() + (scales[rows:] != 0xA5).sum()) == 0
+        g = torch.tensor(g, dtype=torch.float32).double().item()
+        ref.assert_quantised(data[:rows], scales[:rows], want, fmt, g, slack=norm_slack(n) + 2 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [256, 1001, 8192])
+def test_gpu_norm_in_place_and_strided(ct, dev, n):
+    """residual_out is residual, then x; rows with a stride, a transposed residual, weights with a stride"""
+    dt = torch.bfloat16
+    for alias in ("residual", "x", "strided"):
+        x, r = normal((9, n), 1, dev, dt), normal((9, n), 2, dev, dt)
+        w = (1 + 0.3 * normal((2 * n,), 3, dev)).to(dt)[:n]
+        if alias == "strided":
+            x, r, w = normal((9, 2 * n), 1, dev, dt)[:, ::2], normal((n, 9), 2, dev, dt).t(), (1 + 0.3 * normal((2 * n,), 3, dev)).to(dt)[::2]
+        total = x.float() + r.float()
+        c = x.double() + r.double()
+        want = c / torch.sqrt(c.square().mean(-1, keepdim=True) + 1e-5) * w.double()
+        ro = {"residual": r, "x": x, "strided": torch.zeros((n, 9), dtype=dt, device=dev).t()}[alias]
+        data, scales = ref.buffers(9, ref.padded(n, "mxfp8"), "mxfp8", dev)
+        ct.add_rms_norm_quantize(r, x, w, whole(ct, data), whole(ct, scales), whole(ct, ro), 1e-5, "mxfp8")
+        torch.cuda.synchronize()
+        assert torch.equal(ro, total.to(dt)), alias
+        ref.assert_quantised(data, scales, want, "mxfp8", slack=norm_slack(n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gpu_norm_special_rows(ct, dev, fmt):
+    """a row of zeros (with and without eps), of one NaN, of an infinity (its block is NaN, the others are 0), of the largest values
+    (whose squares overflow f32 for bf16: the norm is 0)"""
+    n, b = 256, ref.BLOCK[fmt]
+    x = normal((6, n), 4, dev, torch.bfloat16)
+    x[0] = 0
+    x[1, 70] = math.nan
+    x[2, 70] = math.inf
+    x[3] = torch.finfo(torch.bfloat16).max
+    w = torch.ones(n, dtype=torch.bfloat16, device=dev)
+    for eps in (1e-6, 0.0):
+        data, scales = ref.buffers(6, n, fmt, dev)
+        ct.rms_norm_quantize(x, w, whole(ct, data), whole(ct, scales), eps, fmt, 0.01 if fmt == "nvfp4" else 1.0)
+        v = ref.values(data, scales, fmt, 0.01 if fmt == "nvfp4" else 1.0)
+        assert bool((v[0] == 0).all()) if eps else bool(torch.isnan(v[0]).all())
+        assert bool(torch.isnan(v[1]).all())
+        at = slice(70 // b * b, 70 // b * b + b)
+        assert bool(torch.isnan(v[2, at]).all()) and int(torch.isnan(v[2]).sum()) == b and float(torch.nan_to_num(v[2]).abs().max()) == 0
+        assert bool((v[3] == 0).all())
+        assert bool(torch.isfinite(v[4:]).all()) and float(v[4:].abs().min(-1).values.max()) >= 0 and float(v[4:].abs().max()) > 1
+
+
+# ---- gated activation --------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", LENGTHS)
+def test_gpu_silu_mul(ct, dev, fmt, dtype, n):
+    dt = TYPES[dtype]
+    for rows, halves in ((1, True), (5, True), (19, False)):
+        both = normal((rows, 2 * n), n + rows, dev, dt, 3.0)
+        gate, up = (both[:, :n], both[:, n:]) if halves else (both[:, ::2], both[:, 1::2])
+        x = gate.double()
+        want = x / (1 + torch.exp(-x)) * up.double()
+        g = g_of(want, fmt)
+        data, scales = ref.buffers(rows, ref.padded(n, fmt), fmt, dev, extra_rows=1)
+        ct.silu_mul_quantize(gate, up, whole(ct, data[:rows]), whole(ct, scales[:rows]), fmt, g)
+        torch.cuda.synchronize()
+        assert int((data[rows:] != 0xA5).sum() + (scales[rows:] != 0xA5).sum()) == 0
+        g = torch.tensor(g, dtype=torch.float32).double().item()
+        # exponential (2 steps), sum, quotient (2), product, each relative to the result at most; nvfp4's scale
+        ref.assert_quantised(data[:rows], scales[:rows], want, fmt, g, slack=(6 + 2) * 2.0 ** -24, tiny=2.0 ** -126)
+
+
+@pytest.mark.gpu
+def test_gpu_silu_mul_far_gates(ct, dev):
+    """gates from -300 to 300: nothing overflows on the way; a NaN or an infinity takes its block"""
+    gate = torch.linspace(-300, 300, 1024, device=dev).to(torch.bfloat16)[None].clone()
+    up = normal((1, 1024), 6, dev, torch.bfloat16)
+    gate[0, 512 + 5], up[0, 640 + 7], gate[0, 704 + 2] = math.nan, math.inf, -math.inf
+    data, scales = ref.buffers(1, 1024, "mxfp8", dev)
+    ct.silu_mul_quantize(gate, up, whole(ct, data), whole(ct, scales), "mxfp8")
+    x = gate.double()
+    want = x / (1 + torch.exp(-x)) * up.double()
+    assert [int(i) for i in torch.nonzero(~torch.isfinite(want[0]))] == [517, 647, 706]
+    ref.assert_quantised(data, scales, want, "mxfp8", slack=6 * 2.0 ** -24, tiny=2.0 ** -126)

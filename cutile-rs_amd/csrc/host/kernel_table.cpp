@@ -481,14 +481,26 @@ std::vector<KernelEntry> build_table() {
       add("linear_tile_mxfp4", keep(v), keep("linear_tile_mxfp4_entry__" + v), IMG_MXFP4_FLAT, 512, (uint32_t)(std::max(stages, sums) + 4), 0, t[1], 0, t[0], dt, 0, 2);
     }
 
-  // ---- block-scaled rows (block_scale.hip) ----
+  // ---- block-scaled rows (block_scale.hip): any strides, rows of unit stride, and norms of rows held in registers (as above: capacity
+  // in values, tile[2] = units of 8 values per lane, tile[3] = wavefronts per row) ----
   for (const char* fmt : {"mxfp8", "mxfp4", "nvfp4"})
-    for (const char* dt : {"f16", "bf16", "f32"})
-      for (const char* fn : {"block_quantize", "block_dequantize", "silu_mul_quantize", "rms_norm_quantize", "add_rms_norm_quantize"}) {
-        if (dt[1] == '3' && strncmp(fn, "block_", 6) != 0) continue;   // (the fused forms read 16-bit rows)
-        const std::string v = std::string(fmt) + "_" + dt + "_any";
-        add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_BLOCK_SCALE, 256, strstr(fn, "norm") ? 16 : 0, 0, 0, 0, 0, dt, 0, 2);
+    for (const char* dt : {"f16", "bf16", "f32"}) {
+      const std::string base = std::string(fmt) + "_" + dt + "_";
+      for (const char* fn : {"block_quantize", "block_dequantize", "silu_mul_quantize"}) {
+        if (dt[1] == '3' && fn[0] == 's') continue;   // (the fused forms read 16-bit rows)
+        for (const char* kind : {"rows", "any"}) add(fn, keep(base + kind), keep(std::string(fn) + "_entry__" + base + kind), IMG_BLOCK_SCALE, 256, 0, 0, 0, 0, 0, dt, 0, 2);
       }
+      if (dt[1] == '3') continue;
+      static const RowVariant kHeld[] = {{1, 1}, {1, 2}, {4, 2}, {4, 3}, {4, 4}, {8, 4}, {16, 4}};   // the first that holds a row is taken
+      for (const char* fn : {"rms_norm_quantize", "add_rms_norm_quantize"}) {
+        for (auto rv : kHeld) {
+          const std::string v = base + "w" + std::to_string(rv.wpr) + "v" + std::to_string(rv.vpl);
+          add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_BLOCK_SCALE, (uint32_t)std::max(256, rv.wpr * 64), rv.wpr > 1 ? (uint32_t)std::max(4, rv.wpr) * 4 : 0, 0, 0, rv.vpl,
+              rv.wpr, dt, (int64_t)rv.wpr * 64 * rv.vpl * 8, 2);
+        }
+        add(fn, keep(base + "any"), keep(std::string(fn) + "_entry__" + base + "any"), IMG_BLOCK_SCALE, 256, 16, 0, 0, 0, 0, dt, 0, 2);
+      }
+    }
   return t;
 }
 

@@ -3337,10 +3337,37 @@ cutile_status_t rows_of(const char* fn, const cutile_partition_arg_t* const* par
 
 bool is_16bit_float(cutile_dtype_t dt) { return dt == CUTILE_DTYPE_F16 || dt == CUTILE_DTYPE_BF16; }
 
-// Workgroups of 256 threads, a unit of 8 values to a thread; the kernels stride over what is beyond.
-void unit_grid(int64_t units, uint32_t grid[3]) {
-  grid[0] = (uint32_t)std::min<int64_t>((units + 255) / 256, 1 << 24);
-  grid[1] = grid[2] = 1;
+// Rows of a launch as the kernels count them: units of 8 values.  `plain`: inner strides of 1, which the "rows" kernels need, and few
+// enough units for their 32-bit count; `one`: nothing lies between one row and the next, so all of them make one row.
+struct UnitRows {
+  int64_t rows, units, n;
+  bool plain;
+};
+constexpr int64_t kMostUnits = (1ll << 31) - 4096;
+UnitRows unit_rows(int64_t rows, int64_t units, int64_t n, bool unit_stride, bool one) {
+  UnitRows u{rows, units, n, unit_stride && rows * units <= kMostUnits};
+  if (u.plain && one) u = {1, rows * units, rows * n, true};
+  return u;
+}
+// Rows r of the tensor lie one behind the other without a gap.
+bool rows_touch(const cutile_tensor_arg_t& t) { return t.shape[0] == 1 || t.strides[0] == t.shape[1]; }
+bool unit_inner(const cutile_tensor_arg_t& t) { return t.shape[t.rank - 1] == 1 || t.strides[t.rank - 1] == 1; }
+
+// Pushes what the quantising and reading kernels take behind their tensors and scales, and launches: four units to a thread ("rows"), or
+// one, strided over what is beyond the grid ("any").
+cutile_status_t launch_units(Resolved& res, cutile_stream_t stream, ArgPacker& args, const UnitRows& u, int64_t rows, int64_t units) {
+  uint32_t grid[3] = {1, 1, 1};
+  if (strstr(res.entry->variant, "_rows")) {
+    args.push_val<uint32_t>((uint32_t)u.rows);
+    args.push_val<uint32_t>((uint32_t)u.units);
+    args.push_val<int64_t>(u.n);
+    grid[0] = div_up((uint64_t)(u.rows * u.units), 256 * 4);
+  } else {
+    args.push_val<int64_t>(rows);
+    args.push_val<int32_t>((int32_t)units);
+    grid[0] = (uint32_t)std::min<int64_t>((rows * units + 255) / 256, 1 << 24);
+  }
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
 
 // block_quantize (up == nullptr) and silu_mul_quantize
@@ -3364,20 +3391,21 @@ cutile_status_t launch_quantize(const char* fn, cutile_stream_t stream, const cu
   if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
   const cutile_partition_arg_t* parts[2] = {out, scales};
   if (cutile_status_t s = rows_of(fn, parts, 2, opts, &rows)) return s;
-  const Name any = Name(f.name) + "_" + cutile_dtype_name(x->dtype) + "_any";
+  const UnitRows u = unit_rows(rows, k / 8, x->shape[1], unit_inner(*x) && (!up || unit_inner(*up)),
+                               x->shape[1] == k && rows_touch(*x) && (!up || rows_touch(*up)) && rows_touch(out->tensor) && rows_touch(scales->tensor));
+  const Name base = Name(f.name) + "_" + cutile_dtype_name(x->dtype), any = base + "_any", plain = base + "_rows";
+  Names fitting;
+  if (u.plain) fitting.push_back(plain);
+  fitting.push_back(any);
   Resolved res;
-  if (cutile_status_t s = resolve_entry(fn, opts, any, {any}, &res)) return s;
+  if (cutile_status_t s = resolve_entry(fn, opts, fitting[0], fitting, &res)) return s;
   ArgPacker args;
   args.push_tensor(*x);
   if (up) args.push_tensor(*up);
   args.push_partition(*out);
   args.push_partition(*scales);
   args.push_val<TensorScale>(t);
-  args.push_val<int64_t>(rows);
-  args.push_val<int32_t>((int32_t)(k / 8));
-  uint32_t grid[3];
-  unit_grid(rows * (k / 8), grid);
-  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+  return launch_units(res, stream, args, u, rows, k / 8);
 }
 
 // rms_norm_quantize (residual == nullptr) and add_rms_norm_quantize
@@ -3407,9 +3435,14 @@ cutile_status_t launch_norm_quantize(const char* fn, cutile_stream_t stream, con
   if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
   const cutile_partition_arg_t* parts[3] = {out, scales, residual_out};
   if (cutile_status_t s = rows_of(fn, parts, residual ? 3 : 2, opts, &rows)) return s;
-  const Name any = Name(f.name) + "_" + cutile_dtype_name(x->dtype) + "_any";
+  const Name base = Name(f.name) + "_" + cutile_dtype_name(x->dtype) + "_";
+  Names fitting;
+  if (unit_inner(*x) && unit_inner(*w) && (!residual || (unit_inner(*residual) && unit_inner(residual_out->tensor))))
+    for (const KernelEntry* e : kernels_of(fn))
+      if (e->capacity >= k && strncmp(e->variant, base.c_str(), base.size()) == 0) fitting.push_back(e->variant);
+  fitting.push_back(base + "any");
   Resolved res;
-  if (cutile_status_t s = resolve_entry(fn, opts, any, {any}, &res)) return s;
+  if (cutile_status_t s = resolve_entry(fn, opts, fitting[0], fitting, &res)) return s;
   ArgPacker args;
   if (residual) args.push_tensor(*residual);
   args.push_tensor(*x);
@@ -3421,7 +3454,8 @@ cutile_status_t launch_norm_quantize(const char* fn, cutile_stream_t stream, con
   args.push_val<TensorScale>(t);
   args.push_val<int64_t>(rows);
   args.push_val<int32_t>((int32_t)(k / 8));
-  const uint32_t grid[3] = {(uint32_t)std::min<int64_t>(rows, 1 << 24), 1, 1};
+  const int wpr = res.entry->tile[3];   // 0: a workgroup to a row, strided over what is beyond the grid
+  const uint32_t grid[3] = {wpr ? div_up((uint64_t)rows, wpr < 4 ? 4 / wpr : 1) : (uint32_t)std::min<int64_t>(rows, 1 << 24), 1, 1};
   return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
 
@@ -3468,20 +3502,20 @@ cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cut
   if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
   const cutile_partition_arg_t* parts[1] = {out};
   if (cutile_status_t s = rows_of(fn, parts, 1, opts, &rows)) return s;
-  const Name any = Name(f.name) + "_" + cutile_dtype_name(ot.dtype) + "_any";
+  const int64_t units = div_up(ot.shape[1], 8);
+  const UnitRows u = unit_rows(rows, units, ot.shape[1], unit_inner(ot), ot.shape[1] == k && rows_touch(ot) && rows_touch(*x) && rows_touch(*scales));
+  const Name base = Name(f.name) + "_" + cutile_dtype_name(ot.dtype), any = base + "_any", plain = base + "_rows";
+  Names fitting;
+  if (u.plain) fitting.push_back(plain);
+  fitting.push_back(any);
   Resolved res;
-  if (cutile_status_t s = resolve_entry(fn, opts, any, {any}, &res)) return s;
-  const int32_t units = (int32_t)div_up(ot.shape[1], 8);
+  if (cutile_status_t s = resolve_entry(fn, opts, fitting[0], fitting, &res)) return s;
   ArgPacker args;
   args.push_tensor(*x);
   args.push_tensor(*scales);
   args.push_partition(*out);
   args.push_val<float>(t.g);
-  args.push_val<int64_t>(rows);
-  args.push_val<int32_t>(units);
-  uint32_t grid[3];
-  unit_grid(rows * units, grid);
-  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+  return launch_units(res, stream, args, u, rows, units);
 }
 
 cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cutile_partition_arg_t* z, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* y,

@@ -62,6 +62,183 @@ __device__ __forceinline__ void quantize_rows(const TensorArg<2>& x, const Tenso
   }
 }
 
+// ---- rows of unit stride ---------------------------------------------------------------------------------------------
+// A unit as it lies in memory: 16 bytes (f32: 32), read with one (two) loads of any alignment; behind the row 0.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 Unaligned __attribute__((aligned(2)));
+template <typename T>
+struct Unit {
+  static constexpr int kVectors = sizeof(T) / 2, kPer = 8 / kVectors;
+  union {
+    u32x4 raw[kVectors];
+    T v[8];
+  };
+  __device__ __forceinline__ Unit() {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) raw[i] = u32x4{0, 0, 0, 0};
+  }
+  // `left` values of the row from p on; a unit on the row's end goes value by value
+  __device__ __forceinline__ void load(const T* p, int64_t left) {
+    if (left >= 8) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) raw[i] = __builtin_nontemporal_load(reinterpret_cast<const Unaligned*>(p + i * kPer));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) v[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int64_t left) const {
+    if (left >= 8) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) *reinterpret_cast<Unaligned*>(p + i * kPer) = raw[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) p[i] = v[i];
+    }
+  }
+};
+
+// Units of a launch in one sequence, row after row; a workgroup takes kUnits of them for each of its threads, neighbours to
+// neighbouring lanes.  Where everything is contiguous the launcher makes one row of it.
+constexpr int kUnits = 4;
+struct UnitPlace {
+  uint32_t r, u;
+  bool live;
+};
+__device__ __forceinline__ UnitPlace unit_place(int i, uint32_t rows, uint32_t units) {
+  const uint32_t f = blockIdx.x * (kThreads * kUnits) + i * kThreads + threadIdx.x;
+  if (rows == 1) return {0, f, f < units};
+  const uint32_t r = f / units;
+  return {r, f - r * units, r < rows};
+}
+
+template <Format F, typename T, bool SILU>
+__device__ __forceinline__ void quantize_units(const TensorArg<2>& x, const TensorArg<2>* up, const PartitionArg<2>& out, const PartitionArg<2>& scales,
+                                               TensorScale t, uint32_t rows, uint32_t units, int64_t n) {
+  UnitPlace at[kUnits];
+  Unit<T> a[kUnits], b[SILU ? kUnits : 1];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    at[i] = unit_place(i, rows, units);
+    if (!at[i].live) continue;
+    const int64_t j = (int64_t)at[i].u * 8;
+    a[i].load((const T*)x.ptr + (int64_t)at[i].r * x.strides[0] + j, n - j);
+    if constexpr (SILU) b[i].load((const T*)up->ptr + (int64_t)at[i].r * up->strides[0] + j, n - j);
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (!at[i].live) continue;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = SILU ? silu_mul((float)a[i].v[e], (float)b[SILU ? i : 0].v[e]) : (float)a[i].v[e];
+    quantize_unit<F>(v, t, data_at<F>(out, at[i].r, at[i].u), scale_at<F>(scales, at[i].r, at[i].u));
+  }
+}
+
+template <Format F, typename T>
+__device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const TensorArg<2>& scales, const PartitionArg<2>& out, float g, uint32_t rows,
+                                                 uint32_t units, int64_t n) {
+  UnitPlace at[kUnits];
+  uint2 word[kUnits];
+  uint32_t byte[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    at[i] = unit_place(i, rows, units);
+    if (!at[i].live) continue;
+    const uint8_t* d = (const uint8_t*)x.ptr + (int64_t)at[i].r * x.strides[0] + (int64_t)at[i].u * Traits<F>::kUnitBytes;
+    if constexpr (F == kMxfp8)
+      word[i] = *reinterpret_cast<const uint2*>(d);
+    else
+      word[i].x = *reinterpret_cast<const uint32_t*>(d);
+    byte[i] = ((const uint8_t*)scales.ptr)[(int64_t)at[i].r * scales.strides[0] + at[i].u / Traits<F>::kLanes];
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (!at[i].live) continue;
+    float v[8];
+    unpack_unit<F>(word[i].x, word[i].y, byte[i], g, v);
+    Unit<T> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.v[e] = (T)v[e];
+    const int64_t j = (int64_t)at[i].u * 8;
+    o.store((T*)out.ptr + (int64_t)at[i].r * out.strides[0] + j, n - j);
+  }
+}
+
+// A row of up to WPR * 64 * VPL units in the registers of WPR wavefronts: read once, summed, scaled, quantised.  Bound by memory;
+// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 13.4 with a
+// wavefront of one unit a lane, 14.5 with two, 21 with four wavefronts; 4096 x 1024 4.7: 8.9 with one wavefront, 9.5 with four; 2048 x 2048 4.7: 8.5 with four
+// of two units, 9.4 with one of four; 1500 x 5120 8.5: 12.5 with four of three, 13.9 with eight; 16384 x 8192 149: 162 to 165 with four or eight of four
+// units, 172 to 176 with sixteen of one or two; 2048 x 28672 65: 89 with sixteen of four.  Up to 500 rows every shape takes the time of a launch.
+template <Format F, typename T, bool ADD, int WPR, int VPL>
+__device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const TensorArg<2>& x, const TensorArg<1>& w, const PartitionArg<2>& out,
+                                          const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, float eps, TensorScale t, int64_t rows,
+                                          int32_t units) {
+  constexpr int kRows = WPR < 4 ? 4 / WPR : 1;      // of a workgroup
+  __shared__ float part[kRows][WPR];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, slot = wave / WPR, sub = wave % WPR;
+  const int64_t r = (int64_t)blockIdx.x * kRows + slot;
+  const bool live = r < rows;
+  const int32_t n = x.shape[1];
+  Unit<T> a[VPL], b[ADD ? VPL : 1], g[VPL];
+  float c[VPL][8], ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int32_t u = i * (WPR * 64) + sub * 64 + lane;
+    if (!live || u >= units) continue;
+    const int64_t j = (int64_t)u * 8;
+    a[i].load((const T*)x.ptr + r * x.strides[0] + j, n - j);
+    if constexpr (ADD) b[i].load((const T*)residual->ptr + r * residual->strides[0] + j, n - j);
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int32_t u = i * (WPR * 64) + sub * 64 + lane;
+    if (live && u < units) g[i].load((const T*)w.ptr + (int64_t)u * 8, n - (int64_t)u * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[i][e] = ADD ? (float)a[i].v[e] + (float)b[ADD ? i : 0].v[e] : (float)a[i].v[e];
+      s = __builtin_fmaf(c[i][e], c[i][e], s);
+    }
+    ss += s;
+  }
+  ss = lanes::across_wave<lanes::Sum>(ss);
+  if constexpr (WPR > 1) {
+    if (lane == 0) part[slot][sub] = ss;
+    __syncthreads();
+    ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) ss += part[slot][i];
+  }
+  if (!live) return;
+  const float inv = 1.0f / sqrtf(ss / (float)n + eps);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int32_t u = i * (WPR * 64) + sub * 64 + lane;
+    if (u >= units) continue;
+    if constexpr (ADD) {   // (may be residual or x itself: this lane has read what it writes)
+      Unit<T> o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o.v[e] = (T)c[i][e];
+      o.store((T*)residual_out->ptr + r * residual_out->strides[0] + (int64_t)u * 8, n - (int64_t)u * 8);
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c[i][e] * inv * (float)g[i].v[e];
+    if ((int64_t)u * 8 + 8 > n) {   // behind the row nothing but zeros, whatever inv is
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (int64_t)u * 8 + e < n ? v[e] : 0.0f;
+    }
+    quantize_unit<F>(v, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
+  }
+}
+
+// ---- any strides -------------------------------------------------------------------------------------------------------
 // Sum over the workgroup, in every thread.
 __device__ __forceinline__ float workgroup_sum(float v) {
   __shared__ float part[kThreads / 64];
@@ -138,6 +315,39 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
       TensorArg<2> x, TensorArg<2> scales, PartitionArg<2> out, float g, int64_t rows, int32_t units) {                                             \
     dequantize_rows<F, T>(x, scales, out, g, rows, units);                                                                                          \
   }
+#define BLOCK_UNITS(FMT, F, TYPE, T)                                                                                                                \
+  extern "C" __global__ void __launch_bounds__(kThreads) block_quantize_entry__##FMT##_##TYPE##_rows(                                               \
+      TensorArg<2> x, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, uint32_t rows, uint32_t units, int64_t n) {                       \
+    quantize_units<F, T, false>(x, nullptr, out, scales, t, rows, units, n);                                                                        \
+  }                                                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(kThreads) block_dequantize_entry__##FMT##_##TYPE##_rows(                                             \
+      TensorArg<2> x, TensorArg<2> scales, PartitionArg<2> out, float g, uint32_t rows, uint32_t units, int64_t n) {                                \
+    dequantize_units<F, T>(x, scales, out, g, rows, units, n);                                                                                      \
+  }
+#define BLOCK_UNITS_16(FMT, F, TYPE, T)                                                                                                             \
+  BLOCK_UNITS(FMT, F, TYPE, T)                                                                                                                      \
+  extern "C" __global__ void __launch_bounds__(kThreads) silu_mul_quantize_entry__##FMT##_##TYPE##_rows(                                            \
+      TensorArg<2> gate, TensorArg<2> up, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, uint32_t rows, uint32_t units, int64_t n) {   \
+    quantize_units<F, T, true>(gate, &up, out, scales, t, rows, units, n);                                                                          \
+  }
+#define NORM_HELD(FMT, F, TYPE, T, WPR, VPL)                                                                                                        \
+  extern "C" __global__ void __launch_bounds__(WPR < 4 ? 256 : WPR * 64) rms_norm_quantize_entry__##FMT##_##TYPE##_w##WPR##v##VPL(                  \
+      TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, float eps, TensorScale t, int64_t rows, int32_t units) {         \
+    norm_held<F, T, false, WPR, VPL>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units);                                                     \
+  }                                                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(WPR < 4 ? 256 : WPR * 64) add_rms_norm_quantize_entry__##FMT##_##TYPE##_w##WPR##v##VPL(              \
+      TensorArg<2> residual, TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, PartitionArg<2> residual_out, float eps,  \
+      TensorScale t, int64_t rows, int32_t units) {                                                                                                 \
+    norm_held<F, T, true, WPR, VPL>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units);                                              \
+  }
+#define NORMS_HELD(FMT, F, TYPE, T)   \
+  NORM_HELD(FMT, F, TYPE, T, 1, 1)    \
+  NORM_HELD(FMT, F, TYPE, T, 1, 2)    \
+  NORM_HELD(FMT, F, TYPE, T, 4, 2)    \
+  NORM_HELD(FMT, F, TYPE, T, 4, 3)    \
+  NORM_HELD(FMT, F, TYPE, T, 4, 4)    \
+  NORM_HELD(FMT, F, TYPE, T, 8, 4)    \
+  NORM_HELD(FMT, F, TYPE, T, 16, 4)
 #define BLOCK_KERNELS_16(FMT, F, TYPE, T)                                                                                                           \
   BLOCK_KERNELS(FMT, F, TYPE, T)                                                                                                                    \
   extern "C" __global__ void __launch_bounds__(kThreads) silu_mul_quantize_entry__##FMT##_##TYPE##_any(                                             \
@@ -156,7 +366,12 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
 #define BLOCK_FORMAT(FMT, F)               \
   BLOCK_KERNELS_16(FMT, F, f16, _Float16)  \
   BLOCK_KERNELS_16(FMT, F, bf16, __bf16)   \
-  BLOCK_KERNELS(FMT, F, f32, float)
+  BLOCK_KERNELS(FMT, F, f32, float)        \
+  BLOCK_UNITS_16(FMT, F, f16, _Float16)    \
+  BLOCK_UNITS_16(FMT, F, bf16, __bf16)     \
+  BLOCK_UNITS(FMT, F, f32, float)          \
+  NORMS_HELD(FMT, F, f16, _Float16)        \
+  NORMS_HELD(FMT, F, bf16, __bf16)
 BLOCK_FORMAT(mxfp8, kMxfp8)
 BLOCK_FORMAT(mxfp4, kMxfp4)
 BLOCK_FORMAT(nvfp4, kNvfp4)

@@ -3353,15 +3353,15 @@ UnitRows unit_rows(int64_t rows, int64_t units, int64_t n, bool unit_stride, boo
 bool rows_touch(const cutile_tensor_arg_t& t) { return t.shape[0] == 1 || t.strides[0] == t.shape[1]; }
 bool unit_inner(const cutile_tensor_arg_t& t) { return t.shape[t.rank - 1] == 1 || t.strides[t.rank - 1] == 1; }
 
-// Pushes what the quantising and reading kernels take behind their tensors and scales, and launches: four units to a thread ("rows"), or
-// one, strided over what is beyond the grid ("any").
-cutile_status_t launch_units(Resolved& res, cutile_stream_t stream, ArgPacker& args, const UnitRows& u, int64_t rows, int64_t units) {
+// Pushes what the quantising and reading kernels take behind their tensors and scales, and launches: `per_thread` units to a thread ("rows"),
+// or one, strided over what is beyond the grid ("any").
+cutile_status_t launch_units(Resolved& res, cutile_stream_t stream, ArgPacker& args, const UnitRows& u, int64_t rows, int64_t units, int per_thread) {
   uint32_t grid[3] = {1, 1, 1};
   if (strstr(res.entry->variant, "_rows")) {
     args.push_val<uint32_t>((uint32_t)u.rows);
     args.push_val<uint32_t>((uint32_t)u.units);
     args.push_val<int64_t>(u.n);
-    grid[0] = div_up((uint64_t)(u.rows * u.units), 256 * 4);
+    grid[0] = div_up((uint64_t)(u.rows * u.units), 256 * per_thread);
   } else {
     args.push_val<int64_t>(rows);
     args.push_val<int32_t>((int32_t)units);
@@ -3405,7 +3405,7 @@ cutile_status_t launch_quantize(const char* fn, cutile_stream_t stream, const cu
   args.push_partition(*out);
   args.push_partition(*scales);
   args.push_val<TensorScale>(t);
-  return launch_units(res, stream, args, u, rows, k / 8);
+  return launch_units(res, stream, args, u, rows, k / 8, 1);
 }
 
 // rms_norm_quantize (residual == nullptr) and add_rms_norm_quantize
@@ -3515,7 +3515,7 @@ cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cut
   args.push_tensor(*scales);
   args.push_partition(*out);
   args.push_val<float>(t.g);
-  return launch_units(res, stream, args, u, rows, units);
+  return launch_units(res, stream, args, u, rows, units, 4);
 }
 
 cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cutile_partition_arg_t* z, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* y,

@@ -102,19 +102,21 @@ struct Unit {
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) raw[i] = u32x4{0, 0, 0, 0};
   }
-  // `left` values of the row from p on; a unit on the row's end goes value by value
+  // `left` values of the row from p on; a unit on the row's end goes value by value.  WHOLE: the row is units without a rest.
+  template <bool WHOLE>
   __device__ __forceinline__ void load(const T* p, int64_t left) {
-    if (left >= 8) {
+    if (WHOLE || left >= 8) {
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) raw[i] = __builtin_nontemporal_load(reinterpret_cast<const Unaligned*>(p + i * kPer));
+      for (int i = 0; i < kVectors; ++i) raw[i] = *reinterpret_cast<const Unaligned*>(p + i * kPer);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (i < left) v[i] = p[i];
     }
   }
+  template <bool WHOLE>
   __device__ __forceinline__ void store(T* p, int64_t left) const {
-    if (left >= 8) {
+    if (WHOLE || left >= 8) {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) *reinterpret_cast<Unaligned*>(p + i * kPer) = raw[i];
     } else {
@@ -125,35 +127,50 @@ struct Unit {
   }
 };
 
-// Units of a launch in one sequence, row after row; a workgroup takes kUnits of them for each of its threads, neighbours to
-// neighbouring lanes.  Where everything is contiguous the launcher makes one row of it.
-constexpr int kUnits = 4;
+// Units of a launch in one sequence, row after row, neighbours to neighbouring lanes; a workgroup takes U of them for each of its
+// threads (the launcher counts with the same U).  Where everything is contiguous the launcher makes one row of it.
+// One unit a thread for the quantising kernels: later workgroups read while earlier ones write (us with 1, 2, 4, 8 of them: 16384 x 8192 bf16 to mxfp8
+// 71, 75, 73, 78; gated activation of 1500 x 14336 22.2, 24.6, 25.5, 29.3); four for reading back (16384 x 8192 mxfp4 to bf16 65, 69, 61, 65).
+// Loads are ordinary ones: a prompt's rows come out of the memory-side cache, past which nontemporal loads go (1500 x 14336 to mxfp8 13.5 us, so 11.7).
+constexpr int kQuantizeUnits = 1, kDequantizeUnits = 4;
 struct UnitPlace {
   uint32_t r, u;
   bool live;
 };
-__device__ __forceinline__ UnitPlace unit_place(int i, uint32_t rows, uint32_t units) {
-  const uint32_t f = blockIdx.x * (kThreads * kUnits) + i * kThreads + threadIdx.x;
-  if (rows == 1) return {0, f, f < units};
-  const uint32_t r = f / units;
-  return {r, f - r * units, r < rows};
+template <int U>
+__device__ __forceinline__ void unit_places(uint32_t rows, uint32_t units, UnitPlace (&at)[U]) {
+  const uint32_t f = blockIdx.x * (kThreads * U) + threadIdx.x;
+  if (rows == 1) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) at[i] = {0, f + i * kThreads, f + i * kThreads < units};
+    return;
+  }
+  const uint32_t down = kThreads / units, across = kThreads % units;   // from a unit to the thread's next by addition
+  uint32_t r = f / units, u = f % units;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    at[i] = {r, u, r < rows};
+    u += across;
+    r += down + (u >= units);
+    u -= u >= units ? units : 0;
+  }
 }
 
-template <Format F, typename T, bool SILU>
+template <Format F, typename T, bool SILU, bool WHOLE>
 __device__ __forceinline__ void quantize_units(const TensorArg<2>& x, const TensorArg<2>* up, const PartitionArg<2>& out, const PartitionArg<2>& scales,
                                                TensorScale t, uint32_t rows, uint32_t units, int64_t n) {
-  UnitPlace at[kUnits];
-  Unit<T> a[kUnits], b[SILU ? kUnits : 1];
+  UnitPlace at[kQuantizeUnits];
+  unit_places(rows, units, at);
+  Unit<T> a[kQuantizeUnits], b[SILU ? kQuantizeUnits : 1];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    at[i] = unit_place(i, rows, units);
+  for (int i = 0; i < kQuantizeUnits; ++i) {
     if (!at[i].live) continue;
     const int64_t j = (int64_t)at[i].u * 8;
-    a[i].load((const T*)x.ptr + (int64_t)at[i].r * x.strides[0] + j, n - j);
-    if constexpr (SILU) b[i].load((const T*)up->ptr + (int64_t)at[i].r * up->strides[0] + j, n - j);
+    a[i].template load<WHOLE>((const T*)x.ptr + (int64_t)at[i].r * x.strides[0] + j, n - j);
+    if constexpr (SILU) b[i].template load<WHOLE>((const T*)up->ptr + (int64_t)at[i].r * up->strides[0] + j, n - j);
   }
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
+  for (int i = 0; i < kQuantizeUnits; ++i) {
     if (!at[i].live) continue;
     float v[8];
 #pragma unroll
@@ -162,15 +179,15 @@ __device__ __forceinline__ void quantize_units(const TensorArg<2>& x, const Tens
   }
 }
 
-template <Format F, typename T>
+template <Format F, typename T, bool WHOLE>
 __device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const TensorArg<2>& scales, const PartitionArg<2>& out, float g, uint32_t rows,
                                                  uint32_t units, int64_t n) {
-  UnitPlace at[kUnits];
-  uint2 word[kUnits];
-  uint32_t byte[kUnits];
+  UnitPlace at[kDequantizeUnits];
+  unit_places(rows, units, at);
+  uint2 word[kDequantizeUnits];
+  uint32_t byte[kDequantizeUnits];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    at[i] = unit_place(i, rows, units);
+  for (int i = 0; i < kDequantizeUnits; ++i) {
     if (!at[i].live) continue;
     const uint8_t* d = (const uint8_t*)x.ptr + (int64_t)at[i].r * x.strides[0] + (int64_t)at[i].u * Traits<F>::kUnitBytes;
     if constexpr (F == kMxfp8)
@@ -180,7 +197,7 @@ __device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const Te
     byte[i] = ((const uint8_t*)scales.ptr)[(int64_t)at[i].r * scales.strides[0] + at[i].u / Traits<F>::kLanes];
   }
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
+  for (int i = 0; i < kDequantizeUnits; ++i) {
     if (!at[i].live) continue;
     float v[8];
     unpack_unit<F>(word[i].x, word[i].y, byte[i], g, v);
@@ -188,7 +205,7 @@ __device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const Te
 #pragma unroll
     for (int e = 0; e < 8; ++e) o.v[e] = (T)v[e];
     const int64_t j = (int64_t)at[i].u * 8;
-    o.store((T*)out.ptr + (int64_t)at[i].r * out.strides[0] + j, n - j);
+    o.template store<WHOLE>((T*)out.ptr + (int64_t)at[i].r * out.strides[0] + j, n - j);
   }
 }
 
@@ -197,12 +214,11 @@ __device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const Te
 // wavefront of one unit a lane, 14.5 with two, 21 with four wavefronts; 4096 x 1024 4.7: 8.9 with one wavefront, 9.5 with four; 2048 x 2048 4.7: 8.5 with four
 // of two units, 9.4 with one of four; 1500 x 5120 8.5: 12.5 with four of three, 13.9 with eight; 16384 x 8192 149: 162 to 165 with four or eight of four
 // units, 172 to 176 with sixteen of one or two; 2048 x 28672 65: 89 with sixteen of four.  Up to 500 rows every shape takes the time of a launch.
-template <Format F, typename T, bool ADD, int WPR, int VPL>
+template <Format F, typename T, bool ADD, int WPR, int VPL, bool WHOLE>
 __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const TensorArg<2>& x, const TensorArg<1>& w, const PartitionArg<2>& out,
                                           const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, float eps, TensorScale t, int64_t rows,
-                                          int32_t units) {
+                                          int32_t units, float (*part)[WPR]) {
   constexpr int kRows = WPR < 4 ? 4 / WPR : 1;      // of a workgroup
-  __shared__ float part[kRows][WPR];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, slot = wave / WPR, sub = wave % WPR;
   const int64_t r = (int64_t)blockIdx.x * kRows + slot;
   const bool live = r < rows;
@@ -214,13 +230,13 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
     const int32_t u = i * (WPR * 64) + sub * 64 + lane;
     if (!live || u >= units) continue;
     const int64_t j = (int64_t)u * 8;
-    a[i].load((const T*)x.ptr + r * x.strides[0] + j, n - j);
-    if constexpr (ADD) b[i].load((const T*)residual->ptr + r * residual->strides[0] + j, n - j);
+    a[i].template load<WHOLE>((const T*)x.ptr + r * x.strides[0] + j, n - j);
+    if constexpr (ADD) b[i].template load<WHOLE>((const T*)residual->ptr + r * residual->strides[0] + j, n - j);
   }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int32_t u = i * (WPR * 64) + sub * 64 + lane;
-    if (live && u < units) g[i].load((const T*)w.ptr + (int64_t)u * 8, n - (int64_t)u * 8);
+    if (live && u < units) g[i].template load<WHOLE>((const T*)w.ptr + (int64_t)u * 8, n - (int64_t)u * 8);
   }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
@@ -250,12 +266,12 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
       Unit<T> o;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o.v[e] = (T)c[i][e];
-      o.store((T*)residual_out->ptr + r * residual_out->strides[0] + (int64_t)u * 8, n - (int64_t)u * 8);
+      o.template store<WHOLE>((T*)residual_out->ptr + r * residual_out->strides[0] + (int64_t)u * 8, n - (int64_t)u * 8);
     }
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = s.times(c[i][e], (float)g[i].v[e]);
-    if ((int64_t)u * 8 + 8 > n) {   // behind the row nothing but zeros, whatever the norm is
+    if (!WHOLE && (int64_t)u * 8 + 8 > n) {   // behind the row nothing but zeros, whatever the norm is
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = (int64_t)u * 8 + e < n ? v[e] : 0.0f;
     }
@@ -343,27 +359,34 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
 #define BLOCK_UNITS(FMT, F, TYPE, T)                                                                                                                \
   extern "C" __global__ void __launch_bounds__(kThreads) block_quantize_entry__##FMT##_##TYPE##_rows(                                               \
       TensorArg<2> x, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, uint32_t rows, uint32_t units, int64_t n) {                       \
-    quantize_units<F, T, false>(x, nullptr, out, scales, t, rows, units, n);                                                                        \
+    if (n == 8ll * units) quantize_units<F, T, false, true>(x, nullptr, out, scales, t, rows, units, n);                                            \
+    else quantize_units<F, T, false, false>(x, nullptr, out, scales, t, rows, units, n);                                                                        \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kThreads) block_dequantize_entry__##FMT##_##TYPE##_rows(                                             \
       TensorArg<2> x, TensorArg<2> scales, PartitionArg<2> out, float g, uint32_t rows, uint32_t units, int64_t n) {                                \
-    dequantize_units<F, T>(x, scales, out, g, rows, units, n);                                                                                      \
+    if (n == 8ll * units) dequantize_units<F, T, true>(x, scales, out, g, rows, units, n);                                                          \
+    else dequantize_units<F, T, false>(x, scales, out, g, rows, units, n);                                                                                      \
   }
 #define BLOCK_UNITS_16(FMT, F, TYPE, T)                                                                                                             \
   BLOCK_UNITS(FMT, F, TYPE, T)                                                                                                                      \
   extern "C" __global__ void __launch_bounds__(kThreads) silu_mul_quantize_entry__##FMT##_##TYPE##_rows(                                            \
       TensorArg<2> gate, TensorArg<2> up, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, uint32_t rows, uint32_t units, int64_t n) {   \
-    quantize_units<F, T, true>(gate, &up, out, scales, t, rows, units, n);                                                                          \
+    if (n == 8ll * units) quantize_units<F, T, true, true>(gate, &up, out, scales, t, rows, units, n);                                              \
+    else quantize_units<F, T, true, false>(gate, &up, out, scales, t, rows, units, n);                                                                          \
   }
 #define NORM_HELD(FMT, F, TYPE, T, WPR, VPL)                                                                                                        \
   extern "C" __global__ void __launch_bounds__(WPR < 4 ? 256 : WPR * 64) rms_norm_quantize_entry__##FMT##_##TYPE##_w##WPR##v##VPL(                  \
       TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, float eps, TensorScale t, int64_t rows, int32_t units) {         \
-    norm_held<F, T, false, WPR, VPL>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units);                                                     \
+    __shared__ float part[WPR < 4 ? 4 / WPR : 1][WPR];                                                                                              \
+    if (x.shape[1] == 8ll * units) norm_held<F, T, false, WPR, VPL, true>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units, part);          \
+    else norm_held<F, T, false, WPR, VPL, false>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units, part);                                   \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(WPR < 4 ? 256 : WPR * 64) add_rms_norm_quantize_entry__##FMT##_##TYPE##_w##WPR##v##VPL(              \
       TensorArg<2> residual, TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, PartitionArg<2> residual_out, float eps,  \
       TensorScale t, int64_t rows, int32_t units) {                                                                                                 \
-    norm_held<F, T, true, WPR, VPL>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units);                                              \
+    __shared__ float part[WPR < 4 ? 4 / WPR : 1][WPR];                                                                                              \
+    if (x.shape[1] == 8ll * units) norm_held<F, T, true, WPR, VPL, true>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units, part);   \
+    else norm_held<F, T, true, WPR, VPL, false>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units, part);                            \
   }
 #define NORMS_HELD(FMT, F, TYPE, T)   \
   NORM_HELD(FMT, F, TYPE, T, 1, 1)    \

@@ -3396,6 +3396,8 @@ cutile_status_t launch_quantize(const char* fn, cutile_stream_t stream, const cu
   const Name base = Name(f.name) + "_" + cutile_dtype_name(x->dtype), any = base + "_any", plain = base + "_rows";
   Names fitting;
   if (u.plain) fitting.push_back(plain);
+  const uint32_t column_groups = div_up((uint64_t)(k / 8), 32);   // of 32 units, 128 rows each: what a workgroup of the "columns" kernels covers
+  if (!up && x->strides[0] == 1 && div_up((uint64_t)rows, 128) * (uint64_t)column_groups <= 0x7fffffffull / 512) fitting.push_back(base + "_columns");
   fitting.push_back(any);
   Resolved res;
   if (cutile_status_t s = resolve_entry(fn, opts, fitting[0], fitting, &res)) return s;
@@ -3405,6 +3407,13 @@ cutile_status_t launch_quantize(const char* fn, cutile_stream_t stream, const cu
   args.push_partition(*out);
   args.push_partition(*scales);
   args.push_val<TensorScale>(t);
+  if (strstr(res.entry->variant, "_columns")) {
+    args.push_val<int64_t>(rows);
+    args.push_val<int32_t>((int32_t)(k / 8));
+    args.push_val<uint32_t>(column_groups);
+    const uint32_t grid[3] = {div_up((uint64_t)rows, 128) * column_groups, 1, 1};
+    return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+  }
   return launch_units(res, stream, args, u, rows, k / 8, 1);
 }
 

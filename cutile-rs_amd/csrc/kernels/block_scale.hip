@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include "block_scale.h"
+#include "gemm_common.h"
 #include "kernel_args.h"
 
 using namespace cutile;
@@ -209,6 +210,34 @@ __device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const Te
   }
 }
 
+// Columns of unit stride: a weight that is kept [K, N], quantised along K.  A lane reads eight neighbouring rows of eight columns, 16 bytes a
+// column (16 lanes: 256 bytes), and so holds a unit of each of the eight rows; no exchange is needed but the one for the scale.
+// A wavefront covers 128 rows of four units, the eight of a workgroup lie side by side along the row: 128-byte lines of e2m1 are
+// written whole, and neighbours along the row are neighbours on an XCD, whose L2 puts the scale bytes together.
+// (14336 x 4096 bf16 to mxfp4 out of [4096, 14336]: 225 us value by value.)
+constexpr int kColThreads = 512, kColRows = 128, kColUnits = 32;   // of a workgroup
+template <Format F, typename T, bool WHOLE>
+__device__ __forceinline__ void quantize_columns(const TensorArg<2>& x, const PartitionArg<2>& out, const PartitionArg<2>& scales, TensorScale t, int64_t rows,
+                                                 int32_t units, uint32_t groups) {
+  const uint32_t id = gemm::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int lane = threadIdx.x & 63;
+  const int64_t r0 = (int64_t)(id / groups) * kColRows + (lane >> 2) * 8;
+  const int32_t u = (int32_t)(id % groups) * kColUnits + (int)(threadIdx.x >> 6) * 4 + (lane & 3), n = x.shape[1];
+  if (u >= units || r0 >= rows) return;
+  Unit<T> a[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if ((int64_t)u * 8 + e < n) a[e].template load<WHOLE>((const T*)x.ptr + ((int64_t)u * 8 + e) * x.strides[1] + r0, rows - r0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!WHOLE && r0 + i >= rows) break;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)a[e].v[i];
+    quantize_unit<F>(v, t, data_at<F>(out, r0 + i, u), scale_at<F>(scales, r0 + i, u));
+  }
+}
+
 // A row of up to WPR * 64 * VPL units in the registers of WPR wavefronts: read once, summed, scaled, quantised.  Bound by memory;
 // what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 13.4 with a
 // wavefront of one unit a lane, 14.5 with two, 21 with four wavefronts; 4096 x 1024 4.7: 8.9 with one wavefront, 9.5 with four; 2048 x 2048 4.7: 8.5 with four
@@ -361,6 +390,11 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
       TensorArg<2> x, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, uint32_t rows, uint32_t units, int64_t n) {                       \
     if (n == 8ll * units) quantize_units<F, T, false, true>(x, nullptr, out, scales, t, rows, units, n);                                            \
     else quantize_units<F, T, false, false>(x, nullptr, out, scales, t, rows, units, n);                                                                        \
+  }                                                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(kColThreads) block_quantize_entry__##FMT##_##TYPE##_columns(                                         \
+      TensorArg<2> x, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, int64_t rows, int32_t units, uint32_t groups) {                   \
+    if (rows % 8 == 0) quantize_columns<F, T, true>(x, out, scales, t, rows, units, groups);                                                        \
+    else quantize_columns<F, T, false>(x, out, scales, t, rows, units, groups);                                                                     \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kThreads) block_dequantize_entry__##FMT##_##TYPE##_rows(                                             \
       TensorArg<2> x, TensorArg<2> scales, PartitionArg<2> out, float g, uint32_t rows, uint32_t units, int64_t n) {                                \

@@ -490,7 +490,8 @@ std::vector<KernelEntry> build_table() {
         if (dt[1] == '3' && fn[0] == 's') continue;   // (the fused forms read 16-bit rows)
         for (const char* kind : {"rows", "any"}) add(fn, keep(base + kind), keep(std::string(fn) + "_entry__" + base + kind), IMG_BLOCK_SCALE, 256, 0, 0, 0, 0, 0, dt, 0, 2);
       }
-      add("block_quantize", keep(base + "columns"), keep("block_quantize_entry__" + base + "columns"), IMG_BLOCK_SCALE, 512, 0, 0, 0, 0, 0, dt, 0, 2);
+      add("block_quantize", keep(base + "columns"), keep("block_quantize_entry__" + base + "columns"), IMG_BLOCK_SCALE, 512,
+          fmt[0] == 'n' ? 128 * (128 + 16) : 128 * ((fmt[4] == '8' ? 256 : 128) + 8), 0, 0, 0, 0, dt, 0, 2);
       if (dt[1] == '3') continue;
       static const RowVariant kHeld[] = {{1, 1}, {1, 2}, {4, 2}, {4, 3}, {4, 4}, {8, 4}, {16, 4}};   // the first that holds a row is taken
       for (const char* fn : {"rms_norm_quantize", "add_rms_norm_quantize"}) {

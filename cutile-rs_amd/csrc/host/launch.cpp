@@ -3397,10 +3397,13 @@ cutile_status_t launch_quantize(const char* fn, cutile_stream_t stream, const cu
   Names fitting;
   if (u.plain) fitting.push_back(plain);
   const uint32_t column_groups = div_up((uint64_t)(k / 8), 32);   // of 32 units, 128 rows each: what a workgroup of the "columns" kernels covers
-  if (!up && x->strides[0] == 1 && div_up((uint64_t)rows, 128) * (uint64_t)column_groups <= 0x7fffffffull / 512) fitting.push_back(base + "_columns");
+  const Name columns = base + "_columns";
+  if (!up && x->strides[0] == 1 && div_up((uint64_t)rows, 128) * (uint64_t)column_groups <= 0x7fffffffull / 512) fitting.push_back(columns);
   fitting.push_back(any);
   Resolved res;
-  if (cutile_status_t s = resolve_entry(fn, opts, fitting[0], fitting, &res)) return s;
+  // fewer than 64 rows are no work for workgroups of 128 (to mxfp8, us: 16 x 4096 7.0, value by value 5.1; 64 x 4096 5.4, 5.1; 512 x 512 5.7, 5.1; 4096 x 4096 12.6, 70)
+  const Name& usual = fitting[0] == columns && rows < 64 ? any : fitting[0];
+  if (cutile_status_t s = resolve_entry(fn, opts, usual, fitting, &res)) return s;
   ArgPacker args;
   args.push_tensor(*x);
   if (up) args.push_tensor(*up);

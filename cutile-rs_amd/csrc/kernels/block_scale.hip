@@ -212,29 +212,50 @@ __device__ __forceinline__ void dequantize_units(const TensorArg<2>& x, const Te
 
 // Columns of unit stride: a weight that is kept [K, N], quantised along K.  A lane reads eight neighbouring rows of eight columns, 16 bytes a
 // column (16 lanes: 256 bytes), and so holds a unit of each of the eight rows; no exchange is needed but the one for the scale.
-// A wavefront covers 128 rows of four units, the eight of a workgroup lie side by side along the row: 128-byte lines of e2m1 are
-// written whole, and neighbours along the row are neighbours on an XCD, whose L2 puts the scale bytes together.
-// (14336 x 4096 bf16 to mxfp4 out of [4096, 14336]: 225 us value by value.)
+// A wavefront covers 128 rows of four units, the eight of a workgroup lie side by side along the row.  Quantised units and scales
+// go through LDS, so that a row's 32 units leave as whole lines and its scale bytes at once (straight from the lanes, 16 or 32 bytes to a
+// line and byte by byte: 14336 x 4096 bf16 to mxfp4 out of [4096, 14336] 51 us, value by value 242).
 constexpr int kColThreads = 512, kColRows = 128, kColUnits = 32;   // of a workgroup
+template <Format F>
+struct ColumnStage {
+  static constexpr int kRowBytes = kColUnits * Traits<F>::kUnitBytes, kScales = kColUnits / Traits<F>::kLanes;
+  uint8_t data[kColRows * kRowBytes], scale[kColRows * kScales];
+  // unit u of row r; the rows that a store instruction's lanes write are 8 apart: each starts at another place
+  __device__ __forceinline__ uint8_t* unit(int r, int u) { return data + r * kRowBytes + (u * Traits<F>::kUnitBytes + (r >> 3) * (kRowBytes / 8)) % kRowBytes; }
+};
 template <Format F, typename T, bool WHOLE>
 __device__ __forceinline__ void quantize_columns(const TensorArg<2>& x, const PartitionArg<2>& out, const PartitionArg<2>& scales, TensorScale t, int64_t rows,
-                                                 int32_t units, uint32_t groups) {
+                                                 int32_t units, uint32_t groups, ColumnStage<F>& stage) {
   const uint32_t id = gemm::xcd_contiguous(blockIdx.x, gridDim.x);
-  const int lane = threadIdx.x & 63;
-  const int64_t r0 = (int64_t)(id / groups) * kColRows + (lane >> 2) * 8;
-  const int32_t u = (int32_t)(id % groups) * kColUnits + (int)(threadIdx.x >> 6) * 4 + (lane & 3), n = x.shape[1];
-  if (u >= units || r0 >= rows) return;
-  Unit<T> a[8];
+  const int lane = threadIdx.x & 63, r_in = (lane >> 2) * 8, u_in = (int)(threadIdx.x >> 6) * 4 + (lane & 3);
+  const int64_t r0 = (int64_t)(id / groups) * kColRows;
+  const int32_t u0 = (int32_t)(id % groups) * kColUnits, n = x.shape[1];
+  if (u0 + u_in < units && r0 + r_in < rows) {
+    Unit<T> a[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if ((int64_t)u * 8 + e < n) a[e].template load<WHOLE>((const T*)x.ptr + ((int64_t)u * 8 + e) * x.strides[1] + r0, rows - r0);
+    for (int e = 0; e < 8; ++e) {
+      const int64_t j = (int64_t)(u0 + u_in) * 8 + e;
+      if (j < n) a[e].template load<WHOLE>((const T*)x.ptr + j * x.strides[1] + r0 + r_in, rows - r0 - r_in);
+    }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (!WHOLE && r0 + i >= rows) break;
-    float v[8];
+    for (int i = 0; i < 8; ++i) {
+      float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)a[e].v[i];
-    quantize_unit<F>(v, t, data_at<F>(out, r0 + i, u), scale_at<F>(scales, r0 + i, u));
+      for (int e = 0; e < 8; ++e) v[e] = (float)a[e].v[i];
+      quantize_unit<F>(v, t, stage.unit(r_in + i, u_in), stage.scale + (r_in + i) * ColumnStage<F>::kScales + u_in / Traits<F>::kLanes);
+    }
+  }
+  __syncthreads();
+  constexpr int kChunks = ColumnStage<F>::kRowBytes / 8, kUnitsOf8 = 8 / Traits<F>::kUnitBytes;   // 8 bytes to a lane
+#pragma unroll
+  for (int p = 0; p < kColRows * kChunks / kColThreads; ++p) {
+    const int r = p * (kColThreads / kChunks) + threadIdx.x / kChunks, c = threadIdx.x % kChunks;
+    if (r0 + r < rows && u0 + c * kUnitsOf8 < units) *reinterpret_cast<uint2*>(data_at<F>(out, r0 + r, u0 + c * kUnitsOf8)) = *reinterpret_cast<const uint2*>(stage.unit(r, c * kUnitsOf8));
+  }
+  constexpr int kScales = ColumnStage<F>::kScales, kLanes = Traits<F>::kLanes;
+  for (int s = threadIdx.x; s < kColRows * kScales; s += kColThreads) {
+    const int r = s / kScales, b = s % kScales;
+    if (r0 + r < rows && u0 + b * kLanes < units) *scale_at<F>(scales, r0 + r, u0 + b * kLanes) = stage.scale[s];
   }
 }
 
@@ -393,8 +414,9 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kColThreads) block_quantize_entry__##FMT##_##TYPE##_columns(                                         \
       TensorArg<2> x, PartitionArg<2> out, PartitionArg<2> scales, TensorScale t, int64_t rows, int32_t units, uint32_t groups) {                   \
-    if (rows % 8 == 0) quantize_columns<F, T, true>(x, out, scales, t, rows, units, groups);                                                        \
-    else quantize_columns<F, T, false>(x, out, scales, t, rows, units, groups);                                                                     \
+    __shared__ __attribute__((aligned(16))) ColumnStage<F> stage;                                                                                   \
+    if (rows % 8 == 0) quantize_columns<F, T, true>(x, out, scales, t, rows, units, groups, stage);                                                 \
+    else quantize_columns<F, T, false>(x, out, scales, t, rows, units, groups, stage);                                                              \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kThreads) block_dequantize_entry__##FMT##_##TYPE##_rows(                                             \
       TensorArg<2> x, TensorArg<2> scales, PartitionArg<2> out, float g, uint32_t rows, uint32_t units, int64_t n) {                                \

@@ -41,6 +41,7 @@ IMAGES = {
     "mxtiles": "mxfp8_tiles.hip",
     "gemmgroup": "gemm_group.hip",
     "fmhakeys": "fmha_keys.hip",
+    "mxfp4": "mxfp4_gemm.hip",
     "mxfp4flat": "mxfp4_flat.hip",
     "blockscale": "block_scale.hip",
 }

@@ -322,10 +322,11 @@ inline GemmChoice choose_gemm(const GemmShape& s, int cus, uint64_t partial_byte
 }
 
 // ---- block-scaled products ----
+enum ScaledKind { kScaledMxfp8, kScaledNvfp4, kScaledMxfp4 };
 struct ScaledShape {
   int64_t m, n;
   int32_t pieces;          // 64-byte pieces of a row: 64 (fp8) or 128 (fp4) values of K
-  bool fp4;
+  ScaledKind format;
 };
 // K splits of a scaled_flat.hip launch: up to half the compute units busy, at least two 128-byte steps for each of the 8
 // wavefronts (mxfp8, 64 x 1024 x 8192, 32 strips: 16.7, 13.2, 12.5 us with 1, 2, 4 splits; 16 x 4096 x 4096, 64 strips: 9.4,
@@ -376,17 +377,27 @@ struct FlatStrip {
 };
 constexpr FlatStrip kFlat[] = {{"flat16x64", 16, 64, 0.09, 0.20, 0.20, 0.20, 5.5}, {"flat32x64", 32, 64, 0.12, 0.28, 0.28, 0.28, 5.5}, {"flat64x64", 64, 64, 0.155, 0.36, 0.294, 0.297, 4.5},
                                {"flat64x128", 64, 128, 0.27, 0.62, 0.534, 0.561, 4.8}, {"flat128x128", 128, 128, 0.52, 1.12, 1.053, 1.08, 5.4}};
+// MXFP4 (mxfp4_gemm.hip, mxfp4_flat.hip), by name: strips for up to 64 rows, 256 x 256 tiles where they are half as many as compute units or more,
+// 128 x 128 in between.  us on each: 16 x 14336 x 4096 strips of 16 rows 9.1, 128 x 128 14.3; 64 x 14336 x 4096 strips of 64 rows 11.1, 15.4; 200 x 14336 x 4096
+// 128 x 128 16.7, 256 x 256 29; 1000 x 4096 x 4096 17.6, 30; 2048 x 14336 x 4096 89, 79; 4096 x 4096 x 4096 46, 39.
+inline const char* choose_mxfp4(const ScaledShape& s, int own_m, int own_n, int cus) {
+  auto blocks = [&](int64_t b) { return (uint64_t)((s.m + b - 1) / b) * (uint64_t)((s.n + b - 1) / b); };
+  if (s.m <= 64) return s.m <= 16 ? "flat16x64" : s.m <= 32 ? "flat32x64" : "flat64x64";
+  return own_m == 256 && own_n == 256 && blocks(256) * 2 >= (uint64_t)cus ? "256x256x256_e4x2" : "128x128x256_e2x2";
+}
 // The kernel by name, or nullptr: the partition's own (tuning record, then the table's order).  us per 64-byte piece of K for
 // one block on each compute unit, measured at K = 4096 (mxfp8: 16 x 4096 9.4 us, 64 x 4096 13.4, 512 x 4096 21 on 64 x 128 blocks, 24 with
 // 128 x 128 tiles; nvfp4: 9.9, 14.7, 24).  The 256 x 256 kernels are the better ones where their tiles come near to filling the chip.
 // `lone`: what mx_plan says for fp8, where it was asked.
 inline const char* choose_scaled(const ScaledShape& s, int own_m, int own_n, int cus, uint64_t partial_bytes, MxPlan* lone) {
+  if (s.format == kScaledMxfp4) return choose_mxfp4(s, own_m, own_n, cus);
+  const bool fp4 = s.format == kScaledNvfp4;
   // a partition whose output other tiles of nvfp4_gemm.hip may compute too
-  const bool tiled = s.fp4 && own_m == own_n && (own_m == 128 || (own_m == 256 && s.pieces > 4));
+  const bool tiled = fp4 && own_m == own_n && (own_m == 128 || (own_m == 256 && s.pieces > 4));
   auto blocks = [&](int bm, int bn) { return (uint64_t)((s.m + bm - 1) / bm) * (uint64_t)((s.n + bn - 1) / bn); };
   // fp4 of up to 128 values: too short for strips; start and output of a 256 x 256 tile are most of it (us there and on 128 x 128: 256 x 128
   // 9.2, 5.5; 988 x 5056 14.8, 9.7; 381 x 15296 15.0, 10.4; of more than a round of the small ones 1504 x 10432 16.3, 18.4)
-  if (s.fp4 && s.pieces <= 1) return own_m == 256 && own_n == 256 && blocks(128, 128) <= 2 * (uint64_t)cus ? "128x128x64_w2x2" : nullptr;
+  if (fp4 && s.pieces <= 1) return own_m == 256 && own_n == 256 && blocks(128, 128) <= 2 * (uint64_t)cus ? "128x128x64_w2x2" : nullptr;
   if (s.pieces <= 4 && !tiled) return nullptr;   // two steps: nothing to share out
   if (!tiled && s.m > 64 && own_m == 256 && own_n == 256 && blocks(256, 256) * 4 >= (uint64_t)cus * 3) return nullptr;
   // (fp8 on 128 x 128: the direct pipeline below is always the cheaper one; only a name reaches flat128x128 there)
@@ -399,7 +410,7 @@ inline const char* choose_scaled(const ScaledShape& s, int own_m, int own_n, int
   for (const FlatStrip& k : kFlat) {
     const uint64_t b = blocks(k.bm, k.bn), waves = (b + cus - 1) / cus;
     if (s.pieces <= 4) break;
-    const double us = s.fp4 && waves > 1 ? rounds(b, cus, k.few, k.all, k.ends) : (double)waves * ((s.fp4 ? k.fp4 : k.fp8) * s.pieces / scaled_splits(b, s.pieces, cus) + 3.5);
+    const double us = fp4 && waves > 1 ? rounds(b, cus, k.few, k.all, k.ends) : (double)waves * ((fp4 ? k.fp4 : k.fp8) * s.pieces / scaled_splits(b, s.pieces, cus) + 3.5);
     if (us < best) best = us, name = k.name;
   }
   if (tiled) {
@@ -416,11 +427,11 @@ inline const char* choose_scaled(const ScaledShape& s, int own_m, int own_n, int
     if (us256 < best) best = us256, name = "256x256x64_q2x4";
     return name;
   }
-  if (!s.fp4) {
+  if (!fp4) {
     *lone = mx_plan(s.m, s.n, s.pieces, cus, partial_bytes);
     if (lone->splits && lone->us < best) best = lone->us, name = "128x128x128_e2x2";
   }
-  if (!s.fp4 && blocks(128, 128) > (uint64_t)cus) {   // two workgroups to a compute unit
+  if (!fp4 && blocks(128, 128) > (uint64_t)cus) {   // two workgroups to a compute unit
     const uint64_t b = blocks(128, 128), rest = b % (2 * (uint64_t)cus);
     const double us = (double)(b / (2 * (uint64_t)cus)) * (0.58 * s.pieces + 4) + (rest == 0 ? 0.0 : (rest <= (uint64_t)cus ? 0.31 : 0.58) * s.pieces + 4);
     if (us < best) best = us, name = "128x128x128_e2x2";

@@ -29,6 +29,7 @@ extern const unsigned char cutile_img_gemmgroup_start[], cutile_img_gemmgroup_en
 extern const unsigned char cutile_img_fmhakeys_start[], cutile_img_fmhakeys_end[];
 extern const unsigned char cutile_img_gemmtiles_start[], cutile_img_gemmtiles_end[];
 extern const unsigned char cutile_img_scaledflat_start[], cutile_img_scaledflat_end[];
+extern const unsigned char cutile_img_mxfp4_start[], cutile_img_mxfp4_end[];
 extern const unsigned char cutile_img_mxfp4flat_start[], cutile_img_mxfp4flat_end[];
 extern const unsigned char cutile_img_blockscale_start[], cutile_img_blockscale_end[];
 }
@@ -73,6 +74,7 @@ ImageRef image_ref(Image img) {
     case IMG_GEMM_TILES: return {cutile_img_gemmtiles_start, cutile_img_gemmtiles_end};
     case IMG_GEMM_SMALL: return {cutile_img_gemmsmall_start, cutile_img_gemmsmall_end};
     case IMG_SCALED_FLAT: return {cutile_img_scaledflat_start, cutile_img_scaledflat_end};
+    case IMG_MXFP4: return {cutile_img_mxfp4_start, cutile_img_mxfp4_end};
     case IMG_MXFP4_FLAT: return {cutile_img_mxfp4flat_start, cutile_img_mxfp4flat_end};
     case IMG_BLOCK_SCALE: return {cutile_img_blockscale_start, cutile_img_blockscale_end};
     default: return {nullptr, nullptr};
@@ -472,7 +474,13 @@ std::vector<KernelEntry> build_table() {
         add(mx8 ? "linear_tile" : "linear_tile_nvfp4", keep(v), keep((mx8 ? "linear_tile_entry__" : "linear_tile_nvfp4_entry__") + v), IMG_SCALED_FLAT, 512,
             (uint32_t)(std::max(stages, sums) + 4), 0, t[1], 0, t[0], dt, 0, 2);
       }
-  // the same strips on MXFP4 operands (mxfp4_flat.hip)
+  // ---- MXFP4 GEMM: LDS = 2 stages x (BM + BN) x (128 bytes of data + 16 of scales) ----
+  for (const char* out : {"bf16", "f32"})
+    for (int b : {256, 128}) {
+      const std::string v = std::string(out) + (b == 256 ? "_256x256x256_e4x2" : "_128x128x256_e2x2");
+      add("linear_tile_mxfp4", keep(v), keep("linear_tile_mxfp4_entry__" + v), IMG_MXFP4, b == 256 ? 512 : 256, (uint32_t)(2 * 2 * b * (128 + 16)), b, b, 256, 0, out, 0, 2);
+    }
+  // strips on MXFP4 operands (mxfp4_flat.hip)
   for (const char* dt : {"bf16", "f32"})
     for (auto t : {std::array<int, 4>{16, 64, 8, 16}, std::array<int, 4>{32, 64, 8, 32}, std::array<int, 4>{64, 64, 8, 64}, std::array<int, 4>{64, 128, 4, 64},
                    std::array<int, 4>{128, 128, 2, 64}}) {

@@ -417,7 +417,7 @@ cutile_status_t resolve_scaled(const char* function, const char* prefix, const N
   });
   *cus = 256;
   Name sized;
-  if (flat || (shape.fp4 && full_cover && shape.pieces <= 1)) {
+  if (flat || (shape.format == kScaledNvfp4 && full_cover && shape.pieces <= 1)) {
     if (cutile_status_t s = current_device_units(cus)) return s;
     const char* kernel = choose_scaled(shape, fit[0]->tile[0], fit[0]->tile[1], *cus, room->bytes, &room->lone);
     if (kernel && strcmp(kernel, "128x128x128_e2x2") == 0 && room->lone.splits > 1 && g_launch_mode != 2) {
@@ -3213,7 +3213,7 @@ cutile_status_t cutile_launch_linear_tile_mxfp8(cutile_stream_t stream, const cu
   Resolved res;
   int cus = 256;
   ScaledRoom room;
-  if (cutile_status_t s = resolve_scaled("linear_tile", "mxfp8_", dt, bm, bn, full_cover, full_cover, {M, N, K / 64, false}, opts, missing, stream, &cus, &room, &res)) return s;
+  if (cutile_status_t s = resolve_scaled("linear_tile", "mxfp8_", dt, bm, bn, full_cover, full_cover, {M, N, K / 64, kScaledMxfp8}, opts, missing, stream, &cus, &room, &res)) return s;
   return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, K / 64, cus, room);
 }
 
@@ -3275,7 +3275,7 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
   Resolved res;
   int cus = 256;
   ScaledRoom room;
-  if (cutile_status_t s = resolve_scaled("linear_tile_nvfp4", "", dt, bm, bn, full_cover, flat, {M, N, (KP + 63) / 64, true}, opts, missing, stream, &cus, &room, &res)) return s;
+  if (cutile_status_t s = resolve_scaled("linear_tile_nvfp4", "", dt, bm, bn, full_cover, flat, {M, N, (KP + 63) / 64, kScaledNvfp4}, opts, missing, stream, &cus, &room, &res)) return s;
   return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, (KP + 63) / 64, cus, room);
 }
 
@@ -3568,16 +3568,13 @@ cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cu
                  "linear_tile (mxfp4): precompiled variants address an operand with 32-bit byte offsets: x, y, the scales and z must each end below 2 GiB from their first "
                  "element (x spans %lld bytes, y %lld, z %lld)",
                  (long long)extent_bytes_2d(*x), (long long)extent_bytes_2d(*y), (long long)extent_bytes_2d(zt));
-  CUTILE_REQUIRE(full_cover, CUTILE_ERR_KERNEL_NOT_FOUND, "linear_tile (mxfp4): no precompiled variant covers a part of z");
   const Name dt = zt.dtype == CUTILE_DTYPE_F32 ? "f32" : "bf16";
-  Names acceptable;
-  for (const KernelEntry* e : kernels_of("linear_tile_mxfp4"))
-    if (dt == e->dtype) acceptable.push_back(e->variant);
+  auto missing = [&] { return std::string("no precompiled variant of mxfp4 linear_tile<") + num(bm).c_str() + ", " + num(bn).c_str() + "> -> " + dt.c_str(); };
   Resolved res;
   int cus = 256;
-  if (cutile_status_t s = current_device_units(&cus)) return s;
-  if (cutile_status_t s = resolve_entry("linear_tile_mxfp4", opts, dt + (M <= 16 ? "_flat16x64" : M <= 32 ? "_flat32x64" : "_flat64x128"), acceptable, &res)) return s;
-  return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, KP / 64, cus, ScaledRoom{});
+  ScaledRoom room;
+  if (cutile_status_t s = resolve_scaled("linear_tile_mxfp4", "", dt, bm, bn, full_cover, full_cover, {M, N, KP / 64, kScaledMxfp4}, opts, missing, stream, &cus, &room, &res)) return s;
+  return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, KP / 64, cus, room);
 }
 
 }  // extern "C"

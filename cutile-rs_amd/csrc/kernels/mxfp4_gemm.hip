@@ -40,7 +40,11 @@ struct Mxfp4Direct {
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && (BM + BN) % (64 * kWaves) == 0 && BM % 64 == 0, "tile must split evenly");
   static_assert(TN % 2 == 0 && TN >= 4 && TM >= 2, "two y fragment slots: an even number of y blocks keeps a block in its slot from tile to tile");
 
-  __device__ static __forceinline__ int lds_off(int r, int u) { return r * kRow + ((u ^ ((r >> 1) & 7)) << 4); }
+  // Slot s of row r holds the 16-byte unit at position s ^ (r / 2 % 8), positions counted first units of all lane groups first: a 16-byte LDS read
+  // takes lanes of two groups at a time, and only neighbouring positions keep their rows on distinct banks (units in their own order: half of
+  // the LDS cycles were conflicts).
+  __device__ static __forceinline__ int lds_off(int r, int position) { return r * kRow + ((position ^ ((r >> 1) & 7)) << 4); }
+  __device__ static __forceinline__ int unit_at(int position) { return (position & 3) * 2 + (position >> 2); }
 
   __device__ static void run(const PartitionArg<2>& z, const TensorArg<2>& x, const TensorArg<2>& y, const TensorArg<2>& xs, const TensorArg<2>& ys, float alpha,
                              const TileGrid& g) {
@@ -69,12 +73,12 @@ struct Mxfp4Direct {
     uint32_t a_goff[kAInstr], b_goff[kBInstr], s_goff[kSInstr];
 #pragma unroll
     for (int i = 0; i < kAInstr; ++i) {
-      const int r = (wave * kAInstr + i) * 8 + (lane >> 3), u = (lane & 7) ^ ((r >> 1) & 7);
+      const int r = (wave * kAInstr + i) * 8 + (lane >> 3), u = unit_at((lane & 7) ^ ((r >> 1) & 7));
       a_goff[i] = row0 + r < M ? (uint32_t)((int64_t)(row0 + r) * x.strides[0] + u * 16) : kOob;
     }
 #pragma unroll
     for (int i = 0; i < kBInstr; ++i) {
-      const int r = (wave * kBInstr + i) * 8 + (lane >> 3), u = (lane & 7) ^ ((r >> 1) & 7);
+      const int r = (wave * kBInstr + i) * 8 + (lane >> 3), u = unit_at((lane & 7) ^ ((r >> 1) & 7));
       b_goff[i] = col0 + r < N ? (uint32_t)((int64_t)(col0 + r) * y.strides[0] + u * 16) : kOob;
     }
 #pragma unroll
@@ -99,8 +103,8 @@ struct Mxfp4Direct {
       }
     };
     // LDS side: the lane's two 16-byte units of its row and its two scale bytes.
-    const int a_lo = lds_off(wm * WM + l16, 2 * grp), a_hi = lds_off(wm * WM + l16, 2 * grp + 1);   // + tm * 16 rows
-    const int b_lo = lds_off(wn * WN + l16, 2 * grp), b_hi = lds_off(wn * WN + l16, 2 * grp + 1);   // + tn * 16 rows
+    const int a_lo = lds_off(wm * WM + l16, grp), a_hi = lds_off(wm * WM + l16, 4 + grp);   // + tm * 16 rows
+    const int b_lo = lds_off(wn * WN + l16, grp), b_hi = lds_off(wn * WN + l16, 4 + grp);   // + tn * 16 rows
     const int sa_addr = (wm * WM + l16) * 16 + 2 * grp;                                             // + tm * 16 rows, + 8 * (tile % 2)
     const int sb_addr = (BM + wn * WN + l16) * 16 + 2 * grp;                                        // + tn * 16 rows
     struct Frag {

@@ -377,6 +377,12 @@ struct FlatStrip {
 };
 constexpr FlatStrip kFlat[] = {{"flat16x64", 16, 64, 0.09, 0.20, 0.20, 0.20, 5.5}, {"flat32x64", 32, 64, 0.12, 0.28, 0.28, 0.28, 5.5}, {"flat64x64", 64, 64, 0.155, 0.36, 0.294, 0.297, 4.5},
                                {"flat64x128", 64, 128, 0.27, 0.62, 0.534, 0.561, 4.8}, {"flat128x128", 128, 128, 0.52, 1.12, 1.053, 1.08, 5.4}};
+// The 128 x 128 kernel whose launches of a compute unit to each tile take another member, and may share K; "-" if there is none.
+inline const char* lone_tile(ScaledKind format) { return format == kScaledMxfp8 ? "128x128x128_e2x2" : format == kScaledMxfp4 ? "128x128x256_e2x2" : "-"; }
+inline MxPlan mxfp4_plan(int64_t m, int64_t n, int32_t pieces, int cus, uint64_t partial_bytes) {
+  const uint64_t t = tiles_of(m, n, 128, 128);
+  return MxPlan{t <= (uint64_t)cus ? 1u : 0u, 1.0};
+}
 // MXFP4 (mxfp4_gemm.hip, mxfp4_flat.hip), by name: strips for up to 64 rows, 256 x 256 tiles where they are half as many as compute units or more,
 // 128 x 128 in between.  us on each: 16 x 14336 x 4096 strips of 16 rows 9.1, 128 x 128 14.3; 64 x 14336 x 4096 strips of 64 rows 11.1, 15.4; 200 x 14336 x 4096
 // 128 x 128 16.7, 256 x 256 29; 1000 x 4096 x 4096 17.6, 30; 2048 x 14336 x 4096 89, 79; 4096 x 4096 x 4096 46, 39.

@@ -480,6 +480,11 @@ std::vector<KernelEntry> build_table() {
       const std::string v = std::string(out) + (b == 256 ? "_256x256x256_e4x2" : "_128x128x256_e2x2");
       add("linear_tile_mxfp4", keep(v), keep("linear_tile_mxfp4_entry__" + v), IMG_MXFP4, b == 256 ? 512 : 256, (uint32_t)(2 * 2 * b * (128 + 16)), b, b, 256, 0, out, 0, 2);
     }
+  // the member of 128 x 128 for tiles that have a compute unit each: two groups of four wavefronts, four stages, two buffers for the scales of four K tiles
+  for (const char* out : {"bf16", "f32"}) {
+    const std::string v = std::string(out) + "_128x128x256_e2x2";
+    add("linear_tile_mxfp4", keep(v + "+lone"), keep("linear_tile_mxfp4_entry__" + v + "_lone"), IMG_MXFP4, 512, 4 * 256 * 128 + 2 * 256 * 32, 128, 128, 256, 0, out, 0, 2);
+  }
   // strips on MXFP4 operands (mxfp4_flat.hip)
   for (const char* dt : {"bf16", "f32"})
     for (auto t : {std::array<int, 4>{16, 64, 8, 16}, std::array<int, 4>{32, 64, 8, 32}, std::array<int, 4>{64, 64, 8, 64}, std::array<int, 4>{64, 128, 4, 64},

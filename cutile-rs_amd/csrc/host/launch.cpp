@@ -402,7 +402,7 @@ cutile_status_t resolve_scaled(const char* function, const char* prefix, const N
                                ScaledRoom* room, Resolved* res) {
   Few<const KernelEntry*, 12> fit, others;
   for (const KernelEntry* e : kernels_of(function)) {
-    if (e->image == IMG_MX_TILES || dt != e->dtype) continue;   // (members, which only launch_scaled names)
+    if (strchr(e->variant, '+') || dt != e->dtype) continue;   // (members, which only launch_scaled names)
     if (is_scaled_flat(e)) {
       if (flat) others.push_back(e);
     } else if ((e->tile[0] == bm && e->tile[1] == bn) || (full_cover && e->tile[0] % bm == 0 && e->tile[1] % bn == 0)) {
@@ -420,12 +420,12 @@ cutile_status_t resolve_scaled(const char* function, const char* prefix, const N
   if (flat || (shape.format == kScaledNvfp4 && full_cover && shape.pieces <= 1)) {
     if (cutile_status_t s = current_device_units(cus)) return s;
     const char* kernel = choose_scaled(shape, fit[0]->tile[0], fit[0]->tile[1], *cus, room->bytes, &room->lone);
-    if (kernel && strcmp(kernel, "128x128x128_e2x2") == 0 && room->lone.splits > 1 && g_launch_mode != 2) {
+    if (kernel && strcmp(kernel, lone_tile(shape.format)) == 0 && room->lone.splits > 1 && g_launch_mode != 2) {
       // a captured launch has no workspace and takes the best kernel of those that need none: their code object is loaded here
       cutile_device_t device = nullptr;
       hipFunction_t fn;
       if (cutile_status_t s = current_device(&device)) return s;
-      if (cutile_status_t s = load_entry(device, find_entry(function, "mxfp8_bf16_flat64x64"), &fn)) return s;
+      if (cutile_status_t s = load_entry(device, find_entry(function, shape.format == kScaledMxfp4 ? "bf16_flat64x64" : "mxfp8_bf16_flat64x64"), &fn)) return s;
       if (g_launch_mode == 0) {
         room->ws = split_workspace(device, (hipStream_t)stream);
         if (!room->ws.partials) kernel = choose_scaled(shape, fit[0]->tile[0], fit[0]->tile[1], *cus, room->bytes = 0, &room->lone);
@@ -492,9 +492,11 @@ cutile_status_t launch_scaled(Resolved& res, cutile_stream_t stream, const cutil
   }
   args.push_tile_grid(kg);
   uint32_t grid[3] = {kg[0] * kg[1], 1, 1};
-  if (strstr(res.entry->variant, "_128x128x128_e2x2") != nullptr && grid[0] <= (uint32_t)cus && pieces >= 4) {   // a compute unit to each tile
-    uint32_t splits = room.lone.splits ? room.lone.splits
-                                       : mx_plan(zt.shape[0], zt.shape[1], pieces, cus, kg[0] == div_up(zt.shape[0], 128) && kg[1] == div_up(zt.shape[1], 128) ? room.bytes : 0).splits;
+  const ScaledKind format = x->dtype == CUTILE_DTYPE_F8E4M3FN ? kScaledMxfp8 : xs->dtype == CUTILE_DTYPE_F8E8M0FNU ? kScaledMxfp4 : kScaledNvfp4;
+  if (strstr(res.entry->variant, lone_tile(format)) != nullptr && grid[0] <= (uint32_t)cus && pieces >= 4) {   // a compute unit to each tile
+    const uint64_t bytes = kg[0] == div_up(zt.shape[0], 128) && kg[1] == div_up(zt.shape[1], 128) ? room.bytes : 0;
+    uint32_t splits = room.lone.splits ? room.lone.splits : (format == kScaledMxfp4 ? mxfp4_plan : mx_plan)(zt.shape[0], zt.shape[1], pieces, cus, bytes).splits;
+    if (getenv("MX4_SPLITS")) splits = atoi(getenv("MX4_SPLITS"));
     if (splits > 1 && g_launch_mode == 0 && !room.ws.partials) {   // a kernel that the caller or a record names
       room.ws = split_workspace(res.device, (hipStream_t)stream);
       if (!room.ws.partials) splits = 1;

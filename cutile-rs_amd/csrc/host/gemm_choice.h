@@ -377,26 +377,64 @@ struct FlatStrip {
 };
 constexpr FlatStrip kFlat[] = {{"flat16x64", 16, 64, 0.09, 0.20, 0.20, 0.20, 5.5}, {"flat32x64", 32, 64, 0.12, 0.28, 0.28, 0.28, 5.5}, {"flat64x64", 64, 64, 0.155, 0.36, 0.294, 0.297, 4.5},
                                {"flat64x128", 64, 128, 0.27, 0.62, 0.534, 0.561, 4.8}, {"flat128x128", 128, 128, 0.52, 1.12, 1.053, 1.08, 5.4}};
+constexpr int kLonePieces = 4;   // the shortest rows that these kernels take
 // The 128 x 128 kernel whose launches of a compute unit to each tile take another member, and may share K; "-" if there is none.
 inline const char* lone_tile(ScaledKind format) { return format == kScaledMxfp8 ? "128x128x128_e2x2" : format == kScaledMxfp4 ? "128x128x256_e2x2" : "-"; }
+// MXFP4 on 128 x 128 tiles that have a compute unit each (mxfp4_gemm.hip), as mx_plan: K tiles of 256 values, two and more for each workgroup that shares them.
+// 321 x 2824 x 6784 in 1, 2, 3 parts 20.0, 17.0, 17.6 us; 512 x 4096 x 14336 30.4, 26.3 in 1, 2; 512 x 4096 x 4096 12.3, 17.0.
 inline MxPlan mxfp4_plan(int64_t m, int64_t n, int32_t pieces, int cus, uint64_t partial_bytes) {
   const uint64_t t = tiles_of(m, n, 128, 128);
-  return MxPlan{t <= (uint64_t)cus ? 1u : 0u, 1.0};
+  const int64_t kt = (pieces + 1) / 2;
+  MxPlan best{0, 1e30};
+  for (uint32_t s : {1u, 2u, 3u, 4u, 6u, 8u}) {
+    const uint64_t g = t * s;
+    if (g > (uint64_t)cus || (s > 1 && (kt < 2 * s || g * 128 * 128 * 4 > partial_bytes))) break;
+    const double us = (double)((kt + s - 1) / s) * (0.266 + 0.421 * (double)g / cus) + 4.7 + (s > 1 ? 1.2 * s + 0.0126 * (double)g - 0.4 : 0.0);
+    if (us < best.us * 0.98) best = {s, us};
+  }
+  return best;
 }
-// MXFP4 (mxfp4_gemm.hip, mxfp4_flat.hip), by name: strips for up to 64 rows, 256 x 256 tiles where they are half as many as compute units or more,
-// 128 x 128 in between.  us on each: 16 x 14336 x 4096 strips of 16 rows 9.1, 128 x 128 14.3; 64 x 14336 x 4096 strips of 64 rows 11.1, 15.4; 200 x 14336 x 4096
-// 128 x 128 16.7, 256 x 256 29; 1000 x 4096 x 4096 17.6, 30; 2048 x 14336 x 4096 89, 79; 4096 x 4096 x 4096 46, 39.
-inline const char* choose_mxfp4(const ScaledShape& s, int own_m, int own_n, int cus) {
-  auto blocks = [&](int64_t b) { return (uint64_t)((s.m + b - 1) / b) * (uint64_t)((s.n + b - 1) / b); };
-  if (s.m <= 64) return s.m <= 16 ? "flat16x64" : s.m <= 32 ? "flat32x64" : "flat64x64";
-  return own_m == 256 && own_n == 256 && blocks(256) * 2 >= (uint64_t)cus ? "256x256x256_e4x2" : "128x128x256_e2x2";
+// MXFP4 strips (mxfp4_flat.hip), us: a piece of K where few and where all compute units have a workgroup, start and output of a round, of a launch in
+// several rounds, and of each part where K is shared.
+struct Mxfp4Strip {
+  const char* name;
+  int bm, bn;
+  double few, all, ends, rounds, part;
+};
+constexpr Mxfp4Strip kMxfp4Strips[] = {{"flat16x64", 16, 64, 0.071, 0.134, 1.8, 2.9, 1.07}, {"flat32x64", 32, 64, 0.086, 0.148, 3.1, 2.0, 0.92}, {"flat64x64", 64, 64, 0.087, 0.177, 4.1, 0.8, 0.77}};
+// MXFP4 by name.  Strips, 128 x 128 tiles with a compute unit each, two such tiles to a compute unit, or 256 x 256 tiles: the one priced lowest.  Least squares over
+// 220 products of 1 to 8192 rows and 512 to 16384 values of K, operands from memory, every kernel timed (strips 7 % rms, tiles 7 to 8): it takes 1.008 of the best one's
+// time, and 1.19 at most.  us, bf16 out, on the best strips, on 128 x 128 and on 256 x 256: 1 x 14336 x 4096 8.5, 12.3, 28; 64 x 14336 x 4096 11.1, 11.8, 28;
+// 200 x 14336 x 4096 31.8, 13.7, 29; 1000 x 4096 x 4096 22.7, 16.0, 30; 2048 x 14336 x 4096 -, 84, 73; 3661 x 6240 x 6016 -, 105, 99; 4096 x 4096 x 4096 -, 46, 38.
+inline const char* choose_mxfp4(const ScaledShape& s, int cus, uint64_t partial_bytes, MxPlan* lone) {
+  const char* name = nullptr;
+  double best = 1e30;
+  auto offer = [&](const char* kernel, double us) {
+    if (us < best) best = us, name = kernel;
+  };
+  for (const Mxfp4Strip& k : kMxfp4Strips) {
+    const uint64_t b = tiles_of(s.m, s.n, k.bm, k.bn), rest = b % (uint64_t)cus;
+    const uint32_t splits = scaled_launch_splits(b, s.pieces, cus, false, k.bm, k.bn);
+    auto piece = [&](uint64_t busy) { return (k.few + (k.all - k.few) * std::min(1.0, (double)busy / cus)) * s.pieces; };
+    offer(k.name, splits > 1 ? piece(b * splits) / splits + k.ends + k.part * splits
+                             : k.rounds + (double)(b / (uint64_t)cus) * (piece((uint64_t)cus) + k.ends) + (rest ? piece(rest) + k.ends : 0.0));
+  }
+  const uint64_t small = tiles_of(s.m, s.n, 128, 128), large = tiles_of(s.m, s.n, 256, 256), pairs = small % (2 * (uint64_t)cus), last = large % (uint64_t)cus;
+  *lone = s.pieces >= kLonePieces ? mxfp4_plan(s.m, s.n, s.pieces, cus, partial_bytes) : MxPlan{0, 0.0};
+  if (lone->splits) {
+    offer("128x128x256_e2x2", lone->us);
+  } else {
+    offer("128x128x256_e2x2", 1.0 + (double)(small / (2 * (uint64_t)cus)) * (0.592 * s.pieces + 4.4) + (pairs ? (pairs <= (uint64_t)cus ? 0.334 : 0.592) * s.pieces + 4.4 : 0.0));
+  }
+  offer("256x256x256_e4x2", (double)(large / (uint64_t)cus) * (0.971 * s.pieces + 8.0) + (last ? (0.661 + 0.31 * (double)last / cus) * s.pieces + 8.0 : 0.0));
+  return name;
 }
 // The kernel by name, or nullptr: the partition's own (tuning record, then the table's order).  us per 64-byte piece of K for
 // one block on each compute unit, measured at K = 4096 (mxfp8: 16 x 4096 9.4 us, 64 x 4096 13.4, 512 x 4096 21 on 64 x 128 blocks, 24 with
 // 128 x 128 tiles; nvfp4: 9.9, 14.7, 24).  The 256 x 256 kernels are the better ones where their tiles come near to filling the chip.
-// `lone`: what mx_plan says for fp8, where it was asked.
+// `lone`: what the plan of a compute unit to each tile says (fp8 and MXFP4), where it was asked.
 inline const char* choose_scaled(const ScaledShape& s, int own_m, int own_n, int cus, uint64_t partial_bytes, MxPlan* lone) {
-  if (s.format == kScaledMxfp4) return choose_mxfp4(s, own_m, own_n, cus);
+  if (s.format == kScaledMxfp4) return choose_mxfp4(s, cus, partial_bytes, lone);
   const bool fp4 = s.format == kScaledNvfp4;
   // a partition whose output other tiles of nvfp4_gemm.hip may compute too
   const bool tiled = fp4 && own_m == own_n && (own_m == 128 || (own_m == 256 && s.pieces > 4));

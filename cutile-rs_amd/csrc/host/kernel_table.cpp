@@ -487,8 +487,7 @@ std::vector<KernelEntry> build_table() {
   }
   // strips on MXFP4 operands (mxfp4_flat.hip)
   for (const char* dt : {"bf16", "f32"})
-    for (auto t : {std::array<int, 4>{16, 64, 8, 16}, std::array<int, 4>{32, 64, 8, 32}, std::array<int, 4>{64, 64, 8, 64}, std::array<int, 4>{64, 128, 4, 64},
-                   std::array<int, 4>{128, 128, 2, 64}}) {
+    for (auto t : {std::array<int, 4>{16, 64, 8, 16}, std::array<int, 4>{32, 64, 8, 32}, std::array<int, 4>{64, 64, 8, 64}}) {
       const std::string v = std::string(dt) + "_flat" + std::to_string(t[0]) + "x" + std::to_string(t[1]);
       const int stages = 8 * ((64 + t[3]) * (128 + 8) + 32), sums = t[2] * t[0] * (t[1] + 4) * 4;
       add("linear_tile_mxfp4", keep(v), keep("linear_tile_mxfp4_entry__" + v), IMG_MXFP4_FLAT, 512, (uint32_t)(std::max(stages, sums) + 4), 0, t[1], 0, t[0], dt, 0, 2);

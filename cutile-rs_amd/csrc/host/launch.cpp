@@ -493,10 +493,9 @@ cutile_status_t launch_scaled(Resolved& res, cutile_stream_t stream, const cutil
   args.push_tile_grid(kg);
   uint32_t grid[3] = {kg[0] * kg[1], 1, 1};
   const ScaledKind format = x->dtype == CUTILE_DTYPE_F8E4M3FN ? kScaledMxfp8 : xs->dtype == CUTILE_DTYPE_F8E8M0FNU ? kScaledMxfp4 : kScaledNvfp4;
-  if (strstr(res.entry->variant, lone_tile(format)) != nullptr && grid[0] <= (uint32_t)cus && pieces >= 4) {   // a compute unit to each tile
+  if (strstr(res.entry->variant, lone_tile(format)) != nullptr && grid[0] <= (uint32_t)cus && pieces >= kLonePieces) {   // a compute unit to each tile
     const uint64_t bytes = kg[0] == div_up(zt.shape[0], 128) && kg[1] == div_up(zt.shape[1], 128) ? room.bytes : 0;
     uint32_t splits = room.lone.splits ? room.lone.splits : (format == kScaledMxfp4 ? mxfp4_plan : mx_plan)(zt.shape[0], zt.shape[1], pieces, cus, bytes).splits;
-    if (getenv("MX4_SPLITS")) splits = atoi(getenv("MX4_SPLITS"));
     if (splits > 1 && g_launch_mode == 0 && !room.ws.partials) {   // a kernel that the caller or a record names
       room.ws = split_workspace(res.device, (hipStream_t)stream);
       if (!room.ws.partials) splits = 1;

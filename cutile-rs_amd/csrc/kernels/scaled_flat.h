@@ -292,9 +292,11 @@ struct ScaledFlat {
                       uint32_t* counters, uint32_t tiles_m, uint32_t tiles_n, uint32_t splits) {                                      \
     ScaledFlat<FMT, OUT_T, MB, NB, WM, WN, WK, AHEAD>::run(z, x, y, xs, ys, alpha, partials, counters, tiles_m, tiles_n, splits);      \
   }
-#define SCALED_FLAT_FAMILY(ENTRY, PREFIX, FMT, OUT_T, AHEAD16, AHEAD32, AHEAD64)       \
+#define SCALED_FLAT_STRIPS(ENTRY, PREFIX, FMT, OUT_T, AHEAD16, AHEAD32, AHEAD64)       \
   SCALED_FLAT_KERNEL(ENTRY, PREFIX##_flat16x64, FMT, OUT_T, 1, 4, 1, 1, 8, AHEAD16)    \
   SCALED_FLAT_KERNEL(ENTRY, PREFIX##_flat32x64, FMT, OUT_T, 2, 4, 1, 1, 8, AHEAD32)    \
-  SCALED_FLAT_KERNEL(ENTRY, PREFIX##_flat64x64, FMT, OUT_T, 4, 4, 1, 1, 8, AHEAD64)    \
+  SCALED_FLAT_KERNEL(ENTRY, PREFIX##_flat64x64, FMT, OUT_T, 4, 4, 1, 1, 8, AHEAD64)
+#define SCALED_FLAT_FAMILY(ENTRY, PREFIX, FMT, OUT_T, AHEAD16, AHEAD32, AHEAD64)       \
+  SCALED_FLAT_STRIPS(ENTRY, PREFIX, FMT, OUT_T, AHEAD16, AHEAD32, AHEAD64)             \
   SCALED_FLAT_KERNEL(ENTRY, PREFIX##_flat64x128, FMT, OUT_T, 4, 4, 1, 2, 4, AHEAD64)   \
   SCALED_FLAT_KERNEL(ENTRY, PREFIX##_flat128x128, FMT, OUT_T, 4, 4, 2, 2, 2, AHEAD64)

@@ -3336,6 +3336,15 @@ cutile_status_t rows_of(const char* fn, const cutile_partition_arg_t* const* par
   return CUTILE_SUCCESS;
 }
 
+// No two elements of a [rows, columns] output share memory, as far as its strides tell.
+cutile_status_t check_apart(const char* fn, const char* name, const cutile_tensor_arg_t& t) {
+  const int inner = t.shape[0] == 1 || (t.shape[1] != 1 && t.strides[1] <= t.strides[0]) ? 1 : 0, outer = 1 - inner;
+  const int64_t span = t.shape[inner] == 1 ? 1 : (int64_t)(t.shape[inner] - 1) * t.strides[inner] + 1;
+  CUTILE_REQUIRE((t.shape[inner] == 1 || t.strides[inner] > 0) && (t.shape[outer] == 1 || t.strides[outer] >= span), CUTILE_ERR_KERNEL_NOT_FOUND,
+                 "%s: elements of %s overlap (shape [%d, %d], strides [%lld, %lld])", fn, name, t.shape[0], t.shape[1], (long long)t.strides[0], (long long)t.strides[1]);
+  return CUTILE_SUCCESS;
+}
+
 bool is_16bit_float(cutile_dtype_t dt) { return dt == CUTILE_DTYPE_F16 || dt == CUTILE_DTYPE_BF16; }
 
 // Rows of a launch as the kernels count them: units of 8 values.  `plain`: inner strides of 1, which the "rows" kernels need, and few
@@ -3345,6 +3354,7 @@ struct UnitRows {
   bool plain;
 };
 constexpr int64_t kMostUnits = (1ll << 31) - 4096;
+constexpr int64_t kMostBlocks = (1 << 24) - 1;   // workgroups of 256 that one dispatch holds
 UnitRows unit_rows(int64_t rows, int64_t units, int64_t n, bool unit_stride, bool one) {
   UnitRows u{rows, units, n, unit_stride && rows * units <= kMostUnits};
   if (u.plain && one) u = {1, rows * units, rows * n, true};
@@ -3366,7 +3376,7 @@ cutile_status_t launch_units(Resolved& res, cutile_stream_t stream, ArgPacker& a
   } else {
     args.push_val<int64_t>(rows);
     args.push_val<int32_t>((int32_t)units);
-    grid[0] = (uint32_t)std::min<int64_t>((rows * units + 255) / 256, 1 << 24);
+    grid[0] = (uint32_t)std::min<int64_t>((rows * units + 255) / 256, kMostBlocks);
   }
   return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
@@ -3446,13 +3456,20 @@ cutile_status_t launch_norm_quantize(const char* fn, cutile_stream_t stream, con
   if (cutile_status_t s = check_generic(opts, 0, num(n), "N")) return s;
   TensorScale t;
   if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
+  if (residual)
+    if (cutile_status_t s = check_apart(fn, "residual_out", residual_out->tensor)) return s;
   const cutile_partition_arg_t* parts[3] = {out, scales, residual_out};
   if (cutile_status_t s = rows_of(fn, parts, residual ? 3 : 2, opts, &rows)) return s;
   const Name base = Name(f.name) + "_" + cutile_dtype_name(x->dtype) + "_";
+  // tile[3] wavefronts to a row, four of them or more to a workgroup; 0: a workgroup to a row, strided over what is beyond the grid
+  auto blocks_of = [&](const KernelEntry* e) {
+    const int wpr = e->tile[3];
+    return wpr ? (uint64_t)div_up((uint64_t)rows, wpr < 4 ? 4 / wpr : 1) : (uint64_t)std::min(rows, kMostBlocks);
+  };
   Names fitting;
   if (unit_inner(*x) && unit_inner(*w) && (!residual || (unit_inner(*residual) && unit_inner(residual_out->tensor))))
     for (const KernelEntry* e : kernels_of(fn))
-      if (e->capacity >= k && strncmp(e->variant, base.c_str(), base.size()) == 0) fitting.push_back(e->variant);
+      if (e->capacity >= k && strncmp(e->variant, base.c_str(), base.size()) == 0 && blocks_of(e) * e->block[0] <= 0xffffffffull) fitting.push_back(e->variant);
   fitting.push_back(base + "any");
   Resolved res;
   if (cutile_status_t s = resolve_entry(fn, opts, fitting[0], fitting, &res)) return s;
@@ -3467,8 +3484,7 @@ cutile_status_t launch_norm_quantize(const char* fn, cutile_stream_t stream, con
   args.push_val<TensorScale>(t);
   args.push_val<int64_t>(rows);
   args.push_val<int32_t>((int32_t)(k / 8));
-  const int wpr = res.entry->tile[3];   // 0: a workgroup to a row, strided over what is beyond the grid
-  const uint32_t grid[3] = {wpr ? div_up((uint64_t)rows, wpr < 4 ? 4 / wpr : 1) : (uint32_t)std::min<int64_t>(rows, 1 << 24), 1, 1};
+  const uint32_t grid[3] = {(uint32_t)blocks_of(res.entry), 1, 1};
   return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
 
@@ -3513,6 +3529,7 @@ cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cut
   if (cutile_status_t s = check_generic(opts, 0, num(ot.shape[1]), "N")) return s;
   TensorScale t;
   if (cutile_status_t s = tensor_scale_of(fn, f, tensor_scale, &t)) return s;
+  if (cutile_status_t s = check_apart(fn, "out", ot)) return s;
   const cutile_partition_arg_t* parts[1] = {out};
   if (cutile_status_t s = rows_of(fn, parts, 1, opts, &rows)) return s;
   const int64_t units = div_up(ot.shape[1], 8);
@@ -3569,6 +3586,7 @@ cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cu
                  "linear_tile (mxfp4): precompiled variants address an operand with 32-bit byte offsets: x, y, the scales and z must each end below 2 GiB from their first "
                  "element (x spans %lld bytes, y %lld, z %lld)",
                  (long long)extent_bytes_2d(*x), (long long)extent_bytes_2d(*y), (long long)extent_bytes_2d(zt));
+  if (cutile_status_t s = check_apart("linear_tile (mxfp4)", "z", zt)) return s;
   const Name dt = zt.dtype == CUTILE_DTYPE_F32 ? "f32" : "bf16";
   auto missing = [&] { return std::string("no precompiled variant of mxfp4 linear_tile<") + num(bm).c_str() + ", " + num(bn).c_str() + "> -> " + dt.c_str(); };
   Resolved res;

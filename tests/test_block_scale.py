@@ -73,6 +73,8 @@ def test_refusals(fake_hip):
         (lambda: norm(r=x[:, :32]), "must be shared by all tensors"),
         (lambda: norm(ro=x[:2]), "same rows"),
         (lambda: norm(ro=x.float()), "all be f16 or all bf16"),
+        (lambda: norm(ro=x[:1].expand(4, 64)), "elements of residual_out overlap"),
+        (lambda: norm(ro=x[:, :1].expand(4, 64)), "elements of residual_out overlap"),
         (lambda: norm(variant="none"), "does not fit these arguments"),
         (lambda: ct.rms_norm_quantize(x.float(), w.float(), whole(ct, data), whole(ct, scales), 1e-6, "mxfp8"), "all be f16 or all bf16"),
         (lambda: silu(u=x[:, :32]), "up has another shape"),
@@ -81,6 +83,8 @@ def test_refusals(fake_hip):
         (lambda: deq(o=torch.zeros(4, 65, dtype=torch.half)), "x holds 4 rows of 64 values"),
         (lambda: deq(o=torch.zeros(5, 64, dtype=torch.half)), "x holds 4 rows of 64 values"),
         (lambda: deq(o=torch.zeros(4, 64, dtype=torch.double)), "out must be f16, bf16 or f32"),
+        (lambda: deq(o=x[:1].expand(4, 64)), "elements of out overlap"),
+        (lambda: deq(o=x.flatten()[:130].as_strided((4, 64), (20, 1))), "elements of out overlap"),
         (lambda: deq(s=wide), "whole blocks of 32 and scales"),
         (lambda: deq(data, scales, x, "mxfp4", 3.0), "whole blocks of 32 and scales"),
     ]
@@ -135,6 +139,23 @@ def test_launch_modes_and_coverage(fake_hip):
     finally:
         ct.check(ct.lib().cutile_set_launch_mode(0))
     assert ct.lib().cutile_testing_launch_count() == n0
+
+
+def test_rows_beyond_one_dispatch(fake_hip):
+    """fewer than 2^32 lanes make a grid: what has more rows goes to the kernels that stride over them"""
+    from test_host_abi import _last
+
+    ct = fake_hip
+    rows = (1 << 26) + 5
+    data, scales = torch.empty(rows, 16, dtype=torch.uint8), torch.empty(rows, 1, dtype=torch.uint8)      # (never touched)
+    x, w = torch.empty(1, 32, dtype=torch.half).expand(rows, 32), torch.empty(32, dtype=torch.half)
+    ct.rms_norm_quantize(x, w, whole(ct, data), whole(ct, scales), 1e-6, "mxfp4")
+    rec, _ = _last(ct)
+    assert rec.symbol.decode().endswith("mxfp4_f16_any") and rec.grid[0] * rec.block[0] < 1 << 32
+    ct.rms_norm_quantize(x[:-5], w, whole(ct, data[:-5]), whole(ct, scales[:-5]), 1e-6, "mxfp4")
+    assert _last(ct)[0].symbol.decode().endswith("mxfp4_f16_any")
+    ct.rms_norm_quantize(x[:-9], w, whole(ct, data[:-9]), whole(ct, scales[:-9]), 1e-6, "mxfp4")
+    assert _last(ct)[0].symbol.decode().endswith("mxfp4_f16_w1v1")
 
 
 # ---- quantisation ----------------------------------------------------------------------------------------------------------
@@ -403,3 +424,83 @@ def test_gpu_silu_mul_far_gates(ct, dev):
     want = x / (1 + torch.exp(-x)) * up.double()
     assert [int(i) for i in torch.nonzero(~torch.isfinite(want[0]))] == [517, 647, 706]
     ref.assert_quantised(data, scales, want, "mxfp8", slack=6 * 2.0 ** -24, tiny=2.0 ** -126)
+
+
+# ---- every kernel by its name, where the size rule would take another ---------------------------------------------------------
+def variants_of(ct, function, prefix):
+    return [v.split(":")[1] for v in ct.kernel_list() if v.startswith(function + ":" + prefix)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 257, 1024])
+def test_gpu_norm_by_name(ct, dev, fmt, dtype, n):
+    x, r, w = normal((13, n), n, dev, TYPES[dtype]), normal((13, n), n + 1, dev, TYPES[dtype]), normal((n,), n + 2, dev, TYPES[dtype])
+    for function in ("rms_norm_quantize", "add_rms_norm_quantize"):
+        names = variants_of(ct, function, fmt + "_" + dtype + "_")
+        assert len(names) == 8
+        c = x.double() + r.double() if function[0] == "a" else x.double()
+        want = c / torch.sqrt(c.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+        g = g_of(want, fmt)
+        for variant in names:
+            if variant.endswith("w1v1") and n > 512:                      # holds 512 values
+                continue
+            data, scales = ref.buffers(13, ref.padded(n, fmt), fmt, dev)
+            ro = torch.full_like(x, 7.0)
+            args = (whole(ct, data), whole(ct, scales))
+            if function[0] == "a":
+                ct.add_rms_norm_quantize(r, x, w, *args, whole(ct, ro), 1e-6, fmt, g, variant=variant)
+                assert torch.equal(ro, (x.float() + r.float()).to(x.dtype)), variant
+            else:
+                ct.rms_norm_quantize(x, w, *args, 1e-6, fmt, g, variant=variant)
+            ref.assert_quantised(data, scales, want, fmt, torch.tensor(g, dtype=torch.float32).double().item(), slack=norm_slack(n) + 2 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gpu_units_by_name(ct, dev, fmt, dtype):
+    """the three ways through a matrix give the same bytes, and the two ways back the same values"""
+    base = normal((333, 417), 17, dev, TYPES[dtype])
+    plain, column = base, base.t().contiguous().t()
+    g = g_of(base, fmt)
+    prefix = fmt + "_" + dtype + "_"
+    results = [quantised(ct, x, fmt, None, g, variant=prefix + kind) for x, kind in ((plain, "rows"), (plain, "any"), (column, "columns"), (column, "any"), (column[:, :417], "columns"))]
+    for data, scales in results[1:]:
+        assert torch.equal(data, results[0][0]) and torch.equal(scales, results[0][1])
+    ref.assert_quantised(*results[0], base.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+    outs = [torch.full_like(base, 7.0) for _ in range(2)]
+    for out, kind in zip(outs, ("rows", "any")):
+        ct.block_dequantize(*results[0], whole(ct, out), fmt, g, variant=prefix + kind)
+    assert torch.equal(outs[0], outs[1]) and bool(torch.isfinite(outs[0]).all())
+    if dtype != "f32":
+        up = normal(base.shape, 18, dev, base.dtype)
+        got = []
+        for kind in ("rows", "any"):
+            data, scales = ref.buffers(333, ref.padded(417, fmt), fmt, dev)
+            ct.silu_mul_quantize(base, up, whole(ct, data), whole(ct, scales), fmt, g, variant=prefix + kind)
+            got.append((data, scales))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("image,entries", [("blockscale", 153), ("mxfp4", 6), ("mxfp4flat", 6)])
+def test_lds_bytes_and_registers(fake_hip, image, entries):
+    """LDS of the code objects is what the table says; no kernel of block-scaled rows spills"""
+    import os
+    import re
+    import subprocess
+
+    ct = fake_hip
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    notes = subprocess.run(["/opt/rocm/llvm/bin/llvm-readelf", "--notes", os.path.join(root, "cutile-rs_amd", "lib", image + ".hsaco")],
+                           stdout=subprocess.PIPE, text=True, check=True).stdout
+    kernels = notes.split("- .agpr_count")[1:]
+    assert len(kernels) == entries
+    by_symbol = {}
+    for kernel in kernels:
+        symbol = re.search(r"\n    \.name: +(\S+)", kernel)[1]
+        function, variant = symbol.split("_entry__")
+        lds = int(re.search(r"\.group_segment_fixed_size: (\d+)", kernel)[1])
+        assert ct.kernel_lookup(function, variant=variant.replace("_lone", "+lone")).lds_bytes == lds, symbol
+        assert image != "blockscale" or int(re.search(r"\.vgpr_spill_count: (\d+)", kernel)[1]) == 0, symbol

@@ -61,6 +61,7 @@ def test_refusals(fake_hip):
         (lambda: run(xs=u8(16, 9)[:, :8]), "aligned rows"),
         (lambda: run(xs=u8(8, 16).t()), "unit inner strides"),
         (lambda: run(x=big, xs=u8(256, 8), z=torch.zeros(256, 32)), "below 2 GiB"),
+        (lambda: run(z=torch.zeros(1, 32).expand(16, 32)), "elements of z overlap"),
         (lambda: run(generics=[64, 128]), "generic BM"),
         (lambda: run(generics=[128, 128, 96]), "not a multiple of BK"),
         (lambda: run(generics=[128, 128, 128, 32]), "BK_PACKED"),
@@ -85,6 +86,90 @@ def test_null_arguments_of_the_c_entry(fake_hip):
     assert fn(None, *args, C.c_float(1.0), None) == 0
     for i in range(len(args)):
         assert fn(None, *[None if i == j else a for j, a in enumerate(args)], C.c_float(1.0), None) == -2
+
+
+def chosen(ct, m, n, k, tile=(128, 128), out=torch.bfloat16, **kw):
+    """kernel and workgroups of a launch without a GPU (256 compute units)"""
+    from test_host_abi import _last
+
+    u8 = lambda r, c: torch.empty(r, c, dtype=torch.uint8)
+    ct.linear_tile_mxfp4(ct.partition(torch.empty(m, n, dtype=out), list(tile), **({"prefix": True} if "grid" in kw else {})), u8(m, k // 2), u8(n, k // 2), u8(m, k // 32), u8(n, k // 32), **kw)
+    rec, _ = _last(ct)
+    return rec.symbol.decode().split("__")[1], rec.grid[0]
+
+
+# rows, n, k, shares of K on 128 x 128 tiles
+SHARED = [(100, 68, 1152, 1), (130, 260, 4736, 2), (200, 388, 9088, 3), (100, 68, 16256, 4), (100, 68, 37760, 6), (100, 68, 64640, 8)]
+
+
+def test_rule(fake_hip):
+    """what a launch is given to, by extents alone: any tile of z that covers it all may be computed by another one"""
+    ct = fake_hip
+    for tile in ((128, 128), (256, 256)):
+        assert chosen(ct, 1, 14336, 4096, tile) == ("bf16_flat16x64", 224)
+        assert chosen(ct, 64, 14336, 4096, tile) == ("bf16_flat64x64", 224)
+        assert chosen(ct, 200, 14336, 4096, tile) == ("bf16_128x128x256_e2x2_lone", 224)
+        assert chosen(ct, 512, 4096, 14336, tile) == ("bf16_128x128x256_e2x2_lone", 256)      # 128 tiles, K in two
+        assert chosen(ct, 1700, 11000, 6784, tile)[0] in ("bf16_128x128x256_e2x2", "bf16_256x256x256_e4x2")
+        assert chosen(ct, 4096, 4096, 4096, tile) == ("bf16_256x256x256_e4x2", 256)
+    named = {"variant": "bf16_128x128x256_e2x2"}
+    for m, n, k, shares in SHARED:
+        assert chosen(ct, m, n, k, **named) == ("bf16_128x128x256_e2x2_lone", shares * -(-m // 128) * -(-n // 128)), (m, n, k)
+    assert chosen(ct, 2100, 2052, 1024, **named) == ("bf16_128x128x256_e2x2", 17 * 17)
+    assert chosen(ct, 128, 128, 384, **named) == ("bf16_128x128x256_e2x2", 1)                 # too short for two groups
+    assert chosen(ct, 300, 512, 16384, grid=(2, 1, 1)) == ("bf16_128x128x256_e2x2_lone", 2)    # a part of z: its own tiles, whole K
+    assert chosen(ct, 600, 512, 16384, (256, 256), grid=(2, 1, 1)) == ("bf16_256x256x256_e4x2", 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,shares", SHARED)
+def test_gpu_mxfp4_shared_k(ct, dev, m, n, k, shares):
+    """the same sums launch after launch, on two streams at once, and captured (where nobody may share)"""
+    args = operands(m, n, k, k, dev)
+    want, size = product(*args)
+    zs = [torch.full((m, n), math.nan, device=dev) for _ in range(4)]
+    run = lambda i, stream=None: ct.linear_tile_mxfp4(ct.partition(zs[i], [128, 128]), *args, variant="f32_128x128x256_e2x2", stream=stream)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        run(0), run(1, streams[0].cuda_stream), run(2, streams[1].cuda_stream)
+    torch.cuda.synchronize()
+    for z in zs[:3]:
+        assert_product(z, want, size, k)
+    assert torch.equal(zs[0], zs[1]) and torch.equal(zs[0], zs[2])                             # shares are added in their order
+    graph = ct.CapturedGraph().capture(lambda s: run(3, s))
+    for _ in range(3):
+        zs[3].fill_(math.nan)
+        run(0)
+        torch.cuda.synchronize()
+        graph.launch()
+        graph.synchronize()
+        assert_product(zs[3], want, size, k)
+    graph.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,variant", [(2100, 2052, 1152, "128x128x256_e2x2"), (2100, 2052, 640, None), (4300, 4100, 384, "256x256x256_e4x2"), (300, 34000, 256, None)])
+def test_gpu_mxfp4_more_tiles_than_compute_units(ct, dev, m, n, k, variant):
+    args = operands(m, n, k, 3, dev)
+    want, size = product(*args)
+    z = torch.full((m, n), math.nan, dtype=torch.bfloat16, device=dev)
+    ct.linear_tile_mxfp4(ct.partition(z, [256, 256] if variant and variant[0] == "2" else [128, 128]), *args, variant=variant and "bf16_" + variant)
+    assert_product(z, want, size, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("k", [256, 2176])
+def test_gpu_mxfp4_part_of_z(ct, dev, tile, k):
+    """a grid over some tiles of z leaves the others alone"""
+    m, n = 2 * tile + 40, 2 * tile + 36
+    args = operands(m, n, k, 8, dev)
+    want, size = product(*args)
+    z = torch.full((m, n), 7.0, device=dev)
+    ct.linear_tile_mxfp4(ct.partition(z, [tile, tile], prefix=True), *args, grid=(2, 1, 1))
+    assert_product(z[: 2 * tile, :tile], want[: 2 * tile, :tile], size[: 2 * tile, :tile], k)
+    assert bool((z[2 * tile:] == 7.0).all()) and bool((z[:, tile:] == 7.0).all())
 
 
 @pytest.mark.gpu

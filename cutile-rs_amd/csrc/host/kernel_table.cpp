@@ -509,10 +509,10 @@ std::vector<KernelEntry> build_table() {
       for (const char* fn : {"rms_norm_quantize", "add_rms_norm_quantize"}) {
         for (auto rv : kHeld) {
           const std::string v = base + "w" + std::to_string(rv.wpr) + "v" + std::to_string(rv.vpl);
-          add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_BLOCK_SCALE, (uint32_t)std::max(256, rv.wpr * 64), rv.wpr > 1 ? (uint32_t)std::max(4, rv.wpr) * 4 : 0, 0, 0, rv.vpl,
+          add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_BLOCK_SCALE, (uint32_t)std::max(256, rv.wpr * 64), rv.wpr > 1 ? (uint32_t)std::max(4, rv.wpr) * 8 : 0, 0, 0, rv.vpl,
               rv.wpr, dt, (int64_t)rv.wpr * 64 * rv.vpl * 8, 2);
         }
-        add(fn, keep(base + "any"), keep(std::string(fn) + "_entry__" + base + "any"), IMG_BLOCK_SCALE, 256, 16, 0, 0, 0, 0, dt, 0, 2);
+        add(fn, keep(base + "any"), keep(std::string(fn) + "_entry__" + base + "any"), IMG_BLOCK_SCALE, 256, 32, 0, 0, 0, 0, dt, 0, 2);
       }
     }
   return t;

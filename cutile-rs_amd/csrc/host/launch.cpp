@@ -3309,6 +3309,10 @@ cutile_status_t check_blocks(const char* fn, const cutile_tensor_arg_t& data, co
   return CUTILE_SUCCESS;
 }
 
+// As the norms take them: mean(c^2) + eps = sum * inv_n + eps.
+struct NormMean {
+  double inv_n, eps;
+};
 // g and 1 / (6 g), as the kernels take them.
 struct TensorScale {
   float g, inv6g;
@@ -3480,7 +3484,7 @@ cutile_status_t launch_norm_quantize(const char* fn, cutile_stream_t stream, con
   args.push_partition(*out);
   args.push_partition(*scales);
   if (residual) args.push_partition(*residual_out);
-  args.push_val<float>(eps);
+  args.push_val<NormMean>({1.0 / (double)n, (double)eps});
   args.push_val<TensorScale>(t);
   args.push_val<int64_t>(rows);
   args.push_val<int32_t>((int32_t)(k / 8));

@@ -52,21 +52,68 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return __builtin_fmaf(__builtin_fmaf(-y, d, n), q, y) * u;
 }
 
-// 1 / sqrt(a) in two parts, and c / sqrt(a) * w rounded once: each rounding on the way to the quantised value takes some of the values next
-// to a border between two codes to the wrong side of it.  The second part is what one Newton step adds; rows
-// far from 1 (where its products would leave f32) and rows of zeros, infinities or NaN have none.
+// mean(c^2) + eps = sum * inv_n + eps
+struct NormMean {
+  double inv_n, eps;
+};
+// c / sqrt(mean) * w.  A rounded product next to a border between two codes, or next to a power of two, which is a border between two block scales, may lie on
+// the wrong side of it or on the border itself.  So most values take two products (`about`, off by 4.5 x 2^-24 of themselves at most: the mean's rounding, root,
+// quotient and two products), and those within kBorderSlack steps of f32 of a border are found again by `exact`, from 1 / sqrt(mean) in two parts (the
+// second is what one Newton step adds; rows far from 1, where its products would leave f32, and rows of zeros, infinities or NaN have none): rounded
+// once, and where that ends on a border, to the next float on the value's side.  The quantised row is that of the real numbers but for the sum of squares
+// (f32 over four values, then f64) and sums of residual and x beyond f32: of 134 million values 3 or 4 were not, 70 where two f32 roundings are all.
+// nvfp4 elements are products with one more factor; all of its values are rounded once (`times`).
+constexpr uint32_t kBorderSlack = 8;
+// Steps from the nearest border below, plus the slack: up to twice the slack within its reach.  Borders of the mx formats have zeros in
+// all these bits; zeros, which are none, are made 2^-144 (and quantised as zeros).
+constexpr float kTiny = 0x1p-144f;
+template <Format F>
+__device__ __forceinline__ uint32_t border_distance(float v) {
+  return F == kNvfp4 ? ~0u : (__builtin_bit_cast(uint32_t, v) + kBorderSlack) & (F == kMxfp8 ? (1u << 19) - 1 : (1u << 21) - 1);
+}
 struct Scale {
   float r, rest;
+  __device__ __forceinline__ float about(float c, float w) const { return __builtin_fmaf(c * r, w, kTiny); }
+  __device__ __forceinline__ float low(float c, float t) const { return __builtin_fmaf(c, rest, __builtin_fmaf(c, r, -t)); }
   __device__ __forceinline__ float times(float c, float w) const {
-    const float t = c * r, low = __builtin_fmaf(c, rest, __builtin_fmaf(c, r, -t));
-    return __builtin_fmaf(t, w, low * w);
+    const float t = c * r;
+    return __builtin_fmaf(t, w, low(c, t) * w);
+  }
+  template <Format F>
+  __device__ __forceinline__ float exact(float c, float w) const {
+    const float y = times(c, w), t = c * r, left = __builtin_fmaf(t, w, -y) + low(c, t) * w;
+    if (border_distance<F>(y) != kBorderSlack || left == 0.0f || !__builtin_isfinite(left)) return y;
+    const int32_t b = __builtin_bit_cast(int32_t, y);
+    return __builtin_bit_cast(float, b + (((b ^ __builtin_bit_cast(int32_t, left)) >> 31) | 1));
   }
 };
-__device__ __forceinline__ Scale norm_scale(float a) {
+__device__ __forceinline__ Scale norm_scale(double mean) {
+  const float a = (float)mean;
   Scale s{1.0f / sqrtf(a), 0.0f};
-  const float h = a * s.r, off = __builtin_fmaf(-h, s.r, 1.0f) - __builtin_fmaf(a, s.r, -h) * s.r;   // 1 - a r^2
+  const float h = a * s.r, off = __builtin_fmaf(-h, s.r, 1.0f) - (__builtin_fmaf(a, s.r, -h) + (float)(mean - (double)a) * s.r) * s.r;   // 1 - mean r^2
   if (a > 0x1p-100f && a < 0x1p100f) s.rest = 0.5f * s.r * off;
   return s;
+}
+// Sum over the wavefront, in every lane.
+__device__ __forceinline__ double wave_sum(double v) {
+  union Words {
+    double d;
+    int32_t w[2];
+  };
+  auto add = [&](auto exchange) {
+    Words a{v}, b;
+    b.w[0] = exchange(a.w[0]), b.w[1] = exchange(a.w[1]);
+    v = a.d + b.d;
+  };
+  add([](int32_t w) { return lanes::dpp<lanes::kQuadXor1>(w); });
+  add([](int32_t w) { return lanes::dpp<lanes::kQuadXor2>(w); });
+  add([](int32_t w) { return lanes::dpp<lanes::kHalfMirror>(w); });
+  add([](int32_t w) { return lanes::dpp<lanes::kRowMirror>(w); });
+  Words a{v}, e, o;
+  for (int i = 0; i < 2; ++i) lanes::split_row_pairs(a.w[i], &e.w[i], &o.w[i]);
+  a.d = e.d + o.d;
+  for (int i = 0; i < 2; ++i) lanes::split_halves(a.w[i], &e.w[i], &o.w[i]);
+  return e.d + o.d;
 }
 
 template <Format F, typename T, bool SILU>
@@ -260,21 +307,22 @@ __device__ __forceinline__ void quantize_columns(const TensorArg<2>& x, const Pa
 }
 
 // A row of up to WPR * 64 * VPL units in the registers of WPR wavefronts: read once, summed, scaled, quantised.  Bound by memory;
-// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 13.4 with a
-// wavefront of one unit a lane, 14.5 with two, 21 with four wavefronts; 4096 x 1024 4.7: 8.9 with one wavefront, 9.5 with four; 2048 x 2048 4.7: 8.5 with four
-// of two units, 9.4 with one of four; 1500 x 5120 8.5: 12.5 with four of three, 13.9 with eight; 16384 x 8192 149: 162 to 165 with four or eight of four
-// units, 172 to 176 with sixteen of one or two; 2048 x 28672 65: 89 with sixteen of four.  Up to 500 rows every shape takes the time of a launch.
+// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 11.6 with a
+// wavefront of one unit a lane, 11.8 with two, 21 with four wavefronts; 4096 x 1024 4.7: 8.0 with one wavefront, 9.2 with four; 2048 x 2048 4.7: 8.2 with four
+// of two units, 8.6 of three; 1500 x 5120 8.5: 11.4 with four of three, 13.1 with eight of four; 16384 x 8192 149: 162 to 165 with four or eight of four
+// units, 234 with sixteen; 4096 x 16384 75: 87 with eight, 101 with sixteen; 2048 x 28672 65: 89 with sixteen.  Up to 500 rows every shape takes the time of a launch.
 template <Format F, typename T, bool ADD, int WPR, int VPL, bool WHOLE>
 __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const TensorArg<2>& x, const TensorArg<1>& w, const PartitionArg<2>& out,
-                                          const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, float eps, TensorScale t, int64_t rows,
-                                          int32_t units, float (*part)[WPR]) {
+                                          const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, NormMean m, TensorScale t, int64_t rows,
+                                          int32_t units, double (*part)[WPR]) {
   constexpr int kRows = WPR < 4 ? 4 / WPR : 1;      // of a workgroup
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, slot = wave / WPR, sub = wave % WPR;
   const int64_t r = (int64_t)blockIdx.x * kRows + slot;
   const bool live = r < rows;
   const int32_t n = x.shape[1];
   Unit<T> a[VPL], b[ADD ? VPL : 1], g[VPL];
-  float c[VPL][8], ss = 0.0f;
+  float c[VPL][8];
+  double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int32_t u = i * (WPR * 64) + sub * 64 + lane;
@@ -290,37 +338,46 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
   }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      c[i][e] = ADD ? (float)a[i].v[e] + (float)b[ADD ? i : 0].v[e] : (float)a[i].v[e];
-      s = __builtin_fmaf(c[i][e], c[i][e], s);
+    for (int e = 0; e < 8; ++e) c[i][e] = ADD ? (float)a[i].v[e] + (float)b[ADD ? i : 0].v[e] : (float)a[i].v[e];
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+      const float *d = c[i] + h, low = __builtin_fmaf(d[1], d[1], d[0] * d[0]);
+      ss += (double)__builtin_fmaf(d[3], d[3], __builtin_fmaf(d[2], d[2], low));
     }
-    ss += s;
   }
-  ss = lanes::across_wave<lanes::Sum>(ss);
+  ss = wave_sum(ss);
   if constexpr (WPR > 1) {
     if (lane == 0) part[slot][sub] = ss;
     __syncthreads();
-    ss = 0.0f;
+    ss = 0.0;
 #pragma unroll
     for (int i = 0; i < WPR; ++i) ss += part[slot][i];
   }
   if (!live) return;
-  const Scale s = norm_scale(ss / (float)n + eps);
+  const Scale s = norm_scale(__builtin_fma(ss, m.inv_n, m.eps));
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int32_t u = i * (WPR * 64) + sub * 64 + lane;
     if (u >= units) continue;
+    float v[8];
+    uint32_t border = ~0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = F == kNvfp4 ? s.times(c[i][e], (float)g[i].v[e]) : s.about(c[i][e], (float)g[i].v[e]);
+      border = min(border, border_distance<F>(v[e]));
+    }
+    if (border <= 2 * kBorderSlack) {   // one wavefront in sixty
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (border_distance<F>(v[e]) <= 2 * kBorderSlack) v[e] = s.exact<F>(c[i][e], (float)g[i].v[e]);
+    }
     if constexpr (ADD) {   // (may be residual or x itself: this lane has read what it writes)
       Unit<T> o;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o.v[e] = (T)c[i][e];
       o.template store<WHOLE>((T*)residual_out->ptr + r * residual_out->strides[0] + (int64_t)u * 8, n - (int64_t)u * 8);
     }
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = s.times(c[i][e], (float)g[i].v[e]);
     if (!WHOLE && (int64_t)u * 8 + 8 > n) {   // behind the row nothing but zeros, whatever the norm is
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = (int64_t)u * 8 + e < n ? v[e] : 0.0f;
@@ -331,9 +388,9 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
 
 // ---- any strides -------------------------------------------------------------------------------------------------------
 // Sum over the workgroup, in every thread.
-__device__ __forceinline__ float workgroup_sum(float v) {
-  __shared__ float part[kThreads / 64];
-  v = lanes::across_wave<lanes::Sum>(v);
+__device__ __forceinline__ double workgroup_sum(double v) {
+  __shared__ double part[kThreads / 64];
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -342,7 +399,7 @@ __device__ __forceinline__ float workgroup_sum(float v) {
 
 template <Format F, typename T, bool ADD>
 __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const TensorArg<2>& x, const TensorArg<1>& w, const PartitionArg<2>& out,
-                                          const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, float eps, TensorScale t, int64_t rows,
+                                          const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, NormMean m, TensorScale t, int64_t rows,
                                           int32_t units) {
   const int32_t n = x.shape[1];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -355,13 +412,14 @@ __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const Te
         for (int e = 0; e < 8; ++e) c[e] += a[e];
       }
     };
-    float c[8], ss = 0.0f;
+    float c[8];
+    double ss = 0.0;
     for (int32_t u = threadIdx.x; u < units; u += kThreads) {
       load(u, c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(c[e], c[e], ss);
+      for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)c[e], (double)c[e], ss);
     }
-    const Scale s = norm_scale(workgroup_sum(ss) / (float)n + eps);
+    const Scale s = norm_scale(__builtin_fma(workgroup_sum(ss), m.inv_n, m.eps));
     for (int32_t u = threadIdx.x; u < units; u += kThreads) {
       load(u, c);
 #pragma unroll
@@ -369,7 +427,7 @@ __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const Te
         const int32_t j = u * 8 + e;
         if (j >= n) continue;
         if constexpr (ADD) *at<T>(*residual_out, r, j) = (T)c[e];   // (may be residual or x itself: this thread has read the element)
-        c[e] = s.times(c[e], (float)((const T*)w.ptr)[(int64_t)j * w.strides[0]]);
+        c[e] = s.exact<F>(c[e], (float)((const T*)w.ptr)[(int64_t)j * w.strides[0]]);
       }
       quantize_unit<F>(c, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
     }
@@ -432,17 +490,17 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
   }
 #define NORM_HELD(FMT, F, TYPE, T, WPR, VPL)                                                                                                        \
   extern "C" __global__ void __launch_bounds__(WPR < 4 ? 256 : WPR * 64) rms_norm_quantize_entry__##FMT##_##TYPE##_w##WPR##v##VPL(                  \
-      TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, float eps, TensorScale t, int64_t rows, int32_t units) {         \
-    __shared__ float part[WPR < 4 ? 4 / WPR : 1][WPR];                                                                                              \
-    if (x.shape[1] == 8ll * units) norm_held<F, T, false, WPR, VPL, true>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units, part);          \
-    else norm_held<F, T, false, WPR, VPL, false>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units, part);                                   \
+      TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, NormMean m, TensorScale t, int64_t rows, int32_t units) {         \
+    __shared__ double part[WPR < 4 ? 4 / WPR : 1][WPR];                                                                                              \
+    if (x.shape[1] == 8ll * units) norm_held<F, T, false, WPR, VPL, true>(nullptr, x, w, out, scales, nullptr, m, t, rows, units, part);          \
+    else norm_held<F, T, false, WPR, VPL, false>(nullptr, x, w, out, scales, nullptr, m, t, rows, units, part);                                   \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(WPR < 4 ? 256 : WPR * 64) add_rms_norm_quantize_entry__##FMT##_##TYPE##_w##WPR##v##VPL(              \
-      TensorArg<2> residual, TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, PartitionArg<2> residual_out, float eps,  \
+      TensorArg<2> residual, TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, PartitionArg<2> residual_out, NormMean m,  \
       TensorScale t, int64_t rows, int32_t units) {                                                                                                 \
-    __shared__ float part[WPR < 4 ? 4 / WPR : 1][WPR];                                                                                              \
-    if (x.shape[1] == 8ll * units) norm_held<F, T, true, WPR, VPL, true>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units, part);   \
-    else norm_held<F, T, true, WPR, VPL, false>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units, part);                            \
+    __shared__ double part[WPR < 4 ? 4 / WPR : 1][WPR];                                                                                              \
+    if (x.shape[1] == 8ll * units) norm_held<F, T, true, WPR, VPL, true>(&residual, x, w, out, scales, &residual_out, m, t, rows, units, part);   \
+    else norm_held<F, T, true, WPR, VPL, false>(&residual, x, w, out, scales, &residual_out, m, t, rows, units, part);                            \
   }
 #define NORMS_HELD(FMT, F, TYPE, T)   \
   NORM_HELD(FMT, F, TYPE, T, 1, 1)    \
@@ -459,13 +517,13 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
     quantize_rows<F, T, true>(gate, &up, out, scales, t, rows, units);                                                                              \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kThreads) rms_norm_quantize_entry__##FMT##_##TYPE##_any(                                             \
-      TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, float eps, TensorScale t, int64_t rows, int32_t units) {         \
-    norm_rows<F, T, false>(nullptr, x, w, out, scales, nullptr, eps, t, rows, units);                                                               \
+      TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, NormMean m, TensorScale t, int64_t rows, int32_t units) {         \
+    norm_rows<F, T, false>(nullptr, x, w, out, scales, nullptr, m, t, rows, units);                                                               \
   }                                                                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kThreads) add_rms_norm_quantize_entry__##FMT##_##TYPE##_any(                                         \
-      TensorArg<2> residual, TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, PartitionArg<2> residual_out, float eps,  \
+      TensorArg<2> residual, TensorArg<2> x, TensorArg<1> w, PartitionArg<2> out, PartitionArg<2> scales, PartitionArg<2> residual_out, NormMean m,  \
       TensorScale t, int64_t rows, int32_t units) {                                                                                                 \
-    norm_rows<F, T, true>(&residual, x, w, out, scales, &residual_out, eps, t, rows, units);                                                        \
+    norm_rows<F, T, true>(&residual, x, w, out, scales, &residual_out, m, t, rows, units);                                                        \
   }
 #define BLOCK_FORMAT(FMT, F)               \
   BLOCK_KERNELS_16(FMT, F, f16, _Float16)  \

@@ -762,11 +762,11 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
  * x: [M, N] f16, bf16 or f32 with any strides; N of any length up to K.  out: K whole blocks a row, columns N .. K - 1 zeros
  * (so rows can be made as long as the product that reads them wants).  out and scales are partitioned [BM, whole row] alike
  * and may have fewer rows than x; their rows are contiguous and apart, those of out on 8-byte boundaries.  tensor_scale is 1 for
- * the mx formats and between 2^-100 and 2^100 for nvfp4.  Generic 0, when given, is N. */
+ * the mx formats and between 2^-100 and 2^100 for nvfp4.  Generic 0, when given, is N.  Outputs share no memory with inputs. */
 cutile_status_t cutile_launch_block_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_partition_arg_t* out,
                                              const cutile_partition_arg_t* scales, float tensor_scale, const cutile_launch_opts_t* opts);
 /* block_dequantize: out [M, N] <- the values that x and scales stand for, N up to K, rounded once to f16, bf16 or f32; out has
- * any strides and is partitioned [BM, N]; the block of a NaN scale is NaN. */
+ * any strides that keep its elements apart and is partitioned [BM, N]; the block of a NaN scale is NaN. */
 cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* scales,
                                                float tensor_scale, const cutile_partition_arg_t* out, const cutile_launch_opts_t* opts);
 /* The kernels in front of a block-scaled product with its operand as their output (x, w, gate, up f16 or bf16 alike, any

@@ -60,8 +60,9 @@ struct NormMean {
 // the wrong side of it or on the border itself.  So most values take two products (`about`, off by 4.5 x 2^-24 of themselves at most: the mean's rounding, root,
 // quotient and two products), and those within kBorderSlack steps of f32 of a border are found again by `exact`, from 1 / sqrt(mean) in two parts (the
 // second is what one Newton step adds; rows far from 1, where its products would leave f32, and rows of zeros, infinities or NaN have none): rounded
-// once, and where that ends on a border, to the next float on the value's side.  The quantised row is that of the real numbers but for the sum of squares
-// (f32 over four values, then f64) and sums of residual and x beyond f32: of 134 million values 3 or 4 were not, 70 where two f32 roundings are all.
+// once, and where that ends on a border, to the next float on the value's side.  (Both parts are right to 2^-45: what is closer to a border than 2^-44
+// is on it, as rows of equal values are.)  The quantised row is that of the real numbers but for sums of residual and x beyond f32: of
+// 134 million values at most one was not, 70 where two f32 roundings are all.
 // nvfp4 elements are products with one more factor; all of its values are rounded once (`times`).
 constexpr uint32_t kBorderSlack = 8;
 // Steps from the nearest border below, plus the slack: up to twice the slack within its reach.  Borders of the mx formats have zeros in
@@ -82,7 +83,7 @@ struct Scale {
   template <Format F>
   __device__ __forceinline__ float exact(float c, float w) const {
     const float y = times(c, w), t = c * r, left = __builtin_fmaf(t, w, -y) + low(c, t) * w;
-    if (border_distance<F>(y) != kBorderSlack || left == 0.0f || !__builtin_isfinite(left)) return y;
+    if (border_distance<F>(y) != kBorderSlack || !(__builtin_fabsf(left) > __builtin_fabsf(y) * 0x1p-44f) || !__builtin_isfinite(left)) return y;
     const int32_t b = __builtin_bit_cast(int32_t, y);
     return __builtin_bit_cast(float, b + (((b ^ __builtin_bit_cast(int32_t, left)) >> 31) | 1));
   }
@@ -307,10 +308,11 @@ __device__ __forceinline__ void quantize_columns(const TensorArg<2>& x, const Pa
 }
 
 // A row of up to WPR * 64 * VPL units in the registers of WPR wavefronts: read once, summed, scaled, quantised.  Bound by memory;
-// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 11.6 with a
-// wavefront of one unit a lane, 11.8 with two, 21 with four wavefronts; 4096 x 1024 4.7: 8.0 with one wavefront, 9.2 with four; 2048 x 2048 4.7: 8.2 with four
-// of two units, 8.6 of three; 1500 x 5120 8.5: 11.4 with four of three, 13.1 with eight of four; 16384 x 8192 149: 162 to 165 with four or eight of four
-// units, 234 with sixteen; 4096 x 16384 75: 87 with eight, 101 with sixteen; 2048 x 28672 65: 89 with sixteen.  Up to 500 rows every shape takes the time of a launch.
+// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 11.5 with a
+// wavefront of one unit a lane, 12.3 with two, 23 with four wavefronts; 4096 x 1024 4.7: 8.2 with one wavefront, 9.3 with four; 2048 x 2048 4.7: 8.2 with four
+// of two units, 8.8 of three; 1500 x 5120 8.5: 11.4 with four of three, 13.2 with eight of four; 16384 x 8192 149: 163 to 165 with four or eight of four
+// units, 245 with sixteen; 4096 x 16384 75: 87 with eight, 101 with sixteen; 2048 x 28672 65: 89 with sixteen.  Up to 500 rows every shape takes the time of a
+// launch.  The sum of squares in f64 costs 2 % of the short ones (f32 over four values, then f64: 1500 x 5120 11.2, and 4 of 134 million codes off).
 template <Format F, typename T, bool ADD, int WPR, int VPL, bool WHOLE>
 __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const TensorArg<2>& x, const TensorArg<1>& w, const PartitionArg<2>& out,
                                           const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, NormMean m, TensorScale t, int64_t rows,
@@ -340,11 +342,10 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
   for (int i = 0; i < VPL; ++i) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) c[i][e] = ADD ? (float)a[i].v[e] + (float)b[ADD ? i : 0].v[e] : (float)a[i].v[e];
+    double sum = 0.0;
 #pragma unroll
-    for (int h = 0; h < 8; h += 4) {
-      const float *d = c[i] + h, low = __builtin_fmaf(d[1], d[1], d[0] * d[0]);
-      ss += (double)__builtin_fmaf(d[3], d[3], __builtin_fmaf(d[2], d[2], low));
-    }
+    for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)c[i][e], (double)c[i][e], sum);
+    ss += sum;
   }
   ss = wave_sum(ss);
   if constexpr (WPR > 1) {

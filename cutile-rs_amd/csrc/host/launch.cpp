@@ -3322,7 +3322,7 @@ cutile_status_t tensor_scale_of(const char* fn, const BlockFormat& f, float g, T
     CUTILE_REQUIRE(g >= 0x1p-100f && g <= 0x1p100f, CUTILE_ERR_KERNEL_LAUNCH, "%s: tensor_scale must lie between 2^-100 and 2^100, got %g", fn, (double)g);
   else
     CUTILE_REQUIRE(g == 1.0f, CUTILE_ERR_KERNEL_LAUNCH, "%s: %s has no tensor_scale (nvfp4 has): it must be 1, got %g", fn, f.name, (double)g);
-  *t = {g, (float)(1.0 / (6.0 * (double)g))};
+  *t = {g, 1.0f / (6.0f * g)};   // as the rest of the scale in f32: what a program that computes it in f32 gets
   return CUTILE_SUCCESS;
 }
 

@@ -7,7 +7,9 @@
 //   mx      byte = clamp(floor(log2 a) - emax + 127, 0, 254), emax = 8 (e4m3) or 2 (e2m1), a = 0: byte 0;
 //           elements round(v * 2^(127 - byte)), to nearest even, saturated to 448 or 6 (the conversion of the OCP MX
 //           specification 1.0, section 6.3)
-//   nvfp4   s = e4m3(min(a / (6 g), 448)); elements e2m1(v * (1 / (s g))), 0 where s is 0
+//   nvfp4   s = e4m3(min(a * (1 / (6 g)), 448)); elements e2m1(v * (1 / (s g))), 0 where s is 0, every operation in f32.  (With g = largest / (6 * 448),
+//           as tensors are calibrated, many a / (6 g) lie on a border between two scales: in f32 throughout the bytes are those that any program that
+//           takes these steps gets; 1 / (6 g) rounded once instead moves one scale in eighty of some such tensors to its neighbour.)
 //   a block that holds a NaN or an infinity: scale NaN (0xff or 0x7f), elements 0 - the whole block stands for NaN
 // The exponent of a is that of its f32 bits, so the mx scale is an integer subtraction and the scaling exact.  Magnitudes are
 // compared as integers: they order like floats, with infinities and NaN on top, where a float maximum would drop a NaN.
@@ -28,7 +30,7 @@ struct Traits {
   static constexpr int kLanes = kBlock / 8;           // lanes of a block
 };
 
-// The scale of the tensor as the kernels take it: g, and 1 / (6 g) rounded once.
+// The scale of the tensor as the kernels take it: g, and 1 / (6 g).
 struct TensorScale {
   float g, inv6g;
 };

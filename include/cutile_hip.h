@@ -757,7 +757,8 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
  * block_quantize: for the largest magnitude a of a block (32 values, nvfp4 16)
  *   mxfp8, mxfp4   byte = clamp(floor(log2 a) - emax + 127, 0, 254), emax 8 (e4m3) or 2 (e2m1); a = 0: byte 0; elements
  *                  round(x * 2^(127 - byte)) to nearest even, saturated at 448 or 6   (OCP MX 1.0, section 6.3)
- *   nvfp4          scale = e4m3(min(a / (6 tensor_scale), 448)), elements e2m1(x / (scale * tensor_scale)), 0 where the scale is
+ *   nvfp4          scale = e4m3(min(a * (1 / (6 tensor_scale)), 448)), elements e2m1(x * (1 / (scale * tensor_scale))), 0 where the
+ *                  scale is; every operation in f32
  *   A block that holds a NaN or an infinity gets a NaN scale (0xff, 0x7f) and elements 0: it stands for NaN throughout.
  * x: [M, N] f16, bf16 or f32 with any strides; N of any length up to K.  out: K whole blocks a row, columns N .. K - 1 zeros
  * (so rows can be made as long as the product that reads them wants).  out and scales are partitioned [BM, whole row] alike
@@ -765,7 +766,7 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
  * the mx formats and between 2^-100 and 2^100 for nvfp4.  Generic 0, when given, is N.  Outputs share no memory with inputs. */
 cutile_status_t cutile_launch_block_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_partition_arg_t* out,
                                              const cutile_partition_arg_t* scales, float tensor_scale, const cutile_launch_opts_t* opts);
-/* block_dequantize: out [M, N] <- the values that x and scales stand for, N up to K, rounded once to f16, bf16 or f32; out has
+/* block_dequantize: out [M, N] <- the values that x and scales stand for (nvfp4: in f32), N up to K, rounded once to f16, bf16 or f32; out has
  * any strides that keep its elements apart and is partitioned [BM, N]; the block of a NaN scale is NaN. */
 cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* scales,
                                                float tensor_scale, const cutile_partition_arg_t* out, const cutile_launch_opts_t* opts);

@@ -12,6 +12,11 @@ TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 LENGTHS = [1, 15, 16, 31, 32, 33, 100, 256, 1000, 5001, 8192, 20000]
 
 
+# of nvfp4's scale, relative: f32 roundings of tensor_scale, of 6 tensor_scale, of its reciprocal and of the product with it (what follows in
+# the elements is in assert_quantised)
+NVFP4_SLACK = 4 * 2.0 ** -24
+
+
 def whole(ct, t):
     return ct.partition(t, [1, t.shape[1]])
 
@@ -174,14 +179,14 @@ def quantised(ct, x, fmt, k=None, g=1.0, rows=None, **kw):
 @pytest.mark.parametrize("n", LENGTHS)
 def test_gpu_quantize(ct, dev, fmt, dtype, n):
     """rows of any length, from tight to wide apart; the input is exact, so every code is the rounding (nvfp4: its scale is found with
-    two f32 roundings)"""
+    roundings of f32)"""
     for rows, pad in ((1, 0), (5, 0), (37, 3)):
         x = normal((rows, n + pad), 100 + n + rows, dev, TYPES[dtype]) * torch.exp2(torch.arange(rows, device=dev) % 13 - 6.0).to(TYPES[dtype])[:, None]
         x = x[:, pad:]
         g = g_of(x, fmt)
         k = ref.padded(n, fmt) + (ref.BLOCK[fmt] * 3 if rows == 5 else 0)      # blocks of nothing but padding
         data, scales = quantised(ct, x, fmt, k, g)
-        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=NVFP4_SLACK if fmt == "nvfp4" else 0.0)
 
 
 @pytest.mark.gpu
@@ -194,7 +199,7 @@ def test_gpu_quantize_strides(ct, dev, fmt, dtype):
     for x in (base.t(), base[:, ::2], base[:1].expand(9, 517), wide[:, 3:1027], wide[1:, 1:130], wide[:, 6:70], base.t()[5:, 3:200], base[::3].t()):
         g = g_of(x, fmt)
         data, scales = quantised(ct, x, fmt, None, g)
-        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=NVFP4_SLACK if fmt == "nvfp4" else 0.0)
 
 
 @pytest.mark.gpu
@@ -217,7 +222,7 @@ def test_gpu_quantize_special_values(ct, dev, fmt):
         x = torch.stack(rows).to(dt).reshape(1, -1).to(dev)
         g = 2.0 ** -9 if fmt == "nvfp4" else 1.0
         data, scales = quantised(ct, x, fmt, None, g)
-        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+        ref.assert_quantised(data, scales, x.double(), fmt, g, slack=NVFP4_SLACK if fmt == "nvfp4" else 0.0)
         back = torch.zeros(x.shape, device=dev)
         ct.block_dequantize(data, scales, whole(ct, back), fmt, g)
         lost = ~torch.isfinite(x.view(-1, b)).all(-1)
@@ -230,7 +235,26 @@ def test_gpu_quantize_tensor_scale_range(ct, dev):
     x = torch.cat([normal((1, 64), 3, dev) * s for s in (1e-30, 1e-6, 1.0, 1e6, 1e30)], 1)
     for g in (2.0 ** -100, 1.0, 1e3, 2.0 ** 100):
         data, scales = quantised(ct, x, "nvfp4", None, g)
-        ref.assert_quantised(data, scales, x.double(), "nvfp4", g, slack=2 * 2.0 ** -24)
+        ref.assert_quantised(data, scales, x.double(), "nvfp4", g, slack=NVFP4_SLACK)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1.0, 14.0, 81.5, 0.8984375, 3.359375, 110.5])
+def test_gpu_quantize_calibrated_tensor_scale(ct, dev, most):
+    """g = largest / (6 * 448): many blocks' scales lie on a border between two; the bytes are those of the definition in f32"""
+    x = normal((300, 512), 21, dev, torch.bfloat16)
+    x = (x / x.abs().max() * most).bfloat16()
+    x[7, 9] = most
+    g = float(x.abs().max().float()) / (6.0 * 448.0)
+    data, scales = quantised(ct, x, "nvfp4", None, g)
+    g32 = torch.tensor(g, dtype=torch.float32)
+    v = x.float().cpu().view(300, 32, 16)
+    s = (v.abs().amax(-1) * (1.0 / (6.0 * g32))).clamp(max=448.0).to(torch.float8_e4m3fn)
+    assert torch.equal(scales.cpu(), s.view(torch.uint8))
+    unit = s.float()
+    q = torch.where(unit > 0, 1.0 / (unit * g32), 0.0).unsqueeze(-1) * v
+    codes = ref.nearest(q.double(), ref.grid_of("nvfp4")).view(300, 512)
+    assert torch.equal(ref.unpack(data, "nvfp4").cpu().long() & 7, codes)
 
 
 @pytest.mark.gpu
@@ -342,7 +366,7 @@ def test_gpu_norm(ct, dev, fmt, dtype, n, add):
         torch.cuda.synchronize()
         assert int((data[rows:] != 0xA5).sum() + (scales[rows:] != 0xA5).sum()) == 0
         g = torch.tensor(g, dtype=torch.float32).double().item()
-        ref.assert_quantised(data[:rows], scales[:rows], want, fmt, g, slack=norm_slack(n) + 2 * 2.0 ** -24)
+        ref.assert_quantised(data[:rows], scales[:rows], want, fmt, g, slack=norm_slack(n) + NVFP4_SLACK)
 
 
 @pytest.mark.gpu
@@ -409,7 +433,7 @@ def test_gpu_silu_mul(ct, dev, fmt, dtype, n):
         assert int((data[rows:] != 0xA5).sum() + (scales[rows:] != 0xA5).sum()) == 0
         g = torch.tensor(g, dtype=torch.float32).double().item()
         # exponential (2 steps), sum, quotient (2), product, each relative to the result at most; nvfp4's scale
-        ref.assert_quantised(data[:rows], scales[:rows], want, fmt, g, slack=(6 + 2) * 2.0 ** -24, tiny=2.0 ** -126)
+        ref.assert_quantised(data[:rows], scales[:rows], want, fmt, g, slack=6 * 2.0 ** -24 + NVFP4_SLACK, tiny=2.0 ** -126)
 
 
 @pytest.mark.gpu
@@ -454,7 +478,7 @@ def test_gpu_norm_by_name(ct, dev, fmt, dtype, n):
                 assert torch.equal(ro, (x.float() + r.float()).to(x.dtype)), variant
             else:
                 ct.rms_norm_quantize(x, w, *args, 1e-6, fmt, g, variant=variant)
-            ref.assert_quantised(data, scales, want, fmt, torch.tensor(g, dtype=torch.float32).double().item(), slack=norm_slack(n) + 2 * 2.0 ** -24)
+            ref.assert_quantised(data, scales, want, fmt, torch.tensor(g, dtype=torch.float32).double().item(), slack=norm_slack(n) + NVFP4_SLACK)
 
 
 @pytest.mark.gpu
@@ -469,7 +493,7 @@ def test_gpu_units_by_name(ct, dev, fmt, dtype):
     results = [quantised(ct, x, fmt, None, g, variant=prefix + kind) for x, kind in ((plain, "rows"), (plain, "any"), (column, "columns"), (column, "any"), (column[:, :417], "columns"))]
     for data, scales in results[1:]:
         assert torch.equal(data, results[0][0]) and torch.equal(scales, results[0][1])
-    ref.assert_quantised(*results[0], base.double(), fmt, g, slack=2 * 2.0 ** -24 if fmt == "nvfp4" else 0.0)
+    ref.assert_quantised(*results[0], base.double(), fmt, g, slack=NVFP4_SLACK if fmt == "nvfp4" else 0.0)
     outs = [torch.full_like(base, 7.0) for _ in range(2)]
     for out, kind in zip(outs, ("rows", "any")):
         ct.block_dequantize(*results[0], whole(ct, out), fmt, g, variant=prefix + kind)

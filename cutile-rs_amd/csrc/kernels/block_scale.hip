@@ -41,60 +41,93 @@ __device__ __forceinline__ void load_unit(const TensorArg<2>& t, int64_t r, int3
   for (int i = 0; i < 8; ++i) v[i] = u * 8 + i < n ? (float)*at<T>(t, r, u * 8 + i) : 0.0f;
 }
 
+// ---- values next to a border ---------------------------------------------------------------------------------------------
+// A value that is the result of f32 roundings and lies next to a border between two codes, or next to a power of two, which is a border between two block
+// scales, may be on the wrong side of it or on the border itself.  So the fused kernels of the mx formats compute in f32, and what comes within some steps
+// of f32 (`slack`, what the f32 result may be off) of a border they compute again in f64: the quantised row is that of the real numbers.  (nvfp4
+// elements are products with one more factor, which has borders of its own.)
+// Steps from the nearest border below, plus the slack: up to twice the slack within reach.  Borders of the mx formats have zeros in all these
+// bits; zeros, which are none, are made 2^-142 (and quantised as zeros).
+constexpr float kTiny = 0x1p-142f;
+template <Format F>
+__device__ __forceinline__ uint32_t border_distance(float v, uint32_t slack) {
+  return F == kNvfp4 ? ~0u : (__builtin_bit_cast(uint32_t, v) + slack) & (F == kMxfp8 ? (1u << 19) - 1 : (1u << 21) - 1);
+}
+// y as a float on the same side of every border; what is closer to one than 2^-49 is on it (f64 results are off by 2^-51).
+template <Format F>
+__device__ __forceinline__ float settled(double y) {
+  const float f = (float)y;
+  const double left = y - (double)f;
+  if (border_distance<F>(f, 0) != 0 || !(__builtin_fabs(left) > __builtin_fabs(y) * 0x1p-49) || !__builtin_isfinite(left)) return f;
+  const int32_t b = __builtin_bit_cast(int32_t, f);
+  return __builtin_bit_cast(float, b + (((b >> 31) ^ (left < 0.0 ? -1 : 0)) | 1));
+}
+// A unit's values within `slack` steps of a border by `again(e)` of them; one iteration or none as a rule.
+template <Format F, class Again>
+__device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, Again again) {
+  if constexpr (F == kNvfp4) return;
+  uint32_t border = ~0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) border = min(border, border_distance<F>(v[e], slack));
+  if (border > 2 * slack) return;
+  uint32_t near = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) near |= border_distance<F>(v[e], slack) <= 2 * slack ? 1u << e : 0u;
+#pragma unroll 1
+  while (near != 0) {
+    const int at = __builtin_ctz(near);
+    near &= near - 1;
+    const float f = settled<F>(again(at));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e == at ? f : v[e];
+  }
+}
+
 // g / (1 + exp(-g)) * u, through E = exp(-|g|) <= 1, which nothing overflows: (max(g, 0) + min(g, 0) E) / (1 + E).  E is the square of
-// exp(-|g| / 2): the exponential instruction flushes results below 2^-126, a product does not.  The quotient is corrected once
-// by its remainder.  (With the library's exponential and division 45 vector instructions a value, 31 us for 1500 x 14336
-// where memory takes 17.)
+// exp(-|g| / 2): the exponential instruction flushes results below 2^-126, a product does not.  Off by less than kSiluSlack steps for g above -12
+// (what E loses grows with |g|).  nvfp4: the quotient is corrected once by its remainder.
+// (With the library's exponential and division 45 vector instructions a value, 31 us for 1500 x 14336 where memory takes 17.)
+constexpr uint32_t kSiluSlack = 32;
+template <Format F>
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float h = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0.72134752f);   // log2(e) / 2
   const float e = h * h, d = 1.0f + e, q = __builtin_amdgcn_rcpf(d);
   const float n = __builtin_fmaf(fminf(g, 0.0f), e, fmaxf(g, 0.0f)), y = n * q;
+  if constexpr (F != kNvfp4) return __builtin_fmaf(y, u, kTiny);
   return __builtin_fmaf(__builtin_fmaf(-y, d, n), q, y) * u;
 }
+__device__ __forceinline__ double silu_mul_f64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
 
 // mean(c^2) + eps = sum * inv_n + eps
 struct NormMean {
   double inv_n, eps;
 };
-// c / sqrt(mean) * w.  A rounded product next to a border between two codes, or next to a power of two, which is a border between two block scales, may lie on
-// the wrong side of it or on the border itself.  So most values take two products (`about`, off by 4.5 x 2^-24 of themselves at most: the mean's rounding, root,
-// quotient and two products), and those within kBorderSlack steps of f32 of a border are found again by `exact`, from 1 / sqrt(mean) in two parts (the
-// second is what one Newton step adds; rows far from 1, where its products would leave f32, and rows of zeros, infinities or NaN have none): rounded
-// once, and where that ends on a border, to the next float on the value's side.  (Both parts are right to 2^-45: what is closer to a border than 2^-44
-// is on it, as rows of equal values are.)  The quantised row is that of the real numbers but for sums of residual and x beyond f32: of
-// 134 million values at most one was not, 70 where two f32 roundings are all.
-// nvfp4 elements are products with one more factor; all of its values are rounded once (`times`).
-constexpr uint32_t kBorderSlack = 8;
-// Steps from the nearest border below, plus the slack: up to twice the slack within its reach.  Borders of the mx formats have zeros in
-// all these bits; zeros, which are none, are made 2^-144 (and quantised as zeros).
-constexpr float kTiny = 0x1p-144f;
-template <Format F>
-__device__ __forceinline__ uint32_t border_distance(float v) {
-  return F == kNvfp4 ? ~0u : (__builtin_bit_cast(uint32_t, v) + kBorderSlack) & (F == kMxfp8 ? (1u << 19) - 1 : (1u << 21) - 1);
-}
+// c / sqrt(mean) * w: two products of f32 are off by 4.5 x 2^-24 of themselves at most (the mean's rounding, root, quotient and the products); in f64 two
+// Newton steps from there (nvfp4: rounded once, with r in two parts).  Of 134 million values at most one differed from the 64-bit result, 70 where the two f32 products are all.
+constexpr uint32_t kNormSlack = 8;
 struct Scale {
-  float r, rest;
-  __device__ __forceinline__ float about(float c, float w) const { return __builtin_fmaf(c * r, w, kTiny); }
-  __device__ __forceinline__ float low(float c, float t) const { return __builtin_fmaf(c, rest, __builtin_fmaf(c, r, -t)); }
+  float r, rest;   // exact = r + rest
+  double exact;
+  template <Format F>
   __device__ __forceinline__ float times(float c, float w) const {
     const float t = c * r;
-    return __builtin_fmaf(t, w, low(c, t) * w);
+    return F == kNvfp4 ? __builtin_fmaf(t, w, __builtin_fmaf(c, rest, __builtin_fmaf(c, r, -t)) * w) : __builtin_fmaf(t, w, kTiny);
   }
-  template <Format F>
-  __device__ __forceinline__ float exact(float c, float w) const {
-    const float y = times(c, w), t = c * r, left = __builtin_fmaf(t, w, -y) + low(c, t) * w;
-    if (border_distance<F>(y) != kBorderSlack || !(__builtin_fabsf(left) > __builtin_fabsf(y) * 0x1p-44f) || !__builtin_isfinite(left)) return y;
-    const int32_t b = __builtin_bit_cast(int32_t, y);
-    return __builtin_bit_cast(float, b + (((b ^ __builtin_bit_cast(int32_t, left)) >> 31) | 1));
-  }
+  __device__ __forceinline__ double in_f64(float c, float w) const { return (double)c * exact * (double)w; }
 };
 __device__ __forceinline__ Scale norm_scale(double mean) {
-  const float a = (float)mean;
-  Scale s{1.0f / sqrtf(a), 0.0f};
-  const float h = a * s.r, off = __builtin_fmaf(-h, s.r, 1.0f) - (__builtin_fmaf(a, s.r, -h) + (float)(mean - (double)a) * s.r) * s.r;   // 1 - mean r^2
-  if (a > 0x1p-100f && a < 0x1p100f) s.rest = 0.5f * s.r * off;
+  Scale s;
+  s.r = 1.0f / sqrtf((float)mean);
+  s.exact = (double)s.r;
+  if (s.r > 0.0f && s.r < __builtin_inff()) {   // (rows of zeros, infinities and NaN, and beyond f32, stay as they are)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) s.exact = __builtin_fma(0.5 * s.exact, __builtin_fma(-mean * s.exact, s.exact, 1.0), s.exact);
+  }
+  s.rest = (float)(s.exact - (double)s.r);
+  if (!__builtin_isfinite(s.rest)) s.rest = 0.0f;   // (infinity less infinity)
   return s;
 }
+
 // Sum over the wavefront, in every lane.
 __device__ __forceinline__ double wave_sum(double v) {
   union Words {
@@ -130,7 +163,8 @@ __device__ __forceinline__ void quantize_rows(const TensorArg<2>& x, const Tenso
       float w[8];
       load_unit<T>(*up, r, u, n, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = silu_mul(v[e], w[e]);
+      for (int e = 0; e < 8; ++e) v[e] = silu_mul<F>(v[e], w[e]);
+      settle<F>(v, kSiluSlack, [&](int e) { return u * 8 + e < n ? silu_mul_f64((double)*at<T>(x, r, u * 8 + e), (double)*at<T>(*up, r, u * 8 + e)) : 0.0; });
     }
     quantize_unit<F>(v, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
   }
@@ -223,7 +257,12 @@ __device__ __forceinline__ void quantize_units(const TensorArg<2>& x, const Tens
     if (!at[i].live) continue;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = SILU ? silu_mul((float)a[i].v[e], (float)b[SILU ? i : 0].v[e]) : (float)a[i].v[e];
+    for (int e = 0; e < 8; ++e) v[e] = SILU ? silu_mul<F>((float)a[i].v[e], (float)b[SILU ? i : 0].v[e]) : (float)a[i].v[e];
+    if constexpr (SILU)
+      settle<F>(v, kSiluSlack, [&](int e) {
+        const int64_t j = (int64_t)at[i].u * 8 + e;
+        return j < n ? silu_mul_f64((double)((const T*)x.ptr)[(int64_t)at[i].r * x.strides[0] + j], (double)((const T*)up->ptr)[(int64_t)at[i].r * up->strides[0] + j]) : 0.0;
+      });
     quantize_unit<F>(v, t, data_at<F>(out, at[i].r, at[i].u), scale_at<F>(scales, at[i].r, at[i].u));
   }
 }
@@ -362,17 +401,14 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
     const int32_t u = i * (WPR * 64) + sub * 64 + lane;
     if (u >= units) continue;
     float v[8];
-    uint32_t border = ~0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = F == kNvfp4 ? s.times(c[i][e], (float)g[i].v[e]) : s.about(c[i][e], (float)g[i].v[e]);
-      border = min(border, border_distance<F>(v[e]));
-    }
-    if (border <= 2 * kBorderSlack) {   // one wavefront in sixty
+    for (int e = 0; e < 8; ++e) v[e] = s.times<F>(c[i][e], (float)g[i].v[e]);
+    settle<F>(v, kNormSlack, [&](int at) {   // (from registers: a load here is what a row's last wavefront would wait for)
+      float cv = 0.0f, gv = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (border_distance<F>(v[e]) <= 2 * kBorderSlack) v[e] = s.exact<F>(c[i][e], (float)g[i].v[e]);
-    }
+      for (int e = 0; e < 8; ++e) cv = e == at ? c[i][e] : cv, gv = e == at ? (float)g[i].v[e] : gv;
+      return s.in_f64(cv, gv);
+    });
     if constexpr (ADD) {   // (may be residual or x itself: this lane has read what it writes)
       Unit<T> o;
 #pragma unroll
@@ -428,7 +464,7 @@ __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const Te
         const int32_t j = u * 8 + e;
         if (j >= n) continue;
         if constexpr (ADD) *at<T>(*residual_out, r, j) = (T)c[e];   // (may be residual or x itself: this thread has read the element)
-        c[e] = s.exact<F>(c[e], (float)((const T*)w.ptr)[(int64_t)j * w.strides[0]]);
+        c[e] = settled<F>(s.in_f64(c[e], (float)((const T*)w.ptr)[(int64_t)j * w.strides[0]]));
       }
       quantize_unit<F>(c, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
     }

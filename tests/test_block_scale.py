@@ -554,6 +554,32 @@ def test_gpu_norm_rounds_the_value_itself(ct, dev, fmt, dtype, rows, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,n", [(3000, 480), (700, 4096), (90, 20001)])
+def test_gpu_silu_mul_rounds_the_value_itself(ct, dev, fmt, dtype, rows, n):
+    """as above; gates within 12 of 0, where the f32 result is within 32 steps, and some far above: their products with 1 are a power of two less a
+    little, which f32 does not hold"""
+    gate = normal((rows, n), 61, dev, torch.float32, 2.5).clamp(-11.9, 40.0).to(TYPES[dtype])
+    up = normal((rows, n), 62, dev, TYPES[dtype])
+    gate[:, 5], up[:, 5] = 16.0, 2.0
+    gate[:, 70], up[:, 70] = 32.0, -4.0
+    g = gate.double()
+    want = g / (1 + torch.exp(-g)) * up.double()
+    k = ref.padded(n, fmt)
+    for view in (lambda t: t, lambda t: t.t().contiguous().t()):
+        data, scales = ref.buffers(rows, k, fmt, dev)
+        ct.silu_mul_quantize(view(gate), view(up), whole(ct, data), whole(ct, scales), fmt)
+        full = torch.zeros((rows, k), dtype=torch.float64, device=dev)
+        full[:, :n] = want
+        blocks = full.view(rows, k // 32, 32)
+        exponents = ref._scale_codes(blocks.abs().amax(-1), fmt, 1.0)
+        assert torch.equal(scales.long(), exponents)
+        codes = ref.nearest(blocks / torch.exp2(exponents.double() - 127).unsqueeze(-1), ref.grid_of(fmt)).view(rows, k)
+        assert torch.equal(codes, (ref.unpack(data, fmt) & (127 if fmt == "mxfp8" else 7)).long())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 @pytest.mark.parametrize("n", [32, 100, 5120])
 def test_gpu_norm_of_equal_values(ct, dev, fmt, n):
     """rows of one value c each and eps = 0: the norm is w, wherever w lies - on a power of two (a border between scales), between two codes, above or below"""

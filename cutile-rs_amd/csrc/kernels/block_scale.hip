@@ -87,6 +87,7 @@ __device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, Again agai
 // exp(-|g| / 2): the exponential instruction flushes results below 2^-126, a product does not.  Off by less than kSiluSlack steps for g above -12
 // (what E loses grows with |g|).  nvfp4: the quotient is corrected once by its remainder.
 // (With the library's exponential and division 45 vector instructions a value, 31 us for 1500 x 14336 where memory takes 17.)
+// (What the values in f64 cost: 1500 x 14336 in a row of passes 20.7 us without them, 21.3 with; 52, 10 and 111 of 21.5 million codes were off, now 2, 1 and 3.)
 constexpr uint32_t kSiluSlack = 32;
 template <Format F>
 __device__ __forceinline__ float silu_mul(float g, float u) {
@@ -213,7 +214,7 @@ struct Unit {
 // Units of a launch in one sequence, row after row, neighbours to neighbouring lanes; a workgroup takes U of them for each of its
 // threads (the launcher counts with the same U).  Where everything is contiguous the launcher makes one row of it.
 // One unit a thread for the quantising kernels: later workgroups read while earlier ones write (us with 1, 2, 4, 8 of them: 16384 x 8192 bf16 to mxfp8
-// 71, 75, 73, 78; gated activation of 1500 x 14336 22.2, 24.6, 25.5, 29.3); four for reading back (16384 x 8192 mxfp4 to bf16 65, 69, 61, 65).
+// 71, 75, 73, 78; gated activation of 1500 x 14336, without values in f64, 22.2, 24.6, 25.5, 29.3); four for reading back (16384 x 8192 mxfp4 to bf16 65, 69, 61, 65).
 // Loads are ordinary ones: a prompt's rows come out of the memory-side cache, past which nontemporal loads go (1500 x 14336 to mxfp8 13.5 us, so 11.7).
 constexpr int kQuantizeUnits = 1, kDequantizeUnits = 4;
 struct UnitPlace {
@@ -347,11 +348,11 @@ __device__ __forceinline__ void quantize_columns(const TensorArg<2>& x, const Pa
 }
 
 // A row of up to WPR * 64 * VPL units in the registers of WPR wavefronts: read once, summed, scaled, quantised.  Bound by memory;
-// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 11.5 with a
-// wavefront of one unit a lane, 12.3 with two, 23 with four wavefronts; 4096 x 1024 4.7: 8.2 with one wavefront, 9.3 with four; 2048 x 2048 4.7: 8.2 with four
-// of two units, 8.8 of three; 1500 x 5120 8.5: 11.4 with four of three, 13.2 with eight of four; 16384 x 8192 149: 163 to 165 with four or eight of four
-// units, 245 with sixteen; 4096 x 16384 75: 87 with eight, 101 with sixteen; 2048 x 28672 65: 89 with sixteen.  Up to 500 rows every shape takes the time of a
-// launch.  The sum of squares in f64 costs 2 % of the short ones (f32 over four values, then f64: 1500 x 5120 11.2, and 4 of 134 million codes off).
+// what the shapes are for, bf16 with residual to mxfp8, us (rows read and written once at the rate of a large copy in front): 16384 x 512 9.3: 11.7 with a
+// wavefront of one unit a lane, 12.3 with two, 23 with four wavefronts; 4096 x 1024 4.7: 7.9 with one wavefront, 9.7 with four; 2048 x 2048 4.7: 8.4 with four
+// of two units, 8.9 of three; 1500 x 5120 8.5: 11.6 with four of three, 14.1 with eight of four; 16384 x 8192 149: 164 to 166 with four or eight of four
+// units, 240 with sixteen; 4096 x 16384 75: 89 with eight, 101 with sixteen; 2048 x 28672 65: 89 with sixteen.  Up to 500 rows every shape takes the time of a
+// launch.  The sum of squares in f64 costs 2 % of the short ones (f32 over four values, then f64: 1500 x 5120 11.4, and 4 of 134 million codes off).
 template <Format F, typename T, bool ADD, int WPR, int VPL, bool WHOLE>
 __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const TensorArg<2>& x, const TensorArg<1>& w, const PartitionArg<2>& out,
                                           const PartitionArg<2>& scales, const PartitionArg<2>* residual_out, NormMean m, TensorScale t, int64_t rows,

@@ -3,8 +3,8 @@
 //   block_dequantize     out <- values of (x, scales)
 //   rms_norm_quantize    out, scales <- c r w with c = x or residual + x, r = 1 / sqrt(mean(c^2) + eps); residual_out <- c
 //   silu_mul_quantize    out, scales <- gate / (1 + exp(-gate)) * up
-// Everything between the loads and the quantised store is f32 and stays in registers: the 16-bit rows that separate kernels would
-// hand on are neither written nor rounded to.  Rows of N values fill the first N columns of out, the columns behind them
+// Everything between the loads and the quantised store is f32 (sums of squares, and values next to a border of their format, f64) and stays in registers: the
+// 16-bit rows that separate kernels would hand on are neither written nor rounded to.  Rows of N values fill the first N columns of out, the columns behind them
 // (up to whole blocks, or to the K of the product that reads them) are zeros.
 //
 // A lane holds a unit of 8 consecutive values, the lanes of a block are neighbours (4, or 2 for nvfp4), and its scale is found

@@ -596,3 +596,36 @@ def test_gpu_norm_of_equal_values(ct, dev, fmt, n):
             other = ref.buffers(8, ref.padded(n, fmt), fmt, dev)
             ct.rms_norm_quantize(x.t().contiguous().t(), weights, whole(ct, other[0]), whole(ct, other[1]), 0.0, fmt)
             assert torch.equal(other[0], data) and torch.equal(other[1], scales)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp8", "nvfp4"])
+@pytest.mark.parametrize("rows", [1, 70, 300])
+def test_gpu_operands_of_the_products(ct, dev, fmt, rows):
+    """norm -> product -> gated activation -> product on 8-bit, and on nvfp4 operands made here: each product is that of the values its bytes
+    stand for, to what its own kernels are held to (1e-4 and 1e-5 of the norm in f32)"""
+    hidden, inter, kh, ki = 500, 700, 512, 768
+    dt = torch.bfloat16
+    x, r, w = normal((rows, hidden), 71, dev, dt), normal((rows, hidden), 72, dev, dt), (1 + 0.3 * normal((hidden,), 73, dev)).to(dt)
+    gate_up, down = normal((hidden, 2 * inter), 74, dev, dt, hidden ** -0.5).t(), normal((hidden, inter), 75, dev, dt, inter ** -0.5)
+
+    def operand(count, k, make, g):
+        data, scales = ref.buffers(count, k, fmt, dev)
+        make(whole(ct, data), whole(ct, scales), g)
+        return data, scales, ref.values(data, scales, fmt), torch.tensor(g, dtype=torch.float32).double().item()
+
+    def product(a, b, out):
+        run, alpha = (ct.linear_tile_mxfp8, 1.0) if fmt == "mxfp8" else (ct.linear_tile_nvfp4, a[3] * b[3])
+        run(ct.partition(out, [128, 128]), a[0], b[0], a[1], b[1], alpha)
+        want = alpha * (a[2] @ b[2].t())
+        assert float((out.double() - want).norm() / want.norm()) <= (1e-4 if fmt == "mxfp8" else 1e-5)
+
+    scale = lambda t: g_of(t, fmt)
+    wa = operand(2 * inter, kh, lambda d, s, g: ct.block_quantize(gate_up, d, s, fmt, g), scale(gate_up))
+    wd = operand(hidden, ki, lambda d, s, g: ct.block_quantize(down, d, s, fmt, g), scale(down))
+    a = operand(rows, kh, lambda d, s, g: ct.add_rms_norm_quantize(r, x, w, d, s, whole(ct, r), 1e-6, fmt, g), 8.0 / (6 * 448) if fmt == "nvfp4" else 1.0)
+    both = torch.zeros(rows, 2 * inter, device=dev)
+    product(a, wa, both)
+    half = both.to(dt)
+    h = operand(rows, ki, lambda d, s, g: ct.silu_mul_quantize(half[:, :inter], half[:, inter:], d, s, fmt, g), 16.0 / (6 * 448) if fmt == "nvfp4" else 1.0)
+    product(h, wd, torch.zeros(rows, hidden, device=dev))

@@ -34,11 +34,12 @@ __device__ __forceinline__ uint8_t* data_at(const PartitionArg<2>& out, int64_t 
 template <Format F>
 __device__ __forceinline__ uint8_t* scale_at(const PartitionArg<2>& scales, int64_t r, int32_t u) { return (uint8_t*)scales.ptr + r * scales.strides[0] + u / Traits<F>::kLanes; }
 
-// The eight values of unit u of a row of n, any stride; 0 behind the row.
+// The eight values of unit u of a row of n, any stride; 0 behind the row.  (Columns in 64 bits: 4-bit rows of 2^30 bytes and more have 2^31 values.)
 template <typename T>
 __device__ __forceinline__ void load_unit(const TensorArg<2>& t, int64_t r, int32_t u, int32_t n, float (&v)[8]) {
+  const int64_t j = (int64_t)u * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = u * 8 + i < n ? (float)*at<T>(t, r, u * 8 + i) : 0.0f;
+  for (int i = 0; i < 8; ++i) v[i] = j + i < n ? (float)*at<T>(t, r, j + i) : 0.0f;
 }
 
 // ---- values next to a border ---------------------------------------------------------------------------------------------
@@ -165,7 +166,10 @@ __device__ __forceinline__ void quantize_rows(const TensorArg<2>& x, const Tenso
       load_unit<T>(*up, r, u, n, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = silu_mul<F>(v[e], w[e]);
-      settle<F>(v, kSiluSlack, [&](int e) { return u * 8 + e < n ? silu_mul_f64((double)*at<T>(x, r, u * 8 + e), (double)*at<T>(*up, r, u * 8 + e)) : 0.0; });
+      settle<F>(v, kSiluSlack, [&](int e) {
+        const int64_t j = (int64_t)u * 8 + e;
+        return j < n ? silu_mul_f64((double)*at<T>(x, r, j), (double)*at<T>(*up, r, j)) : 0.0;
+      });
     }
     quantize_unit<F>(v, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
   }
@@ -462,10 +466,10 @@ __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const Te
       load(u, c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int32_t j = u * 8 + e;
+        const int64_t j = (int64_t)u * 8 + e;
         if (j >= n) continue;
         if constexpr (ADD) *at<T>(*residual_out, r, j) = (T)c[e];   // (may be residual or x itself: this thread has read the element)
-        c[e] = settled<F>(s.in_f64(c[e], (float)((const T*)w.ptr)[(int64_t)j * w.strides[0]]));
+        c[e] = settled<F>(s.in_f64(c[e], (float)((const T*)w.ptr)[j * w.strides[0]]));
       }
       quantize_unit<F>(c, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
     }
@@ -487,7 +491,7 @@ __device__ __forceinline__ void dequantize_rows(const TensorArg<2>& x, const Ten
     unpack_unit<F>(word[0], word[1], ((const uint8_t*)scales.ptr)[r * scales.strides[0] + u / Traits<F>::kLanes], g, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (u * 8 + e < n) *at<T>(out, r, u * 8 + e) = (T)v[e];
+      if ((int64_t)u * 8 + e < n) *at<T>(out, r, (int64_t)u * 8 + e) = (T)v[e];
   }
 }
 

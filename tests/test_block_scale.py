@@ -629,3 +629,40 @@ def test_gpu_operands_of_the_products(ct, dev, fmt, rows):
     half = both.to(dt)
     h = operand(rows, ki, lambda d, s, g: ct.silu_mul_quantize(half[:, :inter], half[:, inter:], d, s, fmt, g), 16.0 / (6 * 448) if fmt == "nvfp4" else 1.0)
     product(h, wd, torch.zeros(rows, hidden, device=dev))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["rows", "any", "silu", "norm", "add_norm"])
+def test_gpu_rows_padded_beyond_32_bit_columns(ct, dev, kind):
+    """4-bit rows of more than 2^31 values, a short row in front of zeros: what lies behind the row is neither read nor, in residual_out, written"""
+    k = (1 << 31) + 256
+    n = 100
+    data, scales = torch.full((1, k // 2), 0xA5, dtype=torch.uint8, device=dev), torch.full((1, k // 32), 0xA5, dtype=torch.uint8, device=dev)
+    outs = whole(ct, data), whole(ct, scales)
+    base = normal((2 * n, 4), 81, dev, torch.bfloat16)
+    x = base[::2, 1:2].t()                                                   # a stride between the columns
+    want = x.double()
+    if kind == "rows":
+        ct.block_quantize(x.contiguous(), *outs, "mxfp4", variant="mxfp4_bf16_rows")
+    elif kind == "any":
+        ct.block_quantize(x, *outs, "mxfp4", variant="mxfp4_bf16_any")
+    elif kind == "silu":
+        up = base[1::2, 2:3].t()
+        want = want / (1 + torch.exp(-want)) * up.double()
+        ct.silu_mul_quantize(x, up, *outs, "mxfp4", variant="mxfp4_bf16_any")
+    else:
+        w = torch.ones(n, dtype=torch.bfloat16, device=dev)
+        around = torch.full((1, n + 2000), 7.0, dtype=torch.bfloat16, device=dev)
+        if kind == "norm":
+            ct.rms_norm_quantize(x, w, *outs, 1e-6, "mxfp4")
+        else:
+            r = base[1::2, 2:3].t()
+            want = (x.float() + r.float()).double()
+            ct.add_rms_norm_quantize(r, x, w, *outs, whole(ct, around[:, 1000:1000 + n]), 1e-6, "mxfp4")
+            assert torch.equal(around[:, 1000:1000 + n], want.to(torch.bfloat16))
+        want = want / torch.sqrt(want.square().mean(-1, keepdim=True) + 1e-6)
+        assert bool((around[:, :1000] == 7.0).all()) and bool((around[:, 1000 + n:] == 7.0).all())
+    assert ct.last_resolved()["variant"].endswith("_rows" if kind == "rows" else "_any")
+    torch.cuda.synchronize()
+    ref.assert_quantised(data[:, :64], scales[:, :4], want, "mxfp4", slack=32 * 2.0 ** -24 if kind in ("silu", "norm", "add_norm") else 0.0)
+    assert int(torch.count_nonzero(data[:, 64:])) == 0 and int(torch.count_nonzero(scales[:, 4:])) == 0

@@ -54,18 +54,18 @@ template <Format F>
 __device__ __forceinline__ uint32_t border_distance(float v, uint32_t slack) {
   return F == kNvfp4 ? ~0u : (__builtin_bit_cast(uint32_t, v) + slack) & (F == kMxfp8 ? (1u << 19) - 1 : (1u << 21) - 1);
 }
-// y as a float on the same side of every border; what is closer to one than 2^-49 is on it (f64 results are off by 2^-51).
+// y as a float on the same side of every border; what is not further from one than `tie` of itself is on it.
 template <Format F>
-__device__ __forceinline__ float settled(double y) {
+__device__ __forceinline__ float settled(double y, double tie) {
   const float f = (float)y;
   const double left = y - (double)f;
-  if (border_distance<F>(f, 0) != 0 || !(__builtin_fabs(left) > __builtin_fabs(y) * 0x1p-49) || !__builtin_isfinite(left)) return f;
+  if (border_distance<F>(f, 0) != 0 || !(__builtin_fabs(left) > __builtin_fabs(y) * tie) || !__builtin_isfinite(left)) return f;
   const int32_t b = __builtin_bit_cast(int32_t, f);
   return __builtin_bit_cast(float, b + (((b >> 31) ^ (left < 0.0 ? -1 : 0)) | 1));
 }
 // A unit's values within `slack` steps of a border by `again(e)` of them; one iteration or none as a rule.
 template <Format F, class Again>
-__device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, Again again) {
+__device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, double tie, Again again) {
   if constexpr (F == kNvfp4) return;
   uint32_t border = ~0u;
 #pragma unroll
@@ -78,7 +78,7 @@ __device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, Again agai
   while (near != 0) {
     const int at = __builtin_ctz(near);
     near &= near - 1;
-    const float f = settled<F>(again(at));
+    const float f = settled<F>(again(at), tie);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e == at ? f : v[e];
   }
@@ -88,8 +88,11 @@ __device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, Again agai
 // exp(-|g| / 2): the exponential instruction flushes results below 2^-126, a product does not.  Off by less than kSiluSlack steps for g above -12
 // (what E loses grows with |g|).  nvfp4: the quotient is corrected once by its remainder.
 // (With the library's exponential and division 45 vector instructions a value, 31 us for 1500 x 14336 where memory takes 17.)
-// (What the values in f64 cost: 1500 x 14336 in a row of passes 20.7 us without them, 21.3 with; 52, 10 and 111 of 21.5 million codes were off, now 2, 1 and 3.)
+// (What the values in f64 cost: 1500 x 14336 in a row of passes 20.7 us without them, 21.3 with; 52, 10 and 111 of 21.5 million codes were off, now none.)
 constexpr uint32_t kSiluSlack = 32;
+// exp(-g) is no rational number, so no product is a border but where 1 + exp(-g) is 1 in f64, and there f64 has the product exactly: only what equals a
+// border is on it (gate 36 and factor 1.5 are 2^-52 below one).
+constexpr double kSiluTie = 0.0;
 template <Format F>
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float h = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0.72134752f);   // log2(e) / 2
@@ -107,6 +110,7 @@ struct NormMean {
 // c / sqrt(mean) * w: two products of f32 are off by 4.5 x 2^-24 of themselves at most (the mean's rounding, root, quotient and the products); in f64 two
 // Newton steps from there (nvfp4: rounded once, with r in two parts).  Of 134 million values at most one differed from the 64-bit result, 70 where the two f32 products are all.
 constexpr uint32_t kNormSlack = 8;
+constexpr double kNormTie = 0x1p-49;   // (f64 results are off by 2^-51)
 struct Scale {
   float r, rest;   // exact = r + rest
   double exact;
@@ -166,7 +170,7 @@ __device__ __forceinline__ void quantize_rows(const TensorArg<2>& x, const Tenso
       load_unit<T>(*up, r, u, n, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = silu_mul<F>(v[e], w[e]);
-      settle<F>(v, kSiluSlack, [&](int e) {
+      settle<F>(v, kSiluSlack, kSiluTie, [&](int e) {
         const int64_t j = (int64_t)u * 8 + e;
         return j < n ? silu_mul_f64((double)*at<T>(x, r, j), (double)*at<T>(*up, r, j)) : 0.0;
       });
@@ -264,7 +268,7 @@ __device__ __forceinline__ void quantize_units(const TensorArg<2>& x, const Tens
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = SILU ? silu_mul<F>((float)a[i].v[e], (float)b[SILU ? i : 0].v[e]) : (float)a[i].v[e];
     if constexpr (SILU)
-      settle<F>(v, kSiluSlack, [&](int e) {
+      settle<F>(v, kSiluSlack, kSiluTie, [&](int e) {
         const int64_t j = (int64_t)at[i].u * 8 + e;
         return j < n ? silu_mul_f64((double)((const T*)x.ptr)[(int64_t)at[i].r * x.strides[0] + j], (double)((const T*)up->ptr)[(int64_t)at[i].r * up->strides[0] + j]) : 0.0;
       });
@@ -408,7 +412,7 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = s.times<F>(c[i][e], (float)g[i].v[e]);
-    settle<F>(v, kNormSlack, [&](int at) {   // (from registers: a load here is what a row's last wavefront would wait for)
+    settle<F>(v, kNormSlack, kNormTie, [&](int at) {   // (from registers: a load here is what a row's last wavefront would wait for)
       float cv = 0.0f, gv = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) cv = e == at ? c[i][e] : cv, gv = e == at ? (float)g[i].v[e] : gv;
@@ -469,7 +473,7 @@ __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const Te
         const int64_t j = (int64_t)u * 8 + e;
         if (j >= n) continue;
         if constexpr (ADD) *at<T>(*residual_out, r, j) = (T)c[e];   // (may be residual or x itself: this thread has read the element)
-        c[e] = settled<F>(s.in_f64(c[e], (float)((const T*)w.ptr)[j * w.strides[0]]));
+        c[e] = settled<F>(s.in_f64(c[e], (float)((const T*)w.ptr)[j * w.strides[0]]), kNormTie);
       }
       quantize_unit<F>(c, t, data_at<F>(out, r, u), scale_at<F>(scales, r, u));
     }

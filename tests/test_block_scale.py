@@ -666,3 +666,42 @@ def test_gpu_rows_padded_beyond_32_bit_columns(ct, dev, kind):
     torch.cuda.synchronize()
     ref.assert_quantised(data[:, :64], scales[:, :4], want, "mxfp4", slack=32 * 2.0 ** -24 if kind in ("silu", "norm", "add_norm") else 0.0)
     assert int(torch.count_nonzero(data[:, 64:])) == 0 and int(torch.count_nonzero(scales[:, 4:])) == 0
+
+
+def assert_codes_of(data, scales, want, fmt):
+    """data and scales (mx formats) are the rounding of `want` itself, code by code"""
+    rows, n = want.shape
+    k = scales.shape[1] * 32
+    full = torch.zeros((rows, k), dtype=torch.float64, device=want.device)
+    full[:, :n] = want
+    blocks = full.view(rows, k // 32, 32)
+    exponents = ref._scale_codes(blocks.abs().amax(-1), fmt, 1.0)
+    assert torch.equal(scales.long(), exponents), int((scales.long() != exponents).sum())
+    codes = ref.nearest(blocks / torch.exp2(exponents.double() - 127).unsqueeze(-1), ref.grid_of(fmt)).view(rows, k)
+    got = (ref.unpack(data, fmt) & (127 if fmt == "mxfp8" else 7)).long()
+    assert torch.equal(codes, got), int((codes != got).sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sign", [1])
+def test_gpu_silu_mul_of_every_gate(ct, dev, fmt, dtype, sign):
+    """Every gate of the type from 1/2 to 84 of one sign, a row each, times every factor from 1 to 2, by both kernels: in the mx formats every code is the rounding of the
+    product itself, next to borders (36 x 1.5 is 2^-52 below one) and however far below 0 the gate is; nvfp4 within its roundings of f32"""
+    dt = TYPES[dtype]
+    every = torch.arange(1 << 15, dtype=torch.int32).to(torch.int16).view(dt)
+    every = sign * every[(every >= 0.5) & (every <= 84)].to(dev)
+    up = (1 + torch.arange(1 << (10 if dtype == "f16" else 7), device=dev) * torch.finfo(dt).eps).to(dt)
+    gate, up = every[:, None].expand(-1, up.numel()).contiguous(), up[None].expand(every.numel(), -1).contiguous()
+    x = gate.double()
+    want = x / (1 + torch.exp(-x)) * up.double()
+    rows, n = gate.shape
+    g = 2.0 ** (-60 if sign < 0 else -6) if fmt == "nvfp4" else 1.0
+    for view in (lambda t: t, lambda t: t.t().contiguous().t()):
+        data, scales = ref.buffers(rows, n, fmt, dev)
+        ct.silu_mul_quantize(view(gate), view(up), whole(ct, data), whole(ct, scales), fmt, g)
+        if fmt == "nvfp4":
+            ref.assert_quantised(data, scales, want, fmt, g, slack=6 * 2.0 ** -24 + NVFP4_SLACK)
+        else:
+            assert_codes_of(data, scales, want, fmt)

@@ -84,24 +84,30 @@ __device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, double tie
   }
 }
 
-// g / (1 + exp(-g)) * u, through E = exp(-|g|) <= 1, which nothing overflows: (max(g, 0) + min(g, 0) E) / (1 + E).  E is the square of
-// exp(-|g| / 2): the exponential instruction flushes results below 2^-126, a product does not.  Off by less than kSiluSlack steps for g above -12
-// (what E loses grows with |g|).  nvfp4: the quotient is corrected once by its remainder.
+// g / (1 + exp(-g)) * u, through h = exp(-|g| / 2) <= 1, which nothing overflows: g / (1 + h^2) times u, or u h^2 where g is below 0.  The square leaves f32 at
+// |g| = 87, its product with a large u need not, so u is multiplied by h twice; from 174 on h itself is 0 (the product is below 2^-115 there).
+// Off by less than 16 + 2 |min(g, 0)| steps: exponential twice 4, the products with it 2, sum 1, reciprocal 2, products 2, and 1.23 |g| where h is a factor of the
+// result (the argument's rounding 1, that of log2(e) 0.23).  nvfp4: the quotient is corrected once by its remainder.
 // (With the library's exponential and division 45 vector instructions a value, 31 us for 1500 x 14336 where memory takes 17.)
-// (What the values in f64 cost: 1500 x 14336 in a row of passes 20.7 us without them, 21.3 with; 52, 10 and 111 of 21.5 million codes were off, now none.)
-constexpr uint32_t kSiluSlack = 32;
-// exp(-g) is no rational number, so no product is a border but where 1 + exp(-g) is 1 in f64, and there f64 has the product exactly: only what equals a
-// border is on it (gate 36 and factor 1.5 are 2^-52 below one).
-constexpr double kSiluTie = 0.0;
 template <Format F>
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float h = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -0.72134752f);   // log2(e) / 2
-  const float e = h * h, d = 1.0f + e, q = __builtin_amdgcn_rcpf(d);
-  const float n = __builtin_fmaf(fminf(g, 0.0f), e, fmaxf(g, 0.0f)), y = n * q;
-  if constexpr (F != kNvfp4) return __builtin_fmaf(y, u, kTiny);
-  return __builtin_fmaf(__builtin_fmaf(-y, d, n), q, y) * u;
+  const float d = __builtin_fmaf(h, h, 1.0f), q = __builtin_amdgcn_rcpf(d), y = g * q, s = g > 0.0f ? u : u * h * h;
+  if constexpr (F != kNvfp4) return __builtin_fmaf(y, s, kTiny);
+  return __builtin_fmaf(__builtin_fmaf(-y, d, g), q, y) * s;
 }
 __device__ __forceinline__ double silu_mul_f64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+// The unit's gates `v` and factors `w` to their products, those next to a border by `again(e)` in f64.  exp(-g) is no rational number, so no product is a border
+// but where 1 + exp(-g) is 1 in f64, and there f64 has the product exactly: only what equals a border is on it (gate 36 and factor 1.5 are 2^-52 below one).
+template <Format F, class Again>
+__device__ __forceinline__ void silu_unit(float (&v)[8], const float (&w)[8], Again again) {
+  float low = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) low = fminf(low, v[e]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = silu_mul<F>(v[e], w[e]);
+  settle<F>(v, (uint32_t)__builtin_fmaf(-2.0f, fmaxf(low, -175.0f), 16.0f), 0.0, again);
+}
 
 // mean(c^2) + eps = sum * inv_n + eps
 struct NormMean {
@@ -168,9 +174,7 @@ __device__ __forceinline__ void quantize_rows(const TensorArg<2>& x, const Tenso
     if constexpr (SILU) {
       float w[8];
       load_unit<T>(*up, r, u, n, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = silu_mul<F>(v[e], w[e]);
-      settle<F>(v, kSiluSlack, kSiluTie, [&](int e) {
+      silu_unit<F>(v, w, [&](int e) {
         const int64_t j = (int64_t)u * 8 + e;
         return j < n ? silu_mul_f64((double)*at<T>(x, r, j), (double)*at<T>(*up, r, j)) : 0.0;
       });
@@ -266,12 +270,16 @@ __device__ __forceinline__ void quantize_units(const TensorArg<2>& x, const Tens
     if (!at[i].live) continue;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = SILU ? silu_mul<F>((float)a[i].v[e], (float)b[SILU ? i : 0].v[e]) : (float)a[i].v[e];
-    if constexpr (SILU)
-      settle<F>(v, kSiluSlack, kSiluTie, [&](int e) {
+    for (int e = 0; e < 8; ++e) v[e] = (float)a[i].v[e];
+    if constexpr (SILU) {
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = (float)b[i].v[e];
+      silu_unit<F>(v, w, [&](int e) {
         const int64_t j = (int64_t)at[i].u * 8 + e;
         return j < n ? silu_mul_f64((double)((const T*)x.ptr)[(int64_t)at[i].r * x.strides[0] + j], (double)((const T*)up->ptr)[(int64_t)at[i].r * up->strides[0] + j]) : 0.0;
       });
+    }
     quantize_unit<F>(v, t, data_at<F>(out, at[i].r, at[i].u), scale_at<F>(scales, at[i].r, at[i].u));
   }
 }

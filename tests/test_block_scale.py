@@ -682,10 +682,16 @@ def assert_codes_of(data, scales, want, fmt):
     assert torch.equal(codes, got), int((codes != got).sum())
 
 
+def silu_steps(gate):
+    """what an nvfp4 gated product is off by, relative: exponential twice 4 steps of 2^-24, products with it 2, sum 1, quotient 1, product 1, and for negative gates
+    1.23 |g|, the rounding of the exponential's argument"""
+    return (9 + 1.23 * float(gate.abs().max())) * 2.0 ** -24
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("sign", [1])
+@pytest.mark.parametrize("sign", [-1, 1])
 def test_gpu_silu_mul_of_every_gate(ct, dev, fmt, dtype, sign):
     """Every gate of the type from 1/2 to 84 of one sign, a row each, times every factor from 1 to 2, by both kernels: in the mx formats every code is the rounding of the
     product itself, next to borders (36 x 1.5 is 2^-52 below one) and however far below 0 the gate is; nvfp4 within its roundings of f32"""
@@ -702,6 +708,27 @@ def test_gpu_silu_mul_of_every_gate(ct, dev, fmt, dtype, sign):
         data, scales = ref.buffers(rows, n, fmt, dev)
         ct.silu_mul_quantize(view(gate), view(up), whole(ct, data), whole(ct, scales), fmt, g)
         if fmt == "nvfp4":
-            ref.assert_quantised(data, scales, want, fmt, g, slack=6 * 2.0 ** -24 + NVFP4_SLACK)
+            ref.assert_quantised(data, scales, want, fmt, g, slack=silu_steps(gate) + NVFP4_SLACK)
+        else:
+            assert_codes_of(data, scales, want, fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gpu_silu_mul_of_far_gates_and_large_factors(ct, dev, fmt):
+    """exp(g) below what f32 holds, times a factor that brings the product back: gates from -64 to -150, factors up to 2^127; beside them far positive gates"""
+    rows, n = 300, 512
+    gate = (-64 - 86 * torch.rand((rows, n), generator=torch.Generator().manual_seed(93))).to(dev).bfloat16()
+    up = (torch.exp2(torch.floor(-gate.double() * 1.442) - 20).clamp(max=2.0 ** 126) * (1 + normal((rows, n), 94, dev).double().abs().clamp(max=0.99))).bfloat16()
+    steps = silu_steps(gate)
+    gate[:, 64:96] = 3e38
+    up[:, 64:96] = 0.1
+    x = gate.double()
+    want = x / (1 + torch.exp(-x)) * up.double()
+    for view in (lambda t: t, lambda t: t.t().contiguous().t()):
+        data, scales = ref.buffers(rows, n, fmt, dev)
+        ct.silu_mul_quantize(view(gate), view(up), whole(ct, data), whole(ct, scales), fmt, 2.0 ** -20 if fmt == "nvfp4" else 1.0)
+        if fmt == "nvfp4":
+            ref.assert_quantised(data, scales, want, fmt, 2.0 ** -20, slack=steps + NVFP4_SLACK)
         else:
             assert_codes_of(data, scales, want, fmt)

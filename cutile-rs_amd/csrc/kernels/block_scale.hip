@@ -63,7 +63,19 @@ __device__ __forceinline__ float settled(double y, double tie) {
   const int32_t b = __builtin_bit_cast(int32_t, f);
   return __builtin_bit_cast(float, b + (((b >> 31) ^ (left < 0.0 ? -1 : 0)) | 1));
 }
-// A unit's values within `slack` steps of a border by `again(e)` of them; one iteration or none as a rule.
+// The values of the bits in `which` by `again(e)` of them.
+template <Format F, class Again>
+__device__ __forceinline__ void retake(float (&v)[8], uint32_t which, double tie, Again again) {
+#pragma unroll 1
+  while (which != 0) {
+    const int at = __builtin_ctz(which);
+    which &= which - 1;
+    const float f = settled<F>(again(at), tie);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e == at ? f : v[e];
+  }
+}
+// Those of a unit within `slack` steps of a border; one or none as a rule.
 template <Format F, class Again>
 __device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, double tie, Again again) {
   if constexpr (F == kNvfp4) return;
@@ -74,14 +86,7 @@ __device__ __forceinline__ void settle(float (&v)[8], uint32_t slack, double tie
   uint32_t near = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) near |= border_distance<F>(v[e], slack) <= 2 * slack ? 1u << e : 0u;
-#pragma unroll 1
-  while (near != 0) {
-    const int at = __builtin_ctz(near);
-    near &= near - 1;
-    const float f = settled<F>(again(at), tie);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e == at ? f : v[e];
-  }
+  retake<F>(v, near, tie, again);
 }
 
 // g / (1 + exp(-g)) * u, through h = exp(-|g| / 2) <= 1, which nothing overflows: g / (1 + h^2) times u, or u h^2 where g is below 0.  The square leaves f32 at
@@ -127,14 +132,20 @@ struct Scale {
   }
   __device__ __forceinline__ double in_f64(float c, float w) const { return (double)c * exact * (double)w; }
 };
+// The root is taken in f32, of a mean whose f32 is neither 0 nor subnormal: one below 2^-100 (eps = 0) is scaled by an even power of two.  A mean of 2^128 and more,
+// of rows whose root mean square is 2^64 and more, is infinite in f32, and the row 0.
 __device__ __forceinline__ Scale norm_scale(double mean) {
+  const bool small = mean > 0.0 && mean < 0x1p-100;
+  const double m = small ? mean * 0x1p200 : mean;
   Scale s;
-  s.r = 1.0f / sqrtf((float)mean);
-  s.exact = (double)s.r;
-  if (s.r > 0.0f && s.r < __builtin_inff()) {   // (rows of zeros, infinities and NaN, and beyond f32, stay as they are)
+  const float r = 1.0f / sqrtf((float)m);
+  s.exact = (double)r;
+  if (r > 0.0f && r < __builtin_inff()) {   // (rows of zeros, infinities and NaN, and beyond f32, stay as they are)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) s.exact = __builtin_fma(0.5 * s.exact, __builtin_fma(-mean * s.exact, s.exact, 1.0), s.exact);
+    for (int i = 0; i < 2; ++i) s.exact = __builtin_fma(0.5 * s.exact, __builtin_fma(-m * s.exact, s.exact, 1.0), s.exact);
   }
+  if (small) s.exact *= 0x1p100;
+  s.r = (float)s.exact;
   s.rest = (float)(s.exact - (double)s.r);
   if (!__builtin_isfinite(s.rest)) s.rest = 0.0f;   // (infinity less infinity)
   return s;
@@ -420,12 +431,14 @@ __device__ __forceinline__ void norm_held(const TensorArg<2>* residual, const Te
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = s.times<F>(c[i][e], (float)g[i].v[e]);
-    settle<F>(v, kNormSlack, kNormTie, [&](int at) {   // (from registers: a load here is what a row's last wavefront would wait for)
+    auto again = [&](int at) {   // (from registers: a load here is what a row's last wavefront would wait for)
       float cv = 0.0f, gv = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) cv = e == at ? c[i][e] : cv, gv = e == at ? (float)g[i].v[e] : gv;
       return s.in_f64(cv, gv);
-    });
+    };
+    if (F == kNvfp4 && s.r == __builtin_inff()) retake<F>(v, 0xff, kNormTie, again);   // a row of subnormals: f32 does not hold its r (infinities lie on a border of the mx formats)
+    settle<F>(v, kNormSlack, kNormTie, again);
     if constexpr (ADD) {   // (may be residual or x itself: this lane has read what it writes)
       Unit<T> o;
 #pragma unroll

@@ -772,7 +772,8 @@ cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cut
                                                float tensor_scale, const cutile_partition_arg_t* out, const cutile_launch_opts_t* opts);
 /* The kernels in front of a block-scaled product with its operand as their output (x, w, gate, up f16 or bf16 alike, any
  * strides; f32 or more from the loads to the one rounding of block_quantize, nothing rounded to 16 bits in between):
- *   rms_norm_quantize       x / sqrt(mean(x^2) + eps) * w
+ *   rms_norm_quantize       x / sqrt(mean(x^2) + eps) * w, squares summed in f64; a mean of 2^128 and more (bf16 rows whose root mean square is 2^64
+ *                           and more) counts as infinite: the row is 0
  *   add_rms_norm_quantize   the same of c = residual + x; residual_out <- c, rounded once; it may be residual or x itself
  *   silu_mul_quantize       gate / (1 + exp(-gate)) * up */
 cutile_status_t cutile_launch_rms_norm_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* w,

@@ -732,3 +732,28 @@ def test_gpu_silu_mul_of_far_gates_and_large_factors(ct, dev, fmt):
             ref.assert_quantised(data, scales, want, fmt, 2.0 ** -20, slack=steps + NVFP4_SLACK)
         else:
             assert_codes_of(data, scales, want, fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("add", [False, True])
+def test_gpu_norm_of_small_rows(ct, dev, fmt, add):
+    """eps = 0 and rows whose mean square f32 holds badly (below 2^-126) or not at all, down to rows of nothing but subnormals: an ordinary norm of about w, by every kernel"""
+    exponents = [-40, -55, -62, -64, -70, -75, -90, -120, -126, -130, -132]
+    n = 500
+    x, r = (torch.stack([normal((n,), 100 * i + j, dev) * 2.0 ** e for j, e in enumerate(exponents)]).bfloat16() for i in (1, 2))
+    w = (1 + 0.3 * normal((n,), 3, dev)).bfloat16()
+    c = (x.float() + r.float()).double() if add else x.double()
+    want = c / torch.sqrt(c.square().mean(-1, keepdim=True)) * w.double()
+    k, g = 512, 2.0 ** -9 if fmt == "nvfp4" else 1.0
+    function = "add_rms_norm_quantize" if add else "rms_norm_quantize"
+    for variant in variants_of(ct, function, fmt + "_bf16_"):
+        data, scales = ref.buffers(len(exponents), k, fmt, dev)
+        if add:
+            ct.add_rms_norm_quantize(r, x, w, whole(ct, data), whole(ct, scales), whole(ct, torch.empty_like(x)), 0.0, fmt, g, variant=variant)
+        else:
+            ct.rms_norm_quantize(x, w, whole(ct, data), whole(ct, scales), 0.0, fmt, g, variant=variant)
+        if fmt == "nvfp4":
+            ref.assert_quantised(data, scales, want, fmt, g, slack=2.0 ** -24 + NVFP4_SLACK)       # one rounding to f32
+        else:
+            assert_codes_of(data, scales, want, fmt)

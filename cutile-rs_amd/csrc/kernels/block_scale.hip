@@ -121,7 +121,9 @@ struct NormMean {
 // c / sqrt(mean) * w: two products of f32 are off by 4.5 x 2^-24 of themselves at most (the mean's rounding, root, quotient and the products); in f64 two
 // Newton steps from there (nvfp4: rounded once, with r in two parts).  Of 134 million values at most one differed from the 64-bit result, 70 where the two f32 products are all.
 constexpr uint32_t kNormSlack = 8;
-constexpr double kNormTie = 0x1p-49;   // (f64 results are off by 2^-51)
+// What the norm in f64 may be off by: half of what the sum of squares collects, 2^-53 for each of the additions that a value passes (held rows 8 + 4 in its lane, 6 + 16
+// across lanes and wavefronts; otherwise n / 2048 + 8 and 10), and 4 for mean, root and products: below 2^-44 for rows of up to 2^20 values.
+constexpr double kNormTie = 0x1p-44;
 struct Scale {
   float r, rest;   // exact = r + rest
   double exact;
@@ -483,8 +485,10 @@ __device__ __forceinline__ void norm_rows(const TensorArg<2>* residual, const Te
     double ss = 0.0;
     for (int32_t u = threadIdx.x; u < units; u += kThreads) {
       load(u, c);
+      double sum = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)c[e], (double)c[e], ss);
+      for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)c[e], (double)c[e], sum);
+      ss += sum;
     }
     const Scale s = norm_scale(__builtin_fma(workgroup_sum(ss), m.inv_n, m.eps));
     for (int32_t u = threadIdx.x; u < units; u += kThreads) {

@@ -757,3 +757,40 @@ def test_gpu_norm_of_small_rows(ct, dev, fmt, add):
             ref.assert_quantised(data, scales, want, fmt, g, slack=2.0 ** -24 + NVFP4_SLACK)       # one rounding to f32
         else:
             assert_codes_of(data, scales, want, fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("n", [5000, 32768, 40000, 262144])
+def test_gpu_norm_of_equal_values_whose_squares_do_not_add_up(ct, dev, fmt, n):
+    """as test_gpu_norm_of_equal_values, with c of 24 bits: sums of its squares are rounded (by 2^-47 of themselves and more where each thread adds a thousand), and the norm is w
+    all the same - on a border between two codes or scales"""
+    r = torch.tensor([1.0, -1.0, 1.5, 1.25, 1.0], device=dev).bfloat16()[:, None].expand(-1, n).contiguous()
+    x = torch.tensor([2.0 ** -23, -2.0 ** -23, 2.0 ** -23, 1.5 * 2.0 ** -22, 2.0 ** -22], device=dev).bfloat16()[:, None].expand(-1, n).contiguous()
+    k = ref.padded(n, fmt)
+    for w in (1.0, 2.0, 1.0625, 1.1875, 2.5, 5.0, 1.75):
+        weights = torch.full((n,), w, dtype=torch.bfloat16, device=dev)
+        for last in (1.0, 4.0):
+            weights[::32] = last * w
+            want = torch.sign(r.double()) * weights.double()
+            for view in (lambda t: t, lambda t: t.t().contiguous().t()):
+                data, scales = ref.buffers(5, k, fmt, dev)
+                ct.add_rms_norm_quantize(view(r), view(x), weights, whole(ct, data), whole(ct, scales), whole(ct, torch.empty_like(x)), 0.0, fmt)
+                assert_codes_of(data, scales, want, fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,n,strided", [(300, 4096, True), (60, 20001, True), (40, 40000, False), (12, 100003, True)])
+def test_gpu_norm_of_any_rows_rounds_the_value_itself(ct, dev, fmt, dtype, rows, n, strided):
+    """test_gpu_norm_rounds_the_value_itself where no kernel holds the row: strides, and more than 32768 values"""
+    dt = TYPES[dtype]
+    x, r, w = normal((rows, n), 55, dev, dt), normal((rows, n), 56, dev, dt, 3.0), (1 + 0.3 * normal((n,), 57, dev)).to(dt)
+    c = (x.float() + r.float()).double()                                     # the sum is one of f32
+    want = c / torch.sqrt(c.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+    view = (lambda t: t.t().contiguous().t()) if strided else (lambda t: t)
+    data, scales = ref.buffers(rows, ref.padded(n, fmt), fmt, dev)
+    ct.add_rms_norm_quantize(view(r), view(x), w, whole(ct, data), whole(ct, scales), whole(ct, torch.empty_like(x)), 1e-6, fmt)
+    assert ct.last_resolved()["variant"].endswith("_any")
+    assert_codes_of(data, scales, want, fmt)

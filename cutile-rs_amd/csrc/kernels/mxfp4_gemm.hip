@@ -30,6 +30,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // hand-over of the stages sits one product before the last y block, where every read of the stage has had a block's products to complete; the
 // refill of the stage just drained is dealt out over the products behind it.
 // Scales: 16 bytes of a row serve two K tiles; they are fetched with the first of these into one of two buffers.
+// (256 x 256: all 256 registers; 3 more, 5 with f32 out, are stored in front of the K loop and read back behind it.)
 template <int BM, int BN, int WAVES_M, int WAVES_N, typename OutT>
 struct Mxfp4Direct {
   static constexpr int kRow = 128;                                             // bytes of a row in a K tile of 256 values

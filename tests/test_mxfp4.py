@@ -121,6 +121,21 @@ def test_rule(fake_hip):
     assert chosen(ct, 600, 512, 16384, (256, 256), grid=(2, 1, 1)) == ("bf16_256x256x256_e4x2", 2)
 
 
+def test_registers_of_the_products(fake_hip):
+    """only the 256 x 256 kernels, which take every register, keep some in memory, outside their K loop"""
+    import os
+    import re
+    import subprocess
+
+    lib = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cutile-rs_amd", "lib")
+    for image in ("mxfp4", "mxfp4flat"):
+        notes = subprocess.run(["/opt/rocm/llvm/bin/llvm-readelf", "--notes", os.path.join(lib, image + ".hsaco")], stdout=subprocess.PIPE, text=True, check=True).stdout
+        for kernel in notes.split("- .agpr_count")[1:]:
+            symbol = re.search(r"\n    \.name: +(\S+)", kernel)[1]
+            most = 0 if "256x256x256" not in symbol else 3 if "bf16" in symbol else 5
+            assert int(re.search(r"\.vgpr_spill_count: (\d+)", kernel)[1]) <= most, symbol
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k,shares", SHARED)
 def test_gpu_mxfp4_shared_k(ct, dev, m, n, k, shares):

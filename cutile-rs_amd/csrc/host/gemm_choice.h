@@ -403,9 +403,10 @@ struct Mxfp4Strip {
 };
 constexpr Mxfp4Strip kMxfp4Strips[] = {{"flat16x64", 16, 64, 0.071, 0.134, 1.8, 2.9, 1.07}, {"flat32x64", 32, 64, 0.086, 0.148, 3.1, 2.0, 0.92}, {"flat64x64", 64, 64, 0.087, 0.177, 4.1, 0.8, 0.77}};
 // MXFP4 by name.  Strips, 128 x 128 tiles with a compute unit each, two such tiles to a compute unit, or 256 x 256 tiles: the one priced lowest.  Least squares over
-// 220 products of 1 to 8192 rows and 512 to 16384 values of K, operands from memory, every kernel timed (strips 7 % rms, tiles 7 to 8): it takes 1.008 of the best one's
-// time, and 1.19 at most.  us, bf16 out, on the best strips, on 128 x 128 and on 256 x 256: 1 x 14336 x 4096 8.5, 12.3, 28; 64 x 14336 x 4096 11.1, 11.8, 28;
-// 200 x 14336 x 4096 31.8, 13.7, 29; 1000 x 4096 x 4096 22.7, 16.0, 30; 2048 x 14336 x 4096 -, 84, 73; 3661 x 6240 x 6016 -, 105, 99; 4096 x 4096 x 4096 -, 46, 38.
+// 220 products of 1 to 8192 rows and 512 to 16384 values of K, operands from memory, every kernel timed (strips 7 % rms, tiles 7 to 8).  Over 220 others, 128 to 16384 values of
+// K, it takes 0.99 of the time of the best one by name (the noise of two timings), 1.15 at most.  us, bf16 out, on the best strips, on 128 x 128 and on 256 x 256, and what
+// memory or matrix pipes alone would take: 1 x 14336 x 4096 8.5, 12.3, 28 (4.9); 64 x 14336 x 4096 11.1, 11.8, 28 (5.2); 200 x 14336 x 4096 31.8, 13.7, 29 (5.9);
+// 1000 x 4096 x 4096 22.7, 16.0, 30 (5.7); 2048 x 14336 x 4096 -, 84, 73 (41); 3661 x 6240 x 6016 -, 105, 99 (47); 4096 x 4096 x 4096 -, 46, 38 (23.5).
 inline const char* choose_mxfp4(const ScaledShape& s, int cus, uint64_t partial_bytes, MxPlan* lone) {
   const char* name = nullptr;
   double best = 1e30;

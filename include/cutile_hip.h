@@ -763,7 +763,8 @@ cutile_status_t cutile_launch_linear_tile_nvfp4(cutile_stream_t stream, const cu
  * x: [M, N] f16, bf16 or f32 with any strides; N of any length up to K.  out: K whole blocks a row, columns N .. K - 1 zeros
  * (so rows can be made as long as the product that reads them wants).  out and scales are partitioned [BM, whole row] alike
  * and may have fewer rows than x; their rows are contiguous and apart, those of out on 8-byte boundaries.  tensor_scale is 1 for
- * the mx formats and between 2^-100 and 2^100 for nvfp4.  Generic 0, when given, is N.  Outputs share no memory with inputs. */
+ * the mx formats and between 2^-100 and 2^100 for nvfp4 (a number of the host: it is not found here, and a captured launch keeps
+ * it).  Generic 0, when given, is N.  Outputs share no memory with inputs. */
 cutile_status_t cutile_launch_block_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_partition_arg_t* out,
                                              const cutile_partition_arg_t* scales, float tensor_scale, const cutile_launch_opts_t* opts);
 /* block_dequantize: out [M, N] <- the values that x and scales stand for (nvfp4: in f32), N up to K, rounded once to f16, bf16 or f32; out has
@@ -774,8 +775,9 @@ cutile_status_t cutile_launch_block_dequantize(cutile_stream_t stream, const cut
  * strides; f32 or more from the loads to the one rounding of block_quantize, nothing rounded to 16 bits in between):
  *   rms_norm_quantize       x / sqrt(mean(x^2) + eps) * w, squares summed in f64; a mean of 2^128 and more (bf16 rows whose root mean square is 2^64
  *                           and more) counts as infinite: the row is 0
- *   add_rms_norm_quantize   the same of c = residual + x; residual_out <- c, rounded once; it may be residual or x itself
- *   silu_mul_quantize       gate / (1 + exp(-gate)) * up */
+ *   add_rms_norm_quantize   the same of c = residual + x, a sum of f32; residual_out <- c, rounded once; it may be residual or x itself
+ *   silu_mul_quantize       gate / (1 + exp(-gate)) * up
+ * mxfp8 and mxfp4 rows are the rounding of the 64-bit results (values below 2^-118: of the f32 ones), nvfp4 rows of f32 results. */
 cutile_status_t cutile_launch_rms_norm_quantize(cutile_stream_t stream, const cutile_tensor_arg_t* x, const cutile_tensor_arg_t* w,
                                                 const cutile_partition_arg_t* out, const cutile_partition_arg_t* scales, float eps,
                                                 float tensor_scale, const cutile_launch_opts_t* opts);

@@ -172,6 +172,10 @@ def lib() -> C.CDLL:
             "cutile_launch_add_rms_norm_quantize": [vp, P(TensorArg), P(TensorArg), P(TensorArg), P(PartitionArg), P(PartitionArg), P(PartitionArg),
                                                     f32, f32, P(LaunchOpts)],
             "cutile_launch_silu_mul_quantize": [vp, P(TensorArg), P(TensorArg), P(PartitionArg), P(PartitionArg), f32, P(LaunchOpts)],
+            "cutile_launch_paged_cache_write": [vp] + [P(TensorArg)] * 9 + [P(LaunchOpts)],
+            "cutile_launch_paged_cache_read": [vp] + [P(TensorArg)] * 7 + [P(PartitionArg), P(PartitionArg), P(LaunchOpts)],
+            "cutile_launch_paged_attention": [vp] + [P(TensorArg)] * 8 + [P(PartitionArg), f32, i32, i32, i32, P(TensorArg), P(LaunchOpts)],
+            "cutile_launch_adjust_logits": [vp, P(TensorArg), P(PartitionArg)] + [P(TensorArg)] * 9 + [P(LaunchOpts)],
             "cutile_partition_grid": [P(PartitionArg), P(C.c_uint32 * 3)],
             "cutile_mapped_partition_grid": [P(MappedPartitionArg), P(C.c_uint32 * 3)],
             "cutile_mapped_partition_index": [P(MappedPartitionArg), C.c_uint32, P(C.c_uint32 * 3), P(C.c_uint32)],
@@ -832,6 +836,59 @@ def silu_mul_quantize(gate, up, out: Partition, scales: Partition, fmt: str, ten
     """silu(gate) * up as block-scaled rows (formats: block_quantize); gate and up f16 or bf16"""
     o, s = _block_outputs(fmt, out, scales)
     _c.silu_mul_quantize(stream, gate, up, o, s, float(tensor_scale), (grid, generics, variant))
+
+
+# ---- a serving step over a paged cache ------------------------------------------------------------------------------------
+def _cache_types(k_cache, v_cache, k_scales, v_scales):
+    """the caches and scales with the element types that they stand for: mxfp8 where there are scales"""
+    for t in (k_cache, v_cache, k_scales, v_scales):
+        if t is not None and any(n > 1 and s >= 2 ** 31 for n, s in zip(t.shape, t.stride())):
+            raise CutileError(-2, "a cache's strides must be below 2^31 elements")
+    if k_scales is None and v_scales is None:
+        return k_cache, v_cache, None, None
+    if k_scales is None or v_scales is None:
+        raise CutileError(-2, "k_scales and v_scales come together")
+    _block_types("mxfp8", k_cache, v_cache, k_scales, v_scales)
+    return (k_cache, F8E4M3FN), (v_cache, F8E4M3FN), (k_scales, F8E8M0FNU), (v_scales, F8E8M0FNU)
+
+
+def paged_cache_write(new_k, new_v, k_cache, v_cache, page_table, starts, context_lens, *, k_scales=None, v_scales=None, stream=None,
+                      variant=None) -> None:
+    """New tokens' K and V [tokens, kv_heads, D] into the pages of caches [pages, page_size, kv_heads, D]: f16, bf16, or mxfp8 with scales
+    [pages, page_size, kv_heads, D/32].  Rows starts[b] .. starts[b+1] are the last of the context_lens[b] tokens of sequence b, and position p lies on
+    page page_table[b, p // page_size], row p % page_size; tokens whose page is none of the cache's are left out."""
+    k, v, ks, vs = _cache_types(k_cache, v_cache, k_scales, v_scales)
+    _c.paged_cache_write(stream, new_k, new_v, k, v, ks, vs, page_table, starts, context_lens, (None, None, variant))
+
+
+def paged_cache_read(k_cache, v_cache, page_table, starts, context_lens, out_k: Partition, out_v: Partition, *, k_scales=None, v_scales=None,
+                     stream=None, grid=None, variant=None) -> None:
+    """the inverse of paged_cache_write: out_k, out_v [tokens, kv_heads, D] (f16, bf16; partitions [BM, kv_heads, D]) <- what lies at
+    the places of their rows, zeros where there is no such place"""
+    k, v, ks, vs = _cache_types(k_cache, v_cache, k_scales, v_scales)
+    _c.paged_cache_read(stream, k, v, ks, vs, page_table, starts, context_lens, out_k, out_v, (grid, None, variant))
+
+
+PAGED_ATTENTION_WORKSPACE_BYTES = (40 << 20) + (16 << 10)
+
+
+def paged_attention(q, k_cache, v_cache, page_table, starts, context_lens, out: Partition, qk_scale: float, *, window: int = 0, max_new: int = 0,
+                    max_context: int = 0, k_scales=None, v_scales=None, workspace=None, stream=None, grid=None, variant=None) -> None:
+    """Causal attention of new tokens q [tokens, q_heads, D] over a paged cache that holds them already (arguments as in paged_cache_write); out of q's shape,
+    partitioned [BM, G, D].  A token sees the keys up to its own position, the last ``window`` of them where that is not 0.  ``max_new``: at least the most
+    new tokens of a sequence, ``max_context``: about the longest context (0: not known).  ``workspace``: device memory for a launch that is
+    captured, zeros before its first use, one stream at a time; up to PAGED_ATTENTION_WORKSPACE_BYTES are used."""
+    k, v, ks, vs = _cache_types(k_cache, v_cache, k_scales, v_scales)
+    _c.paged_attention(stream, q, k, v, ks, vs, page_table, starts, context_lens, out, float(qk_scale), window, max_new, max_context, workspace, (grid, None, variant))
+
+
+def adjust_logits(logits, out: Partition, *, tokens=None, prompt_lens=None, token_lens=None, repetition=None, presence=None, frequency=None,
+                  bias_ids=None, bias_values=None, allowed=None, stream=None, grid=None, variant=None) -> None:
+    """Logits [rows, vocab] (f16, bf16, f32) -> out (may be logits), partitioned [1, vocab], before a token is chosen.  Tokens among ``tokens``
+    [rows, most] (the first token_lens of them) have l / repetition or, below 0, l * repetition; those c > 0 times behind the first prompt_lens
+    l - (presence + frequency c); then l + biases (ids and values [rows, n], n <= 1024); then -inf where bit t % 32 of allowed[row, t // 32] is not
+    set."""
+    _c.adjust_logits(stream, logits, out, tokens, prompt_lens, token_lens, repetition, presence, frequency, bias_ids, bias_values, allowed, (grid, None, variant))
 
 
 # ---- table / device helpers -------------------------------------------------------------------

@@ -44,6 +44,9 @@ IMAGES = {
     "mxfp4": "mxfp4_gemm.hip",
     "mxfp4flat": "mxfp4_flat.hip",
     "blockscale": "block_scale.hip",
+    "pagedcache": "paged_cache.hip",
+    "pagedattention": "paged_attention.hip",
+    "logits": "adjust_logits.hip",
 }
 HOST_SOURCES = ["hip_api.cpp", "driver.cpp", "kernel_table.cpp", "launch.cpp", "runtime.cpp", "tuning.cpp", "workspace.cpp"]
 # The recording stand-in for the HIP runtime (include/cutile_hip_testing.h) is not part of the product library: the CPU

@@ -32,6 +32,9 @@ extern const unsigned char cutile_img_scaledflat_start[], cutile_img_scaledflat_
 extern const unsigned char cutile_img_mxfp4_start[], cutile_img_mxfp4_end[];
 extern const unsigned char cutile_img_mxfp4flat_start[], cutile_img_mxfp4flat_end[];
 extern const unsigned char cutile_img_blockscale_start[], cutile_img_blockscale_end[];
+extern const unsigned char cutile_img_pagedcache_start[], cutile_img_pagedcache_end[];
+extern const unsigned char cutile_img_pagedattention_start[], cutile_img_pagedattention_end[];
+extern const unsigned char cutile_img_logits_start[], cutile_img_logits_end[];
 }
 
 namespace cutile {
@@ -77,6 +80,9 @@ ImageRef image_ref(Image img) {
     case IMG_MXFP4: return {cutile_img_mxfp4_start, cutile_img_mxfp4_end};
     case IMG_MXFP4_FLAT: return {cutile_img_mxfp4flat_start, cutile_img_mxfp4flat_end};
     case IMG_BLOCK_SCALE: return {cutile_img_blockscale_start, cutile_img_blockscale_end};
+    case IMG_PAGED_CACHE: return {cutile_img_pagedcache_start, cutile_img_pagedcache_end};
+    case IMG_PAGED_ATTENTION: return {cutile_img_pagedattention_start, cutile_img_pagedattention_end};
+    case IMG_LOGITS: return {cutile_img_logits_start, cutile_img_logits_end};
     default: return {nullptr, nullptr};
   }
 }
@@ -514,6 +520,21 @@ std::vector<KernelEntry> build_table() {
         }
         add(fn, keep(base + "any"), keep(std::string(fn) + "_entry__" + base + "any"), IMG_BLOCK_SCALE, 256, 32, 0, 0, 0, 0, dt, 0, 2);
       }
+    }
+  // ---- a paged cache: writing, reading back, attention (256 or 512 threads; tile = (rows of a tile, -, D, -)) ----
+  for (const char* dt : {"f16", "bf16"})
+    for (const char* kept : {"", "_mxfp8"})
+      for (int d : {64, 128, 256}) {
+        const std::string v = std::string(dt) + kept + "_d" + std::to_string(d);
+        for (const char* fn : {"paged_cache_write", "paged_cache_read"}) add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_PAGED_CACHE, 256, 0, 0, 0, d, 0, dt, 0, 3);
+        const int waves = d == 256 ? 4 : 8;
+        add("paged_attention", keep(v), keep("paged_attention_entry__" + v), IMG_PAGED_ATTENTION, (uint32_t)waves * 64, (uint32_t)waves * (32 * d * 4 + 256 + 16) + 12, waves * 32, 0, d, 0, dt, 0, 3);
+      }
+  // ---- logits in front of the choice of a token (512 threads; tile = (-, columns of a workgroup, -, -)) ----
+  for (const char* dt : {"f16", "bf16", "f32"})
+    for (int c : {16384, 4096, 1024}) {
+      const std::string v = std::string(dt) + "_" + std::to_string(c);
+      add("adjust_logits", keep(v), keep("adjust_logits_entry__" + v), IMG_LOGITS, 512, (uint32_t)c * 4 + 1024 * 8 + 4, 0, c, 0, 0, dt, 0, 2);
     }
   return t;
 }

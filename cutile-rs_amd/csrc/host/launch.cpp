@@ -29,6 +29,7 @@
 #include "scratch.h"
 #include "../kernels/key_steps.h"
 #include "../kernels/mapped_partition.h"
+#include "../kernels/paged.h"
 
 using cutile::MappedArg;
 using cutile::MappedRangeArg;
@@ -3598,6 +3599,363 @@ cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cu
   ScaledRoom room;
   if (cutile_status_t s = resolve_scaled("linear_tile_mxfp4", "", dt, bm, bn, full_cover, full_cover, {M, N, KP / 64, kScaledMxfp4}, opts, missing, stream, &cus, &room, &res)) return s;
   return launch_scaled(res, stream, z, x, y, xs, ys, alpha, tg, KP / 64, cus, room);
+}
+
+}  // extern "C"
+
+// ---- a paged cache: paged_cache.hip, paged_attention.hip, and logits: adjust_logits.hip ---------------------------------
+namespace {
+
+// No two elements of a tensor share memory, as far as its strides tell: every axis steps over all that the axes of smaller strides span.
+cutile_status_t check_distinct(const char* fn, const char* name, const cutile_tensor_arg_t& t) {
+  int order[CUTILE_MAX_RANK], n = 0;
+  for (int i = 0; i < t.rank; ++i)
+    if (t.shape[i] > 1) order[n++] = i;
+  std::sort(order, order + n, [&](int a, int b) { return t.strides[a] < t.strides[b]; });
+  int64_t span = 1;
+  for (int i = 0; i < n; ++i) {
+    CUTILE_REQUIRE(t.strides[order[i]] >= span, CUTILE_ERR_KERNEL_NOT_FOUND, "%s: elements of %s overlap", fn, name);
+    span += (int64_t)(t.shape[order[i]] - 1) * t.strides[order[i]];
+  }
+  return CUTILE_SUCCESS;
+}
+
+// Unit inner stride, every row of the innermost axis on a 16-byte boundary, no axis that runs backwards.
+cutile_status_t check_rows_aligned(const char* fn, const char* name, const cutile_tensor_arg_t& t) {
+  const int64_t size = (int64_t)cutile_dtype_size(t.dtype);
+  bool ok = t.strides[t.rank - 1] == 1 && aligned16(t.ptr);
+  for (int i = 0; i + 1 < t.rank; ++i) ok = ok && (t.shape[i] == 1 || (t.strides[i] >= 0 && t.strides[i] * size % 16 == 0));
+  CUTILE_REQUIRE(ok, CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants need a unit inner stride and 16-byte aligned rows of %s", fn, name);
+  return CUTILE_SUCCESS;
+}
+
+cutile_status_t check_list(const char* fn, const char* name, const cutile_tensor_arg_t* t, cutile_dtype_t dt, int64_t least) {
+  if (cutile_status_t s = check_tensor(t, name, 1, 1)) return s;
+  CUTILE_REQUIRE(t->dtype == dt && t->shape[0] >= least && (t->shape[0] == 1 || t->strides[0] == 1) && ((uintptr_t)t->ptr & 3) == 0, CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: %s must be %lld contiguous, aligned %s", fn, name, (long long)least, cutile_dtype_name(dt));
+  return CUTILE_SUCCESS;
+}
+
+// A table whose rows are contiguous; `dt2`: another element type that will do.
+cutile_status_t check_table(const char* fn, const char* name, const cutile_tensor_arg_t* t, cutile_dtype_t dt, cutile_dtype_t dt2, int64_t rows) {
+  if (cutile_status_t s = check_tensor(t, name, 2, 2)) return s;
+  CUTILE_REQUIRE((t->dtype == dt || t->dtype == dt2) && t->shape[0] >= rows && (t->shape[1] == 1 || t->strides[1] == 1) && (t->shape[0] == 1 || t->strides[0] >= 0) &&
+                     ((uintptr_t)t->ptr & 3) == 0,
+                 CUTILE_ERR_KERNEL_LAUNCH, "%s: %s must be %lld contiguous rows of %s", fn, name, (long long)rows, cutile_dtype_name(dt));
+  return CUTILE_SUCCESS;
+}
+
+struct PagedLaunch {
+  PagedCache c{};
+  Name variant;
+  int32_t d = 0;
+};
+
+// The cache, its pages and sequences; `rows`: new_k, q or out, [tokens, heads, D].
+cutile_status_t check_paged(const char* fn, const cutile_tensor_arg_t& rows, const cutile_tensor_arg_t* k, const cutile_tensor_arg_t* v, const cutile_tensor_arg_t* ks,
+                            const cutile_tensor_arg_t* vs, const cutile_tensor_arg_t* table, const cutile_tensor_arg_t* starts, const cutile_tensor_arg_t* lens, PagedLaunch* l) {
+  if (cutile_status_t s = check_tensor(k, "k_cache", 4, 4)) return s;
+  if (cutile_status_t s = check_tensor(v, "v_cache", 4, 4)) return s;
+  CUTILE_REQUIRE(is_16bit_float(rows.dtype), CUTILE_ERR_KERNEL_NOT_FOUND, "%s: the tokens' rows must be f16 or bf16", fn);
+  CUTILE_REQUIRE(!ks == !vs, CUTILE_ERR_INVALID_ARGUMENT, "%s: k_scales and v_scales come together", fn);
+  const bool mx = ks != nullptr;
+  CUTILE_REQUIRE(v->dtype == k->dtype && k->dtype == (mx ? CUTILE_DTYPE_F8E4M3FN : rows.dtype), CUTILE_ERR_KERNEL_NOT_FOUND,
+                 "%s: the caches must be f8e4m3fn with scales or, without, of the rows' type %s (k_cache is %s, v_cache %s)", fn, cutile_dtype_name(rows.dtype),
+                 cutile_dtype_name(k->dtype), cutile_dtype_name(v->dtype));
+  const int32_t d = k->shape[3];
+  CUTILE_REQUIRE(same_shape(*k, *v) && rows.shape[2] == d, CUTILE_ERR_KERNEL_LAUNCH, "%s: k_cache and v_cache must have one shape, and D = %d that of the rows (%d)", fn, d, rows.shape[2]);
+  CUTILE_REQUIRE(d == 64 || d == 128 || d == 256, CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants take D = 64, 128 or 256, got %d", fn, d);
+  auto alike = [](const cutile_tensor_arg_t& a, const cutile_tensor_arg_t& b) {
+    for (int i = 0; i < a.rank; ++i)
+      if (a.shape[i] > 1 && a.strides[i] != b.strides[i]) return false;
+    return true;
+  };
+  CUTILE_REQUIRE(alike(*k, *v), CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants need k_cache and v_cache laid out alike", fn);
+  if (cutile_status_t s = check_rows_aligned(fn, "k_cache", *k)) return s;
+  if (cutile_status_t s = check_rows_aligned(fn, "v_cache", *v)) return s;
+  if (cutile_status_t s = check_table(fn, "page_table", table, CUTILE_DTYPE_I32, CUTILE_DTYPE_I32, 1)) return s;
+  const int32_t batch = table->shape[0];
+  if (cutile_status_t s = check_list(fn, "starts", starts, CUTILE_DTYPE_I32, (int64_t)batch + 1)) return s;
+  if (cutile_status_t s = check_list(fn, "context_lens", lens, CUTILE_DTYPE_I32, batch)) return s;
+  PagedCache& c = l->c;
+  const int64_t size = (int64_t)cutile_dtype_size(k->dtype);
+  c.k = k->ptr, c.v = v->ptr;
+  c.page_bytes = k->strides[0] * size, c.row_bytes = k->strides[1] * size, c.head_bytes = k->strides[2] * size;
+  if (mx) {
+    const cutile_tensor_arg_t* both[2] = {ks, vs};
+    for (int i = 0; i < 2; ++i) {
+      if (cutile_status_t s = check_tensor(both[i], i ? "v_scales" : "k_scales", 4, 4)) return s;
+      const cutile_tensor_arg_t& t = *both[i];
+      CUTILE_REQUIRE(t.dtype == CUTILE_DTYPE_F8E8M0FNU && t.shape[0] == k->shape[0] && t.shape[1] == k->shape[1] && t.shape[2] == k->shape[2] && t.shape[3] == d / 32,
+                     CUTILE_ERR_KERNEL_LAUNCH, "%s: scales must be f8e8m0fnu [%d, %d, %d, %d]", fn, k->shape[0], k->shape[1], k->shape[2], d / 32);
+      bool forward = t.strides[3] == 1;
+      for (int j = 0; j < 3; ++j) forward = forward && (t.shape[j] == 1 || t.strides[j] >= 0);
+      CUTILE_REQUIRE(forward && alike(*ks, t), CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants need k_scales and v_scales laid out alike, with a unit inner stride", fn);
+    }
+    c.ks = (const uint8_t*)ks->ptr, c.vs = (const uint8_t*)vs->ptr;
+    c.s_page = ks->strides[0], c.s_row = ks->strides[1], c.s_head = ks->strides[2];
+  }
+  c.table = (const int32_t*)table->ptr, c.starts = (const int32_t*)starts->ptr, c.lens = (const int32_t*)lens->ptr;
+  c.table_row = table->shape[0] == 1 ? 0 : table->strides[0];
+  c.pages = k->shape[0], c.page_size = k->shape[1], c.heads = k->shape[2];
+  c.table_pages = table->shape[1], c.batch = batch, c.tokens = rows.shape[0];
+  l->variant = Name(cutile_dtype_name(rows.dtype)) + (mx ? "_mxfp8_d" : "_d") + num(d);
+  l->d = d;
+  return CUTILE_SUCCESS;
+}
+
+// new_k, new_v or out_k, out_v as the kernels of paged_cache.hip take them.
+struct CacheRows {
+  void *k, *v;
+  int64_t k_token, k_head, v_token, v_head;
+};
+CacheRows cache_rows(const cutile_tensor_arg_t& k, const cutile_tensor_arg_t& v) {
+  return {k.ptr, v.ptr, 2 * (int64_t)k.strides[0], 2 * (int64_t)k.strides[1], 2 * (int64_t)v.strides[0], 2 * (int64_t)v.strides[1]};
+}
+cutile_status_t launch_paged_cache(const char* fn, cutile_stream_t stream, const PagedLaunch& l, const CacheRows& rows, const cutile_launch_opts_t* opts) {
+  Resolved res;
+  if (cutile_status_t s = resolve_entry(fn, opts, l.variant, {l.variant}, &res)) return s;
+  ArgPacker args;
+  args.push_val<PagedCache>(l.c);
+  args.push_val<CacheRows>(rows);
+  const uint32_t grid[3] = {div_up((uint64_t)l.c.tokens, 4), 1, 1};   // a wavefront to a token
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+}
+
+// Every element of `out` belongs to a tile of the launch.
+cutile_status_t check_covered(const char* fn, const cutile_partition_arg_t* const* parts, int n, const cutile_launch_opts_t* opts) {
+  uint32_t explicit_grid[3] = {0, 0, 0}, tg[3];
+  if (opts) memcpy(explicit_grid, opts->grid, sizeof(explicit_grid));
+  if (cutile_status_t s = cutile_infer_launch_grid(explicit_grid, parts, n, tg)) return s;
+  for (int i = 0; i < parts[0]->tensor.rank; ++i)
+    CUTILE_REQUIRE((int64_t)tg[i] * parts[0]->partition_shape[i] >= parts[0]->tensor.shape[i], CUTILE_ERR_KERNEL_LAUNCH, "%s: the launch grid must cover all of the output", fn);
+  return CUTILE_SUCCESS;
+}
+
+// How keys are dealt out (see PagedPlan): `keys` to a workgroup so that `items` tiles of about `context` keys make about `wanted` workgroups, `step` keys at a time.
+struct Deal {
+  int32_t keys = INT32_MAX, shares = 1;
+};
+Deal deal_keys(int64_t items, int64_t context, int64_t wanted, int64_t step, int64_t most_shares) {
+  Deal d;
+  const int64_t shares = std::min({most_shares, (wanted + items - 1) / items, (context + step - 1) / step});
+  if (shares <= 1) return d;
+  const int64_t each = ((context + shares - 1) / shares + step - 1) / step * step;
+  d.keys = (int32_t)each;
+  d.shares = (int32_t)((context + each - 1) / each);
+  return d;
+}
+
+}  // namespace
+
+extern "C" {
+
+cutile_status_t cutile_launch_paged_cache_write(cutile_stream_t stream, const cutile_tensor_arg_t* new_k, const cutile_tensor_arg_t* new_v, const cutile_tensor_arg_t* k_cache,
+                                                const cutile_tensor_arg_t* v_cache, const cutile_tensor_arg_t* k_scales, const cutile_tensor_arg_t* v_scales,
+                                                const cutile_tensor_arg_t* page_table, const cutile_tensor_arg_t* starts, const cutile_tensor_arg_t* context_lens,
+                                                const cutile_launch_opts_t* opts) {
+  const char* const fn = "paged_cache_write";
+  if (cutile_status_t s = check_tensor(new_k, "new_k", 3, 3)) return s;
+  if (cutile_status_t s = check_tensor(new_v, "new_v", 3, 3)) return s;
+  PagedLaunch l;
+  if (cutile_status_t s = check_paged(fn, *new_k, k_cache, v_cache, k_scales, v_scales, page_table, starts, context_lens, &l)) return s;
+  CUTILE_REQUIRE(new_v->dtype == new_k->dtype && same_shape(*new_k, *new_v) && new_k->shape[1] == l.c.heads, CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: new_k and new_v must be [tokens, %d, %d] of one type", fn, l.c.heads, l.d);
+  if (cutile_status_t s = check_rows_aligned(fn, "new_k", *new_k)) return s;
+  if (cutile_status_t s = check_rows_aligned(fn, "new_v", *new_v)) return s;
+  const cutile_tensor_arg_t* written[4] = {k_cache, v_cache, k_scales, v_scales};
+  const char* const names[4] = {"k_cache", "v_cache", "k_scales", "v_scales"};
+  for (int i = 0; i < 4; ++i)
+    if (written[i])
+      if (cutile_status_t s = check_distinct(fn, names[i], *written[i])) return s;
+  return launch_paged_cache(fn, stream, l, cache_rows(*new_k, *new_v), opts);
+}
+
+cutile_status_t cutile_launch_paged_cache_read(cutile_stream_t stream, const cutile_tensor_arg_t* k_cache, const cutile_tensor_arg_t* v_cache, const cutile_tensor_arg_t* k_scales,
+                                               const cutile_tensor_arg_t* v_scales, const cutile_tensor_arg_t* page_table, const cutile_tensor_arg_t* starts,
+                                               const cutile_tensor_arg_t* context_lens, const cutile_partition_arg_t* out_k, const cutile_partition_arg_t* out_v,
+                                               const cutile_launch_opts_t* opts) {
+  const char* const fn = "paged_cache_read";
+  if (cutile_status_t s = check_partition(out_k, "out_k", 3, 3)) return s;
+  if (cutile_status_t s = check_partition(out_v, "out_v", 3, 3)) return s;
+  const cutile_tensor_arg_t &kt = out_k->tensor, &vt = out_v->tensor;
+  PagedLaunch l;
+  if (cutile_status_t s = check_paged(fn, kt, k_cache, v_cache, k_scales, v_scales, page_table, starts, context_lens, &l)) return s;
+  CUTILE_REQUIRE(vt.dtype == kt.dtype && same_shape(kt, vt) && kt.shape[1] == l.c.heads && out_k->partition_shape[1] == l.c.heads && out_k->partition_shape[2] == l.d,
+                 CUTILE_ERR_KERNEL_LAUNCH, "%s: out_k and out_v must be [tokens, %d, %d] of one type, partitioned [BM, %d, %d]", fn, l.c.heads, l.d, l.c.heads, l.d);
+  if (cutile_status_t s = check_rows_aligned(fn, "out_k", kt)) return s;
+  if (cutile_status_t s = check_rows_aligned(fn, "out_v", vt)) return s;
+  if (cutile_status_t s = check_distinct(fn, "out_k", kt)) return s;
+  if (cutile_status_t s = check_distinct(fn, "out_v", vt)) return s;
+  const cutile_partition_arg_t* parts[2] = {out_k, out_v};
+  if (cutile_status_t s = check_covered(fn, parts, 2, opts)) return s;
+  return launch_paged_cache(fn, stream, l, cache_rows(kt, vt), opts);
+}
+
+cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cutile_tensor_arg_t* q, const cutile_tensor_arg_t* k_cache, const cutile_tensor_arg_t* v_cache,
+                                              const cutile_tensor_arg_t* k_scales, const cutile_tensor_arg_t* v_scales, const cutile_tensor_arg_t* page_table,
+                                              const cutile_tensor_arg_t* starts, const cutile_tensor_arg_t* context_lens, const cutile_partition_arg_t* out, float qk_scale,
+                                              int32_t window, int32_t max_new, int32_t max_context, const cutile_tensor_arg_t* workspace, const cutile_launch_opts_t* opts) {
+  const char* const fn = "paged_attention";
+  if (cutile_status_t s = check_tensor(q, "q", 3, 3)) return s;
+  if (cutile_status_t s = check_partition(out, "out", 3, 3)) return s;
+  const cutile_tensor_arg_t& ot = out->tensor;
+  PagedLaunch l;
+  if (cutile_status_t s = check_paged(fn, *q, k_cache, v_cache, k_scales, v_scales, page_table, starts, context_lens, &l)) return s;
+  const int32_t heads = l.c.heads, group = q->shape[1] / heads, tokens = l.c.tokens, batch = l.c.batch, d = l.d;
+  CUTILE_REQUIRE(group > 0 && q->shape[1] % heads == 0, CUTILE_ERR_KERNEL_LAUNCH, "%s: %d query heads are no multiple of the cache's %d", fn, q->shape[1], heads);
+  CUTILE_REQUIRE(ot.dtype == q->dtype && same_shape(ot, *q) && out->partition_shape[2] == d, CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: out must be q's shape [%d, %d, %d] and type, partitioned [BM, G, %d]", fn, q->shape[0], q->shape[1], d, d);
+  CUTILE_REQUIRE(window >= 0 && max_new >= 0 && max_context >= 0, CUTILE_ERR_KERNEL_LAUNCH, "%s: window, max_new and max_context must not be negative", fn);
+  CUTILE_REQUIRE(std::isfinite(qk_scale), CUTILE_ERR_KERNEL_LAUNCH, "%s: qk_scale must be a finite number", fn);
+  CUTILE_REQUIRE((int64_t)tokens * group <= INT32_MAX - 256, CUTILE_ERR_KERNEL_LAUNCH, "%s: %d tokens of %d heads to a KV head are too many", fn, tokens, group);
+  if (cutile_status_t s = check_rows_aligned(fn, "q", *q)) return s;
+  if (cutile_status_t s = check_rows_aligned(fn, "out", ot)) return s;
+  if (cutile_status_t s = check_distinct(fn, "out", ot)) return s;
+  const cutile_partition_arg_t* parts[1] = {out};
+  if (cutile_status_t s = check_covered(fn, parts, 1, opts)) return s;
+  SplitWorkspace ws;
+  int64_t room = 0;
+  if (workspace) {
+    if (cutile_status_t s = check_tensor(workspace, "workspace", 1, CUTILE_MAX_RANK)) return s;
+    const int64_t bytes = numel(*workspace) * (int64_t)cutile_dtype_size(workspace->dtype), counters = (int64_t)(kSplitCounters * sizeof(uint32_t));
+    CUTILE_REQUIRE(is_contiguous(*workspace) && aligned16(workspace->ptr) && bytes > counters, CUTILE_ERR_KERNEL_LAUNCH,
+                   "%s: workspace must be contiguous, 16-byte aligned and of more than %lld bytes", fn, (long long)counters);
+    ws.counters = (uint32_t*)workspace->ptr;
+    ws.partials = (float*)((unsigned char*)workspace->ptr + counters);
+    room = std::min<int64_t>(bytes - counters, kSplitPartialBytes);
+  }
+  Resolved res;
+  if (cutile_status_t s = resolve_entry(fn, opts, l.variant, {l.variant}, &res)) return s;
+  int cus = 256;
+  if (cutile_status_t s = current_device_units(&cus)) return s;
+  const int64_t bm = res.entry->tile[0], most_new = max_new ? std::min(max_new, tokens) : tokens;
+  const int64_t held = (int64_t)l.c.table_pages * l.c.page_size, context = std::max<int64_t>(1, max_context ? std::min<int64_t>(max_context, held) : std::min<int64_t>(held, INT32_MAX));
+  PagedPlan p{};
+  // the kernels look for the largest score before they scale it: a negative scale turns q around, and a scale of 0 makes it zeros
+  p.scale_log2e = qk_scale == 0.0f ? 1.0f : std::fabs(qk_scale) * 1.4426950408889634f;
+  p.q_and = qk_scale == 0.0f ? 0u : ~0u;
+  p.q_xor = qk_scale < 0.0f ? 0x80008000u : 0u;
+  p.window = window, p.group = group;
+  const bool any_long = most_new * group > 32;
+  p.few_rows = any_long && most_new * batch == tokens ? 0 : 32;   // all alike: no tiles of short sequences beside the others
+  p.few_slot_rows = (int32_t)std::min<int64_t>(32, most_new * group);
+  p.long_tiles = any_long ? (int32_t)((int64_t)tokens * group / bm + batch) : 0;
+  auto plan = [&](bool may_share) {
+    const int64_t row_bytes = (d + 2) * 4, few_items = p.few_rows ? (int64_t)batch * heads : 0;
+    const int64_t long_slots = (int64_t)p.long_tiles * heads, long_items = any_long ? ((int64_t)tokens * group + bm - 1) / bm * heads : 0;
+    Deal of_long, of_few;
+    if (may_share && long_slots + few_items <= (int64_t)kSplitCounters) {
+      if (long_items) of_long = deal_keys(long_items, context, cus, 256, std::max<int64_t>(1, room / (few_items ? 2 : 1) / (long_slots * bm * row_bytes)));
+      const int64_t left = room - (of_long.shares > 1 ? of_long.shares * long_slots * bm * row_bytes : 0);
+      if (few_items) of_few = deal_keys(few_items, context, cus * 4, 512, std::max<int64_t>(1, left / (few_items * p.few_slot_rows * row_bytes)));
+    }
+    p.long_shares = of_long.shares, p.long_keys = of_long.keys;
+    p.few_shares = of_few.shares, p.few_keys = of_few.keys;
+  };
+  if (!workspace) room = kSplitPartialBytes;
+  plan(true);
+  if (!workspace && (p.long_shares > 1 || p.few_shares > 1) && g_launch_mode == 0) {
+    ws = split_workspace(res.device, (hipStream_t)stream);
+    if (!ws.partials) plan(false);
+  }
+  p.partials = ws.partials, p.counters = ws.counters;
+  const uint64_t items = (uint64_t)p.long_tiles * p.long_shares + (p.few_rows ? (uint64_t)batch * p.few_shares : 0);
+  CUTILE_REQUIRE(items * heads <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %llu tiles do not fit a launch grid axis", fn, (unsigned long long)(items * heads));
+  ArgPacker args;
+  args.push_tensor(*q);
+  args.push_partition(*out);
+  args.push_val<PagedCache>(l.c);
+  args.push_val<PagedPlan>(p);
+  const uint32_t grid[3] = {(uint32_t)(items * heads), 1, 1};
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
+}
+
+cutile_status_t cutile_launch_adjust_logits(cutile_stream_t stream, const cutile_tensor_arg_t* logits, const cutile_partition_arg_t* out, const cutile_tensor_arg_t* tokens,
+                                            const cutile_tensor_arg_t* prompt_lens, const cutile_tensor_arg_t* token_lens, const cutile_tensor_arg_t* repetition,
+                                            const cutile_tensor_arg_t* presence, const cutile_tensor_arg_t* frequency, const cutile_tensor_arg_t* bias_ids,
+                                            const cutile_tensor_arg_t* bias_values, const cutile_tensor_arg_t* allowed, const cutile_launch_opts_t* opts) {
+  const char* const fn = "adjust_logits";
+  if (cutile_status_t s = check_tensor(logits, "logits", 2, 2)) return s;
+  if (cutile_status_t s = check_partition(out, "out", 2, 2)) return s;
+  const cutile_tensor_arg_t& ot = out->tensor;
+  const int32_t rows = logits->shape[0], vocab = logits->shape[1];
+  CUTILE_REQUIRE(is_16bit_float(logits->dtype) || logits->dtype == CUTILE_DTYPE_F32, CUTILE_ERR_KERNEL_NOT_FOUND, "%s: logits must be f16, bf16 or f32", fn);
+  CUTILE_REQUIRE(ot.dtype == logits->dtype && same_shape(ot, *logits) && out->partition_shape[1] == vocab, CUTILE_ERR_KERNEL_LAUNCH,
+                 "%s: out must be [%d, %d] of logits' type, partitioned [BM, %d]", fn, rows, vocab, vocab);
+  CUTILE_REQUIRE(unit_inner(*logits) && unit_inner(ot) && (rows == 1 || logits->strides[0] >= 0), CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants need a unit inner stride", fn);
+  if (cutile_status_t s = check_distinct(fn, "out", ot)) return s;
+  CUTILE_REQUIRE(tokens || (!prompt_lens && !token_lens && !repetition && !presence && !frequency), CUTILE_ERR_INVALID_ARGUMENT,
+                 "%s: lengths and penalties are nothing without tokens", fn);
+  CUTILE_REQUIRE(!bias_ids == !bias_values, CUTILE_ERR_INVALID_ARGUMENT, "%s: bias_ids and bias_values come together", fn);
+  struct LogitsArgs {   // as in adjust_logits.hip
+    const void* in;
+    void* out;
+    int64_t in_row, out_row;
+    const void *tokens, *prompt_lens, *token_lens;
+    int64_t tokens_row;
+    const void *repetition, *presence, *frequency;
+    const void *bias_ids, *bias_values;
+    int64_t ids_row, values_row;
+    const void* allowed;
+    int64_t allowed_row;
+    int32_t vocab, most, biases, blocks, vectors, pad;
+  } a{};
+  const struct {
+    const cutile_tensor_arg_t* t;
+    const char* name;
+    cutile_dtype_t dt;
+    const void** to;
+  } lists[] = {{prompt_lens, "prompt_lens", CUTILE_DTYPE_I32, &a.prompt_lens}, {token_lens, "token_lens", CUTILE_DTYPE_I32, &a.token_lens},
+               {repetition, "repetition", CUTILE_DTYPE_F32, &a.repetition}, {presence, "presence", CUTILE_DTYPE_F32, &a.presence},
+               {frequency, "frequency", CUTILE_DTYPE_F32, &a.frequency}};
+  for (const auto& x : lists)
+    if (x.t) {
+      if (cutile_status_t s = check_list(fn, x.name, x.t, x.dt, rows)) return s;
+      *x.to = x.t->ptr;
+    }
+  auto row_stride = [](const cutile_tensor_arg_t& t) { return t.shape[0] == 1 ? (int64_t)0 : (int64_t)t.strides[0]; };
+  if (tokens) {
+    if (cutile_status_t s = check_table(fn, "tokens", tokens, CUTILE_DTYPE_I32, CUTILE_DTYPE_I32, rows)) return s;
+    a.tokens = tokens->ptr, a.tokens_row = row_stride(*tokens), a.most = tokens->shape[1];
+  }
+  if (bias_ids) {
+    if (cutile_status_t s = check_table(fn, "bias_ids", bias_ids, CUTILE_DTYPE_I32, CUTILE_DTYPE_I32, rows)) return s;
+    if (cutile_status_t s = check_table(fn, "bias_values", bias_values, CUTILE_DTYPE_F32, CUTILE_DTYPE_F32, rows)) return s;
+    CUTILE_REQUIRE(bias_ids->shape[1] == bias_values->shape[1] && bias_ids->shape[1] <= 1024, CUTILE_ERR_KERNEL_LAUNCH, "%s: a row has up to 1024 biases, as many ids as values (%d and %d)",
+                   fn, bias_ids->shape[1], bias_values->shape[1]);
+    a.bias_ids = bias_ids->ptr, a.bias_values = bias_values->ptr, a.biases = bias_ids->shape[1];
+    a.ids_row = row_stride(*bias_ids), a.values_row = row_stride(*bias_values);
+  }
+  if (allowed) {
+    if (cutile_status_t s = check_table(fn, "allowed", allowed, CUTILE_DTYPE_I32, CUTILE_DTYPE_U32, rows)) return s;
+    CUTILE_REQUIRE(allowed->shape[1] >= (vocab + 31) / 32, CUTILE_ERR_KERNEL_LAUNCH, "%s: allowed needs %d words a row, got %d", fn, (vocab + 31) / 32, allowed->shape[1]);
+    a.allowed = allowed->ptr, a.allowed_row = row_stride(*allowed);
+  }
+  const cutile_partition_arg_t* parts[1] = {out};
+  if (cutile_status_t s = check_covered(fn, parts, 1, opts)) return s;
+  int cus = 256;
+  if (cutile_status_t s = current_device_units(&cus)) return s;
+  Names fitting;
+  Name sized;
+  for (const KernelEntry* e : kernels_of(fn))
+    if (strcmp(e->dtype, cutile_dtype_name(logits->dtype)) == 0) {
+      fitting.push_back(e->variant);
+      if (sized.empty() && (int64_t)rows * div_up(vocab, e->tile[1]) >= 2 * cus) sized = e->variant;   // the widest that fills the chip
+    }
+  if (sized.empty()) sized = fitting[fitting.size() - 1];
+  Resolved res;
+  if (cutile_status_t s = resolve_entry(fn, opts, sized, fitting, &res)) return s;
+  a.in = logits->ptr, a.out = ot.ptr;
+  a.in_row = row_stride(*logits), a.out_row = row_stride(ot);
+  a.vocab = vocab, a.blocks = (int32_t)div_up(vocab, res.entry->tile[1]);
+  const int64_t per16 = 16 / (int64_t)cutile_dtype_size(logits->dtype);
+  a.vectors = aligned16(a.in) && aligned16(a.out) && a.in_row % per16 == 0 && a.out_row % per16 == 0;
+  ArgPacker args;
+  args.push_val<LogitsArgs>(a);
+  CUTILE_REQUIRE((uint64_t)rows * a.blocks <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %d rows of %d do not fit a launch grid axis", fn, rows, vocab);
+  const uint32_t grid[3] = {(uint32_t)rows * a.blocks, 1, 1};
+  return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
 
 }  // extern "C"

@@ -1,0 +1,616 @@
+// Attention of the new tokens of a batch of sequences over a paged cache (paged.h), from one token a sequence to whole prompts:
+//   out[i, h, :] = sum_j softmax_j(scale q[i, h, :] . k_j) v_j      over the keys j of the sequence's KV head h / group with p - window < j <= p,
+// p the position of token i; no key: zeros.
+//
+// The rows of a tile are pairs (token, query head of one KV head), token by token: group heads share every key that is read, and a decode step of 8 heads or a
+// chunk of 4 tokens fill the 32 columns of a matrix instruction.  Products, masks and softmax are those of fmha_common.h / fmha.hip: S^T = K Q^T and
+// O^T = V^T P^T, so that a lane owns one row.
+//  * Tiles of up to 32 rows (decode, speculation): every wavefront has keys of its own, 32 at a time, through registers into LDS that no other
+//    wavefront reads: no barrier in the loop.  HBM's rate bounds it.
+//  * Larger tiles: R wavefronts side by side hold 32 rows each, S = wavefronts / R share the keys of a step; the matrix cores and exponentials bound it.
+// At the end the partial outputs go through LDS, and where the keys of a tile are dealt to several workgroups through the launch's workspace: the one that
+// arrives last adds them up in the order of the keys.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "fmha_common.h"
+#include "kernel_args.h"
+#include "paged.h"
+#include "split_k.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr uint32_t kOob = 0x80000000u;
+
+__device__ u32x4 paged_zeros;   // what a key that is not there reads; never written
+
+// 16 e4m3 values of one block as 16-bit ones.
+template <typename T>
+__device__ __forceinline__ void widen(const u32x4& raw, uint32_t scale_byte, u32x4& lo, u32x4& hi) {
+  const float s = __builtin_bit_cast(float, scale_byte << 23);   // the conversion takes the scale by its exponent: byte 0 is 2^-127, 255 NaN
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a, b;
+    if constexpr (std::is_same<T, _Float16>::value) {
+      a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[i], s, false));
+      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[i], s, true));
+    } else {
+      a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[i], s, false));
+      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[i], s, true));
+    }
+    u32x4& to = i < 2 ? lo : hi;
+    to[i * 2 % 4] = a, to[i * 2 % 4 + 1] = b;
+  }
+}
+
+// What a workgroup works on: the rows of a tile and its share of their keys.
+struct Tile {
+  int32_t head;            // KV head
+  int32_t row0, rows;      // first packed row of the sequence, number of rows
+  int32_t first;           // row of q and out of the sequence's first token
+  int32_t pos0;            // position of that token
+  int32_t k0, k1;          // keys [k0, k1)
+  uint32_t share, shares;
+  uint32_t slot;           // of the workspace's counters
+  const int32_t* pages;    // the sequence's pages
+};
+
+template <typename T, bool MX, int D, int W>
+struct Paged {
+  using E = Elem<T>;
+  using vec8 = typename E::vec8;
+  static constexpr int kThreads = W * 64, BM = W * 32;
+  static constexpr int DB = D / 32, KS = D / 16, kUnits = D / 8;   // 16-byte units of a 16-bit row
+  static constexpr int kBlockBytes = 32 * D * 2;                   // 32 rows of K or V in LDS
+  static constexpr int kBandBytes = 32 * D * 4;                    // a wavefront's partial output
+  static constexpr int kLdsBytes = W * kBandBytes;                 // = W x (K and V of 32 keys)
+  static constexpr int kMostMissed = 4;                            // steps that hold a border of what the 32 rows see: two at either end
+  static constexpr int kStep = D == 64 ? 2 : 1;                    // key blocks of a step are doubled where rows are short: a load each for the threads
+  static constexpr int kLoadUnits = D * (MX ? 1 : 2) / 16;         // 16-byte loads of a row of the cache
+
+  __device__ static __forceinline__ int k_off(int r, int u) { return r * (D * 2) + ((u ^ (r & (kUnits - 1) & 15)) << 4); }
+  __device__ static __forceinline__ int v_off(int r, int u) { return r * (D * 2) + ((u ^ ((r & (kUnits >= 16 ? 3 : 1)) << 2)) << 4); }
+
+  // The largest magnitudes so far of 16-bit values in the halves of a dword, as integers: NaN and infinities are on top.
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint16_t kInfinite = std::is_same<T, _Float16>::value ? 0x7c00 : 0x7f80;
+  __device__ static __forceinline__ void most_of(u16x2& most, const u32x4& v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+  }
+  // 16 bytes of K and of V of row r into LDS.
+  __device__ static __forceinline__ void put(u16x2& most, unsigned char* sk, unsigned char* sv, int r, int unit, const u32x4& k, const u32x4& v, uint32_t ks, uint32_t vs) {
+    if constexpr (MX) {
+      u32x4 lo, hi;
+      widen<T>(k, ks, lo, hi);
+      *reinterpret_cast<u32x4*>(sk + k_off(r, unit * 2)) = lo;
+      *reinterpret_cast<u32x4*>(sk + k_off(r, unit * 2 + 1)) = hi;
+      widen<T>(v, vs, lo, hi);
+      most_of(most, lo);
+      most_of(most, hi);
+      *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2)) = lo;
+      *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2 + 1)) = hi;
+    } else {
+      most_of(most, v);
+      *reinterpret_cast<u32x4*>(sk + k_off(r, unit)) = k;
+      *reinterpret_cast<u32x4*>(sv + v_off(r, unit)) = v;
+    }
+  }
+
+  // The cache rows of N keys on their way to LDS, by THREADS threads: key r of a step is key `at + r`.
+  template <int N, int THREADS>
+  struct Loader {
+    static constexpr int kLoads = N * kLoadUnits / THREADS, kRowsApart = THREADS / kLoadUnits;
+    static_assert(N * kLoadUnits % THREADS == 0 && THREADS % kLoadUnits == 0, "equal shares");
+    const PagedCache& c;
+    const Tile& t;
+    int unit;
+    int32_t page_at[kLoads], row_at[kLoads];   // of the next step to be asked for
+    int32_t entry[kLoads];                     // its entries of the page table
+    int32_t key[kLoads], step;
+    u32x4 k[kLoads], v[kLoads];
+    uint32_t ks[MX ? kLoads : 1], vs[MX ? kLoads : 1];
+
+    __device__ __forceinline__ Loader(const PagedCache& cache, const Tile& tile, int tid, int32_t start, int32_t by) : c(cache), t(tile), step(by) {
+      unit = tid % kLoadUnits;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        key[i] = start + tid / kLoadUnits + i * kRowsApart;
+        page_at[i] = key[i] / c.page_size;
+        row_at[i] = key[i] % c.page_size;
+      }
+      ask();
+    }
+    __device__ __forceinline__ void ask() {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) entry[i] = key[i] < t.k1 ? t.pages[page_at[i]] : -1;
+    }
+    // Asks for the step's rows, and for the page-table entries of the next.
+    __device__ __forceinline__ void load() {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const bool there = (uint32_t)entry[i] < (uint32_t)c.pages;
+        const int64_t off = (int64_t)entry[i] * c.page_bytes + (int64_t)row_at[i] * c.row_bytes + (int64_t)t.head * c.head_bytes + unit * 16;
+        k[i] = *(there ? (const u32x4*)((const unsigned char*)c.k + off) : &paged_zeros);
+        v[i] = *(there ? (const u32x4*)((const unsigned char*)c.v + off) : &paged_zeros);
+        if constexpr (MX) {
+          const int64_t s = (int64_t)entry[i] * c.s_page + (int64_t)row_at[i] * c.s_row + (int64_t)t.head * c.s_head + unit / 2;
+          ks[i] = *(there ? c.ks + s : (const uint8_t*)&paged_zeros);
+          vs[i] = *(there ? c.vs + s : (const uint8_t*)&paged_zeros);
+        }
+        key[i] += step;
+        page_at[i] += step / c.page_size;
+        row_at[i] += step % c.page_size;
+        if (row_at[i] >= c.page_size) row_at[i] -= c.page_size, ++page_at[i];
+      }
+      ask();
+    }
+    // True in a lane that held a value of V that is no finite number.
+    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv, int tid) {
+      u16x2 most = {0, 0};
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) put(most, sk, sv, tid / kLoadUnits + i * kRowsApart, unit, k[i], v[i], ks[MX ? i : 0], vs[MX ? i : 0]);
+      return most[0] >= kInfinite || most[1] >= kInfinite;
+    }
+  };
+
+  // The same of 32 keys by one wavefront: lane r looks key r up (and lane r + 32), and the lanes that fetch its row get the place from there.
+  struct OwnLoader {
+    static constexpr int kLoads = 32 * kLoadUnits / 64, kRowsAtOnce = 64 / kLoadUnits;
+    const PagedCache& c;
+    const Tile& t;
+    int32_t key, page_at, row_at, entry, step;
+    u32x4 k[kLoads], v[kLoads];
+    uint32_t ks[MX ? kLoads : 1], vs[MX ? kLoads : 1];
+
+    __device__ __forceinline__ OwnLoader(const PagedCache& cache, const Tile& tile, int32_t start, int32_t by) : c(cache), t(tile), step(by) {
+      key = start + (threadIdx.x & 31);
+      page_at = key / c.page_size, row_at = key % c.page_size;
+      ask();
+    }
+    __device__ __forceinline__ void ask() { entry = key < t.k1 ? t.pages[page_at] : -1; }
+    __device__ __forceinline__ static int64_t of_lane(int64_t v, int lane) {
+      const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)v), hi = __builtin_amdgcn_ds_bpermute(lane * 4, (int)(v >> 32));
+      return (int64_t)((uint64_t)hi << 32 | lo);
+    }
+    __device__ __forceinline__ void load() {
+      const int lane = threadIdx.x & 63, unit = lane % kLoadUnits;
+      const bool there = (uint32_t)entry < (uint32_t)c.pages;
+      const int64_t off = there ? (int64_t)entry * c.page_bytes + (int64_t)row_at * c.row_bytes : -1, s_off = (int64_t)entry * c.s_page + (int64_t)row_at * c.s_row;
+      const unsigned char *kb = (const unsigned char*)c.k + (int64_t)t.head * c.head_bytes + unit * 16, *vb = (const unsigned char*)c.v + (int64_t)t.head * c.head_bytes + unit * 16;
+      const uint8_t *ksb = c.ks + (int64_t)t.head * c.s_head + unit / 2, *vsb = c.vs + (int64_t)t.head * c.s_head + unit / 2;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = lane / kLoadUnits + i * kRowsAtOnce;
+        const int64_t at = of_lane(off, r);
+        k[i] = *(at >= 0 ? (const u32x4*)(kb + at) : &paged_zeros);
+        v[i] = *(at >= 0 ? (const u32x4*)(vb + at) : &paged_zeros);
+        if constexpr (MX) {
+          const int64_t s_at = of_lane(s_off, r);
+          ks[i] = *(at >= 0 ? ksb + s_at : (const uint8_t*)&paged_zeros);
+          vs[i] = *(at >= 0 ? vsb + s_at : (const uint8_t*)&paged_zeros);
+        }
+      }
+      key += step;
+      page_at += step / c.page_size;
+      row_at += step % c.page_size;
+      if (row_at >= c.page_size) row_at -= c.page_size, ++page_at;
+      ask();
+    }
+    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv) {
+      const int lane = threadIdx.x & 63, unit = lane % kLoadUnits;
+      u16x2 most = {0, 0};
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) put(most, sk, sv, lane / kLoadUnits + i * kRowsAtOnce, unit, k[i], v[i], ks[MX ? i : 0], vs[MX ? i : 0]);
+      return most[0] >= kInfinite || most[1] >= kInfinite;
+    }
+  };
+
+  // 32 rows of a tile as a wavefront holds them.
+  struct Rows {
+    vec8 q[KS];
+    f32x16 o[DB];
+    float m, l;               // of the lane's row; l of the lane's half of the keys
+    int32_t lo, hi;           // keys the lane's row sees
+    int32_t all_lo, all_hi;   // that every row of the wavefront sees
+    int32_t any_lo, any_hi;   // that one of them sees
+    bool used;
+    int missed;               // steps whose second product is still to be done
+  };
+
+  __device__ static __forceinline__ void begin(Rows& w, const Tile& t, const TensorArg<3>& q, const PagedPlan& p, int row_block) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+    const int32_t r0 = row_block * 32, n = min(32, t.rows - r0);
+    w.used = n > 0;
+    const int32_t r = t.row0 + r0 + min(l32, max(n, 1) - 1), token = r / p.group, head = r % p.group;   // (lanes beyond the last row repeat it)
+    const T* from = (const T*)q.ptr + (int64_t)(t.first + token) * q.strides[0] + (int64_t)(t.head * p.group + head) * q.strides[1];
+    if (w.used) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) w.q[ks] = __builtin_bit_cast(vec8, (*reinterpret_cast<const u32x4*>(from + ks * 16 + half * 8) & p.q_and) ^ p.q_xor);
+    }
+    auto low = [&](int32_t pos) { return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0; };
+    const int32_t pos = t.pos0 + token, first = t.pos0 + (t.row0 + r0) / p.group, last = t.pos0 + (t.row0 + r0 + max(n, 1) - 1) / p.group;
+    w.lo = low(pos), w.hi = min(pos, t.k1 - 1);
+    w.any_lo = low(first), w.all_lo = low(last);
+    w.all_hi = min(first, t.k1 - 1), w.any_hi = min(last, t.k1 - 1);
+    w.m = -INFINITY, w.l = 0.0f, w.missed = 0;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w.o[i][e] = 0.0f;
+  }
+
+  __device__ static __forceinline__ vec8 v_frag(const unsigned char* sv, int t, int db, int lane) {
+    const int grp = lane >> 4, l16 = lane & 15;
+    const int dcol = db * 32 + (grp & 1) * 16 + (l16 & 3) * 4, kr = t * 16 + (grp >> 1) * 4 + (l16 >> 2);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(sv + v_off(kr, dcol >> 3) + (dcol & 7) * 2));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(sv + v_off(kr + 8, dcol >> 3) + (dcol & 7) * 2));
+    return __builtin_bit_cast(vec8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+
+  // B blocks of 32 keys from `key0` on, K and V at sk and sv: their products with the rows, and the softmax so far.  `apart`: V holds values that are no finite
+  // numbers.  They must not reach rows that do not see their keys, and 0 times them would: where some rows see a part of such keys the second product is
+  // left for later (add_missed).
+  template <int B>
+  __device__ static __forceinline__ void keys(Rows& w, const unsigned char* sk, const unsigned char* sv, int32_t key0, float c, bool apart, int32_t* missed) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+    if (!w.used || key0 > w.any_hi || key0 + B * 32 - 1 < w.any_lo) return;
+    f32x16 s[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[b] = E::mfma(*reinterpret_cast<const vec8*>(sk + k_off(b * 32 + l32, ks * 2 + half)), w.q[ks], s[b]);
+    }
+    // s[b][e] belongs to key key0 + b * 32 + (e / 4) * 8 + half * 4 + e % 4 and to this lane's row
+    const bool masked = key0 + B * 32 - 1 > w.all_hi || key0 < w.all_lo;
+    if (masked) {
+      const int32_t hi = w.hi - key0 - half * 4, lo = w.lo - key0 - half * 4;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int kk = b * 32 + (e >> 2) * 8 + (e & 3);
+          s[b][e] = kk <= hi && kk >= lo ? s[b][e] : -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
+    mx = max_across_halves(mx);
+    constexpr float kSlack = 8.0f;   // the reference point only has to bound the exponents: it moves when a row's maximum has risen by more
+    const float m_cand = fmaxf(w.m, mx * c);
+    const bool moved = __builtin_amdgcn_ballot_w64(m_cand > w.m + kSlack) != 0;
+    const float m_new = moved ? m_cand : w.m;
+    const float m_use = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen so far: keep exp2 finite
+    float p[B][16], rs = 0.0f;
+    vec8 pf[B][2];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        p[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], c, -m_use));
+        rs += p[b][e];
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {   // P in 16 bits, as V is: the weights' rounding stays below that of V
+        const u32x4 v = {E::pack2(p[b][t * 8 + 0], p[b][t * 8 + 1]), E::pack2(p[b][t * 8 + 2], p[b][t * 8 + 3]), E::pack2(p[b][t * 8 + 4], p[b][t * 8 + 5]),
+                         E::pack2(p[b][t * 8 + 6], p[b][t * 8 + 7])};
+        pf[b][t] = __builtin_bit_cast(vec8, v);
+      }
+    }
+    if (moved) {
+      const float alpha = __builtin_amdgcn_exp2f(w.m - m_use);
+      w.l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w.o[i][e] *= alpha;
+      w.m = m_new;
+    }
+    w.l += rs;
+    if (masked && apart) {
+      if (w.missed < kMostMissed) missed[w.missed++] = key0;
+    } else {
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) w.o[db] = E::mfma(v_frag(sv + b * kBlockBytes, t, db, lane), pf[b][t], w.o[db]);
+    }
+  }
+
+  // LDS operations of one wavefront happen in order; the compiler is kept to it.
+  __device__ static __forceinline__ void ordered() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // O^T += V^T P^T of the steps of `blocks` x 32 keys that keys() left out, m and l being those of all keys: what is no finite number is taken out of V, and what it makes
+  // of the rows that see it found by a product of its own, of marks with 0 and 1.
+  __device__ static __forceinline__ void add_missed(Rows& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, const int32_t* missed, int blocks) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    constexpr bool kHalf = std::is_same<T, _Float16>::value;
+    constexpr uint16_t kOne = kHalf ? 0x3c00 : 0x3f80, k64 = kHalf ? 0x5400 : 0x4280, k4096 = kHalf ? 0x6c00 : 0x4580;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned char *sk = lds + wave * (2 * kBlockBytes), *sv = sk + kBlockBytes;
+#pragma unroll 1
+    for (int n = 0; n < w.missed * blocks; ++n) {
+      const int32_t key0 = missed[wave * kMostMissed + n / blocks] + n % blocks * 32;
+      OwnLoader in(c, t, key0, 32);
+      in.load();
+      in.store(sk, sv);
+      ordered();
+      f32x16 s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = E::mfma(*reinterpret_cast<const vec8*>(sk + k_off(l32, ks * 2 + half)), w.q[ks], s);
+      vec8 pf[2], sees[2];   // weights, and 1 where the lane's row sees the key
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        u32x4 p;
+        u16x8 x;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          float by[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int32_t kk = key0 + t * 16 + ((i + j) >> 2) * 8 + half * 4 + ((i + j) & 3);
+            const bool there = kk >= w.lo && kk <= w.hi;
+            by[j] = there ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t * 8 + i + j], scale, -w.m)) : 0.0f;
+            x[i + j] = there ? kOne : 0;
+          }
+          p[i / 2] = E::pack2(by[0], by[1]);
+        }
+        pf[t] = __builtin_bit_cast(vec8, p), sees[t] = __builtin_bit_cast(vec8, x);
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        f32x16 marks;   // of the keys that the row sees: 1 for each NaN, 64 for each infinity, 4096 for each negative one
+#pragma unroll
+        for (int e = 0; e < 16; ++e) marks[e] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u16x8 f = __builtin_bit_cast(u16x8, v_frag(sv, t, db, lane)), mark;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint16_t mag = f[i] & 0x7fff;
+            mark[i] = mag > kInfinite ? kOne : mag < kInfinite ? (uint16_t)0 : f[i] >> 15 ? k4096 : k64;
+            f[i] = mag < kInfinite ? f[i] : (uint16_t)0;
+          }
+          w.o[db] = E::mfma(__builtin_bit_cast(vec8, f), pf[t], w.o[db]);
+          marks = E::mfma(__builtin_bit_cast(vec8, mark), sees[t], marks);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int n = (int)marks[e];
+          w.o[db][e] += (n & 63 ? NAN : 0.0f) + (n & 4032 ? INFINITY : 0.0f) - (n >> 12 ? INFINITY : 0.0f);
+        }
+      }
+      ordered();
+    }
+  }
+
+  // Up to 32 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ...
+  __device__ static __forceinline__ void own_keys(Rows& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* missed) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned char *sk = lds + wave * (2 * kBlockBytes), *sv = sk + kBlockBytes;
+    int32_t key = t.k0 + wave * 32;
+    if (key >= t.k1) return;
+    OwnLoader in(c, t, key, W * 32);
+    in.load();
+    bool apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv)) != 0;
+    ordered();
+#pragma unroll 1
+    for (; key < t.k1; key += W * 32) {
+      const bool more = key + W * 32 < t.k1;
+      if (more) in.load();
+      keys<1>(w, sk, sv, key, scale, apart, missed + wave * kMostMissed);
+      ordered();
+      if (more) apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv)) != 0;
+      ordered();
+    }
+  }
+
+  // R x 32 rows: wavefront (r, s) has the rows of block r and the key blocks s * B .. of every step of S * B * 32 keys, which all wavefronts fetch together.
+  template <int R, int B>
+  __device__ static __forceinline__ void shared_keys(Rows& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* apart_at, int32_t* missed) {
+    constexpr int S = W / R, N = S * B * 32, kTile = N * D * 2;
+    static_assert(4 * kTile <= kLdsBytes, "two stages");
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ws = wave % S;
+    if (t.k0 >= t.k1) return;
+    Loader<N, kThreads> in(c, t, threadIdx.x, t.k0, N);
+    // the step whose V, in that stage, holds a value that is no finite number: known to all behind the barrier
+    if (threadIdx.x < 2) apart_at[threadIdx.x] = -1;
+    __syncthreads();
+    in.load();
+    if (in.store(lds, lds + kTile, threadIdx.x)) apart_at[0] = t.k0;
+    __syncthreads();
+    int cur = 0;
+#pragma unroll 1
+    for (int32_t key = t.k0; key < t.k1; key += N) {
+      const bool more = key + N < t.k1;
+      if (more) in.load();
+      const unsigned char* sk = lds + cur * (2 * kTile) + ws * B * kBlockBytes;
+      keys<B>(w, sk, sk + kTile, key + ws * B * 32, scale, apart_at[cur] == key, missed + wave * kMostMissed);
+      cur ^= 1;
+      if (more && in.store(lds + cur * (2 * kTile), lds + cur * (2 * kTile) + kTile, threadIdx.x)) apart_at[cur] = key + N;
+      __syncthreads();
+    }
+  }
+
+  // Columns 4 u .. of a row, divided and rounded.
+  __device__ static __forceinline__ void store_row(const PartitionArg<3>& out, const Tile& t, const PagedPlan& p, int32_t row, int u, const f32x4& o, float l) {
+    const int32_t r = t.row0 + row, token = r / p.group, head = r % p.group;
+    const float sum = l == 0.0f ? 1.0f : l;   // a row that saw no key: 0
+    const u32x2 v = {E::pack2(o[0] / sum, o[1] / sum), E::pack2(o[2] / sum, o[3] / sum)};
+    *reinterpret_cast<u32x2*>((T*)out.ptr + (int64_t)(t.first + token) * out.strides[0] + (int64_t)(t.head * p.group + head) * out.strides[1] + u * 4) = v;
+  }
+
+  // The results of the wavefronts, S to 32 rows, and of the tile's other workgroups to out.
+  __device__ static __forceinline__ void finish(Rows& w, const Tile& t, const PartitionArg<3>& out, const PagedPlan& p, unsigned char* partials, int32_t slot_rows, unsigned char* lds,
+                                                float (*stat)[2][32], uint32_t* flag, int S) {
+    constexpr int U = D / 4, kRowsAtOnce = kThreads / U;
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float l = sum_across_halves(w.l);
+    if (half == 0) stat[wave][0][l32] = w.m, stat[wave][1][l32] = l;
+    unsigned char* band = lds + wave * kBandBytes + l32 * (D * 4);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(band + (((db * 8 + g * 2 + half) ^ (l32 & 15)) << 4)) = f32x4{w.o[db][g * 4], w.o[db][g * 4 + 1], w.o[db][g * 4 + 2], w.o[db][g * 4 + 3]};
+    __syncthreads();
+    const uint32_t bytes = (uint32_t)slot_rows * (D + 2) * 4, stats = (uint32_t)slot_rows * D * 4;   // of a share of the workspace
+    const __amdgpu_buffer_rsrc_t part = make_rsrc(partials, bytes * t.shares);
+    const int u = tid % U;
+#pragma unroll 1
+    for (int row = tid / U; row < t.rows; row += kRowsAtOnce) {
+      const int first = row / 32 * S, r = row % 32;
+      float top = -INFINITY;
+      for (int s = 0; s < S; ++s) top = fmaxf(top, stat[first + s][0][r]);
+      const float use = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s = 0; s < S; ++s) {
+        const float by = __builtin_amdgcn_exp2f(stat[first + s][0][r] - use);
+        sum = __builtin_fmaf(stat[first + s][1][r], by, sum);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (first + s) * kBandBytes + r * (D * 4) + ((u ^ (r & 15)) << 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[e], by, o[e]);
+      }
+      if (t.shares == 1) {
+        store_row(out, t, p, row, u, o, sum);
+      } else {
+        gemm::store_partial(o, part, t.share * bytes + (uint32_t)row * (D * 4) + u * 16);
+        if (u == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{top, sum}), part, t.share * bytes + stats + row * 8, 0, gemm::kAgentScope);
+      }
+    }
+    if (t.shares == 1 || !gemm::last_to_arrive(p.counters + t.slot, t.shares, flag)) return;
+#pragma unroll 1
+    for (int row = tid / U; row < t.rows; row += kRowsAtOnce) {
+      constexpr uint32_t kAtOnce = 4;   // shares whose reads are under way together
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+      float m = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+      for (uint32_t k = 0; k < t.shares; k += kAtOnce) {
+        u32x4 v[kAtOnce];
+        f32x2 st[kAtOnce];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+          const bool there = k + i < t.shares;
+          v[i] = __builtin_amdgcn_raw_buffer_load_b128(part, there ? (k + i) * bytes + (uint32_t)row * (D * 4) + u * 16 : kOob, 0, gemm::kAgentScope);
+          st[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(part, there ? (k + i) * bytes + stats + row * 8 : kOob, 0, gemm::kAgentScope));
+        }
+        float top = m;
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) top = fmaxf(top, k + i < t.shares ? st[i][0] : -INFINITY);
+        const float use = top == -INFINITY ? 0.0f : top, was = __builtin_amdgcn_exp2f(m - use);
+        m = top, sum *= was, o *= was;
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+          const float by = k + i < t.shares ? __builtin_amdgcn_exp2f(st[i][0] - use) : 0.0f;
+          const f32x4 x = __builtin_bit_cast(f32x4, v[i]);
+          sum = __builtin_fmaf(st[i][1], by, sum);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], by, o[e]);
+        }
+      }
+      store_row(out, t, p, row, u, o, sum);
+    }
+  }
+
+  __device__ static __forceinline__ void run(const TensorArg<3>& q, const PartitionArg<3>& out, const PagedCache& c, const PagedPlan& p) {
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
+    __shared__ float stat[W][2][32];
+    __shared__ uint32_t flag;
+    __shared__ int32_t apart_at[2], missed[W * kMostMissed];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t heads = (uint32_t)c.heads, of_long = (uint32_t)p.long_tiles * p.long_shares;
+    const uint32_t head = blockIdx.x % heads, item = blockIdx.x / heads;
+    const bool is_long = item < of_long;
+    Tile t;
+    t.head = (int32_t)head;
+    int32_t b;
+    uint32_t most, keys_each;
+    paged::Sequence s;
+    if (is_long) {
+      // Tiles of sequence b have the numbers from starts[b] * group / BM + b on: more than there are, so that nobody has to count them.  The last ones, whose rows see
+      // the most keys, come first.
+      const int32_t n = p.long_tiles - 1 - (int32_t)(item / p.long_shares);
+      t.share = item % p.long_shares;
+      auto number = [&](int32_t i) { return (int64_t)min(max(c.starts[i], 0), c.tokens) * p.group / BM + i; };
+      b = paged::find_sequence(c.batch, n, number);
+      s = paged::sequence(c, b);
+      const int64_t row0 = ((int64_t)n - number(b)) * BM;
+      if (s.count * p.group <= p.few_rows || row0 < 0 || row0 >= (int64_t)s.count * p.group) return;
+      t.row0 = (int32_t)row0;
+      t.rows = min(BM, s.count * p.group - t.row0);
+      most = p.long_shares, keys_each = p.long_keys;
+      t.slot = (uint32_t)n * heads + head;
+    } else {
+      const uint32_t k = item - of_long;
+      b = (int32_t)(k / p.few_shares);
+      t.share = k % p.few_shares;
+      s = paged::sequence(c, b);
+      t.row0 = 0;
+      t.rows = s.count * p.group;
+      if (t.rows == 0 || t.rows > p.few_rows) return;
+      most = p.few_shares, keys_each = p.few_keys;
+      t.slot = ((uint32_t)p.long_tiles + b) * heads + head;
+    }
+    t.first = s.first;
+    t.pos0 = s.position(0);
+    t.pages = c.table + (int64_t)b * c.table_row;
+    const int32_t first = t.pos0 + t.row0 / p.group, last = t.pos0 + (t.row0 + t.rows - 1) / p.group;
+    const int32_t lo = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, hi = max(min(last + 1, s.held), lo);
+    t.shares = min(max((uint32_t)(hi - lo + keys_each - 1) / keys_each, 1u), most);
+    if (t.share >= t.shares) return;
+    t.k0 = lo + (int32_t)(t.share * keys_each);
+    t.k1 = t.share + 1 == t.shares ? hi : t.k0 + (int32_t)keys_each;
+
+    // long tiles' partial results first, [tile][head][share]
+    const int32_t slot_rows = is_long ? BM : p.few_slot_rows;
+    const uint64_t share_bytes = (uint64_t)slot_rows * (D + 2) * 4, long_bytes = p.long_shares > 1 ? (uint64_t)p.long_tiles * heads * p.long_shares * ((uint64_t)BM * (D + 2) * 4) : 0;
+    unsigned char* partials = (unsigned char*)p.partials + (is_long ? (uint64_t)t.slot * p.long_shares * share_bytes
+                                                                     : long_bytes + (uint64_t)(t.slot - (uint32_t)p.long_tiles * heads) * p.few_shares * share_bytes);
+    const int shared_by = t.rows <= 32 ? W : t.rows <= 64 ? W / 2 : W == 8 && t.rows <= 128 ? 2 : 1;   // wavefronts to the keys of 32 rows
+    int blocks = 1;
+    Rows w;
+    begin(w, t, q, p, wave / shared_by);
+    if (shared_by == W) {
+      own_keys(w, t, c, p.scale_log2e, lds, missed);
+    } else if (shared_by == W / 2) {
+      shared_keys<2, 1>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+    } else if (W == 8 && shared_by == 2) {
+      shared_keys<4, kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+      blocks = kStep;
+    } else {
+      shared_keys<W, 2 * kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+      blocks = 2 * kStep;
+    }
+    __syncthreads();   // everybody is done with the stages
+    add_missed(w, t, c, p.scale_log2e, lds, missed, blocks);
+    finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, shared_by);
+  }
+};
+
+}  // namespace
+
+#define ATTENTION(NAME, T, MX, D, W)                                                                                                                                        \
+  extern "C" __global__ void __launch_bounds__(W * 64) paged_attention_entry__##NAME##_d##D(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) { \
+    Paged<T, MX, D, W>::run(q, out, c, p);                                                                                                                                  \
+  }
+#define ATTENTION_D(NAME, T, MX) ATTENTION(NAME, T, MX, 64, 8) ATTENTION(NAME, T, MX, 128, 8) ATTENTION(NAME, T, MX, 256, 4)
+ATTENTION_D(f16, _Float16, false)
+ATTENTION_D(bf16, __bf16, false)
+ATTENTION_D(f16_mxfp8, _Float16, true)
+ATTENTION_D(bf16_mxfp8, __bf16, true)

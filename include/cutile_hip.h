@@ -797,6 +797,56 @@ cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cu
                                                 const cutile_tensor_arg_t* y, const cutile_tensor_arg_t* x_scales,
                                                 const cutile_tensor_arg_t* y_scales, float alpha, const cutile_launch_opts_t* opts);
 
+/* ---- a serving step over a paged cache: no counterpart in the reference, whose caches are one contiguous tensor a sequence (kv_cache.rs, attention.rs) and whose block
+ * copies (experimental/kvbm.rs) move blocks between layouts. ---------------------------------------------------------------
+ * A batch of B sequences shares the pages of one cache.  All of them take these tensors:
+ *   k_cache, v_cache  [pages, page_size, kv_heads, D], D 64, 128 or 256, of any strides but a unit inner one (the same for both), rows on 16-byte boundaries, either
+ *                     f16 or bf16 like the new tokens (k_scales, v_scales NULL), or f8e4m3fn with k_scales, v_scales [pages, page_size, kv_heads, D/32] f8e8m0fnu: mxfp8 as
+ *                     block_quantize makes it
+ *   page_table        [B, most pages of a sequence] i32, contiguous rows: position p of sequence b is row p % page_size of page page_table[b, p / page_size]
+ *   starts            [B + 1] i32, not falling: the new tokens of sequence b are the rows starts[b] .. starts[b+1] of new_k, new_v, q or out (rows that are nobody's stay as they
+ *                     are)
+ *   context_lens      [B] i32: tokens of the sequence with the new ones, which are the last: new token i stands at position context_lens[b] - (starts[b+1] - starts[b]) + i
+ * Their contents are device memory that a launch does not look at on the host, so a captured launch takes new ones at every replay.  A position before 0 or behind the
+ * table, and a page that the cache does not have (-1, say), is not written, reads as zeros and is never touched.  Sequences may share pages that a launch only reads. */
+/* paged_cache_write: the rows of new_k, new_v [tokens, kv_heads, D] (unit inner stride, rows on 16-byte boundaries) to their places; mxfp8 rounds them as block_quantize
+ * does.  Two tokens of one launch must not have the same place. */
+cutile_status_t cutile_launch_paged_cache_write(cutile_stream_t stream, const cutile_tensor_arg_t* new_k, const cutile_tensor_arg_t* new_v,
+                                                const cutile_tensor_arg_t* k_cache, const cutile_tensor_arg_t* v_cache, const cutile_tensor_arg_t* k_scales,
+                                                const cutile_tensor_arg_t* v_scales, const cutile_tensor_arg_t* page_table, const cutile_tensor_arg_t* starts,
+                                                const cutile_tensor_arg_t* context_lens, const cutile_launch_opts_t* opts);
+/* paged_cache_read: its inverse: out_k, out_v [tokens, kv_heads, D], f16 or bf16, partitioned [BM, kv_heads, D], get what lies at the places of their rows (starts that add
+ * up context_lens: all of every sequence), mxfp8 rounded once. */
+cutile_status_t cutile_launch_paged_cache_read(cutile_stream_t stream, const cutile_tensor_arg_t* k_cache, const cutile_tensor_arg_t* v_cache,
+                                               const cutile_tensor_arg_t* k_scales, const cutile_tensor_arg_t* v_scales, const cutile_tensor_arg_t* page_table,
+                                               const cutile_tensor_arg_t* starts, const cutile_tensor_arg_t* context_lens, const cutile_partition_arg_t* out_k,
+                                               const cutile_partition_arg_t* out_v, const cutile_launch_opts_t* opts);
+/* paged_attention: out[i, h, :] = sum_j softmax_j(qk_scale q[i, h, :] . k_j) v_j over the keys j of the sequence's KV head h / group, p - window < j <= p (window 0: all up to
+ * p), p the position of token i, group = q heads / kv_heads; q, out [tokens, q_heads, D], unit inner stride, rows on 16-byte boundaries, out partitioned [BM, G, D].  One token a
+ * sequence is a decode step, several a chunk of a prompt or a draft to be checked; a launch may hold all of them.  A row that sees no key is zeros; what a row does not see, NaN
+ * and infinities included, is nothing to it.  Softmax and sums in f32, the weights rounded to q's type for the second product.  Values of an mxfp8 cache have to be in the range of
+ * q's type.
+ * max_new: at least the most new tokens of a sequence, 0: not known; rows of a sequence beyond it are not promised.  max_context: about the longest of context_lens, 0: not known;
+ * it only decides how keys are dealt out.
+ * workspace: NULL, or device memory of the caller's (a contiguous tensor, 16-byte aligned, zeros before its first use; 40 MiB + 16 KiB are the most that is used) for
+ * the results of workgroups that share the keys of a tile.  One workspace serves one stream at a time; every launch leaves it fit for the next.  Without it the stream's own is
+ * taken, and a launch that is captured, for which there is none, runs unshared: much slower where few sequences have long contexts, in another order of summation. */
+cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cutile_tensor_arg_t* q, const cutile_tensor_arg_t* k_cache, const cutile_tensor_arg_t* v_cache,
+                                              const cutile_tensor_arg_t* k_scales, const cutile_tensor_arg_t* v_scales, const cutile_tensor_arg_t* page_table,
+                                              const cutile_tensor_arg_t* starts, const cutile_tensor_arg_t* context_lens, const cutile_partition_arg_t* out, float qk_scale,
+                                              int32_t window, int32_t max_new, int32_t max_context, const cutile_tensor_arg_t* workspace, const cutile_launch_opts_t* opts);
+/* adjust_logits: logits [rows, vocab] (f16, bf16 or f32, unit inner stride) to out of their type, partitioned [1, vocab], which may be logits itself.  Of every token t of a row,
+ * in f32 and in this order (each tensor may be NULL):
+ *   t among tokens[row, 0 .. token_lens[row]) ([rows, most] i32; token_lens NULL: all):   l <- l > 0 ? l / repetition[row] : l * repetition[row]
+ *   c > 0 times among those from prompt_lens[row] on (NULL: from 0):                       l <- l - (presence[row] + frequency[row] * c)
+ *   bias_ids, bias_values [rows, n], n up to 1024:  l <- l + the sum, in their order, of the values whose id is t
+ *   allowed [rows, words] i32 or u32, bit t % 32 of word t / 32 not set:                   l <- -infinity
+ * Ids outside the vocabulary (-1, say) count for nothing.  repetition, presence, frequency are f32 [rows]; the others i32. */
+cutile_status_t cutile_launch_adjust_logits(cutile_stream_t stream, const cutile_tensor_arg_t* logits, const cutile_partition_arg_t* out, const cutile_tensor_arg_t* tokens,
+                                            const cutile_tensor_arg_t* prompt_lens, const cutile_tensor_arg_t* token_lens, const cutile_tensor_arg_t* repetition,
+                                            const cutile_tensor_arg_t* presence, const cutile_tensor_arg_t* frequency, const cutile_tensor_arg_t* bias_ids,
+                                            const cutile_tensor_arg_t* bias_values, const cutile_tensor_arg_t* allowed, const cutile_launch_opts_t* opts);
+
 /* ======================================================================== */
 /* Part E — asynchronous runtime                                             */
 /* ======================================================================== */

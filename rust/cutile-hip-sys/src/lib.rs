@@ -328,6 +328,10 @@ extern "C" {
     pub fn cutile_launch_add_rms_norm_quantize(stream: cutile_stream_t, residual: *const cutile_tensor_arg_t, x: *const cutile_tensor_arg_t, w: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, scales: *const cutile_partition_arg_t, residual_out: *const cutile_partition_arg_t, eps: f32, tensor_scale: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
     pub fn cutile_launch_silu_mul_quantize(stream: cutile_stream_t, gate: *const cutile_tensor_arg_t, up: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, scales: *const cutile_partition_arg_t, tensor_scale: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
     pub fn cutile_launch_linear_tile_mxfp4(stream: cutile_stream_t, z: *const cutile_partition_arg_t, x: *const cutile_tensor_arg_t, y: *const cutile_tensor_arg_t, x_scales: *const cutile_tensor_arg_t, y_scales: *const cutile_tensor_arg_t, alpha: f32, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_paged_cache_write(stream: cutile_stream_t, new_k: *const cutile_tensor_arg_t, new_v: *const cutile_tensor_arg_t, k_cache: *const cutile_tensor_arg_t, v_cache: *const cutile_tensor_arg_t, k_scales: *const cutile_tensor_arg_t, v_scales: *const cutile_tensor_arg_t, page_table: *const cutile_tensor_arg_t, starts: *const cutile_tensor_arg_t, context_lens: *const cutile_tensor_arg_t, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_paged_cache_read(stream: cutile_stream_t, k_cache: *const cutile_tensor_arg_t, v_cache: *const cutile_tensor_arg_t, k_scales: *const cutile_tensor_arg_t, v_scales: *const cutile_tensor_arg_t, page_table: *const cutile_tensor_arg_t, starts: *const cutile_tensor_arg_t, context_lens: *const cutile_tensor_arg_t, out_k: *const cutile_partition_arg_t, out_v: *const cutile_partition_arg_t, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_paged_attention(stream: cutile_stream_t, q: *const cutile_tensor_arg_t, k_cache: *const cutile_tensor_arg_t, v_cache: *const cutile_tensor_arg_t, k_scales: *const cutile_tensor_arg_t, v_scales: *const cutile_tensor_arg_t, page_table: *const cutile_tensor_arg_t, starts: *const cutile_tensor_arg_t, context_lens: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, qk_scale: f32, window: i32, max_new: i32, max_context: i32, workspace: *const cutile_tensor_arg_t, opts: *const cutile_launch_opts_t) -> cutile_status_t;
+    pub fn cutile_launch_adjust_logits(stream: cutile_stream_t, logits: *const cutile_tensor_arg_t, out: *const cutile_partition_arg_t, tokens: *const cutile_tensor_arg_t, prompt_lens: *const cutile_tensor_arg_t, token_lens: *const cutile_tensor_arg_t, repetition: *const cutile_tensor_arg_t, presence: *const cutile_tensor_arg_t, frequency: *const cutile_tensor_arg_t, bias_ids: *const cutile_tensor_arg_t, bias_values: *const cutile_tensor_arg_t, allowed: *const cutile_tensor_arg_t, opts: *const cutile_launch_opts_t) -> cutile_status_t;
     pub fn cutile_execution_lock_acquire() -> cutile_status_t;
     pub fn cutile_execution_lock_release();
     pub fn cutile_execution_lock_held() -> i32;

@@ -528,7 +528,7 @@ std::vector<KernelEntry> build_table() {
         const std::string v = std::string(dt) + kept + "_d" + std::to_string(d);
         for (const char* fn : {"paged_cache_write", "paged_cache_read"}) add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_PAGED_CACHE, 256, 0, 0, 0, d, 0, dt, 0, 3);
         const int waves = d == 256 ? 4 : 8;
-        add("paged_attention", keep(v), keep("paged_attention_entry__" + v), IMG_PAGED_ATTENTION, (uint32_t)waves * 64, (uint32_t)waves * (32 * d * 4 + 256 + 16) + 12, waves * 32, 0, d, 0, dt, 0, 3);
+        add("paged_attention", keep(v), keep("paged_attention_entry__" + v), IMG_PAGED_ATTENTION, (uint32_t)waves * 64, (uint32_t)waves * (32 * (d * 4 + 48) + 256 + 16) + 12, waves * 32, 0, d, 0, dt, 0, 3);
       }
   // ---- logits in front of the choice of a token (512 threads; tile = (-, columns of a workgroup, -, -)) ----
   for (const char* dt : {"f16", "bf16", "f32"})

@@ -3732,6 +3732,7 @@ cutile_status_t check_covered(const char* fn, const cutile_partition_arg_t* cons
   return CUTILE_SUCCESS;
 }
 
+static const int kFewRounds = getenv("FEW_ROUNDS") ? atoi(getenv("FEW_ROUNDS")) : 1;
 // How keys are dealt out (see PagedPlan): `keys` to a workgroup so that `items` tiles of about `context` keys make about `wanted` workgroups, `step` keys at a time.
 struct Deal {
   int32_t keys = INT32_MAX, shares = 1;
@@ -3848,7 +3849,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     if (may_share && long_slots + few_items <= (int64_t)kSplitCounters) {
       if (long_items) of_long = deal_keys(long_items, context, cus, 256, std::max<int64_t>(1, room / (few_items ? 2 : 1) / (long_slots * bm * row_bytes)));
       const int64_t left = room - (of_long.shares > 1 ? of_long.shares * long_slots * bm * row_bytes : 0);
-      if (few_items) of_few = deal_keys(few_items, context, cus * 4, 512, std::max<int64_t>(1, left / (few_items * p.few_slot_rows * row_bytes)));
+      if (few_items) of_few = deal_keys(few_items, context, cus * kFewRounds, 512, std::max<int64_t>(1, left / (few_items * p.few_slot_rows * row_bytes)));
     }
     p.long_shares = of_long.shares, p.long_keys = of_long.keys;
     p.few_shares = of_few.shares, p.few_keys = of_few.keys;

@@ -3,9 +3,9 @@
 // p the position of token i; no key: zeros.
 //
 // The rows of a tile are pairs (token, query head of one KV head), token by token: group heads share every key that is read, and a decode step of 8 heads or a
-// chunk of 4 tokens fill the 32 columns of a matrix instruction.  Products, masks and softmax are those of fmha_common.h / fmha.hip: S^T = K Q^T and
+// chunk of 4 tokens fill the columns of a matrix instruction.  Products, masks and softmax are those of fmha_common.h / fmha.hip: S^T = K Q^T and
 // O^T = V^T P^T, so that a lane owns one row.
-//  * Tiles of up to 32 rows (decode, speculation): every wavefront has keys of its own, 32 at a time, through registers into LDS that no other
+//  * Tiles of up to 16 rows (decode, speculation): every wavefront has keys of its own, 32 at a time, through registers into LDS that no other
 //    wavefront reads: no barrier in the loop.  HBM's rate bounds it.
 //  * Larger tiles: R wavefronts side by side hold 32 rows each, S = wavefronts / R share the keys of a step; the matrix cores and exponentials bound it.
 // At the end the partial outputs go through LDS, and where the keys of a tile are dealt to several workgroups through the launch's workspace: the one that
@@ -46,6 +46,38 @@ __device__ __forceinline__ void widen(const u32x4& raw, uint32_t scale_byte, u32
   }
 }
 
+// How a wavefront holds X rows (32 or 16) of a tile: S^T and O^T have a row to a column of the matrix instruction, X columns wide, so that lane l has row l % X and, of
+// 32 keys, the S values of its group g = l / X; what a lane holds of P^T are then its operands of O^T += V^T P^T, the keys taken in that order.
+template <typename T, int D, int X>
+struct Shape;
+template <typename T, int D>
+struct Shape<T, D, 32> {
+  using vec8 = typename Elem<T>::vec8;
+  using Acc = f32x16;
+  static constexpr int kScores = 16, kSteps = 2;            // of 32 keys: values of S a lane holds, matrix products of P
+  static constexpr int kInner = 16, kOuter = 32;            // values of D to a product of S, to one of O
+  __device__ static __forceinline__ Acc mfma(vec8 a, vec8 b, Acc c) { return Elem<T>::mfma(a, b, c); }
+  __device__ static __forceinline__ int key_of(int e, int g) { return (e >> 2) * 8 + g * 4 + (e & 3); }
+  __device__ static __forceinline__ int col_of(int e, int g) { return (e >> 2) * 8 + g * 4 + (e & 3); }   // of O^T's rows
+  __device__ static __forceinline__ float most(float v) { return max_across_halves(v); }
+  __device__ static __forceinline__ float sum(float v) { return sum_across_halves(v); }
+};
+template <typename T, int D>
+struct Shape<T, D, 16> {
+  using vec8 = typename Elem<T>::vec8;
+  using Acc = f32x4;
+  static constexpr int kScores = 8, kSteps = 1;
+  static constexpr int kInner = 32, kOuter = 16;
+  __device__ static __forceinline__ Acc mfma(vec8 a, vec8 b, Acc c) {
+    if constexpr (std::is_same<T, _Float16>::value) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ int key_of(int e, int g) { return (e >> 2) * 16 + g * 4 + (e & 3); }
+  __device__ static __forceinline__ int col_of(int e, int g) { return g * 4 + e; }
+  __device__ static __forceinline__ float most(float v) { return max_across_rows(v); }
+  __device__ static __forceinline__ float sum(float v) { return sum_across_rows(v); }
+};
+
 // What a workgroup works on: the rows of a tile and its share of their keys.
 struct Tile {
   int32_t head;            // KV head
@@ -64,15 +96,20 @@ struct Paged {
   using vec8 = typename E::vec8;
   static constexpr int kThreads = W * 64, BM = W * 32;
   static constexpr int DB = D / 32, KS = D / 16, kUnits = D / 8;   // 16-byte units of a 16-bit row
-  static constexpr int kBlockBytes = 32 * D * 2;                   // 32 rows of K or V in LDS
+  // Rows of K and V in LDS are padded so that the lanes of a read meet different banks: 16 bytes for reads of a row a lane, 32 for the transposing ones of
+  // four rows.  (Swizzled units, as in fmha.hip, take a register for every address; here they are one address and constants.)
+  static constexpr int kRowK = D * 2 + 16, kRowV = D * 2 + 32;
+  static constexpr int kOwnBytes = 32 * (kRowK + kRowV);           // 32 keys of a wavefront
   static constexpr int kBandBytes = 32 * D * 4;                    // a wavefront's partial output
-  static constexpr int kLdsBytes = W * kBandBytes;                 // = W x (K and V of 32 keys)
+  static constexpr int kLdsBytes = W * kOwnBytes;
+  static_assert(kBandBytes <= kOwnBytes, "the partial outputs lie where the keys were");
   static constexpr int kMostMissed = 4;                            // steps that hold a border of what the 32 rows see: two at either end
-  static constexpr int kStep = D == 64 ? 2 : 1;                    // key blocks of a step are doubled where rows are short: a load each for the threads
+  // Key blocks of a step: short rows leave a load for every thread, long ones the registers that the operands need.
+  static constexpr int kStep = D == 64 ? 2 : 1, kWideStep = D == 64 ? 4 : D == 128 ? 2 : 1;
   static constexpr int kLoadUnits = D * (MX ? 1 : 2) / 16;         // 16-byte loads of a row of the cache
 
-  __device__ static __forceinline__ int k_off(int r, int u) { return r * (D * 2) + ((u ^ (r & (kUnits - 1) & 15)) << 4); }
-  __device__ static __forceinline__ int v_off(int r, int u) { return r * (D * 2) + ((u ^ ((r & (kUnits >= 16 ? 3 : 1)) << 2)) << 4); }
+  __device__ static __forceinline__ int k_off(int r, int u) { return r * kRowK + u * 16; }
+  __device__ static __forceinline__ int v_off(int r, int u) { return r * kRowV + u * 16; }
 
   // The largest magnitudes so far of 16-bit values in the halves of a dword, as integers: NaN and infinities are on top.
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
@@ -209,11 +246,13 @@ struct Paged {
     }
   };
 
-  // 32 rows of a tile as a wavefront holds them.
+  // X rows of a tile as a wavefront holds them.
+  template <int X>
   struct Rows {
-    vec8 q[KS];
-    f32x16 o[DB];
-    float m, l;               // of the lane's row; l of the lane's half of the keys
+    using H = Shape<T, D, X>;
+    vec8 q[D / H::kInner];
+    typename H::Acc o[D / H::kOuter];
+    float m, l;               // of the lane's row; l of the lane's share of the keys
     int32_t lo, hi;           // keys the lane's row sees
     int32_t all_lo, all_hi;   // that every row of the wavefront sees
     int32_t any_lo, any_hi;   // that one of them sees
@@ -221,15 +260,17 @@ struct Paged {
     int missed;               // steps whose second product is still to be done
   };
 
-  __device__ static __forceinline__ void begin(Rows& w, const Tile& t, const TensorArg<3>& q, const PagedPlan& p, int row_block) {
-    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-    const int32_t r0 = row_block * 32, n = min(32, t.rows - r0);
+  template <int X>
+  __device__ static __forceinline__ void begin(Rows<X>& w, const Tile& t, const TensorArg<3>& q, const PagedPlan& p, int row_block) {
+    using H = Shape<T, D, X>;
+    const int lane = threadIdx.x & 63;
+    const int32_t r0 = row_block * X, n = min(X, t.rows - r0);
     w.used = n > 0;
-    const int32_t r = t.row0 + r0 + min(l32, max(n, 1) - 1), token = r / p.group, head = r % p.group;   // (lanes beyond the last row repeat it)
+    const int32_t r = t.row0 + r0 + min(lane % X, max(n, 1) - 1), token = r / p.group, head = r % p.group;   // (lanes beyond the last row repeat it)
     const T* from = (const T*)q.ptr + (int64_t)(t.first + token) * q.strides[0] + (int64_t)(t.head * p.group + head) * q.strides[1];
     if (w.used) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) w.q[ks] = __builtin_bit_cast(vec8, (*reinterpret_cast<const u32x4*>(from + ks * 16 + half * 8) & p.q_and) ^ p.q_xor);
+      for (int ks = 0; ks < D / H::kInner; ++ks) w.q[ks] = __builtin_bit_cast(vec8, (*reinterpret_cast<const u32x4*>(from + ks * H::kInner + lane / X * 8) & p.q_and) ^ p.q_xor);
     }
     auto low = [&](int32_t pos) { return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0; };
     const int32_t pos = t.pos0 + token, first = t.pos0 + (t.row0 + r0) / p.group, last = t.pos0 + (t.row0 + r0 + max(n, 1) - 1) / p.group;
@@ -238,43 +279,54 @@ struct Paged {
     w.all_hi = min(first, t.k1 - 1), w.any_hi = min(last, t.k1 - 1);
     w.m = -INFINITY, w.l = 0.0f, w.missed = 0;
 #pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) w.o[i][e] = 0.0f;
+    for (auto& o : w.o) o = typename H::Acc{};
   }
 
-  __device__ static __forceinline__ vec8 v_frag(const unsigned char* sv, int t, int db, int lane) {
-    const int grp = lane >> 4, l16 = lane & 15;
-    const int dcol = db * 32 + (grp & 1) * 16 + (l16 & 3) * 4, kr = t * 16 + (grp >> 1) * 4 + (l16 >> 2);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(sv + v_off(kr, dcol >> 3) + (dcol & 7) * 2));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(sv + v_off(kr + 8, dcol >> 3) + (dcol & 7) * 2));
+  // S^T of 32 keys.
+  template <int X>
+  __device__ static __forceinline__ void scores(const Rows<X>& w, const unsigned char* sk, float (&s)[Shape<T, D, X>::kScores]) {
+    using H = Shape<T, D, X>;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 32 / X; ++i) {
+      typename H::Acc acc = {};
+#pragma unroll
+      for (int ks = 0; ks < D / H::kInner; ++ks)
+        acc = H::mfma(*reinterpret_cast<const vec8*>(sk + k_off(i * X + lane % X, ks * (H::kInner / 8) + lane / X)), w.q[ks], acc);
+#pragma unroll
+      for (int e = 0; e < H::kScores * X / 32; ++e) s[i * (H::kScores * X / 32) + e] = acc[e];
+    }
+  }
+
+  // The operand V^T of O's rows ob * kOuter .. and the keys of step t.
+  template <int X>
+  __device__ static __forceinline__ vec8 v_frag(const unsigned char* sv, int t, int ob) {
+    const int lane = threadIdx.x & 63, grp = lane >> 4, l16 = lane & 15;
+    const int col = ob * Shape<T, D, X>::kOuter + (X == 32 ? (grp & 1) * 16 : 0) + (l16 & 3) * 4, row = t * 16 + (X == 32 ? grp >> 1 : grp) * 4 + (l16 >> 2);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(sv + v_off(row, 0) + col * 2));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(sv + v_off(row + (X == 32 ? 8 : 16), 0) + col * 2));
     return __builtin_bit_cast(vec8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
   // B blocks of 32 keys from `key0` on, K and V at sk and sv: their products with the rows, and the softmax so far.  `apart`: V holds values that are no finite
   // numbers.  They must not reach rows that do not see their keys, and 0 times them would: where some rows see a part of such keys the second product is
   // left for later (add_missed).
-  template <int B>
-  __device__ static __forceinline__ void keys(Rows& w, const unsigned char* sk, const unsigned char* sv, int32_t key0, float c, bool apart, int32_t* missed) {
-    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  template <int X, int B>
+  __device__ static __forceinline__ void keys(Rows<X>& w, const unsigned char* sk, const unsigned char* sv, int32_t key0, float c, bool apart, int32_t* missed) {
+    using H = Shape<T, D, X>;
+    const int lane = threadIdx.x & 63, g = lane / X;
     if (!w.used || key0 > w.any_hi || key0 + B * 32 - 1 < w.any_lo) return;
-    f32x16 s[B];
+    float s[B][H::kScores];   // s[b][e] belongs to key key0 + b * 32 + key_of(e, g) and to this lane's row
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[b] = E::mfma(*reinterpret_cast<const vec8*>(sk + k_off(b * 32 + l32, ks * 2 + half)), w.q[ks], s[b]);
-    }
-    // s[b][e] belongs to key key0 + b * 32 + (e / 4) * 8 + half * 4 + e % 4 and to this lane's row
+    for (int b = 0; b < B; ++b) scores<X>(w, sk + b * 32 * kRowK, s[b]);
     const bool masked = key0 + B * 32 - 1 > w.all_hi || key0 < w.all_lo;
     if (masked) {
-      const int32_t hi = w.hi - key0 - half * 4, lo = w.lo - key0 - half * 4;
+      const int32_t hi = w.hi - key0 - g * 4, lo = w.lo - key0 - g * 4;
 #pragma unroll
       for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int kk = b * 32 + (e >> 2) * 8 + (e & 3);
+        for (int e = 0; e < H::kScores; ++e) {
+          const int kk = b * 32 + H::key_of(e, 0);
           s[b][e] = kk <= hi && kk >= lo ? s[b][e] : -INFINITY;
         }
     }
@@ -282,36 +334,33 @@ struct Paged {
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
-    mx = max_across_halves(mx);
+      for (int e = 0; e < H::kScores; ++e) mx = fmaxf(mx, s[b][e]);
+    mx = H::most(mx);
     constexpr float kSlack = 8.0f;   // the reference point only has to bound the exponents: it moves when a row's maximum has risen by more
     const float m_cand = fmaxf(w.m, mx * c);
     const bool moved = __builtin_amdgcn_ballot_w64(m_cand > w.m + kSlack) != 0;
     const float m_new = moved ? m_cand : w.m;
     const float m_use = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen so far: keep exp2 finite
-    float p[B][16], rs = 0.0f;
-    vec8 pf[B][2];
+    float rs = 0.0f;
+    vec8 pf[B][H::kSteps];
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
+    for (int b = 0; b < B; ++b)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        p[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], c, -m_use));
-        rs += p[b][e];
-      }
+      for (int t = 0; t < H::kSteps; ++t) {   // P in 16 bits, as V is: the weights' rounding stays below that of V
+        u32x4 v;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {   // P in 16 bits, as V is: the weights' rounding stays below that of V
-        const u32x4 v = {E::pack2(p[b][t * 8 + 0], p[b][t * 8 + 1]), E::pack2(p[b][t * 8 + 2], p[b][t * 8 + 3]), E::pack2(p[b][t * 8 + 4], p[b][t * 8 + 5]),
-                         E::pack2(p[b][t * 8 + 6], p[b][t * 8 + 7])};
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][t * 8 + 2 * i], c, -m_use)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][t * 8 + 2 * i + 1], c, -m_use));
+          rs += p0, rs += p1;
+          v[i] = E::pack2(p0, p1);
+        }
         pf[b][t] = __builtin_bit_cast(vec8, v);
       }
-    }
     if (moved) {
       const float alpha = __builtin_amdgcn_exp2f(w.m - m_use);
       w.l *= alpha;
 #pragma unroll
-      for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w.o[i][e] *= alpha;
+      for (auto& o : w.o) o *= alpha;
       w.m = m_new;
     }
     w.l += rs;
@@ -321,9 +370,9 @@ struct Paged {
 #pragma unroll
       for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < H::kSteps; ++t)
 #pragma unroll
-          for (int db = 0; db < DB; ++db) w.o[db] = E::mfma(v_frag(sv + b * kBlockBytes, t, db, lane), pf[b][t], w.o[db]);
+          for (int ob = 0; ob < D / H::kOuter; ++ob) w.o[ob] = H::mfma(v_frag<X>(sv + b * 32 * kRowV, t, ob), pf[b][t], w.o[ob]);
     }
   }
 
@@ -335,12 +384,14 @@ struct Paged {
 
   // O^T += V^T P^T of the steps of `blocks` x 32 keys that keys() left out, m and l being those of all keys: what is no finite number is taken out of V, and what it makes
   // of the rows that see it found by a product of its own, of marks with 0 and 1.
-  __device__ static __forceinline__ void add_missed(Rows& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, const int32_t* missed, int blocks) {
+  template <int X>
+  __device__ static __forceinline__ void add_missed(Rows<X>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, const int32_t* missed, int blocks) {
+    using H = Shape<T, D, X>;
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
     constexpr bool kHalf = std::is_same<T, _Float16>::value;
     constexpr uint16_t kOne = kHalf ? 0x3c00 : 0x3f80, k64 = kHalf ? 0x5400 : 0x4280, k4096 = kHalf ? 0x6c00 : 0x4580;
-    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char *sk = lds + wave * (2 * kBlockBytes), *sv = sk + kBlockBytes;
+    const int lane = threadIdx.x & 63, g = lane / X, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned char *sk = lds + wave * kOwnBytes, *sv = sk + 32 * kRowK;
 #pragma unroll 1
     for (int n = 0; n < w.missed * blocks; ++n) {
       const int32_t key0 = missed[wave * kMostMissed + n / blocks] + n % blocks * 32;
@@ -348,14 +399,11 @@ struct Paged {
       in.load();
       in.store(sk, sv);
       ordered();
-      f32x16 s;
+      float s[H::kScores];
+      scores<X>(w, sk, s);
+      vec8 pf[H::kSteps], sees[H::kSteps];   // weights, and 1 where the lane's row sees the key
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = E::mfma(*reinterpret_cast<const vec8*>(sk + k_off(l32, ks * 2 + half)), w.q[ks], s);
-      vec8 pf[2], sees[2];   // weights, and 1 where the lane's row sees the key
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < H::kSteps; ++t) {
         u32x4 p;
         u16x8 x;
 #pragma unroll
@@ -363,7 +411,7 @@ struct Paged {
           float by[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int32_t kk = key0 + t * 16 + ((i + j) >> 2) * 8 + half * 4 + ((i + j) & 3);
+            const int32_t kk = key0 + H::key_of(t * 8 + i + j, g);
             const bool there = kk >= w.lo && kk <= w.hi;
             by[j] = there ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t * 8 + i + j], scale, -w.m)) : 0.0f;
             x[i + j] = there ? kOne : 0;
@@ -373,36 +421,34 @@ struct Paged {
         pf[t] = __builtin_bit_cast(vec8, p), sees[t] = __builtin_bit_cast(vec8, x);
       }
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        f32x16 marks;   // of the keys that the row sees: 1 for each NaN, 64 for each infinity, 4096 for each negative one
+      for (int ob = 0; ob < D / H::kOuter; ++ob) {
+        typename H::Acc marks = {};   // of the keys that the row sees: 1 for each NaN, 64 for each infinity, 4096 for each negative one
 #pragma unroll
-        for (int e = 0; e < 16; ++e) marks[e] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          u16x8 f = __builtin_bit_cast(u16x8, v_frag(sv, t, db, lane)), mark;
+        for (int t = 0; t < H::kSteps; ++t) {
+          u16x8 f = __builtin_bit_cast(u16x8, v_frag<X>(sv, t, ob)), mark;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint16_t mag = f[i] & 0x7fff;
             mark[i] = mag > kInfinite ? kOne : mag < kInfinite ? (uint16_t)0 : f[i] >> 15 ? k4096 : k64;
             f[i] = mag < kInfinite ? f[i] : (uint16_t)0;
           }
-          w.o[db] = E::mfma(__builtin_bit_cast(vec8, f), pf[t], w.o[db]);
-          marks = E::mfma(__builtin_bit_cast(vec8, mark), sees[t], marks);
+          w.o[ob] = H::mfma(__builtin_bit_cast(vec8, f), pf[t], w.o[ob]);
+          marks = H::mfma(__builtin_bit_cast(vec8, mark), sees[t], marks);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int n = (int)marks[e];
-          w.o[db][e] += (n & 63 ? NAN : 0.0f) + (n & 4032 ? INFINITY : 0.0f) - (n >> 12 ? INFINITY : 0.0f);
+        for (int e = 0; e < (int)(sizeof(marks) / 4); ++e) {
+          const int of = (int)marks[e];
+          w.o[ob][e] += (of & 63 ? NAN : 0.0f) + (of & 4032 ? INFINITY : 0.0f) - (of >> 12 ? INFINITY : 0.0f);
         }
       }
       ordered();
     }
   }
 
-  // Up to 32 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ...
-  __device__ static __forceinline__ void own_keys(Rows& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* missed) {
+  // Up to 16 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ...
+  __device__ static __forceinline__ void own_keys(Rows<16>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* missed) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char *sk = lds + wave * (2 * kBlockBytes), *sv = sk + kBlockBytes;
+    unsigned char *sk = lds + wave * kOwnBytes, *sv = sk + 32 * kRowK;
     int32_t key = t.k0 + wave * 32;
     if (key >= t.k1) return;
     OwnLoader in(c, t, key, W * 32);
@@ -413,7 +459,7 @@ struct Paged {
     for (; key < t.k1; key += W * 32) {
       const bool more = key + W * 32 < t.k1;
       if (more) in.load();
-      keys<1>(w, sk, sv, key, scale, apart, missed + wave * kMostMissed);
+      keys<16, 1>(w, sk, sv, key, scale, apart, missed + wave * kMostMissed);
       ordered();
       if (more) apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv)) != 0;
       ordered();
@@ -422,9 +468,9 @@ struct Paged {
 
   // R x 32 rows: wavefront (r, s) has the rows of block r and the key blocks s * B .. of every step of S * B * 32 keys, which all wavefronts fetch together.
   template <int R, int B>
-  __device__ static __forceinline__ void shared_keys(Rows& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* apart_at, int32_t* missed) {
-    constexpr int S = W / R, N = S * B * 32, kTile = N * D * 2;
-    static_assert(4 * kTile <= kLdsBytes, "two stages");
+  __device__ static __forceinline__ void shared_keys(Rows<32>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* apart_at, int32_t* missed) {
+    constexpr int S = W / R, N = S * B * 32, kStage = N * (kRowK + kRowV);
+    static_assert(2 * kStage <= kLdsBytes, "two stages");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ws = wave % S;
     if (t.k0 >= t.k1) return;
     Loader<N, kThreads> in(c, t, threadIdx.x, t.k0, N);
@@ -432,17 +478,17 @@ struct Paged {
     if (threadIdx.x < 2) apart_at[threadIdx.x] = -1;
     __syncthreads();
     in.load();
-    if (in.store(lds, lds + kTile, threadIdx.x)) apart_at[0] = t.k0;
+    if (in.store(lds, lds + N * kRowK, threadIdx.x)) apart_at[0] = t.k0;
     __syncthreads();
     int cur = 0;
 #pragma unroll 1
     for (int32_t key = t.k0; key < t.k1; key += N) {
       const bool more = key + N < t.k1;
       if (more) in.load();
-      const unsigned char* sk = lds + cur * (2 * kTile) + ws * B * kBlockBytes;
-      keys<B>(w, sk, sk + kTile, key + ws * B * 32, scale, apart_at[cur] == key, missed + wave * kMostMissed);
+      const unsigned char* stage = lds + cur * kStage;
+      keys<32, B>(w, stage + ws * B * 32 * kRowK, stage + N * kRowK + ws * B * 32 * kRowV, key + ws * B * 32, scale, apart_at[cur] == key, missed + wave * kMostMissed);
       cur ^= 1;
-      if (more && in.store(lds + cur * (2 * kTile), lds + cur * (2 * kTile) + kTile, threadIdx.x)) apart_at[cur] = key + N;
+      if (more && in.store(lds + cur * kStage, lds + cur * kStage + N * kRowK, threadIdx.x)) apart_at[cur] = key + N;
       __syncthreads();
     }
   }
@@ -455,26 +501,28 @@ struct Paged {
     *reinterpret_cast<u32x2*>((T*)out.ptr + (int64_t)(t.first + token) * out.strides[0] + (int64_t)(t.head * p.group + head) * out.strides[1] + u * 4) = v;
   }
 
-  // The results of the wavefronts, S to 32 rows, and of the tile's other workgroups to out.
-  __device__ static __forceinline__ void finish(Rows& w, const Tile& t, const PartitionArg<3>& out, const PagedPlan& p, unsigned char* partials, int32_t slot_rows, unsigned char* lds,
+  // The results of the wavefronts, S to X rows, and of the tile's other workgroups to out.
+  template <int X>
+  __device__ static __forceinline__ void finish(Rows<X>& w, const Tile& t, const PartitionArg<3>& out, const PagedPlan& p, unsigned char* partials, int32_t slot_rows, unsigned char* lds,
                                                 float (*stat)[2][32], uint32_t* flag, int S) {
+    using H = Shape<T, D, X>;
     constexpr int U = D / 4, kRowsAtOnce = kThreads / U;
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const float l = sum_across_halves(w.l);
-    if (half == 0) stat[wave][0][l32] = w.m, stat[wave][1][l32] = l;
-    unsigned char* band = lds + wave * kBandBytes + l32 * (D * 4);
+    const int tid = threadIdx.x, lane = tid & 63, row_of = lane % X, g = lane / X, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float l = H::sum(w.l);
+    if (g == 0) stat[wave][0][row_of] = w.m, stat[wave][1][row_of] = l;
+    unsigned char* band = lds + wave * kOwnBytes + row_of * (D * 4);   // column unit u of a row lies at u ^ (row % 16)
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int ob = 0; ob < D / H::kOuter; ++ob)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(band + (((db * 8 + g * 2 + half) ^ (l32 & 15)) << 4)) = f32x4{w.o[db][g * 4], w.o[db][g * 4 + 1], w.o[db][g * 4 + 2], w.o[db][g * 4 + 3]};
+      for (int e = 0; e < (int)(sizeof(typename H::Acc) / 4); e += 4)
+        *reinterpret_cast<f32x4*>(band + (((ob * (H::kOuter / 4) + H::col_of(e, g) / 4) ^ (row_of & 15)) << 4)) = f32x4{w.o[ob][e], w.o[ob][e + 1], w.o[ob][e + 2], w.o[ob][e + 3]};
     __syncthreads();
     const uint32_t bytes = (uint32_t)slot_rows * (D + 2) * 4, stats = (uint32_t)slot_rows * D * 4;   // of a share of the workspace
     const __amdgpu_buffer_rsrc_t part = make_rsrc(partials, bytes * t.shares);
     const int u = tid % U;
 #pragma unroll 1
     for (int row = tid / U; row < t.rows; row += kRowsAtOnce) {
-      const int first = row / 32 * S, r = row % 32;
+      const int first = row / X * S, r = row % X;
       float top = -INFINITY;
       for (int s = 0; s < S; ++s) top = fmaxf(top, stat[first + s][0][r]);
       const float use = top == -INFINITY ? 0.0f : top;
@@ -483,7 +531,7 @@ struct Paged {
       for (int s = 0; s < S; ++s) {
         const float by = __builtin_amdgcn_exp2f(stat[first + s][0][r] - use);
         sum = __builtin_fmaf(stat[first + s][1][r], by, sum);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (first + s) * kBandBytes + r * (D * 4) + ((u ^ (r & 15)) << 4));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (first + s) * kOwnBytes + r * (D * 4) + ((u ^ (r & 15)) << 4));
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[e], by, o[e]);
       }
@@ -495,36 +543,53 @@ struct Paged {
       }
     }
     if (t.shares == 1 || !gemm::last_to_arrive(p.counters + t.slot, t.shares, flag)) return;
+    // The shares of few rows are dealt to several groups of threads, whose sums meet in LDS; a read past the L2 takes a microsecond, so eight are under way together.
+    const int rows_at_once = min(kRowsAtOnce, t.rows <= 1 ? 1 : 1 << (32 - __builtin_clz(t.rows - 1))), groups = kRowsAtOnce / rows_at_once, group = tid / U / rows_at_once;
+    const uint32_t each = (t.shares + groups - 1) / groups, k0 = group * each, k1 = min(k0 + each, t.shares);
+    f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+    float* const stats_at = reinterpret_cast<float*>(lds + kThreads * 16);
 #pragma unroll 1
-    for (int row = tid / U; row < t.rows; row += kRowsAtOnce) {
-      constexpr uint32_t kAtOnce = 4;   // shares whose reads are under way together
+    for (int base = 0; base < t.rows; base += rows_at_once) {
+      const int row = base + tid / U % rows_at_once;
+      constexpr uint32_t kAtOnce = 8;
       f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
       float m = -INFINITY, sum = 0.0f;
+      auto add = [&](const f32x4& x, float top_of, float sum_of) {   // in the order of the keys
+        const float top = fmaxf(m, top_of), use = top == -INFINITY ? 0.0f : top, was = __builtin_amdgcn_exp2f(m - use), by = __builtin_amdgcn_exp2f(top_of - use);
+        m = top, sum = __builtin_fmaf(sum_of, by, sum * was);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], by, o[e] * was);
+      };
+      if (row < t.rows) {
 #pragma unroll 1
-      for (uint32_t k = 0; k < t.shares; k += kAtOnce) {
-        u32x4 v[kAtOnce];
-        f32x2 st[kAtOnce];
+        for (uint32_t k = k0; k < k1; k += kAtOnce) {
+          u32x4 v[kAtOnce];
+          u32x2 st[kAtOnce];
 #pragma unroll
-        for (uint32_t i = 0; i < kAtOnce; ++i) {
-          const bool there = k + i < t.shares;
-          v[i] = __builtin_amdgcn_raw_buffer_load_b128(part, there ? (k + i) * bytes + (uint32_t)row * (D * 4) + u * 16 : kOob, 0, gemm::kAgentScope);
-          st[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(part, there ? (k + i) * bytes + stats + row * 8 : kOob, 0, gemm::kAgentScope));
-        }
-        float top = m;
+          for (uint32_t i = 0; i < kAtOnce; ++i) {
+            const bool there = k + i < k1;
+            v[i] = __builtin_amdgcn_raw_buffer_load_b128(part, there ? (k + i) * bytes + (uint32_t)row * (D * 4) + u * 16 : kOob, 0, gemm::kAgentScope);
+            st[i] = __builtin_amdgcn_raw_buffer_load_b64(part, there ? (k + i) * bytes + stats + row * 8 : kOob, 0, gemm::kAgentScope);
+          }
 #pragma unroll
-        for (uint32_t i = 0; i < kAtOnce; ++i) top = fmaxf(top, k + i < t.shares ? st[i][0] : -INFINITY);
-        const float use = top == -INFINITY ? 0.0f : top, was = __builtin_amdgcn_exp2f(m - use);
-        m = top, sum *= was, o *= was;
-#pragma unroll
-        for (uint32_t i = 0; i < kAtOnce; ++i) {
-          const float by = k + i < t.shares ? __builtin_amdgcn_exp2f(st[i][0] - use) : 0.0f;
-          const f32x4 x = __builtin_bit_cast(f32x4, v[i]);
-          sum = __builtin_fmaf(st[i][1], by, sum);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], by, o[e]);
+          for (uint32_t i = 0; i < kAtOnce; ++i) {
+            const f32x2 both = __builtin_bit_cast(f32x2, st[i]);
+            if (k + i < k1) add(__builtin_bit_cast(f32x4, v[i]), both[0], both[1]);
+          }
         }
       }
-      store_row(out, t, p, row, u, o, sum);
+      if (groups > 1) {
+        __syncthreads();
+        sums[tid] = o;
+        if (u == 0) stats_at[tid / U * 2] = m, stats_at[tid / U * 2 + 1] = sum;
+        __syncthreads();
+        if (group != 0) continue;
+        for (int g = 1; g < groups; ++g) {
+          const int at = tid / U + g * rows_at_once;
+          add(sums[at * U + u], stats_at[at * 2], stats_at[at * 2 + 1]);
+        }
+      }
+      if (row < t.rows) store_row(out, t, p, row, u, o, sum);
     }
   }
 
@@ -582,20 +647,27 @@ struct Paged {
     const uint64_t share_bytes = (uint64_t)slot_rows * (D + 2) * 4, long_bytes = p.long_shares > 1 ? (uint64_t)p.long_tiles * heads * p.long_shares * ((uint64_t)BM * (D + 2) * 4) : 0;
     unsigned char* partials = (unsigned char*)p.partials + (is_long ? (uint64_t)t.slot * p.long_shares * share_bytes
                                                                      : long_bytes + (uint64_t)(t.slot - (uint32_t)p.long_tiles * heads) * p.few_shares * share_bytes);
-    const int shared_by = t.rows <= 32 ? W : t.rows <= 64 ? W / 2 : W == 8 && t.rows <= 128 ? 2 : 1;   // wavefronts to the keys of 32 rows
-    int blocks = 1;
-    Rows w;
-    begin(w, t, q, p, wave / shared_by);
-    if (shared_by == W) {
+    if (t.rows <= 16) {
+      Rows<16> w;
+      begin(w, t, q, p, 0);
       own_keys(w, t, c, p.scale_log2e, lds, missed);
-    } else if (shared_by == W / 2) {
+      __syncthreads();   // everybody is done with the keys
+      add_missed(w, t, c, p.scale_log2e, lds, missed, 1);
+      finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, W);
+      return;
+    }
+    const int shared_by = t.rows <= 64 ? W / 2 : W == 8 && t.rows <= 128 ? 2 : 1;   // wavefronts to the keys of 32 rows
+    int blocks = 1;
+    Rows<32> w;
+    begin(w, t, q, p, wave / shared_by);
+    if (shared_by == W / 2) {
       shared_keys<2, 1>(w, t, c, p.scale_log2e, lds, apart_at, missed);
     } else if (W == 8 && shared_by == 2) {
-      shared_keys<4, kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+      shared_keys<W / 2, kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
       blocks = kStep;
     } else {
-      shared_keys<W, 2 * kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
-      blocks = 2 * kStep;
+      shared_keys<W, kWideStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+      blocks = kWideStep;
     }
     __syncthreads();   // everybody is done with the stages
     add_missed(w, t, c, p.scale_log2e, lds, missed, blocks);

@@ -3690,7 +3690,10 @@ cutile_status_t check_paged(const char* fn, const cutile_tensor_arg_t& rows, con
                      CUTILE_ERR_KERNEL_LAUNCH, "%s: scales must be f8e8m0fnu [%d, %d, %d, %d]", fn, k->shape[0], k->shape[1], k->shape[2], d / 32);
       bool forward = t.strides[3] == 1;
       for (int j = 0; j < 3; ++j) forward = forward && (t.shape[j] == 1 || t.strides[j] >= 0);
-      CUTILE_REQUIRE(forward && alike(*ks, t), CUTILE_ERR_KERNEL_NOT_FOUND, "%s: precompiled variants need k_scales and v_scales laid out alike, with a unit inner stride", fn);
+      bool aligned = (uintptr_t)t.ptr % (d / 32) == 0;   // a row's scales are read at once
+      for (int j = 0; j < 3; ++j) aligned = aligned && (t.shape[j] == 1 || t.strides[j] % (d / 32) == 0);
+      CUTILE_REQUIRE(forward && aligned && alike(*ks, t), CUTILE_ERR_KERNEL_NOT_FOUND,
+                     "%s: precompiled variants need k_scales and v_scales laid out alike, with a unit inner stride and rows on %d-byte boundaries", fn, d / 32);
     }
     c.ks = (const uint8_t*)ks->ptr, c.vs = (const uint8_t*)vs->ptr;
     c.s_page = ks->strides[0], c.s_row = ks->strides[1], c.s_head = ks->strides[2];
@@ -3732,7 +3735,6 @@ cutile_status_t check_covered(const char* fn, const cutile_partition_arg_t* cons
   return CUTILE_SUCCESS;
 }
 
-static const int kFewRounds = getenv("FEW_ROUNDS") ? atoi(getenv("FEW_ROUNDS")) : 1;
 // How keys are dealt out (see PagedPlan): `keys` to a workgroup so that `items` tiles of about `context` keys make about `wanted` workgroups, `step` keys at a time.
 struct Deal {
   int32_t keys = INT32_MAX, shares = 1;
@@ -3838,18 +3840,18 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
   p.q_and = qk_scale == 0.0f ? 0u : ~0u;
   p.q_xor = qk_scale < 0.0f ? 0x80008000u : 0u;
   p.window = window, p.group = group;
-  const bool any_long = most_new * group > 32;
+  const bool any_long = most_new * group > 32, few = most_new * group <= 16;
   p.few_rows = any_long && most_new * batch == tokens ? 0 : 32;   // all alike: no tiles of short sequences beside the others
   p.few_slot_rows = (int32_t)std::min<int64_t>(32, most_new * group);
   p.long_tiles = any_long ? (int32_t)((int64_t)tokens * group / bm + batch) : 0;
   auto plan = [&](bool may_share) {
-    const int64_t row_bytes = (d + 2) * 4, few_items = p.few_rows ? (int64_t)batch * heads : 0;
-    const int64_t long_slots = (int64_t)p.long_tiles * heads, long_items = any_long ? ((int64_t)tokens * group + bm - 1) / bm * heads : 0;
+    const int64_t row_bytes = (d + 4) * 4, few_items = p.few_rows ? (int64_t)batch * heads : 0, few_bytes = few_items * p.few_slot_rows * row_bytes;
+    const int64_t long_items = any_long ? ((int64_t)tokens * group + bm - 1) / bm * heads : 0, long_bytes = (int64_t)tokens * group * heads * row_bytes;
     Deal of_long, of_few;
-    if (may_share && long_slots + few_items <= (int64_t)kSplitCounters) {
-      if (long_items) of_long = deal_keys(long_items, context, cus, 256, std::max<int64_t>(1, room / (few_items ? 2 : 1) / (long_slots * bm * row_bytes)));
-      const int64_t left = room - (of_long.shares > 1 ? of_long.shares * long_slots * bm * row_bytes : 0);
-      if (few_items) of_few = deal_keys(few_items, context, cus * kFewRounds, 512, std::max<int64_t>(1, left / (few_items * p.few_slot_rows * row_bytes)));
+    if (may_share && (int64_t)p.long_tiles * heads + few_items <= (int64_t)kSplitCounters) {
+      if (few_items) of_few = deal_keys(few_items, context, cus, few ? 256 : 512, std::max<int64_t>(1, (any_long ? room / 4 : room) / few_bytes));
+      const int64_t left = room - (of_few.shares > 1 ? of_few.shares * few_bytes : 0), seen = window ? std::min<int64_t>(context, window + bm / group) : context;
+      if (long_items) of_long = deal_keys(long_items, seen, cus, 256, std::max<int64_t>(1, left / long_bytes));
     }
     p.long_shares = of_long.shares, p.long_keys = of_long.keys;
     p.few_shares = of_few.shares, p.few_keys = of_few.keys;
@@ -3860,6 +3862,8 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     ws = split_workspace(res.device, (hipStream_t)stream);
     if (!ws.partials) plan(false);
   }
+  if (few)
+    if (cutile_status_t s = use_member(&res, member_of(res.entry, "+few"))) return s;
   p.partials = ws.partials, p.counters = ws.counters;
   const uint64_t items = (uint64_t)p.long_tiles * p.long_shares + (p.few_rows ? (uint64_t)batch * p.few_shares : 0);
   CUTILE_REQUIRE(items * heads <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %llu tiles do not fit a launch grid axis", fn, (unsigned long long)(items * heads));

@@ -94,15 +94,16 @@ template <typename T, bool MX, int D, int W>
 struct Paged {
   using E = Elem<T>;
   using vec8 = typename E::vec8;
-  static constexpr int kThreads = W * 64, BM = W * 32;
+  static constexpr int kRows = D == 256 ? 16 : 32;                 // of a larger tile that a wavefront holds: 32 of D = 256 would not fit its registers
+  static constexpr int kThreads = W * 64, BM = W * kRows;
   static constexpr int DB = D / 32, KS = D / 16, kUnits = D / 8;   // 16-byte units of a 16-bit row
   // Rows of K and V in LDS are padded so that the lanes of a read meet different banks: 16 bytes for reads of a row a lane, 32 for the transposing ones of
   // four rows.  (Swizzled units, as in fmha.hip, take a register for every address; here they are one address and constants.)
   static constexpr int kRowK = D * 2 + 16, kRowV = D * 2 + 32;
   static constexpr int kOwnBytes = 32 * (kRowK + kRowV);           // 32 keys of a wavefront
-  static constexpr int kBandBytes = 32 * D * 4;                    // a wavefront's partial output
-  static constexpr int kLdsBytes = W * kOwnBytes;
-  static_assert(kBandBytes <= kOwnBytes, "the partial outputs lie where the keys were");
+  static constexpr int kOwners = D == 256 ? 4 : W;                 // wavefronts that can have keys of their own: what LDS holds
+  static constexpr int kLdsBytes = kOwners * kOwnBytes, kBandBytes = kLdsBytes / W;
+  static_assert(kBandBytes % 16 == 0 && kBandBytes >= kRows * D * 4 && W % kOwners == 0, "a wavefront's partial output lies where keys were");
   static constexpr int kMostMissed = 4;                            // steps that hold a border of what the 32 rows see: two at either end
   // Key blocks of a step: short rows leave a load for every thread, long ones the registers that the operands need.
   static constexpr int kStep = D == 64 ? 2 : 1, kWideStep = D == 64 ? 4 : D == 128 ? 2 : 1;
@@ -119,19 +120,18 @@ struct Paged {
     for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
   }
   // 16 bytes of K and of V of row r into LDS.
-  __device__ static __forceinline__ void put(u16x2& most, unsigned char* sk, unsigned char* sv, int r, int unit, const u32x4& k, const u32x4& v, uint32_t ks, uint32_t vs) {
+  __device__ static __forceinline__ void put(u16x2& most, unsigned char* sk, unsigned char* sv, int r, int unit, const u32x4& k, const u32x4& v, uint32_t ks, uint32_t vs, bool look = true) {
     if constexpr (MX) {
       u32x4 lo, hi;
       widen<T>(k, ks, lo, hi);
       *reinterpret_cast<u32x4*>(sk + k_off(r, unit * 2)) = lo;
       *reinterpret_cast<u32x4*>(sk + k_off(r, unit * 2 + 1)) = hi;
       widen<T>(v, vs, lo, hi);
-      most_of(most, lo);
-      most_of(most, hi);
+      if (look) most_of(most, lo), most_of(most, hi);
       *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2)) = lo;
       *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2 + 1)) = hi;
     } else {
-      most_of(most, v);
+      if (look) most_of(most, v);
       *reinterpret_cast<u32x4*>(sk + k_off(r, unit)) = k;
       *reinterpret_cast<u32x4*>(sv + v_off(r, unit)) = v;
     }
@@ -194,42 +194,45 @@ struct Paged {
     }
   };
 
-  // The same of 32 keys by one wavefront: lane r looks key r up (and lane r + 32), and the lanes that fetch its row get the place from there.
-  struct OwnLoader {
-    static constexpr int kLoads = 32 * kLoadUnits / 64, kRowsAtOnce = 64 / kLoadUnits;
+  // The same of 32 keys by one wavefront.  Lane r looks key r up, and the lanes that fetch its row have the place from there; of mxfp8 keys lane r holds the scales of K and lane
+  // 32 + r those of V.  (What counts is how often the first-level cache is asked: a load of 64 bytes of each of 16 rows, as the operands of K lie, or a scale byte for
+  // every lane cost as much as one of whole rows: 64 x 8192 mxfp8 189 us that way.)
+  struct OwnKeys {
+    static constexpr int kLoads = 32 * kLoadUnits / 64, kRowsAtOnce = 64 / kLoadUnits, kScaleWords = D == 256 ? 2 : 1;
+    typedef uint32_t Scales __attribute__((ext_vector_type(kScaleWords)));
     const PagedCache& c;
     const Tile& t;
-    int32_t key, page_at, row_at, entry, step;
+    const int lane, step;
+    int32_t key, page_at, row_at, entry;
     u32x4 k[kLoads], v[kLoads];
-    uint32_t ks[MX ? kLoads : 1], vs[MX ? kLoads : 1];
+    Scales scales;
 
-    __device__ __forceinline__ OwnLoader(const PagedCache& cache, const Tile& tile, int32_t start, int32_t by) : c(cache), t(tile), step(by) {
-      key = start + (threadIdx.x & 31);
+    __device__ __forceinline__ OwnKeys(const PagedCache& cache, const Tile& tile, int32_t start, int32_t by) : c(cache), t(tile), lane(threadIdx.x & 63), step(by) {
+      key = start + (lane & 31);
       page_at = key / c.page_size, row_at = key % c.page_size;
       ask();
     }
     __device__ __forceinline__ void ask() { entry = key < t.k1 ? t.pages[page_at] : -1; }
-    __device__ __forceinline__ static int64_t of_lane(int64_t v, int lane) {
-      const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)v), hi = __builtin_amdgcn_ds_bpermute(lane * 4, (int)(v >> 32));
-      return (int64_t)((uint64_t)hi << 32 | lo);
-    }
+    // `word` of lane `from`.
+    __device__ __forceinline__ static uint32_t of_lane(uint32_t word, int from) { return __builtin_amdgcn_ds_bpermute(from * 4, (int)word); }
+    // Asks for the next 32 keys, and for the page-table entries of those behind them.
     __device__ __forceinline__ void load() {
-      const int lane = threadIdx.x & 63, unit = lane % kLoadUnits;
+      const int unit = lane % kLoadUnits;
       const bool there = (uint32_t)entry < (uint32_t)c.pages;
-      const int64_t off = there ? (int64_t)entry * c.page_bytes + (int64_t)row_at * c.row_bytes : -1, s_off = (int64_t)entry * c.s_page + (int64_t)row_at * c.s_row;
+      const int64_t off = there ? (int64_t)entry * c.page_bytes + (int64_t)row_at * c.row_bytes : -1;
+      if constexpr (MX) {
+        const uint8_t* from = (lane < 32 ? c.ks : c.vs) + (int64_t)entry * c.s_page + (int64_t)row_at * c.s_row + (int64_t)t.head * c.s_head;
+        if (!there) from = (const uint8_t*)&paged_zeros;
+        if constexpr (D == 64) scales[0] = *(const uint16_t*)from;
+        else scales = *(const Scales*)from;
+      }
       const unsigned char *kb = (const unsigned char*)c.k + (int64_t)t.head * c.head_bytes + unit * 16, *vb = (const unsigned char*)c.v + (int64_t)t.head * c.head_bytes + unit * 16;
-      const uint8_t *ksb = c.ks + (int64_t)t.head * c.s_head + unit / 2, *vsb = c.vs + (int64_t)t.head * c.s_head + unit / 2;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int r = lane / kLoadUnits + i * kRowsAtOnce;
-        const int64_t at = of_lane(off, r);
-        k[i] = *(at >= 0 ? (const u32x4*)(kb + at) : &paged_zeros);
-        v[i] = *(at >= 0 ? (const u32x4*)(vb + at) : &paged_zeros);
-        if constexpr (MX) {
-          const int64_t s_at = of_lane(s_off, r);
-          ks[i] = *(at >= 0 ? ksb + s_at : (const uint8_t*)&paged_zeros);
-          vs[i] = *(at >= 0 ? vsb + s_at : (const uint8_t*)&paged_zeros);
-        }
+        const int64_t at = (int64_t)((uint64_t)of_lane((uint32_t)(off >> 32), r) << 32 | of_lane((uint32_t)off, r));
+        k[i] = __builtin_nontemporal_load(at >= 0 ? (const u32x4*)(kb + at) : &paged_zeros);
+        v[i] = __builtin_nontemporal_load(at >= 0 ? (const u32x4*)(vb + at) : &paged_zeros);
       }
       key += step;
       page_at += step / c.page_size;
@@ -237,12 +240,26 @@ struct Paged {
       if (row_at >= c.page_size) row_at -= c.page_size, ++page_at;
       ask();
     }
-    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv) {
-      const int lane = threadIdx.x & 63, unit = lane % kLoadUnits;
+    // The scale byte of block `block` of row r; `first`: lane of row 0.
+    __device__ __forceinline__ uint32_t scale_of(int first, int r, int block) const {
+      uint32_t word = of_lane(scales[0], first + r);
+      if constexpr (kScaleWords == 2) {
+        const uint32_t second = of_lane(scales[kScaleWords - 1], first + r);
+        word = block >= 4 ? second : word;
+      }
+      return word >> (block % 4 * 8) & 0xff;
+    }
+    // To LDS; `look`: whether a lane held a value of V that is no finite number.
+    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv, bool look) {
+      const int unit = lane % kLoadUnits;
       u16x2 most = {0, 0};
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) put(most, sk, sv, lane / kLoadUnits + i * kRowsAtOnce, unit, k[i], v[i], ks[MX ? i : 0], vs[MX ? i : 0]);
-      return most[0] >= kInfinite || most[1] >= kInfinite;
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = lane / kLoadUnits + i * kRowsAtOnce;
+        if constexpr (MX) put(most, sk, sv, r, unit, k[i], v[i], scale_of(0, r, unit / 2), scale_of(32, r, unit / 2), look);
+        else put(most, sk, sv, r, unit, k[i], v[i], 0, 0, look);
+      }
+      return look && (most[0] >= kInfinite || most[1] >= kInfinite);
     }
   };
 
@@ -282,11 +299,12 @@ struct Paged {
     for (auto& o : w.o) o = typename H::Acc{};
   }
 
-  // S^T of 32 keys.
+  // S^T of 32 keys in LDS.
   template <int X>
   __device__ static __forceinline__ void scores(const Rows<X>& w, const unsigned char* sk, float (&s)[Shape<T, D, X>::kScores]) {
     using H = Shape<T, D, X>;
     const int lane = threadIdx.x & 63;
+    constexpr int kEach = H::kScores * X / 32;
 #pragma unroll
     for (int i = 0; i < 32 / X; ++i) {
       typename H::Acc acc = {};
@@ -294,7 +312,7 @@ struct Paged {
       for (int ks = 0; ks < D / H::kInner; ++ks)
         acc = H::mfma(*reinterpret_cast<const vec8*>(sk + k_off(i * X + lane % X, ks * (H::kInner / 8) + lane / X)), w.q[ks], acc);
 #pragma unroll
-      for (int e = 0; e < H::kScores * X / 32; ++e) s[i * (H::kScores * X / 32) + e] = acc[e];
+      for (int e = 0; e < kEach; ++e) s[i * kEach + e] = acc[e];
     }
   }
 
@@ -308,17 +326,11 @@ struct Paged {
     return __builtin_bit_cast(vec8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
-  // B blocks of 32 keys from `key0` on, K and V at sk and sv: their products with the rows, and the softmax so far.  `apart`: V holds values that are no finite
-  // numbers.  They must not reach rows that do not see their keys, and 0 times them would: where some rows see a part of such keys the second product is
-  // left for later (add_missed).
-  template <int X, int B>
-  __device__ static __forceinline__ void keys(Rows<X>& w, const unsigned char* sk, const unsigned char* sv, int32_t key0, float c, bool apart, int32_t* missed) {
+  // The softmax of B blocks of 32 keys from `key0` on, whose S^T is s: weights, maximum and sum.  True where some rows see only a part of the keys.
+  template <int X, int B, typename S>
+  __device__ static __forceinline__ bool weights(Rows<X>& w, S (&s)[B], vec8 (&pf)[B][Shape<T, D, X>::kSteps], int32_t key0, float c) {
     using H = Shape<T, D, X>;
-    const int lane = threadIdx.x & 63, g = lane / X;
-    if (!w.used || key0 > w.any_hi || key0 + B * 32 - 1 < w.any_lo) return;
-    float s[B][H::kScores];   // s[b][e] belongs to key key0 + b * 32 + key_of(e, g) and to this lane's row
-#pragma unroll
-    for (int b = 0; b < B; ++b) scores<X>(w, sk + b * 32 * kRowK, s[b]);
+    const int g = (threadIdx.x & 63) / X;
     const bool masked = key0 + B * 32 - 1 > w.all_hi || key0 < w.all_lo;
     if (masked) {
       const int32_t hi = w.hi - key0 - g * 4, lo = w.lo - key0 - g * 4;
@@ -342,7 +354,6 @@ struct Paged {
     const float m_new = moved ? m_cand : w.m;
     const float m_use = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen so far: keep exp2 finite
     float rs = 0.0f;
-    vec8 pf[B][H::kSteps];
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
@@ -364,6 +375,19 @@ struct Paged {
       w.m = m_new;
     }
     w.l += rs;
+    return masked;
+  }
+
+  // B blocks of 32 keys from `key0` on, V at sv: `scores_of`(s) gives S^T, then the softmax so far and O^T.  `apart`: V holds values that are no finite
+  // numbers.  They must not reach rows that do not see their keys, and 0 times them would: where some rows see a part of such keys the second product is
+  // left for later (add_missed).
+  template <int X, int B, typename F>
+  __device__ static __forceinline__ void keys(Rows<X>& w, F&& scores_of, const unsigned char* sv, int32_t key0, float c, bool apart, int32_t* missed) {
+    using H = Shape<T, D, X>;
+    float s[B][H::kScores];   // s[b][e] belongs to key key0 + b * 32 + key_of(e, g) and to this lane's row
+    scores_of(s);
+    vec8 pf[B][H::kSteps];
+    const bool masked = weights<X, B>(w, s, pf, key0, c);
     if (masked && apart) {
       if (w.missed < kMostMissed) missed[w.missed++] = key0;
     } else {
@@ -384,23 +408,19 @@ struct Paged {
 
   // O^T += V^T P^T of the steps of `blocks` x 32 keys that keys() left out, m and l being those of all keys: what is no finite number is taken out of V, and what it makes
   // of the rows that see it found by a product of its own, of marks with 0 and 1.
-  template <int X>
-  __device__ static __forceinline__ void add_missed(Rows<X>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, const int32_t* missed, int blocks) {
+  // `fetch`(key, s): S^T of the 32 keys from there on, whose V then lies at sv.
+  template <int X, typename F>
+  __device__ static __forceinline__ void add_missed(Rows<X>& w, F&& fetch, const unsigned char* sv, float scale, const int32_t* missed, int blocks) {
     using H = Shape<T, D, X>;
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
     constexpr bool kHalf = std::is_same<T, _Float16>::value;
     constexpr uint16_t kOne = kHalf ? 0x3c00 : 0x3f80, k64 = kHalf ? 0x5400 : 0x4280, k4096 = kHalf ? 0x6c00 : 0x4580;
     const int lane = threadIdx.x & 63, g = lane / X, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char *sk = lds + wave * kOwnBytes, *sv = sk + 32 * kRowK;
 #pragma unroll 1
     for (int n = 0; n < w.missed * blocks; ++n) {
       const int32_t key0 = missed[wave * kMostMissed + n / blocks] + n % blocks * 32;
-      OwnLoader in(c, t, key0, 32);
-      in.load();
-      in.store(sk, sv);
-      ordered();
       float s[H::kScores];
-      scores<X>(w, sk, s);
+      fetch(key0, s);
       vec8 pf[H::kSteps], sees[H::kSteps];   // weights, and 1 where the lane's row sees the key
 #pragma unroll
       for (int t = 0; t < H::kSteps; ++t) {
@@ -445,30 +465,55 @@ struct Paged {
     }
   }
 
-  // Up to 16 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ...
-  __device__ static __forceinline__ void own_keys(Rows<16>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* missed) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char *sk = lds + wave * kOwnBytes, *sv = sk + 32 * kRowK;
-    int32_t key = t.k0 + wave * 32;
-    if (key >= t.k1) return;
-    OwnLoader in(c, t, key, W * 32);
-    in.load();
-    bool apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv)) != 0;
-    ordered();
+  // Of the keys at `key`: S^T, with V left at sv, for add_missed.
+  template <int X>
+  __device__ static __forceinline__ void fetch_missed(const Rows<X>& w, const Tile& t, const PagedCache& c, int32_t key, unsigned char* sk, unsigned char* sv,
+                                                      float (&s)[Shape<T, D, X>::kScores]) {
+    const int lane = threadIdx.x & 63, unit = lane % kLoadUnits;
+    u16x2 most;
 #pragma unroll 1
-    for (; key < t.k1; key += W * 32) {
-      const bool more = key + W * 32 < t.k1;
-      if (more) in.load();
-      keys<16, 1>(w, sk, sv, key, scale, apart, missed + wave * kMostMissed);
-      ordered();
-      if (more) apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv)) != 0;
-      ordered();
+    for (int r = lane / kLoadUnits; r < 32; r += 64 / kLoadUnits) {
+      const int32_t at = key + r, entry = at < t.k1 ? t.pages[at / c.page_size] : -1;
+      u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+      uint32_t ks = 0, vs = 0;
+      if ((uint32_t)entry < (uint32_t)c.pages) {
+        const int64_t off = (int64_t)entry * c.page_bytes + (int64_t)(at % c.page_size) * c.row_bytes + (int64_t)t.head * c.head_bytes + unit * 16;
+        k = *(const u32x4*)((const unsigned char*)c.k + off), v = *(const u32x4*)((const unsigned char*)c.v + off);
+        if constexpr (MX) {
+          const int64_t s = (int64_t)entry * c.s_page + (int64_t)(at % c.page_size) * c.s_row + (int64_t)t.head * c.s_head + unit / 2;
+          ks = c.ks[s], vs = c.vs[s];
+        }
+      }
+      put(most, sk, sv, r, unit, k, v, ks, vs, false);
     }
+    ordered();
+    scores<X>(w, sk, s);
   }
 
-  // R x 32 rows: wavefront (r, s) has the rows of block r and the key blocks s * B .. of every step of S * B * 32 keys, which all wavefronts fetch together.
-  template <int R, int B>
-  __device__ static __forceinline__ void shared_keys(Rows<32>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* apart_at, int32_t* missed) {
+  // Up to 16 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ..., 32 of them at a time in LDS at sk and sv.
+  __device__ static __forceinline__ void own_keys(Rows<16>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* sk, unsigned char* sv, int32_t* missed, bool several) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kBy = W * 32;
+    int32_t key0 = t.k0 + wave * 32;
+    if (key0 < t.k1) {
+      OwnKeys in(c, t, key0, kBy);
+      in.load();
+#pragma unroll 1
+      for (; key0 < t.k1; key0 += kBy) {
+        ordered();
+        const bool apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv, several)) != 0;
+        ordered();
+        in.load();
+        keys<16, 1>(w, [&](float (&s)[1][8]) { scores<16>(w, sk, s[0]); }, sv, key0, scale, apart, missed + wave * kMostMissed);
+      }
+    }
+    ordered();
+    add_missed(w, [&](int32_t key, float (&s)[8]) { fetch_missed<16>(w, t, c, key, sk, sv, s); }, sv, scale, missed, 1);
+  }
+
+  // R x X rows: wavefront (r, s) has the rows of block r and the key blocks s * B .. of every step of S * B * 32 keys, which all wavefronts fetch together.
+  template <int X, int R, int B>
+  __device__ static __forceinline__ void shared_keys(Rows<X>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* apart_at, int32_t* missed) {
     constexpr int S = W / R, N = S * B * 32, kStage = N * (kRowK + kRowV);
     static_assert(2 * kStage <= kLdsBytes, "two stages");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ws = wave % S;
@@ -486,7 +531,12 @@ struct Paged {
       const bool more = key + N < t.k1;
       if (more) in.load();
       const unsigned char* stage = lds + cur * kStage;
-      keys<32, B>(w, stage + ws * B * 32 * kRowK, stage + N * kRowK + ws * B * 32 * kRowV, key + ws * B * 32, scale, apart_at[cur] == key, missed + wave * kMostMissed);
+      const int32_t key0 = key + ws * B * 32;
+      if (w.used && key0 <= w.any_hi && key0 + B * 32 > w.any_lo)
+        keys<X, B>(w, [&](float (&s)[B][Shape<T, D, X>::kScores]) {
+#pragma unroll
+          for (int b = 0; b < B; ++b) scores<X>(w, stage + (ws * B + b) * 32 * kRowK, s[b]);
+        }, stage + N * kRowK + ws * B * 32 * kRowV, key0, scale, apart_at[cur] == key, missed + wave * kMostMissed);
       cur ^= 1;
       if (more && in.store(lds + cur * kStage, lds + cur * kStage + N * kRowK, threadIdx.x)) apart_at[cur] = key + N;
       __syncthreads();
@@ -510,14 +560,14 @@ struct Paged {
     const int tid = threadIdx.x, lane = tid & 63, row_of = lane % X, g = lane / X, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float l = H::sum(w.l);
     if (g == 0) stat[wave][0][row_of] = w.m, stat[wave][1][row_of] = l;
-    unsigned char* band = lds + wave * kOwnBytes + row_of * (D * 4);   // column unit u of a row lies at u ^ (row % 16)
+    unsigned char* band = lds + wave * kBandBytes + row_of * (D * 4);   // column unit u of a row lies at u ^ (row % 16)
 #pragma unroll
     for (int ob = 0; ob < D / H::kOuter; ++ob)
 #pragma unroll
       for (int e = 0; e < (int)(sizeof(typename H::Acc) / 4); e += 4)
         *reinterpret_cast<f32x4*>(band + (((ob * (H::kOuter / 4) + H::col_of(e, g) / 4) ^ (row_of & 15)) << 4)) = f32x4{w.o[ob][e], w.o[ob][e + 1], w.o[ob][e + 2], w.o[ob][e + 3]};
     __syncthreads();
-    const uint32_t bytes = (uint32_t)slot_rows * (D + 2) * 4, stats = (uint32_t)slot_rows * D * 4;   // of a share of the workspace
+    const uint32_t bytes = (uint32_t)slot_rows * (D + 4) * 4, stats = (uint32_t)slot_rows * D * 4;   // of a share of the workspace
     const __amdgpu_buffer_rsrc_t part = make_rsrc(partials, bytes * t.shares);
     const int u = tid % U;
 #pragma unroll 1
@@ -531,7 +581,7 @@ struct Paged {
       for (int s = 0; s < S; ++s) {
         const float by = __builtin_amdgcn_exp2f(stat[first + s][0][r] - use);
         sum = __builtin_fmaf(stat[first + s][1][r], by, sum);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (first + s) * kOwnBytes + r * (D * 4) + ((u ^ (r & 15)) << 4));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (first + s) * kBandBytes + r * (D * 4) + ((u ^ (r & 15)) << 4));
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[e], by, o[e]);
       }
@@ -593,6 +643,8 @@ struct Paged {
     }
   }
 
+  // FEW: tiles of up to 16 rows are all there is.
+  template <bool FEW>
   __device__ static __forceinline__ void run(const TensorArg<3>& q, const PartitionArg<3>& out, const PagedCache& c, const PagedPlan& p) {
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
     __shared__ float stat[W][2][32];
@@ -600,8 +652,12 @@ struct Paged {
     __shared__ int32_t apart_at[2], missed[W * kMostMissed];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t heads = (uint32_t)c.heads, of_long = (uint32_t)p.long_tiles * p.long_shares;
-    const uint32_t head = blockIdx.x % heads, item = blockIdx.x / heads;
-    const bool is_long = item < of_long;
+    uint32_t head = blockIdx.x % heads, item = blockIdx.x / heads;
+    if (FEW && MX && gridDim.x / heads % 8 == 0) {   // the heads of one part of a sequence on one XCD, one after another: their scales, and rows of D = 64, share lines
+      const uint32_t slot = blockIdx.x / 8;
+      head = slot % heads, item = slot / heads * 8 + blockIdx.x % 8;
+    }
+    const bool is_long = !FEW && item < of_long;
     Tile t;
     t.head = (int32_t)head;
     int32_t b;
@@ -628,7 +684,7 @@ struct Paged {
       s = paged::sequence(c, b);
       t.row0 = 0;
       t.rows = s.count * p.group;
-      if (t.rows == 0 || t.rows > p.few_rows) return;
+      if (t.rows == 0 || t.rows > (FEW ? 16 : p.few_rows)) return;
       most = p.few_shares, keys_each = p.few_keys;
       t.slot = ((uint32_t)p.long_tiles + b) * heads + head;
     }
@@ -637,51 +693,65 @@ struct Paged {
     t.pages = c.table + (int64_t)b * c.table_row;
     const int32_t first = t.pos0 + t.row0 / p.group, last = t.pos0 + (t.row0 + t.rows - 1) / p.group;
     const int32_t lo = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, hi = max(min(last + 1, s.held), lo);
-    t.shares = min(max((uint32_t)(hi - lo + keys_each - 1) / keys_each, 1u), most);
+    // as many shares as it takes, as even as steps of all wavefronts allow
+    const int32_t span = hi - lo, step = FEW || t.rows <= 16 ? kOwners * 32 : 64, wanted = (int32_t)min(((uint32_t)span + keys_each - 1) / keys_each, most);
+    const int32_t each = max((span + wanted - 1) / max(wanted, 1) + step - 1, step) / step * step;
+    t.shares = max((span + each - 1) / each, 1);
     if (t.share >= t.shares) return;
-    t.k0 = lo + (int32_t)(t.share * keys_each);
-    t.k1 = t.share + 1 == t.shares ? hi : t.k0 + (int32_t)keys_each;
+    t.k0 = lo + (int32_t)t.share * each;
+    t.k1 = min(hi, t.k0 + each);
 
-    // long tiles' partial results first, [tile][head][share]
-    const int32_t slot_rows = is_long ? BM : p.few_slot_rows;
-    const uint64_t share_bytes = (uint64_t)slot_rows * (D + 2) * 4, long_bytes = p.long_shares > 1 ? (uint64_t)p.long_tiles * heads * p.long_shares * ((uint64_t)BM * (D + 2) * 4) : 0;
-    unsigned char* partials = (unsigned char*)p.partials + (is_long ? (uint64_t)t.slot * p.long_shares * share_bytes
-                                                                     : long_bytes + (uint64_t)(t.slot - (uint32_t)p.long_tiles * heads) * p.few_shares * share_bytes);
-    if (t.rows <= 16) {
+    // Partial results: rows of the large tiles first, [head][row of all][share], then the others, [sequence][head][share].
+    const int32_t slot_rows = is_long ? t.rows : p.few_slot_rows;
+    constexpr uint64_t kRowBytes = (D + 4) * 4;
+    const uint64_t all_rows = (uint64_t)c.tokens * p.group, of_shares = p.long_shares > 1 ? p.long_shares : 0;
+    unsigned char* partials = (unsigned char*)p.partials + (is_long ? ((uint64_t)head * all_rows + (uint64_t)t.first * p.group + t.row0) * of_shares * kRowBytes
+                                                                     : heads * all_rows * of_shares * kRowBytes + (uint64_t)(t.slot - (uint32_t)p.long_tiles * heads) * p.few_shares * slot_rows * kRowBytes);
+    unsigned char *const sk = lds + wave % kOwners * kOwnBytes, *const sv = sk + 32 * kRowK;   // of 32 keys of the wavefront's own
+    if (FEW || (D != 256 && t.rows <= 16)) {   // (rows of 256 values on their way take more registers than 8 wavefronts have)
       Rows<16> w;
       begin(w, t, q, p, 0);
-      own_keys(w, t, c, p.scale_log2e, lds, missed);
-      __syncthreads();   // everybody is done with the keys
-      add_missed(w, t, c, p.scale_log2e, lds, missed, 1);
+      own_keys(w, t, c, p.scale_log2e, sk, sv, missed, t.rows > p.group);
+      ordered();   // (a wavefront's results lie where its keys were)
       finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, W);
       return;
     }
-    const int shared_by = t.rows <= 64 ? W / 2 : W == 8 && t.rows <= 128 ? 2 : 1;   // wavefronts to the keys of 32 rows
-    int blocks = 1;
-    Rows<32> w;
-    begin(w, t, q, p, wave / shared_by);
-    if (shared_by == W / 2) {
-      shared_keys<2, 1>(w, t, c, p.scale_log2e, lds, apart_at, missed);
-    } else if (W == 8 && shared_by == 2) {
-      shared_keys<W / 2, kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
-      blocks = kStep;
-    } else {
-      shared_keys<W, kWideStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
-      blocks = kWideStep;
+    if constexpr (!FEW) {
+      constexpr int kMostShared = W * kRows / 64;
+      const int shared_by = t.rows <= 64 ? kMostShared : t.rows <= BM / 2 ? 2 : 1;   // wavefronts to the keys of kRows rows
+      int blocks = 1;
+      Rows<kRows> w;
+      begin(w, t, q, p, wave / shared_by);
+      if (shared_by == 1) {
+        shared_keys<kRows, W, kWideStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+        blocks = kWideStep;
+      } else if (kMostShared > 2 && shared_by > 2) {
+        shared_keys<kRows, W / kMostShared, 1>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+      } else {
+        shared_keys<kRows, W / 2, kStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+        blocks = kStep;
+      }
+      __syncthreads();   // everybody is done with the stages
+#pragma unroll 1
+      for (int i = 0; i < W / kOwners; ++i) {
+        if (wave / kOwners == i) add_missed(w, [&](int32_t key, float (&s)[Shape<T, D, kRows>::kScores]) { fetch_missed<kRows>(w, t, c, key, sk, sv, s); }, sv, p.scale_log2e, missed, blocks);
+        if (kOwners < W) __syncthreads();
+      }
+      finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, shared_by);
     }
-    __syncthreads();   // everybody is done with the stages
-    add_missed(w, t, c, p.scale_log2e, lds, missed, blocks);
-    finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, shared_by);
   }
 };
 
 }  // namespace
 
-#define ATTENTION(NAME, T, MX, D, W)                                                                                                                                        \
-  extern "C" __global__ void __launch_bounds__(W * 64) paged_attention_entry__##NAME##_d##D(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) { \
-    Paged<T, MX, D, W>::run(q, out, c, p);                                                                                                                                  \
+#define ATTENTION(NAME, T, MX, D, W)                                                                                                                                          \
+  extern "C" __global__ void __launch_bounds__(W * 64) paged_attention_entry__##NAME##_d##D(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) {     \
+    Paged<T, MX, D, W>::template run<false>(q, out, c, p);                                                                                                                    \
+  }                                                                                                                                                                           \
+  extern "C" __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) paged_attention_entry__##NAME##_d##D##_few(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) { \
+    Paged<T, MX, D, 4>::template run<true>(q, out, c, p);                                                                                                                     \
   }
-#define ATTENTION_D(NAME, T, MX) ATTENTION(NAME, T, MX, 64, 8) ATTENTION(NAME, T, MX, 128, 8) ATTENTION(NAME, T, MX, 256, 4)
+#define ATTENTION_D(NAME, T, MX) ATTENTION(NAME, T, MX, 64, 8) ATTENTION(NAME, T, MX, 128, 8) ATTENTION(NAME, T, MX, 256, 8)
 ATTENTION_D(f16, _Float16, false)
 ATTENTION_D(bf16, __bf16, false)
 ATTENTION_D(f16_mxfp8, _Float16, true)

@@ -534,9 +534,9 @@ std::vector<KernelEntry> build_table() {
       }
   // ---- logits in front of the choice of a token (512 threads; tile = (-, columns of a workgroup, -, -)) ----
   for (const char* dt : {"f16", "bf16", "f32"})
-    for (int c : {16384, 4096, 1024}) {
+    for (int c : {8192, 4096, 1024}) {
       const std::string v = std::string(dt) + "_" + std::to_string(c);
-      add("adjust_logits", keep(v), keep("adjust_logits_entry__" + v), IMG_LOGITS, 512, (uint32_t)c * 4 + 1024 * 8 + 4, 0, c, 0, 0, dt, 0, 2);
+      add("adjust_logits", keep(v), keep("adjust_logits_entry__" + v), IMG_LOGITS, 512, (uint32_t)c * 4 + 1024 * 6 + 4, 0, c, 0, 0, dt, 0, 2);
     }
   return t;
 }

@@ -3904,7 +3904,7 @@ cutile_status_t cutile_launch_adjust_logits(cutile_stream_t stream, const cutile
     int64_t ids_row, values_row;
     const void* allowed;
     int64_t allowed_row;
-    int32_t vocab, most, biases, blocks, vectors, pad;
+    int32_t vocab, most, biases, blocks, rows, pad;
   } a{};
   const struct {
     const cutile_tensor_arg_t* t;
@@ -3946,7 +3946,7 @@ cutile_status_t cutile_launch_adjust_logits(cutile_stream_t stream, const cutile
   for (const KernelEntry* e : kernels_of(fn))
     if (strcmp(e->dtype, cutile_dtype_name(logits->dtype)) == 0) {
       fitting.push_back(e->variant);
-      if (sized.empty() && (int64_t)rows * div_up(vocab, e->tile[1]) >= 2 * cus) sized = e->variant;   // the widest that fills the chip
+      if (sized.empty() && (int64_t)rows * div_up(vocab, e->tile[1]) >= (int64_t)cus * e->tile[1] / 4096) sized = e->variant;   // wide ones where two or more workgroups to a CU are left (adjust_logits.hip has the times)
     }
   if (sized.empty()) sized = fitting[fitting.size() - 1];
   Resolved res;
@@ -3954,12 +3954,12 @@ cutile_status_t cutile_launch_adjust_logits(cutile_stream_t stream, const cutile
   a.in = logits->ptr, a.out = ot.ptr;
   a.in_row = row_stride(*logits), a.out_row = row_stride(ot);
   a.vocab = vocab, a.blocks = (int32_t)div_up(vocab, res.entry->tile[1]);
-  const int64_t per16 = 16 / (int64_t)cutile_dtype_size(logits->dtype);
-  a.vectors = aligned16(a.in) && aligned16(a.out) && a.in_row % per16 == 0 && a.out_row % per16 == 0;
+  a.rows = rows;
   ArgPacker args;
   args.push_val<LogitsArgs>(a);
-  CUTILE_REQUIRE((uint64_t)rows * a.blocks <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %d rows of %d do not fit a launch grid axis", fn, rows, vocab);
-  const uint32_t grid[3] = {(uint32_t)rows * a.blocks, 1, 1};
+  const uint64_t dealt = rows >= 64 ? (uint64_t)div_up(rows, 8) * 8 : (uint64_t)rows;   // many rows: whole sets of eight, one for each XCD
+  CUTILE_REQUIRE(dealt * a.blocks <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %d rows of %d do not fit a launch grid axis", fn, rows, vocab);
+  const uint32_t grid[3] = {(uint32_t)(dealt * a.blocks), 1, 1};
   return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
 

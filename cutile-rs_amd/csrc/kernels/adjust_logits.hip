@@ -4,7 +4,9 @@
 //   l <- l + sum of the token's biases;   not allowed: l <- -infinity;   all in f32, rounded once
 // A workgroup takes C columns of a row: it counts the row's tokens that fall on them in LDS (integers, so their order is nothing to the result) while its
 // logits are on the way, then reads the counts beside them.  HBM bounds many rows (every logit once in, once out), the two dependent loads (length, tokens)
-// one row.  C trades the two: every workgroup of a row reads all of its tokens, from L2 behind the first.
+// one row.  Every workgroup of a row reads all of its tokens, so wide ones read less and narrow ones are more: 256 rows of 128256 bf16 logits behind 6000
+// tokens take 34 us (4.1 TB/s) with C = 8192, 45 with 4096, 108 with 1024; 16 rows 6.8, 6.2 and 9.8; one row 6.4, 5.5 and 5.3.  16384 columns leave a CU two
+// workgroups, whose loads do not cover their counting: 43 us.  With the workgroups of a row on all XCDs its tokens come from HBM eight times: 65 us that way.
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"
@@ -13,7 +15,7 @@ using namespace cutile;
 
 namespace {
 
-constexpr int kThreads = 512, kMostBiases = 1024;
+constexpr int kThreads = 512, kMostBiases = 1024, kRowsByXcd = 64;
 constexpr uint32_t kPrompt = 0x80000000u, kBiased = 0x40000000u;   // beside the count of generated tokens
 
 struct LogitsArgs {
@@ -29,22 +31,27 @@ struct LogitsArgs {
   const uint32_t* allowed;                           // bit t % 32 of word t / 32
   int64_t allowed_row;
   int32_t vocab, most, biases, blocks;               // blocks: workgroups of a row
-  int32_t vectors;                                   // rows start on 16-byte boundaries
-  int32_t pad;
+  int32_t rows, pad;
 };
 
 template <typename T, int C>
 __device__ __forceinline__ void adjust(const LogitsArgs& a) {
-  constexpr int kUnits = C / 8 / kThreads > 0 ? C / 8 / kThreads : 1, kBytes = 8 * sizeof(T);
+  constexpr int kUnits = C / 8 / kThreads > 0 ? C / 8 / kThreads : 1;
   __shared__ __attribute__((aligned(16))) uint32_t words[C];
-  __shared__ int32_t ids[kMostBiases];
+  __shared__ uint16_t ids[kMostBiases];   // columns: four workgroups of the widest fit a CU
   __shared__ float values[kMostBiases];
   __shared__ int32_t biases;
-  struct __attribute__((aligned(16))) Unit {
+  struct Unit {   // (loads and stores of 16 bytes need no more than the alignment of their elements: rows of odd lengths are no different)
     T v[8];
   };
   const int tid = threadIdx.x;
-  const int32_t row = blockIdx.x / a.blocks, col0 = blockIdx.x % a.blocks * C, cols = min(C, a.vocab - col0);
+  int32_t row = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
+  if (a.rows >= kRowsByXcd) {   // a row's workgroups on one XCD: its tokens are fetched into one L2
+    const int32_t slot = blockIdx.x / 8;
+    row = slot / a.blocks * 8 + blockIdx.x % 8, block = slot % a.blocks;
+    if (row >= a.rows) return;
+  }
+  const int32_t col0 = block * C, cols = min(C, a.vocab - col0);
   const T* in = (const T*)a.in + (int64_t)row * a.in_row + col0;
   T* out = (T*)a.out + (int64_t)row * a.out_row + col0;
 
@@ -52,9 +59,8 @@ __device__ __forceinline__ void adjust(const LogitsArgs& a) {
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
     const int c = (tid + i * kThreads) * 8;
-    if (a.vectors && c + 8 <= cols) {
-#pragma unroll
-      for (int b = 0; b < kBytes / 16; ++b) reinterpret_cast<uint4*>(held[i].v)[b] = reinterpret_cast<const uint4*>(in + c)[b];
+    if (c + 8 <= cols) {
+      held[i] = *reinterpret_cast<const Unit*>(in + c);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) held[i].v[e] = c + e < cols ? in[c + e] : (T)0.0f;
@@ -76,7 +82,7 @@ __device__ __forceinline__ void adjust(const LogitsArgs& a) {
       const uint64_t mask = __builtin_amdgcn_ballot_w64(here);
       if (here) {
         const int32_t at = found + __builtin_popcountll(mask & ((1ull << tid) - 1));
-        ids[at] = c, values[at] = a.bias_values[(int64_t)row * a.values_row + i + tid];
+        ids[at] = (uint16_t)c, values[at] = a.bias_values[(int64_t)row * a.values_row + i + tid];
         atomicOr(&words[c], kBiased);
       }
       found += __builtin_popcountll(mask);
@@ -84,14 +90,28 @@ __device__ __forceinline__ void adjust(const LogitsArgs& a) {
     if (tid == 0) biases = found;
   }
   const int32_t* tokens = a.tokens + (int64_t)row * a.tokens_row;
-#pragma unroll 4
-  for (int32_t i = tid; i < n; i += kThreads) {
-    const int32_t t = tokens[i], c = t - col0;
-    if (t >= col0 && c < cols) {
+  auto count = [&](int32_t i, int32_t t) {
+    const uint32_t c = (uint32_t)t - (uint32_t)col0;
+    if (c < (uint32_t)cols) {
       if (i < prompt) atomicOr(&words[c], kPrompt);
       else atomicAdd(&words[c], 1u);
     }
+  };
+  struct Four {
+    int32_t t[4];
+  };
+  constexpr int kAhead = 4, kStep = kThreads * 4;   // loads under way together
+#pragma unroll 1
+  for (int32_t i = tid * 4; i < (n & ~3); i += kAhead * kStep) {
+    Four four[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) four[k] = i + k * kStep < (n & ~3) ? *reinterpret_cast<const Four*>(tokens + i + k * kStep) : Four{{-1, -1, -1, -1}};
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) count(i + k * kStep + e, four[k].t[e]);
   }
+  if (tid < (n & 3)) count((n & ~3) + tid, tokens[(n & ~3) + tid]);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
@@ -119,9 +139,8 @@ __device__ __forceinline__ void adjust(const LogitsArgs& a) {
       }
       u.v[e] = allowed >> e & 1 ? (T)l : (T)-INFINITY;
     }
-    if (a.vectors && c + 8 <= cols) {
-#pragma unroll
-      for (int b = 0; b < kBytes / 16; ++b) reinterpret_cast<uint4*>(out + c)[b] = reinterpret_cast<const uint4*>(u.v)[b];
+    if (c + 8 <= cols) {
+      *reinterpret_cast<Unit*>(out + c) = u;
     } else {
       for (int e = 0; e < 8 && c + e < cols; ++e) out[c + e] = u.v[e];
     }
@@ -132,7 +151,7 @@ __device__ __forceinline__ void adjust(const LogitsArgs& a) {
 
 #define LOGITS(TYPE, T, C) \
   extern "C" __global__ void __launch_bounds__(kThreads) adjust_logits_entry__##TYPE##_##C(LogitsArgs a) { adjust<T, C>(a); }
-#define LOGITS_C(TYPE, T) LOGITS(TYPE, T, 1024) LOGITS(TYPE, T, 4096) LOGITS(TYPE, T, 16384)
+#define LOGITS_C(TYPE, T) LOGITS(TYPE, T, 1024) LOGITS(TYPE, T, 4096) LOGITS(TYPE, T, 8192)
 LOGITS_C(f16, _Float16)
 LOGITS_C(bf16, __bf16)
 LOGITS_C(f32, float)

@@ -127,7 +127,7 @@ def test_gpu_adjusted(ct, dev, dtype, rows, vocab, history, biases, mask):
     launch(ct, on, out)
     want, size = plain(**x)
     check(out.cpu(), want, size, biases)
-    for v in (1024, 4096, 16384):
+    for v in (1024, 4096, 8192):
         other = torch.full_like(out, 7.0)
         launch(ct, on, other, variant=f"{dtype}_{v}")
         assert torch.equal(other, out)

@@ -85,6 +85,9 @@ struct Tile {
   int32_t first;           // row of q and out of the sequence's first token
   int32_t pos0;            // position of that token
   int32_t k0, k1;          // keys [k0, k1)
+  int32_t all_lo, all_hi;  // keys that all of its rows see, of those that there are
+  // Some rows see only a part of keys [key, key + n).
+  __device__ __forceinline__ bool partly(int32_t key, int32_t n) const { return key + n - 1 > all_hi || key < all_lo; }
   uint32_t share, shares;
   uint32_t slot;           // of the workspace's counters
   const int32_t* pages;    // the sequence's pages
@@ -104,7 +107,7 @@ struct Paged {
   static constexpr int kOwners = D == 256 ? 4 : W;                 // wavefronts that can have keys of their own: what LDS holds
   static constexpr int kLdsBytes = kOwners * kOwnBytes, kBandBytes = kLdsBytes / W;
   static_assert(kBandBytes % 16 == 0 && kBandBytes >= kRows * D * 4 && W % kOwners == 0, "a wavefront's partial output lies where keys were");
-  static constexpr int kMostMissed = 4;                            // steps that hold a border of what the 32 rows see: two at either end
+  static constexpr int kMostMissed = 2 * (BM / 32 + 2);            // steps that hold a border of what the rows see, at either end
   // Key blocks of a step: short rows leave a load for every thread, long ones the registers that the operands need.
   static constexpr int kStep = D == 64 ? 2 : 1, kWideStep = D == 64 ? 4 : D == 128 ? 2 : 1;
   static constexpr int kLoadUnits = D * (MX ? 1 : 2) / 16;         // 16-byte loads of a row of the cache
@@ -112,29 +115,36 @@ struct Paged {
   __device__ static __forceinline__ int k_off(int r, int u) { return r * kRowK + u * 16; }
   __device__ static __forceinline__ int v_off(int r, int u) { return r * kRowV + u * 16; }
 
-  // The largest magnitudes so far of 16-bit values in the halves of a dword, as integers: NaN and infinities are on top.
+  // Takes values that are no finite numbers out of 16-bit ones; true if there were some.
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   static constexpr uint16_t kInfinite = std::is_same<T, _Float16>::value ? 0x7c00 : 0x7f80;
-  __device__ static __forceinline__ void most_of(u16x2& most, const u32x4& v) {
+  __device__ static __forceinline__ bool clean(u32x4& v) {
+    uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bad = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu) >= kInfinite);
+      v[i] &= ~bad, any |= bad;
+    }
+    return any != 0;
   }
-  // 16 bytes of K and of V of row r into LDS.
-  __device__ static __forceinline__ void put(u16x2& most, unsigned char* sk, unsigned char* sv, int r, int unit, const u32x4& k, const u32x4& v, uint32_t ks, uint32_t vs, bool look = true) {
+  // 16 bytes of K and of V of row r into LDS.  `look`: values of V that are no finite numbers stay out (keys()); true if there were some.
+  __device__ static __forceinline__ bool put(unsigned char* sk, unsigned char* sv, int r, int unit, const u32x4& k, u32x4 v, uint32_t ks, uint32_t vs, bool look) {
+    bool found = false;
     if constexpr (MX) {
       u32x4 lo, hi;
       widen<T>(k, ks, lo, hi);
       *reinterpret_cast<u32x4*>(sk + k_off(r, unit * 2)) = lo;
       *reinterpret_cast<u32x4*>(sk + k_off(r, unit * 2 + 1)) = hi;
       widen<T>(v, vs, lo, hi);
-      if (look) most_of(most, lo), most_of(most, hi);
+      if (look) found = clean(lo), found |= clean(hi);
       *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2)) = lo;
       *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2 + 1)) = hi;
     } else {
-      if (look) most_of(most, v);
+      if (look) found = clean(v);
       *reinterpret_cast<u32x4*>(sk + k_off(r, unit)) = k;
       *reinterpret_cast<u32x4*>(sv + v_off(r, unit)) = v;
     }
+    return found;
   }
 
   // The cache rows of N keys on their way to LDS, by THREADS threads: key r of a step is key `at + r`.
@@ -185,12 +195,12 @@ struct Paged {
       }
       ask();
     }
-    // True in a lane that held a value of V that is no finite number.
-    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv, int tid) {
-      u16x2 most = {0, 0};
+    // True in a lane that kept a value of V back.
+    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv, int tid, bool look) {
+      bool found = false;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) put(most, sk, sv, tid / kLoadUnits + i * kRowsApart, unit, k[i], v[i], ks[MX ? i : 0], vs[MX ? i : 0]);
-      return most[0] >= kInfinite || most[1] >= kInfinite;
+      for (int i = 0; i < kLoads; ++i) found |= put(sk, sv, tid / kLoadUnits + i * kRowsApart, unit, k[i], v[i], ks[MX ? i : 0], vs[MX ? i : 0], look);
+      return found;
     }
   };
 
@@ -249,17 +259,16 @@ struct Paged {
       }
       return word >> (block % 4 * 8) & 0xff;
     }
-    // To LDS; `look`: whether a lane held a value of V that is no finite number.
     __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv, bool look) {
       const int unit = lane % kLoadUnits;
-      u16x2 most = {0, 0};
+      bool found = false;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int r = lane / kLoadUnits + i * kRowsAtOnce;
-        if constexpr (MX) put(most, sk, sv, r, unit, k[i], v[i], scale_of(0, r, unit / 2), scale_of(32, r, unit / 2), look);
-        else put(most, sk, sv, r, unit, k[i], v[i], 0, 0, look);
+        if constexpr (MX) found |= put(sk, sv, r, unit, k[i], v[i], scale_of(0, r, unit / 2), scale_of(32, r, unit / 2), look);
+        else found |= put(sk, sv, r, unit, k[i], v[i], 0, 0, look);
       }
-      return look && (most[0] >= kInfinite || most[1] >= kInfinite);
+      return found;
     }
   };
 
@@ -274,7 +283,7 @@ struct Paged {
     int32_t all_lo, all_hi;   // that every row of the wavefront sees
     int32_t any_lo, any_hi;   // that one of them sees
     bool used;
-    int missed;               // steps whose second product is still to be done
+    int missed;               // steps of whose V values were kept back
   };
 
   template <int X>
@@ -326,13 +335,12 @@ struct Paged {
     return __builtin_bit_cast(vec8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
-  // The softmax of B blocks of 32 keys from `key0` on, whose S^T is s: weights, maximum and sum.  True where some rows see only a part of the keys.
+  // The softmax of B blocks of 32 keys from `key0` on, whose S^T is s: weights, maximum and sum.
   template <int X, int B, typename S>
-  __device__ static __forceinline__ bool weights(Rows<X>& w, S (&s)[B], vec8 (&pf)[B][Shape<T, D, X>::kSteps], int32_t key0, float c) {
+  __device__ static __forceinline__ void weights(Rows<X>& w, S (&s)[B], vec8 (&pf)[B][Shape<T, D, X>::kSteps], int32_t key0, float c) {
     using H = Shape<T, D, X>;
     const int g = (threadIdx.x & 63) / X;
-    const bool masked = key0 + B * 32 - 1 > w.all_hi || key0 < w.all_lo;
-    if (masked) {
+    if (key0 + B * 32 - 1 > w.all_hi || key0 < w.all_lo) {
       const int32_t hi = w.hi - key0 - g * 4, lo = w.lo - key0 - g * 4;
 #pragma unroll
       for (int b = 0; b < B; ++b)
@@ -375,29 +383,25 @@ struct Paged {
       w.m = m_new;
     }
     w.l += rs;
-    return masked;
   }
 
-  // B blocks of 32 keys from `key0` on, V at sv: `scores_of`(s) gives S^T, then the softmax so far and O^T.  `apart`: V holds values that are no finite
-  // numbers.  They must not reach rows that do not see their keys, and 0 times them would: where some rows see a part of such keys the second product is
-  // left for later (add_missed).
+  // B blocks of 32 keys from `key0` on, V at sv: `scores_of`(s) gives S^T, then the softmax so far and O^T.  Values of V that are no finite numbers must not reach
+  // rows that do not see their keys, and 0 times them would: of keys that only some rows of the tile see they are kept out of LDS (`apart`), and come to the rows
+  // that see them later (add_missed).
   template <int X, int B, typename F>
   __device__ static __forceinline__ void keys(Rows<X>& w, F&& scores_of, const unsigned char* sv, int32_t key0, float c, bool apart, int32_t* missed) {
     using H = Shape<T, D, X>;
     float s[B][H::kScores];   // s[b][e] belongs to key key0 + b * 32 + key_of(e, g) and to this lane's row
     scores_of(s);
     vec8 pf[B][H::kSteps];
-    const bool masked = weights<X, B>(w, s, pf, key0, c);
-    if (masked && apart) {
-      if (w.missed < kMostMissed) missed[w.missed++] = key0;
-    } else {
+    weights<X, B>(w, s, pf, key0, c);
 #pragma unroll
-      for (int b = 0; b < B; ++b)
+    for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int t = 0; t < H::kSteps; ++t)
+      for (int t = 0; t < H::kSteps; ++t)
 #pragma unroll
-          for (int ob = 0; ob < D / H::kOuter; ++ob) w.o[ob] = H::mfma(v_frag<X>(sv + b * 32 * kRowV, t, ob), pf[b][t], w.o[ob]);
-    }
+        for (int ob = 0; ob < D / H::kOuter; ++ob) w.o[ob] = H::mfma(v_frag<X>(sv + b * 32 * kRowV, t, ob), pf[b][t], w.o[ob]);
+    if (apart && w.missed < kMostMissed) missed[w.missed++] = key0;
   }
 
   // LDS operations of one wavefront happen in order; the compiler is kept to it.
@@ -406,53 +410,60 @@ struct Paged {
     __builtin_amdgcn_wave_barrier();
   }
 
-  // O^T += V^T P^T of the steps of `blocks` x 32 keys that keys() left out, m and l being those of all keys: what is no finite number is taken out of V, and what it makes
-  // of the rows that see it found by a product of its own, of marks with 0 and 1.
-  // `fetch`(key, s): S^T of the 32 keys from there on, whose V then lies at sv.
-  template <int X, typename F>
-  __device__ static __forceinline__ void add_missed(Rows<X>& w, F&& fetch, const unsigned char* sv, float scale, const int32_t* missed, int blocks) {
+  // What the values that were kept back in the noted steps of `blocks` x 32 keys make of the rows that see their keys, found by a product of marks with 0 and 1.
+  // The steps' V goes through LDS at sv.
+  template <int X>
+  __device__ static __forceinline__ void add_missed(Rows<X>& w, const Tile& t, const PagedCache& c, unsigned char* sv, const int32_t* missed, int blocks) {
     using H = Shape<T, D, X>;
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
     constexpr bool kHalf = std::is_same<T, _Float16>::value;
     constexpr uint16_t kOne = kHalf ? 0x3c00 : 0x3f80, k64 = kHalf ? 0x5400 : 0x4280, k4096 = kHalf ? 0x6c00 : 0x4580;
-    const int lane = threadIdx.x & 63, g = lane / X, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, g = lane / X, unit = lane % kLoadUnits;
 #pragma unroll 1
     for (int n = 0; n < w.missed * blocks; ++n) {
-      const int32_t key0 = missed[wave * kMostMissed + n / blocks] + n % blocks * 32;
-      float s[H::kScores];
-      fetch(key0, s);
-      vec8 pf[H::kSteps], sees[H::kSteps];   // weights, and 1 where the lane's row sees the key
+      const int32_t key0 = missed[n / blocks] + n % blocks * 32;
+#pragma unroll 1
+      for (int r = lane / kLoadUnits; r < 32; r += 64 / kLoadUnits) {
+        const int32_t at = key0 + r, entry = at < t.k1 ? t.pages[at / c.page_size] : -1;
+        u32x4 v = {0, 0, 0, 0};
+        uint32_t vs = 0;
+        if ((uint32_t)entry < (uint32_t)c.pages) {
+          v = *(const u32x4*)((const unsigned char*)c.v + (int64_t)entry * c.page_bytes + (int64_t)(at % c.page_size) * c.row_bytes + (int64_t)t.head * c.head_bytes + unit * 16);
+          if constexpr (MX) vs = c.vs[(int64_t)entry * c.s_page + (int64_t)(at % c.page_size) * c.s_row + (int64_t)t.head * c.s_head + unit / 2];
+        }
+        if constexpr (MX) {
+          u32x4 lo, hi;
+          widen<T>(v, vs, lo, hi);
+          *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2)) = lo;
+          *reinterpret_cast<u32x4*>(sv + v_off(r, unit * 2 + 1)) = hi;
+        } else {
+          *reinterpret_cast<u32x4*>(sv + v_off(r, unit)) = v;
+        }
+      }
+      ordered();
+      vec8 sees[H::kSteps];   // 1 where the lane's row sees the key
 #pragma unroll
       for (int t = 0; t < H::kSteps; ++t) {
-        u32x4 p;
         u16x8 x;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          float by[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int32_t kk = key0 + H::key_of(t * 8 + i + j, g);
-            const bool there = kk >= w.lo && kk <= w.hi;
-            by[j] = there ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[t * 8 + i + j], scale, -w.m)) : 0.0f;
-            x[i + j] = there ? kOne : 0;
-          }
-          p[i / 2] = E::pack2(by[0], by[1]);
+        for (int i = 0; i < 8; ++i) {
+          const int32_t kk = key0 + H::key_of(t * 8 + i, g);
+          x[i] = kk >= w.lo && kk <= w.hi ? kOne : 0;
         }
-        pf[t] = __builtin_bit_cast(vec8, p), sees[t] = __builtin_bit_cast(vec8, x);
+        sees[t] = __builtin_bit_cast(vec8, x);
       }
 #pragma unroll
       for (int ob = 0; ob < D / H::kOuter; ++ob) {
         typename H::Acc marks = {};   // of the keys that the row sees: 1 for each NaN, 64 for each infinity, 4096 for each negative one
 #pragma unroll
         for (int t = 0; t < H::kSteps; ++t) {
-          u16x8 f = __builtin_bit_cast(u16x8, v_frag<X>(sv, t, ob)), mark;
+          const u16x8 f = __builtin_bit_cast(u16x8, v_frag<X>(sv, t, ob));
+          u16x8 mark;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint16_t mag = f[i] & 0x7fff;
             mark[i] = mag > kInfinite ? kOne : mag < kInfinite ? (uint16_t)0 : f[i] >> 15 ? k4096 : k64;
-            f[i] = mag < kInfinite ? f[i] : (uint16_t)0;
           }
-          w.o[ob] = H::mfma(__builtin_bit_cast(vec8, f), pf[t], w.o[ob]);
           marks = H::mfma(__builtin_bit_cast(vec8, mark), sees[t], marks);
         }
 #pragma unroll
@@ -465,33 +476,8 @@ struct Paged {
     }
   }
 
-  // Of the keys at `key`: S^T, with V left at sv, for add_missed.
-  template <int X>
-  __device__ static __forceinline__ void fetch_missed(const Rows<X>& w, const Tile& t, const PagedCache& c, int32_t key, unsigned char* sk, unsigned char* sv,
-                                                      float (&s)[Shape<T, D, X>::kScores]) {
-    const int lane = threadIdx.x & 63, unit = lane % kLoadUnits;
-    u16x2 most;
-#pragma unroll 1
-    for (int r = lane / kLoadUnits; r < 32; r += 64 / kLoadUnits) {
-      const int32_t at = key + r, entry = at < t.k1 ? t.pages[at / c.page_size] : -1;
-      u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-      uint32_t ks = 0, vs = 0;
-      if ((uint32_t)entry < (uint32_t)c.pages) {
-        const int64_t off = (int64_t)entry * c.page_bytes + (int64_t)(at % c.page_size) * c.row_bytes + (int64_t)t.head * c.head_bytes + unit * 16;
-        k = *(const u32x4*)((const unsigned char*)c.k + off), v = *(const u32x4*)((const unsigned char*)c.v + off);
-        if constexpr (MX) {
-          const int64_t s = (int64_t)entry * c.s_page + (int64_t)(at % c.page_size) * c.s_row + (int64_t)t.head * c.s_head + unit / 2;
-          ks = c.ks[s], vs = c.vs[s];
-        }
-      }
-      put(most, sk, sv, r, unit, k, v, ks, vs, false);
-    }
-    ordered();
-    scores<X>(w, sk, s);
-  }
-
   // Up to 16 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ..., 32 of them at a time in LDS at sk and sv.
-  __device__ static __forceinline__ void own_keys(Rows<16>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* sk, unsigned char* sv, int32_t* missed, bool several) {
+  __device__ static __forceinline__ void own_keys(Rows<16>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* sk, unsigned char* sv, int32_t* missed) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int kBy = W * 32;
     int32_t key0 = t.k0 + wave * 32;
@@ -501,14 +487,14 @@ struct Paged {
 #pragma unroll 1
       for (; key0 < t.k1; key0 += kBy) {
         ordered();
-        const bool apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv, several)) != 0;
+        const bool apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv, t.partly(key0, 32))) != 0;
         ordered();
         in.load();
-        keys<16, 1>(w, [&](float (&s)[1][8]) { scores<16>(w, sk, s[0]); }, sv, key0, scale, apart, missed + wave * kMostMissed);
+        keys<16, 1>(w, [&](float (&s)[1][8]) { scores<16>(w, sk, s[0]); }, sv, key0, scale, apart, missed);
       }
     }
     ordered();
-    add_missed(w, [&](int32_t key, float (&s)[8]) { fetch_missed<16>(w, t, c, key, sk, sv, s); }, sv, scale, missed, 1);
+    add_missed(w, t, c, sv, missed, 1);
   }
 
   // R x X rows: wavefront (r, s) has the rows of block r and the key blocks s * B .. of every step of S * B * 32 keys, which all wavefronts fetch together.
@@ -519,11 +505,11 @@ struct Paged {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ws = wave % S;
     if (t.k0 >= t.k1) return;
     Loader<N, kThreads> in(c, t, threadIdx.x, t.k0, N);
-    // the step whose V, in that stage, holds a value that is no finite number: known to all behind the barrier
+    // the step whose V in that stage had values kept back: known to all behind the barrier
     if (threadIdx.x < 2) apart_at[threadIdx.x] = -1;
     __syncthreads();
     in.load();
-    if (in.store(lds, lds + N * kRowK, threadIdx.x)) apart_at[0] = t.k0;
+    if (in.store(lds, lds + N * kRowK, threadIdx.x, t.partly(t.k0, N))) apart_at[0] = t.k0;
     __syncthreads();
     int cur = 0;
 #pragma unroll 1
@@ -536,9 +522,9 @@ struct Paged {
         keys<X, B>(w, [&](float (&s)[B][Shape<T, D, X>::kScores]) {
 #pragma unroll
           for (int b = 0; b < B; ++b) scores<X>(w, stage + (ws * B + b) * 32 * kRowK, s[b]);
-        }, stage + N * kRowK + ws * B * 32 * kRowV, key0, scale, apart_at[cur] == key, missed + wave * kMostMissed);
+        }, stage + N * kRowK + ws * B * 32 * kRowV, key0, scale, __builtin_amdgcn_readfirstlane(apart_at[cur]) == key, missed);
       cur ^= 1;
-      if (more && in.store(lds + cur * kStage, lds + cur * kStage + N * kRowK, threadIdx.x)) apart_at[cur] = key + N;
+      if (more && in.store(lds + cur * kStage, lds + cur * kStage + N * kRowK, threadIdx.x, t.partly(key + N, N))) apart_at[cur] = key + N;
       __syncthreads();
     }
   }
@@ -649,7 +635,7 @@ struct Paged {
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
     __shared__ float stat[W][2][32];
     __shared__ uint32_t flag;
-    __shared__ int32_t apart_at[2], missed[W * kMostMissed];
+    __shared__ int32_t apart_at[2], all_missed[W * kMostMissed];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t heads = (uint32_t)c.heads, of_long = (uint32_t)p.long_tiles * p.long_shares;
     uint32_t head = blockIdx.x % heads, item = blockIdx.x / heads;
@@ -692,6 +678,7 @@ struct Paged {
     t.pos0 = s.position(0);
     t.pages = c.table + (int64_t)b * c.table_row;
     const int32_t first = t.pos0 + t.row0 / p.group, last = t.pos0 + (t.row0 + t.rows - 1) / p.group;
+    t.all_lo = p.window > 0 && last >= p.window ? last - p.window + 1 : 0, t.all_hi = first;
     const int32_t lo = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, hi = max(min(last + 1, s.held), lo);
     // as many shares as it takes, as even as steps of all wavefronts allow
     const int32_t span = hi - lo, step = FEW || t.rows <= 16 ? kOwners * 32 : 64, wanted = (int32_t)min(((uint32_t)span + keys_each - 1) / keys_each, most);
@@ -707,11 +694,12 @@ struct Paged {
     const uint64_t all_rows = (uint64_t)c.tokens * p.group, of_shares = p.long_shares > 1 ? p.long_shares : 0;
     unsigned char* partials = (unsigned char*)p.partials + (is_long ? ((uint64_t)head * all_rows + (uint64_t)t.first * p.group + t.row0) * of_shares * kRowBytes
                                                                      : heads * all_rows * of_shares * kRowBytes + (uint64_t)(t.slot - (uint32_t)p.long_tiles * heads) * p.few_shares * slot_rows * kRowBytes);
+    int32_t* const missed = all_missed + wave * kMostMissed;
     unsigned char *const sk = lds + wave % kOwners * kOwnBytes, *const sv = sk + 32 * kRowK;   // of 32 keys of the wavefront's own
     if (FEW || (D != 256 && t.rows <= 16)) {   // (rows of 256 values on their way take more registers than 8 wavefronts have)
       Rows<16> w;
       begin(w, t, q, p, 0);
-      own_keys(w, t, c, p.scale_log2e, sk, sv, missed, t.rows > p.group);
+      own_keys(w, t, c, p.scale_log2e, sk, sv, missed);
       ordered();   // (a wavefront's results lie where its keys were)
       finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, W);
       return;
@@ -734,7 +722,7 @@ struct Paged {
       __syncthreads();   // everybody is done with the stages
 #pragma unroll 1
       for (int i = 0; i < W / kOwners; ++i) {
-        if (wave / kOwners == i) add_missed(w, [&](int32_t key, float (&s)[Shape<T, D, kRows>::kScores]) { fetch_missed<kRows>(w, t, c, key, sk, sv, s); }, sv, p.scale_log2e, missed, blocks);
+        if (wave / kOwners == i) add_missed(w, t, c, sv, missed, blocks);
         if (kOwners < W) __syncthreads();
       }
       finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, shared_by);

@@ -3,13 +3,16 @@
 // p the position of token i; no key: zeros.
 //
 // The rows of a tile are pairs (token, query head of one KV head), token by token: group heads share every key that is read, and a decode step of 8 heads or a
-// chunk of 4 tokens fill the columns of a matrix instruction.  Products, masks and softmax are those of fmha_common.h / fmha.hip: S^T = K Q^T and
-// O^T = V^T P^T, so that a lane owns one row.
+// chunk of 4 tokens fill the columns of a matrix instruction.  S^T = K Q^T and O^T = V^T P^T, so that a lane owns one row and what it holds of P^T is its operand
+// of the second product; the softmax keeps a running reference point and sum of each row, in 32 bits.
 //  * Tiles of up to 16 rows (decode, speculation): every wavefront has keys of its own, 32 at a time, through registers into LDS that no other
-//    wavefront reads: no barrier in the loop.  HBM's rate bounds it.
-//  * Larger tiles: R wavefronts side by side hold 32 rows each, S = wavefronts / R share the keys of a step; the matrix cores and exponentials bound it.
+//    wavefront reads: no barrier in the loop.  HBM's rate bounds it: 1 x 131072 tokens, 8 KV heads, bf16, 91 us (5.9 TB/s).  A launch that has no other tiles runs
+//    a kernel of four wavefronts (two workgroups on a CU), others have eight.
+//  * Larger tiles: R wavefronts side by side hold kRows rows each, W / R share the keys of a step, which all of them fetch together.  Tiles of all W hold their next
+//    scores while the exponentials of the last are made (pipelined_keys).  A prompt of 8192 tokens, 32 heads over 8, D = 128, bf16: 570 us, 960 TFLOP/s of what the
+//    rows see; the loop alone in the order scores, softmax, product 596, and with a branch around the product, which copied O, 669.
 // At the end the partial outputs go through LDS, and where the keys of a tile are dealt to several workgroups through the launch's workspace: the one that
-// arrives last adds them up in the order of the keys.
+// arrives last adds them up in the order of the keys, so that the order of arrival is nothing to the result.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -44,6 +47,15 @@ __device__ __forceinline__ void widen(const u32x4& raw, uint32_t scale_byte, u32
     u32x4& to = i < 2 ? lo : hi;
     to[i * 2 % 4] = a, to[i * 2 % 4 + 1] = b;
   }
+}
+
+// sum + both 16-bit values of `pair`.
+template <typename T>
+__device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (std::is_same<T, _Float16>::value) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{1, 1}, sum, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{1.0f, 1.0f}, sum, false);
 }
 
 // How a wavefront holds X rows (32 or 16) of a tile: S^T and O^T have a row to a column of the matrix instruction, X columns wide, so that lane l has row l % X and, of
@@ -294,6 +306,8 @@ struct Paged {
     w.used = n > 0;
     const int32_t r = t.row0 + r0 + min(lane % X, max(n, 1) - 1), token = r / p.group, head = r % p.group;   // (lanes beyond the last row repeat it)
     const T* from = (const T*)q.ptr + (int64_t)(t.first + token) * q.strides[0] + (int64_t)(t.head * p.group + head) * q.strides[1];
+#pragma unroll
+    for (auto& part : w.q) part = vec8{};
     if (w.used) {
 #pragma unroll
       for (int ks = 0; ks < D / H::kInner; ++ks) w.q[ks] = __builtin_bit_cast(vec8, (*reinterpret_cast<const u32x4*>(from + ks * H::kInner + lane / X * 8) & p.q_and) ^ p.q_xor);
@@ -335,55 +349,95 @@ struct Paged {
     return __builtin_bit_cast(vec8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
-  // The softmax of B blocks of 32 keys from `key0` on, whose S^T is s: weights, maximum and sum.
+  // The softmax of B blocks of 32 keys, in steps.  What the lane's row does not see of S^T, from `key0` on:
   template <int X, int B, typename S>
-  __device__ static __forceinline__ void weights(Rows<X>& w, S (&s)[B], vec8 (&pf)[B][Shape<T, D, X>::kSteps], int32_t key0, float c) {
+  __device__ static __forceinline__ void hide(const Rows<X>& w, S (&s)[B], int32_t key0) {
     using H = Shape<T, D, X>;
+    if (key0 + B * 32 - 1 <= w.all_hi && key0 >= w.all_lo) return;
     const int g = (threadIdx.x & 63) / X;
-    if (key0 + B * 32 - 1 > w.all_hi || key0 < w.all_lo) {
-      const int32_t hi = w.hi - key0 - g * 4, lo = w.lo - key0 - g * 4;
+    const int32_t hi = w.hi - key0 - g * 4, lo = w.lo - key0 - g * 4;
 #pragma unroll
-      for (int b = 0; b < B; ++b)
+    for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int e = 0; e < H::kScores; ++e) {
-          const int kk = b * 32 + H::key_of(e, 0);
-          s[b][e] = kk <= hi && kk >= lo ? s[b][e] : -INFINITY;
-        }
-    }
+      for (int e = 0; e < H::kScores; ++e) {
+        const int kk = b * 32 + H::key_of(e, 0);
+        s[b][e] = kk <= hi && kk >= lo ? s[b][e] : -INFINITY;
+      }
+  }
+  template <int X, int B, typename S>
+  __device__ static __forceinline__ float highest(S (&s)[B]) {
     float mx = -INFINITY;
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
-      for (int e = 0; e < H::kScores; ++e) mx = fmaxf(mx, s[b][e]);
-    mx = H::most(mx);
-    constexpr float kSlack = 8.0f;   // the reference point only has to bound the exponents: it moves when a row's maximum has risen by more
-    const float m_cand = fmaxf(w.m, mx * c);
-    const bool moved = __builtin_amdgcn_ballot_w64(m_cand > w.m + kSlack) != 0;
-    const float m_new = moved ? m_cand : w.m;
-    const float m_use = m_new == -INFINITY ? 0.0f : m_new;   // nothing seen so far: keep exp2 finite
-    float rs = 0.0f;
-#pragma unroll
-    for (int b = 0; b < B; ++b)
-#pragma unroll
-      for (int t = 0; t < H::kSteps; ++t) {   // P in 16 bits, as V is: the weights' rounding stays below that of V
-        u32x4 v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][t * 8 + 2 * i], c, -m_use)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][t * 8 + 2 * i + 1], c, -m_use));
-          rs += p0, rs += p1;
-          v[i] = E::pack2(p0, p1);
-        }
-        pf[b][t] = __builtin_bit_cast(vec8, v);
-      }
-    if (moved) {
-      const float alpha = __builtin_amdgcn_exp2f(w.m - m_use);
-      w.l *= alpha;
-#pragma unroll
-      for (auto& o : w.o) o *= alpha;
-      w.m = m_new;
-    }
-    w.l += rs;
+      for (int e = 0; e < Shape<T, D, X>::kScores; ++e) mx = fmaxf(mx, s[b][e]);
+    return mx;
   }
+  // The row's reference point, `mx` being the lane's highest new score.  It only has to bound the exponents: it moves when a row's maximum has risen by more than kSlack.
+  template <int X>
+  __device__ static __forceinline__ void move(Rows<X>& w, float mx, float c) {
+    constexpr float kSlack = 8.0f;
+    const float to = fmaxf(w.m, Shape<T, D, X>::most(mx) * c);
+    if (__builtin_amdgcn_ballot_w64(to > w.m + kSlack) == 0) return;
+    const float alpha = __builtin_amdgcn_exp2f(w.m - (to == -INFINITY ? 0.0f : to));
+    w.l *= alpha;
+#pragma unroll
+    for (auto& o : w.o) o *= alpha;
+    w.m = to;
+  }
+  // Keeps the compiler from moving the making of x behind this place.
+  template <typename U>
+  __device__ static __forceinline__ void here(U& x) {
+    asm volatile("" : "+v"(x));
+  }
+  // P in 16 bits, as V is: the weights' rounding stays below that of V, and their sum is that of the rounded ones.  All at once, or a part at a time (m of `of`).
+  template <int X, int B>
+  struct Exponentials {
+    using H = Shape<T, D, X>;
+    static constexpr int kPairs = B * H::kScores / 2;
+    Rows<X>& w;
+    float (&s)[B][H::kScores];
+    vec8 (&pf)[B][H::kSteps];
+    const float c, m;
+    float sum[2];
+    u32x4 p[B][H::kSteps];
+    __device__ __forceinline__ Exponentials(Rows<X>& rows, float (&scores)[B][H::kScores], vec8 (&weights)[B][H::kSteps], float scale)
+        : w(rows), s(scores), pf(weights), c(scale), m(rows.m == -INFINITY ? 0.0f : rows.m) {   // (nothing seen so far: keep exp2 finite)
+      sum[0] = w.l, sum[1] = 0.0f;
+    }
+    __device__ __forceinline__ void raise(int i) {
+      float& x = s[i / H::kScores][i % H::kScores];
+      x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -m));
+    }
+    __device__ __forceinline__ void pack(int i) {
+      const int b = i / (H::kScores / 2), r = i % (H::kScores / 2);
+      const uint32_t v = E::pack2(s[b][2 * r], s[b][2 * r + 1]);
+      p[b][r / 4][r % 4] = v;
+      sum[i % 2] = add_pair<T>(v, sum[i % 2]);
+    }
+    __device__ __forceinline__ void operator()(int part, int of) {
+#pragma unroll
+      for (int i = part * kPairs / of; i < (part + 1) * kPairs / of; ++i) raise(2 * i), raise(2 * i + 1);
+#pragma unroll
+      for (int i = part ? (part - 1) * kPairs / of : 0; i < part * kPairs / of; ++i) pack(i);
+      if (part == of - 1) {
+#pragma unroll
+        for (int i = part * kPairs / of; i < kPairs; ++i) pack(i);
+      }
+      if (of > 1) {
+#pragma unroll
+        for (int i = 2 * (part * kPairs / of); i < 2 * ((part + 1) * kPairs / of); ++i) here(s[i / H::kScores][i % H::kScores]);
+        here(sum[0]), here(sum[1]);
+      }
+    }
+    __device__ __forceinline__ void end() {
+      w.l = sum[0] + sum[1];
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int t = 0; t < H::kSteps; ++t) pf[b][t] = __builtin_bit_cast(vec8, p[b][t]);
+    }
+  };
 
   // B blocks of 32 keys from `key0` on, V at sv: `scores_of`(s) gives S^T, then the softmax so far and O^T.  Values of V that are no finite numbers must not reach
   // rows that do not see their keys, and 0 times them would: of keys that only some rows of the tile see they are kept out of LDS (`apart`), and come to the rows
@@ -394,7 +448,11 @@ struct Paged {
     float s[B][H::kScores];   // s[b][e] belongs to key key0 + b * 32 + key_of(e, g) and to this lane's row
     scores_of(s);
     vec8 pf[B][H::kSteps];
-    weights<X, B>(w, s, pf, key0, c);
+    hide<X, B>(w, s, key0);
+    move<X>(w, highest<X, B>(s), c);
+    Exponentials<X, B> weights(w, s, pf, c);
+    weights(0, 1);
+    weights.end();
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
@@ -526,6 +584,167 @@ struct Paged {
       cur ^= 1;
       if (more && in.store(lds + cur * kStage, lds + cur * kStage + N * kRowK, threadIdx.x, t.partly(key + N, N))) apart_at[cur] = key + N;
       __syncthreads();
+    }
+  }
+
+  // K of step g and V of step g - 1 on their way to LDS, by all wavefronts: what pipelined_keys takes together.  A load of a wavefront is a group of kGroup whole rows;
+  // where a group never crosses the end of a page (grouped()) its place is a scalar address, and the vector ALU has nothing to do with it.
+  template <int N>
+  struct GroupLoader {
+    static constexpr int kGroup = 64 / kLoadUnits, kLoads = N / (W * kGroup);
+    static_assert(64 % kLoadUnits == 0 && N % (W * kGroup) == 0, "whole groups, equal shares");
+    typedef const int32_t __attribute__((address_space(4))) * Entries;
+    const PagedCache& c;
+    const Tile& t;
+    const int row, unit, wave;       // the lane's row of a group, its 16 bytes of it
+    const uint32_t at, s_at;         // its place in the group
+    int32_t key[kLoads], page_at[kLoads], row_at[kLoads], entry[kLoads];   // of the groups to be asked for next
+    int64_t off[kLoads], s_off[kLoads];                     // of the groups asked for last, or -1
+    u32x4 k[kLoads], v[kLoads];
+    uint32_t ks[MX ? kLoads : 1], vs[MX ? kLoads : 1];
+
+    __device__ static __forceinline__ bool grouped(const PagedCache& c, const Tile& t) { return c.page_size % kGroup == 0 && t.k0 % kGroup == 0; }
+    __device__ __forceinline__ GroupLoader(const PagedCache& cache, const Tile& tile)
+        : c(cache), t(tile), row((threadIdx.x & 63) / kLoadUnits), unit(threadIdx.x % kLoadUnits), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+          at((uint32_t)(row * c.row_bytes) + unit * 16), s_at((uint32_t)(row * c.s_row) + unit / 2) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        key[i] = t.k0 + (wave + i * W) * kGroup;
+        page_at[i] = key[i] / c.page_size, row_at[i] = key[i] % c.page_size;
+        off[i] = -1, s_off[i] = 0;
+      }
+      ask();
+    }
+    __device__ __forceinline__ void ask() {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) entry[i] = key[i] < t.k1 ? ((Entries)t.pages)[page_at[i]] : -1;
+    }
+    __device__ __forceinline__ void load() {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        v[i] = u32x4{0, 0, 0, 0}, k[i] = u32x4{0, 0, 0, 0};
+        if constexpr (MX) vs[i] = 0, ks[i] = 0;
+        if (off[i] >= 0) {
+          v[i] = *(const u32x4*)((const unsigned char*)c.v + off[i] + at);
+          if constexpr (MX) vs[i] = *(c.vs + s_off[i] + s_at);
+        }
+        off[i] = -1;
+        if ((uint32_t)entry[i] < (uint32_t)c.pages) {
+          off[i] = (int64_t)entry[i] * c.page_bytes + (int64_t)row_at[i] * c.row_bytes + (int64_t)t.head * c.head_bytes;
+          k[i] = *(const u32x4*)((const unsigned char*)c.k + off[i] + at);
+          if constexpr (MX) {
+            s_off[i] = (int64_t)entry[i] * c.s_page + (int64_t)row_at[i] * c.s_row + (int64_t)t.head * c.s_head;
+            ks[i] = *(c.ks + s_off[i] + s_at);
+          }
+        }
+        key[i] += N;
+        page_at[i] += N / c.page_size;
+        row_at[i] += N % c.page_size;
+        if (row_at[i] >= c.page_size) row_at[i] -= c.page_size, ++page_at[i];
+      }
+      ask();
+    }
+    // True in a lane that kept a value of V back: `look`, as put().  What lies behind the context is among what only some rows see.
+    __device__ __forceinline__ bool store(unsigned char* sk, unsigned char* sv, bool look) {
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) found |= put(sk, sv, (wave + i * W) * kGroup + row, unit, k[i], v[i], ks[MX ? i : 0], vs[MX ? i : 0], look);
+      return found;
+    }
+  };
+
+  // Order of what stands in front of this: N matrix products, each with two reads of LDS for the third one behind it and an operation of the vector ALU.
+  template <int N>
+  __device__ static __forceinline__ void dealt() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+    }
+  }
+
+  // W x X rows, a wavefront to X of them, in steps of N = B x 32 keys (D of 128 and 256; rows of 64 are so short that a step is mostly exponentials and larger steps
+  // gain more: 365 us against 390 for the prompt).  The vector ALU has the exponentials of a step while the matrix cores have the scores of the next,
+  // then the highest of those while they have the product with V:  S(j + 1) | exponentials(j),  O(j) | highest(j + 1).
+  // There are two buffers of K and of V; K(j + 2) and V(j + 1) are written over K(j) and V(j - 1) at the start of step j, from registers that were asked for in step j - 1.
+  template <int X, int B>
+  __device__ static __forceinline__ void pipelined_keys(Rows<X>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* lds, int32_t* apart_at, int32_t* missed) {
+    using H = Shape<T, D, X>;
+    constexpr int N = B * 32, kBlocks = N / X, kEach = H::kScores * X / 32, KS = D / H::kInner, OB = D / H::kOuter;
+    static_assert(2 * N * (kRowK + kRowV) <= kLdsBytes, "two buffers of each");
+    const int lane = threadIdx.x & 63;
+    const int32_t steps = (t.k1 - t.k0 + N - 1) / N;
+    if (steps <= 0) return;
+    auto k_at = [&](int32_t j) { return lds + (j & 1) * (N * kRowK); };
+    auto v_at = [&](int32_t j) { return lds + 2 * N * kRowK + (j & 1) * (N * kRowV); };
+    GroupLoader<N> in(c, t);
+    auto store = [&](int32_t j) {   // V of step j, K of the next
+      const int32_t key0 = t.k0 + j * N;
+      if (in.store(k_at(j + 1), v_at(j), t.partly(key0, N))) apart_at[j & 1] = j;
+      in.load();
+    };
+    // `beside`(m, of): what the vector ALU does at matrix product m.
+    auto scores_of = [&](int32_t j, float (&s)[B][H::kScores], auto&& beside) {
+      constexpr int kProducts = kBlocks * KS, kAhead = kProducts < 4 ? kProducts : 4;
+      const unsigned char* sk = k_at(j);
+      auto operand = [&](int m) { return *reinterpret_cast<const vec8*>(sk + k_off(m % kBlocks * X + lane % X, m / kBlocks * (H::kInner / 8) + lane / X)); };
+      typename H::Acc acc[kBlocks] = {};
+      vec8 ahead[kAhead];
+#pragma unroll
+      for (int m = 0; m < kAhead; ++m) ahead[m] = operand(m);
+#pragma unroll
+      for (int m = 0; m < kProducts; ++m) {
+        acc[m % kBlocks] = H::mfma(ahead[m % kAhead], w.q[m / kBlocks], acc[m % kBlocks]);
+        if (m + kAhead < kProducts) ahead[m % kAhead] = operand(m + kAhead);
+        beside(m, kProducts);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) s[i * X / 32][i * kEach % H::kScores + e] = acc[i][e];
+    };
+    if (threadIdx.x < 2) apart_at[threadIdx.x] = -2;
+    in.load();
+    __syncthreads();
+    store(-1);
+    store(0);
+    __syncthreads();
+    float s0[B][H::kScores], s1[B][H::kScores];
+    scores_of(0, s0, [](int, int) {});
+    hide<X, B>(w, s0, t.k0);
+    move<X>(w, highest<X, B>(s0), scale);
+    __syncthreads();
+    auto step = [&](int32_t j, float (&s)[B][H::kScores], float (&next)[B][H::kScores]) {
+      const int32_t key0 = t.k0 + j * N;
+      store(j + 1);
+      if (w.used && key0 <= w.any_hi) {   // (no row of the wavefront sees later keys)
+        vec8 pf[B][H::kSteps];
+        Exponentials<X, B> weights(w, s, pf, scale);
+        scores_of(j + 1, next, weights);
+        weights.end();
+        hide<X, B>(w, next, key0 + N);
+        const unsigned char* sv = v_at(j);
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+          for (int k = 0; k < H::kSteps; ++k)
+#pragma unroll
+            for (int ob = 0; ob < OB; ++ob) w.o[ob] = H::mfma(v_frag<X>(sv + b * 32 * kRowV, k, ob), pf[b][k], w.o[ob]);
+        float mx = highest<X, B>(next);
+        dealt<B * H::kSteps * OB>();
+        here(mx);
+        if (__builtin_amdgcn_readfirstlane(apart_at[j & 1]) == j && w.missed < kMostMissed) missed[w.missed++] = key0;
+        move<X>(w, mx, scale);
+      }
+      __syncthreads();
+    };
+#pragma unroll 1
+    for (int32_t j = 0; j < steps; j += 2) {
+      step(j, s0, s1);
+      if (j + 1 < steps) step(j + 1, s1, s0);
     }
   }
 
@@ -678,8 +897,8 @@ struct Paged {
     t.pos0 = s.position(0);
     t.pages = c.table + (int64_t)b * c.table_row;
     const int32_t first = t.pos0 + t.row0 / p.group, last = t.pos0 + (t.row0 + t.rows - 1) / p.group;
-    t.all_lo = p.window > 0 && last >= p.window ? last - p.window + 1 : 0, t.all_hi = first;
-    const int32_t lo = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, hi = max(min(last + 1, s.held), lo);
+    // (larger tiles start on a multiple of 64: whole groups of rows)
+    const int32_t seen = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, lo = t.rows > 16 ? seen & ~63 : seen, hi = max(min(last + 1, s.held), lo);
     // as many shares as it takes, as even as steps of all wavefronts allow
     const int32_t span = hi - lo, step = FEW || t.rows <= 16 ? kOwners * 32 : 64, wanted = (int32_t)min(((uint32_t)span + keys_each - 1) / keys_each, most);
     const int32_t each = max((span + wanted - 1) / max(wanted, 1) + step - 1, step) / step * step;
@@ -687,6 +906,7 @@ struct Paged {
     if (t.share >= t.shares) return;
     t.k0 = lo + (int32_t)t.share * each;
     t.k1 = min(hi, t.k0 + each);
+    t.all_lo = p.window > 0 && last >= p.window ? last - p.window + 1 : 0, t.all_hi = min(first, t.k1 - 1);
 
     // Partial results: rows of the large tiles first, [head][row of all][share], then the others, [sequence][head][share].
     const int32_t slot_rows = is_long ? t.rows : p.few_slot_rows;
@@ -711,8 +931,11 @@ struct Paged {
       Rows<kRows> w;
       begin(w, t, q, p, wave / shared_by);
       if (shared_by == 1) {
-        shared_keys<kRows, W, kWideStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
         blocks = kWideStep;
+        bool done = false;
+        if constexpr (D > 64)
+          if ((done = GroupLoader<kWideStep * 32>::grouped(c, t))) pipelined_keys<kRows, kWideStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
+        if (!done) shared_keys<kRows, W, kWideStep>(w, t, c, p.scale_log2e, lds, apart_at, missed);
       } else if (kMostShared > 2 && shared_by > 2) {
         shared_keys<kRows, W / kMostShared, 1>(w, t, c, p.scale_log2e, lds, apart_at, missed);
       } else {

@@ -798,53 +798,74 @@ struct Paged {
       }
     }
     if (t.shares == 1 || !gemm::last_to_arrive(p.counters + t.slot, t.shares, flag)) return;
-    // The shares of few rows are dealt to several groups of threads, whose sums meet in LDS; a read past the L2 takes a microsecond, so eight are under way together.
+    // A read past the L2 takes a microsecond, so eight are under way together: of one row where there are many shares, of several where there are few (the chunk of 512
+    // tokens behind 16384, four shares of 256 rows: 157 us, 163 one row at a time).
+    if (W == 4 || t.shares > 4 || t.rows <= kRowsAtOnce) add_shares<1, 8>(t, out, p, part, bytes, lds);
+    else if (t.shares > 2) add_shares<2, 4>(t, out, p, part, bytes, lds);
+    else add_shares<4, 2>(t, out, p, part, bytes, lds);
+  }
+
+  // A row's result so far: columns 4 u .., reference point and sum.
+  struct Sum {
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    __device__ __forceinline__ void add(const f32x4& x, float top_of, float sum_of) {
+      const float top = fmaxf(m, top_of), use = top == -INFINITY ? 0.0f : top, was = __builtin_amdgcn_exp2f(m - use), by = __builtin_amdgcn_exp2f(top_of - use);
+      m = top, l = __builtin_fmaf(sum_of, by, l * was);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], by, o[e] * was);
+    }
+  };
+  // The tile's shares in the order of the keys, R rows and K shares of a thread under way together; of few rows (R = 1) they are dealt to several groups of threads, whose
+  // sums meet in LDS.
+  template <int R, int K>
+  __device__ static __forceinline__ void add_shares(const Tile& t, const PartitionArg<3>& out, const PagedPlan& p, __amdgpu_buffer_rsrc_t part, uint32_t bytes, unsigned char* lds) {
+    constexpr int U = D / 4, kRowsAtOnce = kThreads / U;
+    const int tid = threadIdx.x, u = tid % U;
+    const uint32_t stats = bytes / (D + 4) * D;
     const int rows_at_once = min(kRowsAtOnce, t.rows <= 1 ? 1 : 1 << (32 - __builtin_clz(t.rows - 1))), groups = kRowsAtOnce / rows_at_once, group = tid / U / rows_at_once;
     const uint32_t each = (t.shares + groups - 1) / groups, k0 = group * each, k1 = min(k0 + each, t.shares);
-    f32x4* const sums = reinterpret_cast<f32x4*>(lds);
-    float* const stats_at = reinterpret_cast<float*>(lds + kThreads * 16);
 #pragma unroll 1
-    for (int base = 0; base < t.rows; base += rows_at_once) {
-      const int row = base + tid / U % rows_at_once;
-      constexpr uint32_t kAtOnce = 8;
-      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-      float m = -INFINITY, sum = 0.0f;
-      auto add = [&](const f32x4& x, float top_of, float sum_of) {   // in the order of the keys
-        const float top = fmaxf(m, top_of), use = top == -INFINITY ? 0.0f : top, was = __builtin_amdgcn_exp2f(m - use), by = __builtin_amdgcn_exp2f(top_of - use);
-        m = top, sum = __builtin_fmaf(sum_of, by, sum * was);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], by, o[e] * was);
-      };
-      if (row < t.rows) {
+    for (int base = 0; base < t.rows; base += rows_at_once * R) {
+      const int row0 = base + tid / U % rows_at_once;
+      Sum of[R];
 #pragma unroll 1
-        for (uint32_t k = k0; k < k1; k += kAtOnce) {
-          u32x4 v[kAtOnce];
-          u32x2 st[kAtOnce];
+      for (uint32_t k = k0; k < k1; k += K) {
+        u32x4 v[R][K];
+        u32x2 st[R][K];
 #pragma unroll
-          for (uint32_t i = 0; i < kAtOnce; ++i) {
-            const bool there = k + i < k1;
-            v[i] = __builtin_amdgcn_raw_buffer_load_b128(part, there ? (k + i) * bytes + (uint32_t)row * (D * 4) + u * 16 : kOob, 0, gemm::kAgentScope);
-            st[i] = __builtin_amdgcn_raw_buffer_load_b64(part, there ? (k + i) * bytes + stats + row * 8 : kOob, 0, gemm::kAgentScope);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (uint32_t i = 0; i < K; ++i) {
+            const int row = row0 + r * rows_at_once;
+            const bool there = k + i < k1 && row < t.rows;
+            v[r][i] = __builtin_amdgcn_raw_buffer_load_b128(part, there ? (k + i) * bytes + (uint32_t)row * (D * 4) + u * 16 : kOob, 0, gemm::kAgentScope);
+            st[r][i] = __builtin_amdgcn_raw_buffer_load_b64(part, there ? (k + i) * bytes + stats + row * 8 : kOob, 0, gemm::kAgentScope);
           }
 #pragma unroll
-          for (uint32_t i = 0; i < kAtOnce; ++i) {
-            const f32x2 both = __builtin_bit_cast(f32x2, st[i]);
-            if (k + i < k1) add(__builtin_bit_cast(f32x4, v[i]), both[0], both[1]);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (uint32_t i = 0; i < K; ++i) {
+            const f32x2 both = __builtin_bit_cast(f32x2, st[r][i]);
+            if (k + i < k1) of[r].add(__builtin_bit_cast(f32x4, v[r][i]), both[0], both[1]);
           }
-        }
       }
-      if (groups > 1) {
+      if (R == 1 && groups > 1) {
+        f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+        float* const stats_at = reinterpret_cast<float*>(lds + kThreads * 16);
         __syncthreads();
-        sums[tid] = o;
-        if (u == 0) stats_at[tid / U * 2] = m, stats_at[tid / U * 2 + 1] = sum;
+        sums[tid] = of[0].o;
+        if (u == 0) stats_at[tid / U * 2] = of[0].m, stats_at[tid / U * 2 + 1] = of[0].l;
         __syncthreads();
         if (group != 0) continue;
         for (int g = 1; g < groups; ++g) {
           const int at = tid / U + g * rows_at_once;
-          add(sums[at * U + u], stats_at[at * 2], stats_at[at * 2 + 1]);
+          of[0].add(sums[at * U + u], stats_at[at * 2], stats_at[at * 2 + 1]);
         }
       }
-      if (row < t.rows) store_row(out, t, p, row, u, o, sum);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row0 + r * rows_at_once < t.rows) store_row(out, t, p, row0 + r * rows_at_once, u, of[r].o, of[r].l);
     }
   }
 

@@ -198,6 +198,7 @@ CPP_TESTS = {
     "test_host_surface": ("test_host_surface.cpp", "testing", []),
     "test_gpu_surface": ("test_gpu_surface.cpp", True, []),
     "test_block_scale": ("test_block_scale.cpp", True, []),
+    "test_paged_cache": ("test_paged_cache.cpp", True, []),
     "write_record": ("write_record.cpp", True, []),
     "test_slot_table": ("test_slot_table.cpp", False, []),
     "test_slot_table_tsan": ("test_slot_table.cpp", False, ["-fsanitize=thread"]),

@@ -3841,8 +3841,8 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
   p.q_xor = qk_scale < 0.0f ? 0x80008000u : 0u;
   p.window = window, p.group = group;
   const bool any_long = most_new * group > 32, few = most_new * group <= 16;
-  p.few_rows = any_long && most_new * batch == tokens ? 0 : 32;   // all alike: no tiles of short sequences beside the others
   p.few_slot_rows = (int32_t)std::min<int64_t>(32, most_new * group);
+  p.few_rows = any_long && most_new * batch == tokens ? 0 : p.few_slot_rows;   // all alike: no tiles of short sequences beside the others
   p.long_tiles = any_long ? (int32_t)((int64_t)tokens * group / bm + batch) : 0;
   auto plan = [&](bool may_share) {
     const int64_t row_bytes = (d + 4) * 4, few_items = p.few_rows ? (int64_t)batch * heads : 0, few_bytes = few_items * p.few_slot_rows * row_bytes;

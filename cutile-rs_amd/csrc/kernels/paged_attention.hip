@@ -597,7 +597,7 @@ struct Paged {
     const PagedCache& c;
     const Tile& t;
     const int row, unit, wave;       // the lane's row of a group, its 16 bytes of it
-    const uint32_t at, s_at;         // its place in the group
+    const int64_t at, s_at;          // its place in the group
     int32_t key[kLoads], page_at[kLoads], row_at[kLoads], entry[kLoads];   // of the groups to be asked for next
     int64_t off[kLoads], s_off[kLoads];                     // of the groups asked for last, or -1
     u32x4 k[kLoads], v[kLoads];
@@ -606,7 +606,7 @@ struct Paged {
     __device__ static __forceinline__ bool grouped(const PagedCache& c, const Tile& t) { return c.page_size % kGroup == 0 && t.k0 % kGroup == 0; }
     __device__ __forceinline__ GroupLoader(const PagedCache& cache, const Tile& tile)
         : c(cache), t(tile), row((threadIdx.x & 63) / kLoadUnits), unit(threadIdx.x % kLoadUnits), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
-          at((uint32_t)(row * c.row_bytes) + unit * 16), s_at((uint32_t)(row * c.s_row) + unit / 2) {
+          at(row * c.row_bytes + unit * 16), s_at(row * c.s_row + unit / 2) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         key[i] = t.k0 + (wave + i * W) * kGroup;
@@ -910,7 +910,7 @@ struct Paged {
       s = paged::sequence(c, b);
       t.row0 = 0;
       t.rows = s.count * p.group;
-      if (t.rows == 0 || t.rows > (FEW ? 16 : p.few_rows)) return;
+      if (t.rows == 0 || t.rows > p.few_rows) return;   // (more than max_new allows: not promised)
       most = p.few_shares, keys_each = p.few_keys;
       t.slot = ((uint32_t)p.long_tiles + b) * heads + head;
     }

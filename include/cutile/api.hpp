@@ -520,6 +520,9 @@ auto apply_launcher(std::tuple<Xs...> args) {
   return std::apply([](auto&&... xs) { return make_launcher<Fn>(std::move(xs)...); }, std::move(args));
 }
 
+// Stands for a tensor that a launch does without.
+struct Absent {};
+
 namespace kernels {
 struct SaxpyFn {
   static constexpr const char* name = "saxpy";
@@ -716,6 +719,73 @@ struct SiluMulQuantizeFn {
     auto ga = input_arg(gate), ua = input_arg(up);
     auto op = out.arg(), sp = scales.arg();
     return cutile_launch_silu_mul_quantize(s, &ga, &ua, &op, &sp, tensor_scale, o);
+  }
+};
+// ---- a serving step over a paged cache, logits ----
+template <class X>
+struct OptionalArg {
+  cutile_tensor_arg_t arg;
+  explicit OptionalArg(X& x) : arg(input_arg(x)) {}
+  const cutile_tensor_arg_t* get() const { return &arg; }
+};
+template <>
+struct OptionalArg<Absent> {
+  explicit OptionalArg(Absent&) {}
+  const cutile_tensor_arg_t* get() const { return nullptr; }
+};
+struct PagedCacheWriteFn {
+  static constexpr const char* name = "paged_cache_write";
+  template <class NK, class NV, class K, class V, class P, class S, class L, class KS, class VS>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, NK& new_k, NV& new_v, K& k, V& v, P& page_table, S& starts, L& context_lens, KS& k_scales,
+                                VS& v_scales) {
+    auto nk = input_arg(new_k), nv = input_arg(new_v), ka = input_arg(k), va = input_arg(v), pa = input_arg(page_table), sa = input_arg(starts), la = input_arg(context_lens);
+    OptionalArg<KS> ks(k_scales);
+    OptionalArg<VS> vs(v_scales);
+    return cutile_launch_paged_cache_write(s, &nk, &nv, &ka, &va, ks.get(), vs.get(), &pa, &sa, &la, o);
+  }
+};
+struct PagedCacheReadFn {
+  static constexpr const char* name = "paged_cache_read";
+  template <class K, class V, class P, class S, class L, class OK, class OV, class KS, class VS>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, K& k, V& v, P& page_table, S& starts, L& context_lens, OK& out_k, OV& out_v, KS& k_scales,
+                                VS& v_scales) {
+    auto ka = input_arg(k), va = input_arg(v), pa = input_arg(page_table), sa = input_arg(starts), la = input_arg(context_lens);
+    auto kp = out_k.arg(), vp = out_v.arg();
+    OptionalArg<KS> ks(k_scales);
+    OptionalArg<VS> vs(v_scales);
+    return cutile_launch_paged_cache_read(s, &ka, &va, ks.get(), vs.get(), &pa, &sa, &la, &kp, &vp, o);
+  }
+};
+struct PagedAttentionFn {
+  static constexpr const char* name = "paged_attention";
+  template <class Q, class K, class V, class P, class S, class L, class O, class KS, class VS, class W>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, Q& q, K& k, V& v, P& page_table, S& starts, L& context_lens, O& out, float qk_scale,
+                                int32_t window, int32_t max_new, int32_t max_context, KS& k_scales, VS& v_scales, W& workspace) {
+    auto qa = input_arg(q), ka = input_arg(k), va = input_arg(v), pa = input_arg(page_table), sa = input_arg(starts), la = input_arg(context_lens);
+    auto op = out.arg();
+    OptionalArg<KS> ks(k_scales);
+    OptionalArg<VS> vs(v_scales);
+    OptionalArg<W> wa(workspace);
+    return cutile_launch_paged_attention(s, &qa, &ka, &va, ks.get(), vs.get(), &pa, &sa, &la, &op, qk_scale, window, max_new, max_context, wa.get(), o);
+  }
+};
+struct AdjustLogitsFn {
+  static constexpr const char* name = "adjust_logits";
+  template <class L, class O, class T, class PL, class TL, class R, class P, class F, class BI, class BV, class A>
+  static cutile_status_t launch(cutile_stream_t s, const cutile_launch_opts_t* o, L& logits, O& out, T& tokens, PL& prompt_lens, TL& token_lens, R& repetition, P& presence,
+                                F& frequency, BI& bias_ids, BV& bias_values, A& allowed) {
+    auto la = input_arg(logits);
+    auto op = out.arg();
+    OptionalArg<T> ta(tokens);
+    OptionalArg<PL> pl(prompt_lens);
+    OptionalArg<TL> tl(token_lens);
+    OptionalArg<R> ra(repetition);
+    OptionalArg<P> pa(presence);
+    OptionalArg<F> fa(frequency);
+    OptionalArg<BI> bi(bias_ids);
+    OptionalArg<BV> bv(bias_values);
+    OptionalArg<A> aa(allowed);
+    return cutile_launch_adjust_logits(s, &la, &op, ta.get(), pl.get(), tl.get(), ra.get(), pa.get(), fa.get(), bi.get(), bv.get(), aa.get(), o);
   }
 };
 // ---- transformer-block kernels (cutile-kernels/src/{norms,pointwise,positional}.rs) ----
@@ -948,6 +1018,37 @@ template <class X, class S, class O> auto block_dequantize(X&& x, S&& scales, fl
 template <class X, class W, class O, class S> auto rms_norm_quantize(X&& x, W&& w, O&& out, S&& scales, float eps, float tensor_scale = 1.0f) { return make_launcher<kernels::RmsNormQuantizeFn>(std::forward<X>(x), std::forward<W>(w), std::forward<O>(out), std::forward<S>(scales), eps, tensor_scale); }
 template <class R, class X, class W, class O, class S, class RO> auto add_rms_norm_quantize(R&& residual, X&& x, W&& w, O&& out, S&& scales, RO&& residual_out, float eps, float tensor_scale = 1.0f) { return make_launcher<kernels::AddRmsNormQuantizeFn>(std::forward<R>(residual), std::forward<X>(x), std::forward<W>(w), std::forward<O>(out), std::forward<S>(scales), std::forward<RO>(residual_out), eps, tensor_scale); }
 template <class G, class U, class O, class S> auto silu_mul_quantize(G&& gate, U&& up, O&& out, S&& scales, float tensor_scale = 1.0f) { return make_launcher<kernels::SiluMulQuantizeFn>(std::forward<G>(gate), std::forward<U>(up), std::forward<O>(out), std::forward<S>(scales), tensor_scale); }
+// paged_cache_write(new_k, new_v, k_cache, v_cache, page_table, starts, context_lens, k_scales, v_scales) and what reads such a cache: no counterpart in the reference;
+// shapes and rules in cutile_hip.h.  What a launch does without is Absent.
+template <class NK, class NV, class K, class V, class P, class S, class L, class KS = Absent, class VS = Absent>
+auto paged_cache_write(NK&& new_k, NV&& new_v, K&& k_cache, V&& v_cache, P&& page_table, S&& starts, L&& context_lens, KS&& k_scales = {}, VS&& v_scales = {}) {
+  return make_launcher<kernels::PagedCacheWriteFn>(std::forward<NK>(new_k), std::forward<NV>(new_v), std::forward<K>(k_cache), std::forward<V>(v_cache), std::forward<P>(page_table),
+                                                   std::forward<S>(starts), std::forward<L>(context_lens), std::forward<KS>(k_scales), std::forward<VS>(v_scales));
+}
+// paged_cache_read(k_cache, v_cache, page_table, starts, context_lens, out_k: [BM, heads, D], out_v, k_scales, v_scales)
+template <class K, class V, class P, class S, class L, class OK, class OV, class KS = Absent, class VS = Absent>
+auto paged_cache_read(K&& k_cache, V&& v_cache, P&& page_table, S&& starts, L&& context_lens, OK&& out_k, OV&& out_v, KS&& k_scales = {}, VS&& v_scales = {}) {
+  return make_launcher<kernels::PagedCacheReadFn>(std::forward<K>(k_cache), std::forward<V>(v_cache), std::forward<P>(page_table), std::forward<S>(starts),
+                                                  std::forward<L>(context_lens), std::forward<OK>(out_k), std::forward<OV>(out_v), std::forward<KS>(k_scales),
+                                                  std::forward<VS>(v_scales));
+}
+// paged_attention(q, k_cache, v_cache, page_table, starts, context_lens, out: [BM, G, D], qk_scale, window, max_new, max_context, k_scales, v_scales, workspace)
+template <class Q, class K, class V, class P, class S, class L, class O, class KS = Absent, class VS = Absent, class W = Absent>
+auto paged_attention(Q&& q, K&& k_cache, V&& v_cache, P&& page_table, S&& starts, L&& context_lens, O&& out, float qk_scale, int32_t window = 0, int32_t max_new = 0,
+                     int32_t max_context = 0, KS&& k_scales = {}, VS&& v_scales = {}, W&& workspace = {}) {
+  return make_launcher<kernels::PagedAttentionFn>(std::forward<Q>(q), std::forward<K>(k_cache), std::forward<V>(v_cache), std::forward<P>(page_table), std::forward<S>(starts),
+                                                  std::forward<L>(context_lens), std::forward<O>(out), qk_scale, window, max_new, max_context, std::forward<KS>(k_scales),
+                                                  std::forward<VS>(v_scales), std::forward<W>(workspace));
+}
+// adjust_logits(logits, out: [1, vocab], tokens, prompt_lens, token_lens, repetition, presence, frequency, bias_ids, bias_values, allowed)
+template <class L, class O, class T = Absent, class PL = Absent, class TL = Absent, class R = Absent, class P = Absent, class F = Absent, class BI = Absent, class BV = Absent,
+          class A = Absent>
+auto adjust_logits(L&& logits, O&& out, T&& tokens = {}, PL&& prompt_lens = {}, TL&& token_lens = {}, R&& repetition = {}, P&& presence = {}, F&& frequency = {},
+                   BI&& bias_ids = {}, BV&& bias_values = {}, A&& allowed = {}) {
+  return make_launcher<kernels::AdjustLogitsFn>(std::forward<L>(logits), std::forward<O>(out), std::forward<T>(tokens), std::forward<PL>(prompt_lens), std::forward<TL>(token_lens),
+                                                std::forward<R>(repetition), std::forward<P>(presence), std::forward<F>(frequency), std::forward<BI>(bias_ids),
+                                                std::forward<BV>(bias_values), std::forward<A>(allowed));
+}
 // add_rms_norm_f16(residual, x, w, out: [1,N], residual_out: [1,N], eps)      cutile-kernels/src/norms.rs:76-83
 template <class R, class X, class W, class O, class RO> auto add_rms_norm_f16(R&& residual, X&& x, W&& w, O&& out, RO&& residual_out, float eps) { return make_launcher<kernels::AddRmsNormF16Fn>(std::forward<R>(residual), std::forward<X>(x), std::forward<W>(w), std::forward<O>(out), std::forward<RO>(residual_out), eps); }
 // qk_norm_f16(q, k, q_weight, k_weight, out: [1,N], eps, num_q_rows)          cutile-kernels/src/norms.rs:152-160

@@ -801,8 +801,8 @@ cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cu
  * copies (experimental/kvbm.rs) move blocks between layouts. ---------------------------------------------------------------
  * A batch of B sequences shares the pages of one cache.  All of them take these tensors:
  *   k_cache, v_cache  [pages, page_size, kv_heads, D], D 64, 128 or 256, of any strides but a unit inner one (the same for both), rows on 16-byte boundaries, either
- *                     f16 or bf16 like the new tokens (k_scales, v_scales NULL), or f8e4m3fn with k_scales, v_scales [pages, page_size, kv_heads, D/32] f8e8m0fnu: mxfp8 as
- *                     block_quantize makes it
+ *                     f16 or bf16 like the new tokens (k_scales, v_scales NULL), or f8e4m3fn with k_scales, v_scales [pages, page_size, kv_heads, D/32] f8e8m0fnu (rows on
+ *                     boundaries of D/32 bytes): mxfp8 as block_quantize makes it
  *   page_table        [B, most pages of a sequence] i32, contiguous rows: position p of sequence b is row p % page_size of page page_table[b, p / page_size]
  *   starts            [B + 1] i32, not falling: the new tokens of sequence b are the rows starts[b] .. starts[b+1] of new_k, new_v, q or out (rows that are nobody's stay as they
  *                     are)

@@ -206,29 +206,25 @@ def test_gpu_captured(ct, dev, shared):
     g.close()
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("mx", [False, True])
-@pytest.mark.parametrize("new,held,group,window", [([40], [40], 2, 0), ([200], [300], 1, 0), ([5], [120], 4, 0), ([64], [200], 8, 50), ([3, 100], [70, 100], 1, 33)])
-def test_gpu_what_a_row_does_not_see(ct, dev, dtype, mx, new, held, group, window):
+def unseen(ct, dev, dtype, mx, new, held, group, window, d, page):
     """NaN and infinities behind the context, in later tokens and in front of the window change nothing for the rows that do not see them; rows that do get what
     the definition gives"""
-    b = Batch(new, held, 16, seed=9)
-    q, k, v, scales, real = problem(b, 2, group, 64, dtype, mx, dev)
-    first = check(ct, dev, b, q, k, v, scales, real, 64, window)
+    b = Batch(new, held, page, seed=9)
+    q, k, v, scales, real = problem(b, 2, group, d, dtype, mx, dev)
+    first = check(ct, dev, b, q, k, v, scales, real, d, window)
     kinds = [float("nan")] if mx else [float("nan"), float("inf"), float("-inf")]
     table = b.table.long()
     poisoned = []
     for s, (n, h) in enumerate(zip(new, held)):
-        last = int(table[s, (h - 1) // 16])
-        for r in range((h - 1) % 16 + 1, 16):          # behind the context
+        last = int(table[s, (h - 1) // page])
+        for r in range((h - 1) % page + 1, page):          # behind the context
             if mx:
                 scales["v_scales"][last, r], scales["k_scales"][last, r] = 255, 255
             else:
                 v[last, r], k[last, r] = float("nan"), float("inf")
         p = h - max(1, n // 3)                        # among the new tokens
         for i, kind in enumerate(kinds):
-            at, r = int(table[s, (p + i) // 16]), (p + i) % 16
+            at, r = int(table[s, (p + i) // page]), (p + i) % page
             if p + i >= h:
                 continue
             if mx:
@@ -237,7 +233,7 @@ def test_gpu_what_a_row_does_not_see(ct, dev, dtype, mx, new, held, group, windo
                 v[at, r, 1, 3] = kind
             poisoned.append((s, p + i, kind))
     out = torch.full_like(first, 9.0)
-    ct.paged_attention(q.to(dev), k, v, *b.where(dev), ct.partition(out, [1, 1, 64]), 64 ** -0.5, window=window, **scales)
+    ct.paged_attention(q.to(dev), k, v, *b.where(dev), ct.partition(out, [1, 1, d]), d ** -0.5, window=window, **scales)
     out, first = out.cpu(), first.cpu()
     rows = {}
     for row, s, p, _, _ in b.places():
@@ -256,6 +252,22 @@ def test_gpu_what_a_row_does_not_see(ct, dev, dtype, mx, new, held, group, windo
             inf = {float("inf"), float("-inf")}
             kind = "nan" if set(hit) - inf or inf <= set(hit) else hit[0]
             assert bool(got[group:, cols].isnan().all()) if kind == "nan" else bool((got[group:, cols] == kind).all()), (row, hit)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("new,held,group,window", [([40], [40], 2, 0), ([200], [300], 1, 0), ([5], [120], 4, 0), ([64], [200], 8, 50), ([3, 100], [70, 100], 1, 33)])
+def test_gpu_what_a_row_does_not_see(ct, dev, dtype, mx, new, held, group, window):
+    unseen(ct, dev, dtype, mx, new, held, group, window, 64, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("new,held,group,window,d,page", [([300], [300], 1, 0, 128, 16), ([100], [700], 8, 0, 128, 16), ([200], [900], 2, 333, 128, 16), ([200], [900], 2, 333, 128, 7),
+                                                          ([200], [900], 2, 333, 64, 16), ([130], [700], 2, 90, 256, 16), ([130], [700], 2, 90, 256, 7), ([9], [600], 1, 100, 256, 16)])
+def test_gpu_what_a_row_of_a_larger_tile_does_not_see(ct, dev, mx, new, held, group, window, d, page):
+    unseen(ct, dev, "f16", mx, new, held, group, window, d, page)
 
 
 @pytest.mark.gpu

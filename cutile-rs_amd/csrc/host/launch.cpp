@@ -3832,7 +3832,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
   if (cutile_status_t s = resolve_entry(fn, opts, l.variant, {l.variant}, &res)) return s;
   int cus = 256;
   if (cutile_status_t s = current_device_units(&cus)) return s;
-  const int64_t bm = res.entry->tile[0], most_new = max_new ? std::min(max_new, tokens) : tokens;
+  const int64_t most_new = max_new ? std::min(max_new, tokens) : tokens;
   const int64_t held = (int64_t)l.c.table_pages * l.c.page_size, context = std::max<int64_t>(1, max_context ? std::min<int64_t>(max_context, held) : std::min<int64_t>(held, INT32_MAX));
   PagedPlan p{};
   // the kernels look for the largest score before they scale it: a negative scale turns q around, and a scale of 0 makes it zeros
@@ -3843,18 +3843,34 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
   const bool any_long = most_new * group > 32, few = most_new * group <= 16;
   p.few_slot_rows = (int32_t)std::min<int64_t>(32, most_new * group);
   p.few_rows = any_long && most_new * batch == tokens ? 0 : p.few_slot_rows;   // all alike: no tiles of short sequences beside the others
-  p.long_tiles = any_long ? (int32_t)((int64_t)tokens * group / bm + batch) : 0;
   auto plan = [&](bool may_share) {
     const int64_t row_bytes = (d + 4) * 4, few_items = p.few_rows ? (int64_t)batch * heads : 0, few_bytes = few_items * p.few_slot_rows * row_bytes;
-    const int64_t long_items = any_long ? ((int64_t)tokens * group + bm - 1) / bm * heads : 0, long_bytes = (int64_t)tokens * group * heads * row_bytes;
+    const int64_t rows = (int64_t)tokens * group, long_bytes = rows * heads * row_bytes;
     Deal of_long, of_few;
-    if (may_share && (int64_t)p.long_tiles * heads + few_items <= (int64_t)kSplitCounters) {
-      // A workgroup to a CU, or two where sequences of different lengths are all there is and the small kernel has room for them: 24 ragged sequences of up to 6000 tokens
-      // 39 us against 52, 20 of 8192 87 against 103; a single sequence of 16000 takes 21 us against 17 that way, all else the merging of more shares.
-      if (few_items) of_few = deal_keys(few_items, context, few && batch > 1 ? 2 * cus : cus, few ? 256 : 512, std::max<int64_t>(1, (any_long ? room / 4 : room) / few_bytes));
-      const int64_t left = room - (of_few.shares > 1 ? of_few.shares * few_bytes : 0), seen = window ? std::min<int64_t>(context, window + bm / group) : context;
-      if (long_items) of_long = deal_keys(long_items, seen, cus, 256, std::max<int64_t>(1, left / long_bytes));
+    auto seen_by = [&](int64_t bm) { return window ? std::min<int64_t>(context, window + bm / group) : context; };   // keys that a tile of so many rows sees
+    // A workgroup to a CU, or two where sequences of different lengths are all there is and the small kernel has room for them: 24 ragged sequences of up to 6000 tokens
+    // 39 us against 52, 20 of 8192 87 against 103; a single sequence of 16000 takes 21 us against 17 that way, all else the merging of more shares.
+    if (may_share && few_items && few_items <= (int64_t)kSplitCounters)
+      of_few = deal_keys(few_items, seen_by(32), few && batch > 1 ? 2 * cus : cus, 256, std::max<int64_t>(1, (any_long ? room / 4 : room) / few_bytes));
+    const int64_t left = room - (of_few.shares > 1 ? of_few.shares * few_bytes : 0);
+    // Rows of a tile and shares of its keys: what is done soonest by a count of steps of 64 keys.  A step of half as many rows takes 0.7 of the time, then 0.5 and 0.38 (the
+    // prompt of 8192 tokens 578, 784, 1107 and 1728 us in tiles of 256, 128, 64 and 32 rows); adding shares up, a step's time for every 16 reads of a thread.  672 rows behind
+    // 251 tokens 11 us in tiles of 32 (23 of 256), 512 behind 16448 67 us in tiles of 128 (91), 2048 behind 16896 157 of 256 (213 of 128).
+    double soonest = 0.0;
+    double step = 1.0;
+    p.tile_rows = res.entry->tile[0], p.long_tiles = 0;
+    for (int64_t bm = res.entry->tile[0]; any_long && bm >= 32; bm /= 2, step *= 0.71) {
+      const int64_t tiles = rows / bm + batch, items = (rows + bm - 1) / bm * heads, seen = seen_by(bm);
+      Deal deal;
+      if (may_share && tiles * heads + few_items <= (int64_t)kSplitCounters) deal = deal_keys(items, seen, cus, 256, std::max<int64_t>(1, left / long_bytes));
+      const double longest = step * (double)((seen + deal.shares - 1) / deal.shares + 63) / 64, average = seen < context ? 1.0 : 1.0 - 0.5 * (double)std::min(most_new, context) / (double)context;
+      const int64_t at_once = 512 / (d / 4) * (deal.shares > 4 ? 2 : deal.shares > 2 ? 4 : 8), of_shares = deal.shares > 4 ? 8 : deal.shares > 2 ? 4 : 2;
+      double steps = std::max(longest, longest * average * (double)items * deal.shares / cus);
+      if (deal.shares > 1) steps += (double)(div_up(bm, at_once) * div_up(deal.shares, of_shares));
+      if (p.long_tiles && steps >= soonest) continue;
+      soonest = steps, of_long = deal, p.tile_rows = (int32_t)bm, p.long_tiles = (int32_t)tiles;
     }
+    if (p.long_tiles * (int64_t)heads + few_items > (int64_t)kSplitCounters) of_few = of_long = Deal{};
     p.long_shares = of_long.shares, p.long_keys = of_long.keys;
     p.few_shares = of_few.shares, p.few_keys = of_few.keys;
   };

@@ -27,7 +27,8 @@ struct PagedPlan {
   uint32_t q_and, q_xor;
   int32_t window, group;                // keys a token sees (0: all), query heads of a KV head
   int32_t few_rows;                     // sequences of up to so many rows (token, head of the group) are tiles of their own
-  int32_t long_tiles, long_shares, long_keys;   // numbers of row tiles of the other sequences, workgroups to a tile, keys to a workgroup
+  int32_t tile_rows;                    // of the other sequences
+  int32_t long_tiles, long_shares, long_keys;   // numbers of their tiles, workgroups to a tile, keys to a workgroup
   int32_t few_shares, few_keys;
   int32_t few_slot_rows;                // rows of a small tile's partial result
 };

@@ -798,11 +798,12 @@ struct Paged {
       }
     }
     if (t.shares == 1 || !gemm::last_to_arrive(p.counters + t.slot, t.shares, flag)) return;
-    // A read past the L2 takes a microsecond, so eight are under way together: of one row where there are many shares, of several where there are few (the chunk of 512
-    // tokens behind 16384, four shares of 256 rows: 157 us, 163 one row at a time).
-    if (W == 4 || t.shares > 4 || t.rows <= kRowsAtOnce) add_shares<1, 8>(t, out, p, part, bytes, lds);
-    else if (t.shares > 2) add_shares<2, 4>(t, out, p, part, bytes, lds);
-    else add_shares<4, 2>(t, out, p, part, bytes, lds);
+    // A read past the L2 takes a microsecond, so sixteen are under way together: of one row or two where there are many shares, of several where there are few (the chunk
+    // of 512 tokens behind 16384, four shares of 256 rows: 157 us, 163 one row at a time).
+    if (W == 4 || t.rows <= kRowsAtOnce) add_shares<1, 8>(t, out, p, part, bytes, lds);
+    else if (t.shares > 4) add_shares<2, 8>(t, out, p, part, bytes, lds);
+    else if (t.shares > 2) add_shares<4, 4>(t, out, p, part, bytes, lds);
+    else add_shares<8, 2>(t, out, p, part, bytes, lds);
   }
 
   // A row's result so far: columns 4 u .., reference point and sum.
@@ -890,17 +891,17 @@ struct Paged {
     uint32_t most, keys_each;
     paged::Sequence s;
     if (is_long) {
-      // Tiles of sequence b have the numbers from starts[b] * group / BM + b on: more than there are, so that nobody has to count them.  The last ones, whose rows see
+      // Tiles of sequence b have the numbers from starts[b] * group / tile_rows + b on: more than there are, so that nobody has to count them.  The last ones, whose rows see
       // the most keys, come first.
       const int32_t n = p.long_tiles - 1 - (int32_t)(item / p.long_shares);
       t.share = item % p.long_shares;
-      auto number = [&](int32_t i) { return (int64_t)min(max(c.starts[i], 0), c.tokens) * p.group / BM + i; };
+      auto number = [&](int32_t i) { return (int64_t)min(max(c.starts[i], 0), c.tokens) * p.group / p.tile_rows + i; };
       b = paged::find_sequence(c.batch, n, number);
       s = paged::sequence(c, b);
-      const int64_t row0 = ((int64_t)n - number(b)) * BM;
+      const int64_t row0 = ((int64_t)n - number(b)) * p.tile_rows;
       if (s.count * p.group <= p.few_rows || row0 < 0 || row0 >= (int64_t)s.count * p.group) return;
       t.row0 = (int32_t)row0;
-      t.rows = min(BM, s.count * p.group - t.row0);
+      t.rows = min(p.tile_rows, s.count * p.group - t.row0);
       most = p.long_shares, keys_each = p.long_keys;
       t.slot = (uint32_t)n * heads + head;
     } else {

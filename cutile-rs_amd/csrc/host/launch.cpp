@@ -3940,6 +3940,7 @@ cutile_status_t cutile_launch_adjust_logits(cutile_stream_t stream, const cutile
   auto row_stride = [](const cutile_tensor_arg_t& t) { return t.shape[0] == 1 ? (int64_t)0 : (int64_t)t.strides[0]; };
   if (tokens) {
     if (cutile_status_t s = check_table(fn, "tokens", tokens, CUTILE_DTYPE_I32, CUTILE_DTYPE_I32, rows)) return s;
+    CUTILE_REQUIRE(tokens->shape[1] < 1 << 30, CUTILE_ERR_KERNEL_LAUNCH, "%s: a row has fewer than 2^30 tokens, got %d", fn, tokens->shape[1]);
     a.tokens = tokens->ptr, a.tokens_row = row_stride(*tokens), a.most = tokens->shape[1];
   }
   if (bias_ids) {

@@ -837,7 +837,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
                                               int32_t window, int32_t max_new, int32_t max_context, const cutile_tensor_arg_t* workspace, const cutile_launch_opts_t* opts);
 /* adjust_logits: logits [rows, vocab] (f16, bf16 or f32, unit inner stride) to out of their type, partitioned [1, vocab], which may be logits itself.  Of every token t of a row,
  * in f32 and in this order (each tensor may be NULL):
- *   t among tokens[row, 0 .. token_lens[row]) ([rows, most] i32; token_lens NULL: all):   l <- l > 0 ? l / repetition[row] : l * repetition[row]
+ *   t among tokens[row, 0 .. token_lens[row]) ([rows, most] i32, most < 2^30; token_lens NULL: all):   l <- l > 0 ? l / repetition[row] : l * repetition[row]
  *   c > 0 times among those from prompt_lens[row] on (NULL: from 0):                       l <- l - (presence[row] + frequency[row] * c)
  *   bias_ids, bias_values [rows, n], n up to 1024:  l <- l + the sum, in their order, of the values whose id is t
  *   allowed [rows, words] i32 or u32, bit t % 32 of word t / 32 not set:                   l <- -infinity

@@ -113,6 +113,11 @@ def test_refusals(fake_hip):
     part = p(ct.Partition(out, [1, 100], False, None).arg())
     assert fn(None, t(x["logits"]), part, *[None] * 10) == 0
     assert fn(None, None, part, *[None] * 10) == -2 and fn(None, t(x["logits"]), None, *[None] * 10) == -2
+    many = ct.tensor_arg(x["tokens"], None)
+    many.shape[1], many.strides[0] = 2 ** 30, 2 ** 30
+    n0 = ct.lib().cutile_testing_launch_count()
+    assert fn(None, t(x["logits"]), part, p(many), *[None] * 9) != 0 and b"fewer than 2^30 tokens" in ct.lib().cutile_last_error_message()
+    assert ct.lib().cutile_testing_launch_count() == n0
 
 
 # ---- on a GPU ---------------------------------------------------------------------------------------------------------------

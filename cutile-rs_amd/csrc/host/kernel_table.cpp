@@ -529,8 +529,9 @@ std::vector<KernelEntry> build_table() {
         for (const char* fn : {"paged_cache_write", "paged_cache_read"}) add(fn, keep(v), keep(std::string(fn) + "_entry__" + v), IMG_PAGED_CACHE, 256, 0, 0, 0, d, 0, dt, 0, 3);
         // eight wavefronts of 32 rows, 16 of D = 256; K and V of 32 keys for each of eight, four of D = 256
         add("paged_attention", keep(v), keep("paged_attention_entry__" + v), IMG_PAGED_ATTENTION, 512, (uint32_t)((d == 256 ? 4 : 8) * 32 * (4 * d + 48) + (d == 256 ? 2444 : 2700)), d == 256 ? 128 : 256, 0, d, 0, dt, 0, 3);
-        // launches whose tiles have up to 16 rows: K and V of 32 keys for each of four wavefronts
+        // launches whose tiles have up to 16 or 32 rows: K and V of 32 keys for each of four wavefronts
         add("paged_attention", keep(v + "+few"), keep("paged_attention_entry__" + v + "_few"), IMG_PAGED_ATTENTION, 256, (uint32_t)(4 * 32 * (4 * d + 48) + (d == 256 ? 1156 : 1220)), 16, 0, d, 0, dt, 0, 3);
+        if (d < 256) add("paged_attention", keep(v + "+few32"), keep("paged_attention_entry__" + v + "_few32"), IMG_PAGED_ATTENTION, 256, (uint32_t)(4 * 32 * (4 * d + 48) + 1220), 32, 0, d, 0, dt, 0, 3);
       }
   // ---- logits in front of the choice of a token (512 threads; tile = (-, columns of a workgroup, -, -)) ----
   for (const char* dt : {"f16", "bf16", "f32"})

@@ -3840,7 +3840,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
   p.q_and = qk_scale == 0.0f ? 0u : ~0u;
   p.q_xor = qk_scale < 0.0f ? 0x80008000u : 0u;
   p.window = window, p.group = group;
-  const bool any_long = most_new * group > 32, few = most_new * group <= 16;
+  const bool any_long = most_new * group > 32, few = most_new * group <= (d == 256 ? 16 : 32);
   p.few_slot_rows = (int32_t)std::min<int64_t>(32, most_new * group);
   p.few_rows = any_long && most_new * batch == tokens ? 0 : p.few_slot_rows;   // all alike: no tiles of short sequences beside the others
   auto plan = [&](bool may_share) {
@@ -3881,7 +3881,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     if (!ws.partials) plan(false);
   }
   if (few)
-    if (cutile_status_t s = use_member(&res, member_of(res.entry, "+few"))) return s;
+    if (cutile_status_t s = use_member(&res, member_of(res.entry, most_new * group <= 16 ? "+few" : "+few32"))) return s;
   p.partials = ws.partials, p.counters = ws.counters;
   const uint64_t items = (uint64_t)p.long_tiles * p.long_shares + (p.few_rows ? (uint64_t)batch * p.few_shares : 0);
   CUTILE_REQUIRE(items * heads <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %llu tiles do not fit a launch grid axis", fn, (unsigned long long)(items * heads));

@@ -5,9 +5,10 @@
 // The rows of a tile are pairs (token, query head of one KV head), token by token: group heads share every key that is read, and a decode step of 8 heads or a
 // chunk of 4 tokens fill the columns of a matrix instruction.  S^T = K Q^T and O^T = V^T P^T, so that a lane owns one row and what it holds of P^T is its operand
 // of the second product; the softmax keeps a running reference point and sum of each row, in 32 bits.
-//  * Tiles of up to 16 rows (decode, speculation): every wavefront has keys of its own, 32 at a time, through registers into LDS that no other
-//    wavefront reads: no barrier in the loop.  HBM's rate bounds it: 1 x 131072 tokens, 8 KV heads, bf16, 91 us (5.9 TB/s).  A launch that has no other tiles runs
-//    a kernel of four wavefronts (two workgroups on a CU), others have eight.
+//  * Tiles of up to 32 rows (decode, drafts; 16 at D = 256): every wavefront has all rows, 16 or 32, and keys of its own, 32 at a time, through registers into LDS that
+//    no other wavefront reads: no barrier in the loop.  HBM's rate bounds it: 1 x 131072 tokens, 8 KV heads, bf16, 91 us (5.9 TB/s).  A launch that has no other tiles
+//    runs a kernel of four wavefronts (two workgroups on a CU), others have eight.  Drafts of 8 tokens of 4 heads behind 64 x 8192 mxfp8 tokens take 175 us so, and 321
+//    where the wavefronts share their keys and a barrier a step.
 //  * Larger tiles: R wavefronts side by side hold kRows rows each, W / R share the keys of a step, which all of them fetch together.  Tiles of all W hold their next
 //    scores while the exponentials of the last are made (pipelined_keys).  A prompt of 8192 tokens, 32 heads over 8, D = 128, bf16: 570 us, 960 TFLOP/s of what the
 //    rows see; the loop alone in the order scores, softmax, product 596, and with a branch around the product, which copied O, 669.
@@ -534,8 +535,9 @@ struct Paged {
     }
   }
 
-  // Up to 16 rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ..., 32 of them at a time in LDS at sk and sv.
-  __device__ static __forceinline__ void own_keys(Rows<16>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* sk, unsigned char* sv, int32_t* missed) {
+  // Up to X rows: wavefront w has the keys k0 + 32 w, + 32 (w + W), ..., 32 of them at a time in LDS at sk and sv.
+  template <int X>
+  __device__ static __forceinline__ void own_keys(Rows<X>& w, const Tile& t, const PagedCache& c, float scale, unsigned char* sk, unsigned char* sv, int32_t* missed) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int kBy = W * 32;
     int32_t key0 = t.k0 + wave * 32;
@@ -548,7 +550,7 @@ struct Paged {
         const bool apart = __builtin_amdgcn_ballot_w64(in.store(sk, sv, t.partly(key0, 32))) != 0;
         ordered();
         in.load();
-        keys<16, 1>(w, [&](float (&s)[1][8]) { scores<16>(w, sk, s[0]); }, sv, key0, scale, apart, missed);
+        keys<X, 1>(w, [&](float (&s)[1][Shape<T, D, X>::kScores]) { scores<X>(w, sk, s[0]); }, sv, key0, scale, apart, missed);
       }
     }
     ordered();
@@ -870,8 +872,8 @@ struct Paged {
     }
   }
 
-  // FEW: tiles of up to 16 rows are all there is.
-  template <bool FEW>
+  // FEW: tiles of up to so many rows, 16 or 32, are all there is (0: of any).
+  template <int FEW>
   __device__ static __forceinline__ void run(const TensorArg<3>& q, const PartitionArg<3>& out, const PagedCache& c, const PagedPlan& p) {
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
     __shared__ float stat[W][2][32];
@@ -884,6 +886,8 @@ struct Paged {
       const uint32_t slot = blockIdx.x / 8;
       head = slot % heads, item = slot / heads * 8 + blockIdx.x % 8;
     }
+    // rows that have a wavefront's keys to themselves (of 256 values they take more registers on their way than 8 wavefronts have)
+    constexpr int kMostOwn = FEW ? FEW : D == 256 ? 0 : 32;
     const bool is_long = !FEW && item < of_long;
     Tile t;
     t.head = (int32_t)head;
@@ -922,7 +926,7 @@ struct Paged {
     // (larger tiles start on a multiple of 64: whole groups of rows)
     const int32_t seen = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, lo = t.rows > 16 ? seen & ~63 : seen, hi = max(min(last + 1, s.held), lo);
     // as many shares as it takes, as even as steps of all wavefronts allow
-    const int32_t span = hi - lo, step = FEW || t.rows <= 16 ? kOwners * 32 : 64, wanted = (int32_t)min(((uint32_t)span + keys_each - 1) / keys_each, most);
+    const int32_t span = hi - lo, step = t.rows <= kMostOwn ? kOwners * 32 : 64, wanted = (int32_t)min(((uint32_t)span + keys_each - 1) / keys_each, most);
     const int32_t each = max((span + wanted - 1) / max(wanted, 1) + step - 1, step) / step * step;
     t.shares = max((span + each - 1) / each, 1);
     if (t.share >= t.shares) return;
@@ -938,13 +942,18 @@ struct Paged {
                                                                      : heads * all_rows * of_shares * kRowBytes + (uint64_t)(t.slot - (uint32_t)p.long_tiles * heads) * p.few_shares * slot_rows * kRowBytes);
     int32_t* const missed = all_missed + wave * kMostMissed;
     unsigned char *const sk = lds + wave % kOwners * kOwnBytes, *const sv = sk + 32 * kRowK;   // of 32 keys of the wavefront's own
-    if (FEW || (D != 256 && t.rows <= 16)) {   // (rows of 256 values on their way take more registers than 8 wavefronts have)
-      Rows<16> w;
+    auto own = [&](auto rows) {
+      Rows<decltype(rows)::value> w;
       begin(w, t, q, p, 0);
       own_keys(w, t, c, p.scale_log2e, sk, sv, missed);
       ordered();   // (a wavefront's results lie where its keys were)
       finish(w, t, out, p, partials, slot_rows, lds, stat, &flag, W);
-      return;
+    };
+    if constexpr (FEW > 0) {
+      own(std::integral_constant<int, FEW>{});
+    } else if constexpr (kMostOwn > 0) {
+      if (t.rows <= 16) return own(std::integral_constant<int, 16>{});
+      if (t.rows <= kMostOwn) return own(std::integral_constant<int, kMostOwn>{});
     }
     if constexpr (!FEW) {
       constexpr int kMostShared = W * kRows / 64;
@@ -977,14 +986,18 @@ struct Paged {
 
 }  // namespace
 
-#define ATTENTION(NAME, T, MX, D, W)                                                                                                                                          \
-  extern "C" __global__ void __launch_bounds__(W * 64) paged_attention_entry__##NAME##_d##D(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) {     \
-    Paged<T, MX, D, W>::template run<false>(q, out, c, p);                                                                                                                    \
-  }                                                                                                                                                                           \
-  extern "C" __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) paged_attention_entry__##NAME##_d##D##_few(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) { \
-    Paged<T, MX, D, 4>::template run<true>(q, out, c, p);                                                                                                                     \
+#define ATTENTION(NAME, T, MX, D)                                                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(512) paged_attention_entry__##NAME##_d##D(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) {  \
+    Paged<T, MX, D, 8>::template run<0>(q, out, c, p);                                                                                                             \
   }
-#define ATTENTION_D(NAME, T, MX) ATTENTION(NAME, T, MX, 64, 8) ATTENTION(NAME, T, MX, 128, 8) ATTENTION(NAME, T, MX, 256, 8)
+#define ATTENTION_FEW(NAME, T, MX, D, FEW, SUFFIX)                                                                                                                          \
+  extern "C" __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) paged_attention_entry__##NAME##_d##D##SUFFIX(TensorArg<3> q, PartitionArg<3> out, PagedCache c, PagedPlan p) { \
+    Paged<T, MX, D, 4>::template run<FEW>(q, out, c, p);                                                                                                                   \
+  }
+#define ATTENTION_D(NAME, T, MX)                                                                                                                                    \
+  ATTENTION(NAME, T, MX, 64) ATTENTION(NAME, T, MX, 128) ATTENTION(NAME, T, MX, 256)                                                                                \
+  ATTENTION_FEW(NAME, T, MX, 64, 16, _few) ATTENTION_FEW(NAME, T, MX, 128, 16, _few) ATTENTION_FEW(NAME, T, MX, 256, 16, _few)                                      \
+  ATTENTION_FEW(NAME, T, MX, 64, 32, _few32) ATTENTION_FEW(NAME, T, MX, 128, 32, _few32)
 ATTENTION_D(f16, _Float16, false)
 ATTENTION_D(bf16, __bf16, false)
 ATTENTION_D(f16_mxfp8, _Float16, true)

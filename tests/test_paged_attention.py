@@ -69,7 +69,7 @@ def test_null_arguments_of_the_c_entry(fake_hip):
             assert fn(None, *[None if j == i else b for j, b in enumerate(list_)], None) == -2, i
 
 
-@pytest.mark.parametrize("image,entries", [("pagedcache", 24), ("pagedattention", 24), ("logits", 9)])
+@pytest.mark.parametrize("image,entries", [("pagedcache", 24), ("pagedattention", 32), ("logits", 9)])
 def test_lds_bytes_and_registers(fake_hip, image, entries):
     """LDS of the code objects is what the table says"""
     import os
@@ -142,6 +142,19 @@ def test_gpu_attention(ct, dev, dtype, mx, heads, group, d, page, layout, new, h
 def test_gpu_sliding_window(ct, dev, mx, window, group, d):
     b = Batch([1, 6, 90, 200], [400, 333, 90, 500], 16, seed=window)
     check(ct, dev, b, *problem(b, 2, group, d, "f16", mx, dev), d, window=window, max_new=200, max_context=500)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 70])
+def test_gpu_drafts_of_a_few_tokens(ct, dev, dtype, mx, d, window):
+    """up to 32 rows to every sequence, behind short and long contexts; the same bits every time"""
+    b = Batch([7, 3, 0, 1, 8], [2900, 30, 0, 700, 8], 16, seed=12, rows=21)
+    p = problem(b, 2, 4, d, dtype, mx, dev)
+    out = check(ct, dev, b, *p, d, window=window, max_new=8, max_context=2900)
+    assert torch.equal(out, check(ct, dev, b, *p, d, window=window, max_new=8, max_context=2900))
 
 
 @pytest.mark.gpu
@@ -265,7 +278,8 @@ def test_gpu_what_a_row_does_not_see(ct, dev, dtype, mx, new, held, group, windo
 @pytest.mark.gpu
 @pytest.mark.parametrize("mx", [False, True])
 @pytest.mark.parametrize("new,held,group,window,d,page", [([300], [300], 1, 0, 128, 16), ([100], [700], 8, 0, 128, 16), ([200], [900], 2, 333, 128, 16), ([200], [900], 2, 333, 128, 7),
-                                                          ([200], [900], 2, 333, 64, 16), ([130], [700], 2, 90, 256, 16), ([130], [700], 2, 90, 256, 7), ([9], [600], 1, 100, 256, 16)])
+                                                          ([200], [900], 2, 333, 64, 16), ([130], [700], 2, 90, 256, 16), ([130], [700], 2, 90, 256, 7), ([9], [600], 1, 100, 256, 16), ([8], [300], 4, 100, 128, 16),
+                                                          ([30], [300], 1, 40, 64, 7)])
 def test_gpu_what_a_row_of_a_larger_tile_does_not_see(ct, dev, mx, new, held, group, window, d, page):
     unseen(ct, dev, "f16", mx, new, held, group, window, d, page)
 

@@ -3711,17 +3711,20 @@ cutile_status_t check_paged(const char* fn, const cutile_tensor_arg_t& rows, con
 struct CacheRows {
   void *k, *v;
   int64_t k_token, k_head, v_token, v_head;
+  int32_t per_wave = 1, pad = 0;
 };
 CacheRows cache_rows(const cutile_tensor_arg_t& k, const cutile_tensor_arg_t& v) {
   return {k.ptr, v.ptr, 2 * (int64_t)k.strides[0], 2 * (int64_t)k.strides[1], 2 * (int64_t)v.strides[0], 2 * (int64_t)v.strides[1]};
 }
-cutile_status_t launch_paged_cache(const char* fn, cutile_stream_t stream, const PagedLaunch& l, const CacheRows& rows, const cutile_launch_opts_t* opts) {
+cutile_status_t launch_paged_cache(const char* fn, cutile_stream_t stream, const PagedLaunch& l, CacheRows rows, const cutile_launch_opts_t* opts) {
   Resolved res;
   if (cutile_status_t s = resolve_entry(fn, opts, l.variant, {l.variant}, &res)) return s;
+  // A wavefront to a token, or to several short ones (less than 256 units of K and V) while the chip stays full: it spends most of its time on finding them.
+  while (rows.per_wave < 16 && (int64_t)rows.per_wave * 2 * l.c.heads * (l.d / 8) < 256 && l.c.tokens / (2 * rows.per_wave) >= 8192) rows.per_wave *= 2;
   ArgPacker args;
   args.push_val<PagedCache>(l.c);
   args.push_val<CacheRows>(rows);
-  const uint32_t grid[3] = {div_up((uint64_t)l.c.tokens, 4), 1, 1};   // a wavefront to a token
+  const uint32_t grid[3] = {div_up((uint64_t)l.c.tokens, 4 * (uint64_t)rows.per_wave), 1, 1};
   return launch_packed(res.fn, grid, res.entry->block, 0, stream, args);
 }
 

@@ -237,6 +237,32 @@ def test_gpu_many_sequences(ct, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [20000, 70000, 140000])
+@pytest.mark.parametrize("heads,d", [(1, 64), (3, 64), (1, 128)])
+def test_gpu_many_short_tokens(ct, dev, tokens, heads, d):
+    """wavefronts that take several tokens each, of one sequence, of many, and with more than 64 empty ones between them"""
+    new = [(i * 7) % 13 for i in range(500)] + [0] * 150 + [1] * 70 + [tokens] + [0, 0, 5]
+    b = Batch(new, [x + i % 3 for i, x in enumerate(new)], 64, seed=tokens, rows=sum(new) + 7)
+    x = b.normal(b.rows, heads, d).half()
+    for mx in (False, True):
+        k, v, scales = caches(b, heads, d, "f16", mx, dev)
+        ct.paged_cache_write(x.to(dev), (-x).to(dev), k, v, *b.where(dev), **scales)
+        places = b.places()
+        at, r = (torch.tensor([p[i] for p in places]) for i in (3, 4))
+        want = x[:len(places)]
+        if mx:
+            data, byte = ref.quantized(want)
+            assert torch.equal(k.cpu().view(torch.uint8)[at, r], data) and torch.equal(scales["k_scales"].cpu().view(torch.uint8)[at, r], byte)
+            want = ref.values(data, byte).half()
+        else:
+            assert torch.equal(k.cpu()[at, r], want) and torch.equal(v.cpu()[at, r], -want)
+        out = torch.full((2, b.rows, heads, d), 9.0, dtype=torch.half, device=dev)
+        ct.paged_cache_read(k, v, *b.where(dev), ct.partition(out[0], [4, heads, d]), ct.partition(out[1], [4, heads, d]), **scales)
+        got = out.cpu()
+        assert torch.equal(got[0, :len(places)], want) and torch.equal(got[1, :len(places)], -want) and bool((got[:, len(places):] == 9.0).all())
+
+
+@pytest.mark.gpu
 def test_gpu_offsets_beyond_32_bits(ct, dev):
     """a cache of 6 GiB whose last pages are used: byte and element offsets pass 2^32"""
     pages, page, heads, d = 3 * 2 ** 12, 64, 16, 256

@@ -375,9 +375,12 @@ struct Paged {
     return mx;
   }
   // The row's reference point, `mx` being the lane's highest new score.  It only has to bound the exponents: it moves when a row's maximum has risen by more than kSlack.
+  // Weights are held 2^kLift times what they are against it, and so are O and their sum.  bf16 has the range of f32.  f16's ends at 2^16, and below 2^-14 its steps are 2^-24: lifted to
+  // 2^15 at most, a weight is rounded like the others down to 2^-25 of the reference point and off by 2^-36 of it beyond (without the lift 2^-14 and 2^-25: 40000 keys of 2^-26 of the
+  // largest each, 6 parts in 10000 of the row together, were lost).  A slack of 4 takes no longer than one of 8, whose lift would be 7: prompt of 8192 in f16 626 us against 627; 2: 631.
+  static constexpr float kSlack = std::is_same<T, _Float16>::value ? 4.0f : 8.0f, kLift = std::is_same<T, _Float16>::value ? 15.0f - kSlack : 0.0f;
   template <int X>
   __device__ static __forceinline__ void move(Rows<X>& w, float mx, float c) {
-    constexpr float kSlack = 8.0f;
     const float to = fmaxf(w.m, Shape<T, D, X>::most(mx) * c);
     if (__builtin_amdgcn_ballot_w64(to > w.m + kSlack) == 0) return;
     const float alpha = __builtin_amdgcn_exp2f(w.m - (to == -INFINITY ? 0.0f : to));
@@ -391,7 +394,8 @@ struct Paged {
   __device__ static __forceinline__ void here(U& x) {
     asm volatile("" : "+v"(x));
   }
-  // P in 16 bits, as V is: the weights' rounding stays below that of V, and their sum is that of the rounded ones.  All at once, or a part at a time (m of `of`).
+  // P in 16 bits, as V is: the weights' rounding stays below that of V (f16 weights below its normal range: move()), and their sum is that of the rounded ones.  All at once, or a
+  // part at a time (m of `of`).
   template <int X, int B>
   struct Exponentials {
     using H = Shape<T, D, X>;
@@ -403,7 +407,7 @@ struct Paged {
     float sum[2];
     u32x4 p[B][H::kSteps];
     __device__ __forceinline__ Exponentials(Rows<X>& rows, float (&scores)[B][H::kScores], vec8 (&weights)[B][H::kSteps], float scale)
-        : w(rows), s(scores), pf(weights), c(scale), m(rows.m == -INFINITY ? 0.0f : rows.m) {   // (nothing seen so far: keep exp2 finite)
+        : w(rows), s(scores), pf(weights), c(scale), m((rows.m == -INFINITY ? 0.0f : rows.m) - kLift) {   // (nothing seen so far: keep exp2 finite)
       sum[0] = w.l, sum[1] = 0.0f;
     }
     __device__ __forceinline__ void raise(int i) {

@@ -824,8 +824,8 @@ cutile_status_t cutile_launch_paged_cache_read(cutile_stream_t stream, const cut
 /* paged_attention: out[i, h, :] = sum_j softmax_j(qk_scale q[i, h, :] . k_j) v_j over the keys j of the sequence's KV head h / group, p - window < j <= p (window 0: all up to
  * p), p the position of token i, group = q heads / kv_heads; q, out [tokens, q_heads, D], unit inner stride, rows on 16-byte boundaries, out partitioned [BM, G, D].  One token a
  * sequence is a decode step, several a chunk of a prompt or a draft to be checked; a launch may hold all of them.  A row that sees no key is zeros; what a row does not see, NaN
- * and infinities included, is nothing to it.  Softmax and sums in f32, the weights rounded to q's type for the second product.  Values of an mxfp8 cache have to be in the range of
- * q's type.
+ * and infinities included, is nothing to it.  Softmax and sums in f32, the weights rounded to q's type for the second product, f16 ones
+ * below 2^-25 of the largest to a multiple of 2^-35 of it or less.  Values of an mxfp8 cache have to be in the range of q's type.
  * max_new: at least the most new tokens of a sequence, 0: not known; rows of a sequence beyond it are not promised.  max_context: about the longest of context_lens, 0: not known;
  * it only decides how keys are dealt out.
  * workspace: NULL, or device memory of the caller's (a contiguous tensor, 16-byte aligned, zeros before its first use; 40 MiB + 16 KiB are the most that is used) for

@@ -532,6 +532,9 @@ std::vector<KernelEntry> build_table() {
         // launches whose tiles have up to 16 or 32 rows: K and V of 32 keys for each of four wavefronts
         add("paged_attention", keep(v + "+few"), keep("paged_attention_entry__" + v + "_few"), IMG_PAGED_ATTENTION, 256, (uint32_t)(4 * 32 * (4 * d + 48) + (d == 256 ? 1156 : 1220)), 16, 0, d, 0, dt, 0, 3);
         if (d < 256) add("paged_attention", keep(v + "+few32"), keep("paged_attention_entry__" + v + "_few32"), IMG_PAGED_ATTENTION, 256, (uint32_t)(4 * 32 * (4 * d + 48) + 1220), 32, 0, d, 0, dt, 0, 3);
+        // the first of them with the rows of its larger tiles fixed
+        for (int rows = d == 256 ? 128 : 256; rows >= 32; rows /= 2)
+          add("paged_attention", keep(v + "_rows" + std::to_string(rows)), keep("paged_attention_entry__" + v), IMG_PAGED_ATTENTION, 512, (uint32_t)((d == 256 ? 4 : 8) * 32 * (4 * d + 48) + (d == 256 ? 2444 : 2700)), rows, 0, d, 0, dt, 0, 3);
       }
   // ---- logits in front of the choice of a token (512 threads; tile = (-, columns of a workgroup, -, -)) ----
   for (const char* dt : {"f16", "bf16", "f32"})

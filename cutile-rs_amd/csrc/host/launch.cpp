@@ -3832,7 +3832,15 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     room = std::min<int64_t>(bytes - counters, kSplitPartialBytes);
   }
   Resolved res;
-  if (cutile_status_t s = resolve_entry(fn, opts, l.variant, {l.variant}, &res)) return s;
+  auto fitting = [&](auto f) {
+    if (f(l.variant.c_str())) return true;
+    for (int rows = d == 256 ? 128 : 256; rows >= 32; rows /= 2)
+      if (f((l.variant + "_rows" + num(rows)).c_str())) return true;
+    return false;
+  };
+  if (cutile_status_t s = resolve_among(fn, opts, l.variant, fitting, &res)) return s;
+  const KernelEntry* const family = find_entry(fn, l.variant);
+  const bool fixed = res.entry != family;   // a variant that says how many rows the larger tiles have
   int cus = 256;
   if (cutile_status_t s = current_device_units(&cus)) return s;
   const int64_t most_new = max_new ? std::min(max_new, tokens) : tokens;
@@ -3863,7 +3871,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     double soonest = 0.0;
     double step = 1.0;
     p.tile_rows = res.entry->tile[0], p.long_tiles = 0;
-    for (int64_t bm = res.entry->tile[0]; any_long && bm >= 32; bm /= 2, step *= 0.71) {
+    for (int64_t bm = res.entry->tile[0]; any_long && bm >= (fixed ? res.entry->tile[0] : 32); bm /= 2, step *= 0.71) {
       const int64_t tiles = rows / bm + batch, items = (rows + bm - 1) / bm * heads, seen = seen_by(bm);
       Deal deal;
       if (may_share && tiles * heads + few_items <= (int64_t)kSplitCounters) deal = deal_keys(items, seen, cus, 256, std::max<int64_t>(1, left / long_bytes));
@@ -3884,8 +3892,11 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     ws = split_workspace(res.device, (hipStream_t)stream);
     if (!ws.partials) plan(false);
   }
-  if (few)
-    if (cutile_status_t s = use_member(&res, member_of(res.entry, most_new * group <= 16 ? "+few" : "+few32"))) return s;
+  if (few) {
+    if (cutile_status_t s = use_member(&res, member_of(family, most_new * group <= 16 ? "+few" : "+few32"))) return s;
+  } else if (any_long && !fixed) {   // (the same kernel: its name tells what the rule has chosen)
+    if (cutile_status_t s = use_member(&res, find_entry(fn, l.variant + "_rows" + num(p.tile_rows)))) return s;
+  }
   p.partials = ws.partials, p.counters = ws.counters;
   const uint64_t items = (uint64_t)p.long_tiles * p.long_shares + (p.few_rows ? (uint64_t)batch * p.few_shares : 0);
   CUTILE_REQUIRE(items * heads <= 0x7fffffffull / 512, CUTILE_ERR_KERNEL_LAUNCH, "%s: %llu tiles do not fit a launch grid axis", fn, (unsigned long long)(items * heads));

@@ -828,6 +828,8 @@ cutile_status_t cutile_launch_paged_cache_read(cutile_stream_t stream, const cut
  * below 2^-25 of the largest to a multiple of 2^-35 of it or less.  Values of an mxfp8 cache have to be in the range of q's type.
  * max_new: at least the most new tokens of a sequence, 0: not known; rows of a sequence beyond it are not promised.  max_context: about the longest of context_lens, 0: not known;
  * it only decides how keys are dealt out.
+ * Variants: "<types>_d<D>", whose launches choose how many rows (pairs of a token and a head of the group) a tile of a sequence with more than 32 of them has, or "<types>_d<D>_rows<n>"
+ * with n = 32, 64, 128 or, below D = 256, 256 of them; cutile_last_resolved_kernel has the choice as the tile's first number.
  * workspace: NULL, or device memory of the caller's (a contiguous tensor, 16-byte aligned, zeros before its first use; 40 MiB + 16 KiB are the most that is used) for
  * the results of workgroups that share the keys of a tile.  One workspace serves one stream at a time; every launch leaves it fit for the next.  Without it the stream's own is
  * taken, and a launch that is captured, for which there is none, runs unshared: much slower where few sequences have long contexts, in another order of summation. */

@@ -292,6 +292,7 @@ struct Paged {
     vec8 q[D / H::kInner];
     typename H::Acc o[D / H::kOuter];
     float m, l;               // of the lane's row; l of the lane's share of the keys
+    float limit;              // of the row's scores: m moves where one is above it
     int32_t lo, hi;           // keys the lane's row sees
     int32_t all_lo, all_hi;   // that every row of the wavefront sees
     int32_t any_lo, any_hi;   // that one of them sees
@@ -318,7 +319,7 @@ struct Paged {
     w.lo = low(pos), w.hi = min(pos, t.k1 - 1);
     w.any_lo = low(first), w.all_lo = low(last);
     w.all_hi = min(first, t.k1 - 1), w.any_hi = min(last, t.k1 - 1);
-    w.m = -INFINITY, w.l = 0.0f, w.missed = 0;
+    w.m = w.limit = -INFINITY, w.l = 0.0f, w.missed = 0;
 #pragma unroll
     for (auto& o : w.o) o = typename H::Acc{};
   }
@@ -379,15 +380,19 @@ struct Paged {
   // 2^15 at most, a weight is rounded like the others down to 2^-25 of the reference point and off by 2^-36 of it beyond (without the lift 2^-14 and 2^-25: 40000 keys of 2^-26 of the
   // largest each, 6 parts in 10000 of the row together, were lost).  A slack of 4 takes no longer than one of 8, whose lift would be 7: prompt of 8192 in f16 626 us against 627; 2: 631.
   static constexpr float kSlack = std::is_same<T, _Float16>::value ? 4.0f : 8.0f, kLift = std::is_same<T, _Float16>::value ? 15.0f - kSlack : 0.0f;
+  // What the three roundings between a score and its exponent (the point's own, its lift, the limit) add stays below 2^-22 of the point; of f16, where 2^16 is too much, twice that is left
+  // free above the point and below the limit, up to 2^25 (scores beyond are not told apart by f32 anyway).
   template <int X>
   __device__ static __forceinline__ void move(Rows<X>& w, float mx, float c) {
-    const float to = fmaxf(w.m, Shape<T, D, X>::most(mx) * c);
-    if (__builtin_amdgcn_ballot_w64(to > w.m + kSlack) == 0) return;
+    const float top = Shape<T, D, X>::most(mx) * c;
+    if (__builtin_amdgcn_ballot_w64(top > w.limit) == 0) return;
+    auto free = [](float point) { return kLift > 0.0f ? fminf(fabsf(point) * 0x1p-21f, 16.0f) : 0.0f; };
+    const float to = top > w.m ? top + free(top) : w.m;
     const float alpha = __builtin_amdgcn_exp2f(w.m - (to == -INFINITY ? 0.0f : to));
     w.l *= alpha;
 #pragma unroll
     for (auto& o : w.o) o *= alpha;
-    w.m = to;
+    w.m = to, w.limit = to + (kSlack - free(to));
   }
   // Keeps the compiler from moving the making of x behind this place.
   template <typename U>

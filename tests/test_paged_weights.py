@@ -101,3 +101,35 @@ def test_gpu_scores_that_rise_from_key_to_key(ct, dev, d, rise):
             parts = ref.attention(b, q, kx.half().double(), vx.double(), float(torch.tensor(scale, dtype=torch.float32)))
             off = (out.cpu().double() - parts[0]).abs() / bound(q.dtype, parts, d, held)
             assert bool((off <= 1.0).all()), float(off.nan_to_num(1e9).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("log_score", [16, 20, 23, 24, 25])
+def test_gpu_scores_of_any_magnitude(ct, dev, dtype, d, log_score):
+    """scores of 2^16 to 2^25 (log2 units), all alike or rising by a little from block to block: what f32 leaves of their differences decides, but every output is a mean of values"""
+    held = 640
+    b = Batch([40, 1], [held, held], 16, seed=d)
+    q = torch.zeros(41, 1, d).to(TYPES[dtype])
+    q[..., 0], q[..., 1] = 1024.0, 1.0
+    k, v, _ = caches(b, 1, d, dtype, False, dev)
+    kx, vx = torch.zeros(b.pages, 16, 1, d), (2.0 + b.normal(b.pages, 16, 1, d).clamp(-1, 1)).to(TYPES[dtype])
+    v.copy_(vx)
+    p = torch.arange(held)
+    for i, rise in enumerate([0.0] + [0.25, 0.125, 0.0625, 0.03125] * 4):
+        kx[..., 0] = 1024.0
+        for s in range(2):
+            kx[b.table[s].long()[p // 16], p % 16, 0, 1] = (p // 32).float() * rise
+        k.copy_(kx.to(TYPES[dtype]))
+        for sign in (1.0, -1.0):
+            scale = sign * math.log(2.0) * 2.0 ** (log_score - 20) * (1 + i / 17)
+            out = torch.full_like(q, 9.0).to(dev)
+            ct.paged_attention(q.to(dev), k, v, *b.where(dev), ct.partition(out, [1, 1, d]), scale, max_new=40, max_context=held)
+            got = out.cpu().double()
+            assert bool(((got >= 1.0 - 2.0 ** -8) & (got <= 3.0 + 3 * 2.0 ** -8)).all()), (rise, scale, got.min(), got.max())
+            if rise == 0.0:   # equal scores, whatever they are rounded to: the mean, with weights of no error but that of f32 sums
+                for row, s, at, _, _ in b.places():
+                    mean = vx[b.table[s].long()[p[:at + 1] // 16], p[:at + 1] % 16, 0].double().mean(0)
+                    u = 2.0 ** -11 if dtype == "f16" else 2.0 ** -8
+                    assert bool(((got[row, 0] - mean).abs() <= u * mean + (held / 16 + 64) * 2.0 ** -24 * 3).all()), (row, scale)

@@ -932,8 +932,8 @@ struct Paged {
     t.pos0 = s.position(0);
     t.pages = c.table + (int64_t)b * c.table_row;
     const int32_t first = t.pos0 + t.row0 / p.group, last = t.pos0 + (t.row0 + t.rows - 1) / p.group;
-    // (larger tiles start on a multiple of 64: whole groups of rows)
-    const int32_t seen = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, lo = t.rows > 16 ? seen & ~63 : seen, hi = max(min(last + 1, s.held), lo);
+    // (larger tiles start on a multiple of 64: whole groups of rows; rows whose window lies behind the table have no keys there, and no arithmetic next to 2^31)
+    const int32_t seen = p.window > 0 && first >= p.window ? first - p.window + 1 : 0, hi = max(min(last + 1, s.held), 0), lo = min(t.rows > 16 ? seen & ~63 : seen, hi);
     // as many shares as it takes, as even as steps of all wavefronts allow
     const int32_t span = hi - lo, step = t.rows <= kMostOwn ? kOwners * 32 : 64, wanted = (int32_t)min(((uint32_t)span + keys_each - 1) / keys_each, most);
     const int32_t each = max((span + wanted - 1) / max(wanted, 1) + step - 1, step) / step * step;

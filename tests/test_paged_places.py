@@ -1,0 +1,36 @@
+"""paged_attention on metadata that leaves the table: which keys there are, and what a row sees of them, as cutile_hip.h has it."""
+import pytest
+import torch
+
+import paged_ref as ref
+from paged_ref import Batch
+from test_paged_attention import problem
+from test_paged_tiles import TILES, name
+from test_paged_weights import bound
+
+
+def compare(ct, dev, b, held, heads, group, d, mx, window, wrong_pages=()):
+    """launches for lengths `held` on b's table, in tiles of every number of rows, against 64 bits"""
+    q, k, v, scales, real = problem(b, heads, group, d, "f16", mx, dev)
+    b.held, b.lens = held, torch.tensor(held, dtype=torch.int32)
+    for at, page in wrong_pages:
+        b.table[at] = page
+    parts = ref.attention(b, q, *real, float(torch.tensor(d ** -0.5, dtype=torch.float32)), window)
+    tol = bound(q.dtype, parts, d, b.table.shape[1] * b.page)
+    for rows in (None, *TILES[d]):
+        for kw in ({}, {"max_new": max(b.new), "max_context": 64}):
+            out = torch.full_like(q, 9.0).to(dev)
+            ct.paged_attention(q.to(dev), k, v, *b.where(dev), ct.partition(out, [1, 1, d]), d ** -0.5, window=window, variant=rows and name("f16", mx, d, rows), **scales, **kw)
+            assert bool(((out.cpu().double() - parts[0]).abs() <= tol).all()), (rows, kw)
+    return parts[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("d,group", [(64, 1), (128, 4), (256, 2)])
+@pytest.mark.parametrize("window", [1, 40, 1000, 2 ** 31 - 1])
+def test_gpu_windows_at_the_largest_lengths(ct, dev, mx, d, group, window):
+    """rows at positions next to 2^31, whose window lies behind the table or reaches into it"""
+    b = Batch([3, 1, 50, 40], [64] * 4, 16, table_pages=4, seed=d)
+    want = compare(ct, dev, b, [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 1, 1040], 2, group, d, mx, window)
+    assert bool((want[:54] == 0).all()) == (window < 2 ** 31 - 1)

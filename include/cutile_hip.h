@@ -808,7 +808,8 @@ cutile_status_t cutile_launch_linear_tile_mxfp4(cutile_stream_t stream, const cu
  *                     are)
  *   context_lens      [B] i32: tokens of the sequence with the new ones, which are the last: new token i stands at position context_lens[b] - (starts[b+1] - starts[b]) + i
  * Their contents are device memory that a launch does not look at on the host, so a captured launch takes new ones at every replay.  A position before 0 or behind the
- * table, and a page that the cache does not have (-1, say), is not written, reads as zeros and is never touched.  Sequences may share pages that a launch only reads. */
+ * table, and a page that the cache does not have (-1, say), is not written, reads as zeros and is never touched (what attention makes of them stands there).  Sequences may share
+ * pages that a launch only reads. */
 /* paged_cache_write: the rows of new_k, new_v [tokens, kv_heads, D] (unit inner stride, rows on 16-byte boundaries) to their places; mxfp8 rounds them as block_quantize
  * does.  Two tokens of one launch must not have the same place. */
 cutile_status_t cutile_launch_paged_cache_write(cutile_stream_t stream, const cutile_tensor_arg_t* new_k, const cutile_tensor_arg_t* new_v,
@@ -824,7 +825,8 @@ cutile_status_t cutile_launch_paged_cache_read(cutile_stream_t stream, const cut
 /* paged_attention: out[i, h, :] = sum_j softmax_j(qk_scale q[i, h, :] . k_j) v_j over the keys j of the sequence's KV head h / group, p - window < j <= p (window 0: all up to
  * p), p the position of token i, group = q heads / kv_heads; q, out [tokens, q_heads, D], unit inner stride, rows on 16-byte boundaries, out partitioned [BM, G, D].  One token a
  * sequence is a decode step, several a chunk of a prompt or a draft to be checked; a launch may hold all of them.  A row that sees no key is zeros; what a row does not see, NaN
- * and infinities included, is nothing to it.  Softmax and sums in f32, the weights rounded to q's type for the second product, f16 ones
+ * and infinities included, is nothing to it.  Keys are positions from 0 to the end of the context or of the table: a row in front of position 0 sees none, one behind the table those in
+ * front of its end that its window reaches; the rows of a page that the cache does not have are keys and values of zeros, which count.  Softmax and sums in f32, the weights rounded to q's type for the second product, f16 ones
  * below 2^-25 of the largest to a multiple of 2^-35 of it or less.  Values of an mxfp8 cache have to be in the range of q's type.
  * max_new: at least the most new tokens of a sequence, 0: not known; rows of a sequence beyond it are not promised.  max_context: about the longest of context_lens, 0: not known;
  * it only decides how keys are dealt out.

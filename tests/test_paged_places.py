@@ -34,3 +34,16 @@ def test_gpu_windows_at_the_largest_lengths(ct, dev, mx, d, group, window):
     b = Batch([3, 1, 50, 40], [64] * 4, 16, table_pages=4, seed=d)
     want = compare(ct, dev, b, [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 1, 1040], 2, group, d, mx, window)
     assert bool((want[:54] == 0).all()) == (window < 2 ** 31 - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("d,group", [(64, 1), (128, 4), (256, 2)])
+@pytest.mark.parametrize("window", [0, 3, 40])
+def test_gpu_lengths_that_leave_the_table(ct, dev, mx, d, group, window):
+    """keys behind the table do not exist: rows behind it attend to those in front of its end that their window reaches; rows in front of position 0 are zeros; a page that
+    the cache lacks holds zeros, which count"""
+    b = Batch([2, 50, 4, 60, 1, 3], [64, 64, 64, 64, 40, 64], 16, table_pages=4, seed=window + d)
+    want = compare(ct, dev, b, [66, 90, 2, 30, -7, 2 ** 31 - 1], 2, group, d, mx, window, [((0, 2), -1), ((1, 0), b.pages)])   # (the third and fourth have fewer tokens than new ones)
+    assert bool((want[52:54] == 0).all()) and bool((want[54:56] != 0).all()) and bool((want[56:86] == 0).all()) and bool((want[116] == 0).all())
+    assert bool((want[117:] == 0).all()) == (window > 0) and bool((want[0] != 0).all())

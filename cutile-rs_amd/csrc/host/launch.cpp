@@ -3813,7 +3813,7 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
   CUTILE_REQUIRE(ot.dtype == q->dtype && same_shape(ot, *q) && out->partition_shape[2] == d, CUTILE_ERR_KERNEL_LAUNCH,
                  "%s: out must be q's shape [%d, %d, %d] and type, partitioned [BM, G, %d]", fn, q->shape[0], q->shape[1], d, d);
   CUTILE_REQUIRE(window >= 0 && max_new >= 0 && max_context >= 0, CUTILE_ERR_KERNEL_LAUNCH, "%s: window, max_new and max_context must not be negative", fn);
-  CUTILE_REQUIRE(std::isfinite(qk_scale), CUTILE_ERR_KERNEL_LAUNCH, "%s: qk_scale must be a finite number", fn);
+  CUTILE_REQUIRE(std::isfinite(qk_scale * 1.4426950408889634f), CUTILE_ERR_KERNEL_LAUNCH, "%s: qk_scale must be a finite number, and so 1.4427 times it in f32", fn);
   CUTILE_REQUIRE((int64_t)tokens * group <= INT32_MAX - 256, CUTILE_ERR_KERNEL_LAUNCH, "%s: %d tokens of %d heads to a KV head are too many", fn, tokens, group);
   if (cutile_status_t s = check_rows_aligned(fn, "q", *q)) return s;
   if (cutile_status_t s = check_rows_aligned(fn, "out", ot)) return s;

@@ -6,7 +6,8 @@ import torch
 
 import paged_ref as ref
 from paged_ref import TYPES, Batch
-from test_paged_cache import caches
+from test_paged_attention import attend
+from test_paged_cache import args, caches
 
 LIFT = 11   # f16 weights are held 2^11 times what they are against the row's reference point (paged_attention.hip)
 
@@ -55,6 +56,21 @@ def one_key_above_many(ct, dev, dtype, mx, d, new, held, at, gap, group=1, page=
     return out
 
 
+# ---- without a GPU --------------------------------------------------------------------------------------------------------
+def test_scales_that_f32_does_not_hold(fake_hip):
+    """scores are taken in units of log 2: the scale times 1.4427 has to be a number of f32 as well"""
+    ct, t = fake_hip, args()
+    n0 = ct.lib().cutile_testing_launch_count()
+    for scale in (2.4e38, -2.4e38, 3.4e38, float("inf"), float("nan")):
+        with pytest.raises(ct.CutileError, match="finite number"):
+            attend(ct, t, scale=scale)
+    assert ct.lib().cutile_testing_launch_count() == n0
+    for scale in (2.3e38, -2.3e38, 1e-45, 0.0):
+        attend(ct, t, scale=scale)
+    assert ct.lib().cutile_testing_launch_count() == n0 + 4
+
+
+# ---- on a GPU ---------------------------------------------------------------------------------------------------------------
 GAPS = [12.0, 15.0, 17.4, 17.6, 20.3, 22.0, 22.6, 24.5, 26.0, 30.0]
 
 

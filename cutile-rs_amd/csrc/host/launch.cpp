@@ -3860,10 +3860,14 @@ cutile_status_t cutile_launch_paged_attention(cutile_stream_t stream, const cuti
     Deal of_long, of_few;
     auto seen_by = [&](int64_t bm) { return window ? std::min<int64_t>(context, window + bm / group) : context; };   // keys that a tile of so many rows sees
     // A workgroup to a CU, or two where sequences of different lengths are all there is and the small kernel has room for them: 24 ragged sequences of up to 6000 tokens
-    // 39 us against 52, 20 of 8192 87 against 103; a single sequence of 16000 takes 21 us against 17 that way, all else the merging of more shares.  Shares of
+    // 39 us against 52, 20 of 8192 87 against 103; a single sequence of 16000 takes 21 us against 17 that way, all else the merging of more shares.  At D = 256 a CU holds one: with one to a
+    // CU where that comes out even (a sixteenth over at most) 16 x 2000 of eight heads take 35 us and 46 with two, 20 x 8192 of one head in mxfp8 23 and 31; where it does not, half of a second
+    // round is empty and finer shares fill it: 9 x 6000 of eight heads 81 and 65, 25 x 3000 87 and 76.  Shares of
     // at least 512 keys of 64 values (16 sequences of 500 tokens 8.2 us, 10.5 of 256 keys), 256 of 128 and 128 of 256 (4 sequences of 500 12.3, 15.1 and 19.9 of 256 and 512).
+    const bool even = few_items && (cus + few_items - 1) / few_items * few_items <= cus + cus / 16;
+    const int64_t wanted = few && batch > 1 && !(d == 256 && even) ? 2 * cus : cus;
     if (may_share && few_items && few_items <= (int64_t)kSplitCounters)
-      of_few = deal_keys(few_items, seen_by(32), few && batch > 1 ? 2 * cus : cus, 32768 / d, std::max<int64_t>(1, (any_long ? room / 4 : room) / few_bytes));
+      of_few = deal_keys(few_items, seen_by(32), wanted, 32768 / d, std::max<int64_t>(1, (any_long ? room / 4 : room) / few_bytes));
     const int64_t left = room - (of_few.shares > 1 ? of_few.shares * few_bytes : 0);
     // Rows of a tile and shares of its keys: what is done soonest by a count of steps of 64 keys.  A step of half as many rows takes 0.7 of the time, then 0.5 and 0.38 (the
     // prompt of 8192 tokens 578, 784, 1107 and 1728 us in tiles of 256, 128, 64 and 32 rows); adding shares up, a step's time for every 16 reads of a thread.  672 rows behind

@@ -88,6 +88,18 @@ def test_rows_that_the_caller_fixes(fake_hip, d, mx):
         ct.check(ct.lib().cutile_kernel_set_preferred_variant(b"paged_attention", None))
 
 
+@pytest.mark.parametrize("heads,d,batch,context,shares", [(8, 256, 16, 2000, 2), (1, 256, 20, 8192, 13), (2, 256, 45, 4000, 3), (8, 256, 9, 6000, 8), (8, 256, 25, 3000, 3), (8, 256, 40, 2000, 2), (8, 256, 1, 16000, 32),
+                                                          (8, 128, 16, 2000, 4), (8, 64, 16, 4000, 4), (4, 128, 24, 6000, 6)])
+def test_workgroups_that_share_the_keys_of_single_tokens(fake_hip, heads, d, batch, context, shares):
+    """two to a compute unit, or one where one fits (D = 256) and the tiles come out even"""
+    ct = fake_hip
+    t = args(d=d, heads=heads, pages=4)
+    q = torch.empty((batch, heads * 4, d), dtype=torch.half)
+    ints = lambda *s: torch.zeros(s, dtype=torch.int32)
+    attend(ct, t, new=q, out=q, table=ints(batch, -(-context // 16)), starts=ints(batch + 1), lens=ints(batch), max_new=1, max_context=context)
+    assert _last(ct)[0].grid[0] == heads * batch * shares
+
+
 # ---- on a GPU ---------------------------------------------------------------------------------------------------------------
 class Compared:
     """a batch's problem on the device and its outputs in 64 bits, for launches of different tiles"""

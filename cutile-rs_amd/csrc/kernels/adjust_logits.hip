@@ -5,8 +5,9 @@
 // A workgroup takes C columns of a row: it counts the row's tokens that fall on them in LDS (integers, so their order is nothing to the result) while its
 // logits are on the way, then reads the counts beside them.  HBM bounds many rows (every logit once in, once out), the two dependent loads (length, tokens)
 // one row.  Every workgroup of a row reads all of its tokens, so wide ones read less and narrow ones are more: 256 rows of 128256 bf16 logits behind 6000
-// tokens take 34 us (4.1 TB/s) with C = 8192, 45 with 4096, 108 with 1024; 16 rows 6.8, 6.2 and 9.8; one row 6.4, 5.5 and 5.3.  16384 columns leave a CU two
-// workgroups, whose loads do not cover their counting: 43 us.  With the workgroups of a row on all XCDs its tokens come from HBM eight times: 65 us that way.
+// tokens take 34 to 36 us (3.9 TB/s) with C = 8192, 40 where their tensors are new to the caches, 45 with 4096, 109 with 1024; 16 rows 6.5, 6.1 and 9.9; one row 6.0, 5.1 and 4.9.  Before units with nothing
+// to change were left alone, 16384 columns, which leave a CU two workgroups whose loads do not cover their counting, took 43 us, and the workgroups of a row on all XCDs, where its tokens
+// come from HBM eight times, 65.  Vector issue bounds long histories (69 % of the cycles): nearly every wavefront's columns hold a token of the row, and all of them go through the penalties.
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"

@@ -5,13 +5,14 @@
 // The rows of a tile are pairs (token, query head of one KV head), token by token: group heads share every key that is read, and a decode step of 8 heads or a
 // chunk of 4 tokens fill the columns of a matrix instruction.  S^T = K Q^T and O^T = V^T P^T, so that a lane owns one row and what it holds of P^T is its operand
 // of the second product; the softmax keeps a running reference point and sum of each row, in 32 bits.
-//  * Tiles of up to 32 rows (decode, drafts; 16 at D = 256): every wavefront has all rows, 16 or 32, and keys of its own, 32 at a time, through registers into LDS that
-//    no other wavefront reads: no barrier in the loop.  HBM's rate bounds it: 1 x 131072 tokens, 8 KV heads, bf16, 91 us (5.9 TB/s).  A launch that has no other tiles
-//    runs a kernel of four wavefronts (two workgroups on a CU), others have eight.  Drafts of 8 tokens of 4 heads behind 64 x 8192 mxfp8 tokens take 175 us so, and 321
-//    where the wavefronts share their keys and a barrier a step.
+//  * Tiles of up to 32 rows (decode, drafts): every wavefront has all rows, 16 or 32, and keys of its own, 32 at a time, through registers into LDS that
+//    no other wavefront reads: no barrier in the loop.  HBM's rate bounds it: 1 x 131072 tokens, 8 KV heads, bf16, 92 us (5.8 TB/s).  A launch that has no other tiles
+//    runs a kernel of four wavefronts (two workgroups on a CU; one at D = 256, whose LDS holds no more), others have eight.  Drafts of 8 tokens of 4 heads behind 64 x 8192 mxfp8 tokens
+//    take 174 us so, and 321 where the wavefronts share their keys and a barrier a step.  D = 256 does this for up to 16 rows and only where there are no other tiles: eight wavefronts have no
+//    room for keys of their own, so that 17 to 32 rows, and any small tile beside larger ones, go like the larger ones, two wavefronts to 16 rows (the same drafts 604 us, of 4 tokens 309).
 //  * Larger tiles: R wavefronts side by side hold kRows rows each, W / R share the keys of a step, which all of them fetch together.  Tiles of all W hold their next
-//    scores while the exponentials of the last are made (pipelined_keys).  A prompt of 8192 tokens, 32 heads over 8, D = 128, bf16: 570 us, 960 TFLOP/s of what the
-//    rows see; the loop alone in the order scores, softmax, product 596, and with a branch around the product, which copied O, 669.
+//    scores while the exponentials of the last are made (pipelined_keys).  A prompt of 8192 tokens, 32 heads over 8, D = 128, bf16: 576 us, 954 TFLOP/s of what the
+//    rows see; where it was 570, the loop in the order scores, softmax, product took 596, and with a branch around the product, which copied O, 669.
 // At the end the partial outputs go through LDS, and where the keys of a tile are dealt to several workgroups through the launch's workspace: the one that
 // arrives last adds them up in the order of the keys, so that the order of arrival is nothing to the result.
 #include <hip/hip_runtime.h>

@@ -1,5 +1,8 @@
 """paged_attention in tiles of every number of rows that its launcher chooses from, and what the launcher chooses."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import pytest
 import torch
@@ -98,6 +101,17 @@ def test_workgroups_that_share_the_keys_of_single_tokens(fake_hip, heads, d, bat
     ints = lambda *s: torch.zeros(s, dtype=torch.int32)
     attend(ct, t, new=q, out=q, table=ints(batch, -(-context // 16)), starts=ints(batch + 1), lens=ints(batch), max_new=1, max_context=context)
     assert _last(ct)[0].grid[0] == heads * batch * shares
+
+
+@pytest.mark.parametrize("image", ["pagedcache", "pagedattention", "logits"])
+def test_no_vector_register_is_spilled(image):
+    notes = subprocess.run(["/opt/rocm/llvm/bin/llvm-readelf", "--notes", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cutile-rs_amd", "lib", image + ".hsaco")],
+                           stdout=subprocess.PIPE, text=True, check=True).stdout
+    kernels = notes.split("- .agpr_count")[1:]
+    assert kernels
+    for kernel in kernels:
+        symbol = re.search(r"\n    \.name: +(\S+)", kernel)[1]
+        assert int(re.search(r"\.vgpr_spill_count: (\d+)", kernel)[1]) == 0 and int(re.search(r"\.private_segment_fixed_size: (\d+)", kernel)[1]) == 0, symbol
 
 
 # ---- on a GPU ---------------------------------------------------------------------------------------------------------------

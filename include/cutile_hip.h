@@ -827,7 +827,7 @@ cutile_status_t cutile_launch_paged_cache_read(cutile_stream_t stream, const cut
  * sequence is a decode step, several a chunk of a prompt or a draft to be checked; a launch may hold all of them.  A row that sees no key is zeros; what a row does not see, NaN
  * and infinities included, is nothing to it.  Keys are positions from 0 to the end of the context or of the table: a row in front of position 0 sees none, one behind the
  * table those in front of its end that its window reaches; the rows of a page that the cache does not have are keys and values of zeros, which count.  qk_scale is finite, and
- * 1.4427 times it too.  Softmax and sums in f32, the weights rounded to q's type for the second product, f16 ones below 2^-25 of the largest to a multiple of 2^-35 of it or
+ * 1.4427 times it too; qk_scale q . k is below 2^25 in magnitude.  Softmax and sums in f32, the weights rounded to q's type for the second product, f16 ones below 2^-25 of the largest to a multiple of 2^-35 of it or
  * less.  Values of an mxfp8 cache are widened to q's type: they have to be in its range, and f16 rounds those below 2^-14 to multiples of 2^-24.
  * max_new: at least the most new tokens of a sequence, 0: not known; rows of a sequence beyond it are not promised.  max_context: about the longest of context_lens, 0: not known;
  * it only decides how keys are dealt out.

@@ -183,6 +183,27 @@ def test_gpu_keys_of_every_tile_dealt_out(ct, dev, d, mx, page):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("d,mx", LARGE)
+@pytest.mark.parametrize("new", [[150, 1, 0], [0, 33, 150], [2, 1, 5], [0, 0, 0]])
+def test_gpu_padded_batches(ct, dev, d, mx, new):
+    """as many rows as if every sequence had max_new tokens, which a launch may take for a batch of nothing else"""
+    most = max(*new, 1)
+    b = Batch(new, [400, 700, 200], 16, seed=d, rows=3 * most)
+    b.starts = b.starts + 2 if sum(new) + 2 <= b.rows else b.starts          # rows in front of the first that are nobody's, too
+    q, k, v, scales, real = problem(b, 2, 2, d, "f16", mx, dev)
+    first = int(b.starts[0])
+    parts = ref.attention(b, q[first:], *real, float(torch.tensor(d ** -0.5, dtype=torch.float32)))
+    tol = bound(q.dtype, parts, d, 700)
+    for rows in (None, *TILES[d]):
+        for ws in (None, torch.zeros(ct.PAGED_ATTENTION_WORKSPACE_BYTES, dtype=torch.uint8, device=dev)):
+            out = torch.full_like(q, 9.0).to(dev)
+            ct.paged_attention(q.to(dev), k, v, *b.where(dev), ct.partition(out, [1, 1, d]), d ** -0.5, max_new=most, max_context=700, workspace=ws, variant=rows and name("f16", mx, d, rows), **scales)
+            got, n = out.cpu().double(), sum(new)
+            assert bool((got[:first] == 9.0).all()) and bool((got[first + n:] == 9.0).all())
+            assert bool(((got[first:first + n] - parts[0][:n]).abs() <= tol[:n]).all()), rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,mx", LARGE)
 def test_gpu_every_tile_captured(ct, dev, d, mx):
     """replays for other contents, with eager work between them, equal the eager launch"""
     b = Batch([150, 1], [2000, 700], 16, seed=d)

@@ -47,3 +47,44 @@ def test_gpu_lengths_that_leave_the_table(ct, dev, mx, d, group, window):
     want = compare(ct, dev, b, [66, 90, 2, 30, -7, 2 ** 31 - 1], 2, group, d, mx, window, [((0, 2), -1), ((1, 0), b.pages)])   # (the third and fourth have fewer tokens than new ones)
     assert bool((want[52:54] == 0).all()) and bool((want[54:56] != 0).all()) and bool((want[56:86] == 0).all()) and bool((want[116] == 0).all())
     assert bool((want[117:] == 0).all()) == (window > 0) and bool((want[0] != 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,group", [(64, 4), (128, 4), (256, 2)])
+def test_gpu_several_streams_and_graphs_at_once(ct, dev, d, group):
+    """launches that share keys on two streams (a workspace of each stream's own) beside two graphs (one of the caller's each): the bits of each by itself"""
+    work = []
+    for i, (new, held) in enumerate([([1, 1], [9000, 4000]), ([150, 3], [5000, 2000]), ([1, 1, 1], [3000, 8000, 10]), ([40], [6000])]):
+        b = Batch(new, held, 16, seed=i)
+        q, k, v, _, _ = problem(b, 2, group, d, "bf16", False, dev)
+        work.append((b, q.to(dev), k, v, b.where(dev), torch.zeros_like(q, device=dev)))
+
+    def launch(i, workspace=None, stream=None):
+        b, q, k, v, where, out = work[i]
+        ct.paged_attention(q, k, v, *where, ct.partition(out, [1, 1, d]), d ** -0.5, max_new=max(b.new), max_context=max(b.held), workspace=workspace, stream=stream)
+
+    alone = []
+    for i in range(4):
+        launch(i)
+        torch.cuda.synchronize()
+        alone.append(work[i][-1].clone())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [torch.zeros(ct.PAGED_ATTENTION_WORKSPACE_BYTES, dtype=torch.uint8, device=dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs = [ct.CapturedGraph().capture(lambda s, i=i: launch(2 + i, spaces[i], s)) for i in range(2)]
+    for _ in range(5):
+        for w in work:
+            w[-1].fill_(5.0)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for i in range(2):
+                graphs[i].launch()
+                with torch.cuda.stream(streams[i]):
+                    launch(i)
+        for g in graphs:
+            g.synchronize()
+        torch.cuda.synchronize()
+        for w, want in zip(work, alone):
+            assert torch.equal(w[-1], want)
+    for g in graphs:
+        g.close()
